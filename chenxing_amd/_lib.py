@@ -6,8 +6,10 @@ that already live on the GPU and run on the current torch stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
+import struct
 import threading
 
 import numpy as np
@@ -52,6 +54,16 @@ _SIGS = {
     "cx_lmhead_argmax_bf16": (C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32,
                                         C.c_int32, _P, _P, _P, _P, C.c_size_t, _P]),
     "cx_lmhead_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
+    "cx_kv_append_bf16": (C.c_int, [C.c_char_p, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
+                                    _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int32, C.c_int32,
+                                    C.c_int32, _P, _P, C.c_double, _P, _P]),
+    "cx_paged_attention_bf16": (C.c_int, [C.c_char_p, _P, C.c_int64, C.c_int64, C.c_int32,
+                                          C.c_int32, C.c_double, C.c_int32, C.c_double, _P, _P,
+                                          C.c_size_t, _P]),
+    "cx_paged_attention_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32,
+                                                        C.c_int32]),
+    "cx_kv_copy_pages": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P,
+                                   _P, C.c_int32, _P]),
     "cx_timing_enable": (C.c_int, [C.c_int]),
     "cx_timing_read": (C.c_int, [C.c_int32, _P, _P]),
     "cx_last_error": (C.c_char_p, []),
@@ -234,11 +246,20 @@ class Workspace:
 _ws_sample = Workspace()
 _ws_verify = Workspace()
 _ws_head = Workspace()
+_ws_attend = Workspace()
 
 
 def _stream_ptr(device):
     import torch
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _on(device):
+    """The tensor's device as the current one, where it is not."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def sample_device(logits, prm, u, hist=None, hist_len=None, out_id=None, row_status=None,
@@ -361,6 +382,161 @@ def lmhead_argmax_device(hidden, weight, out_id=None, out_max=None, out_logits=N
     return out_id, out_max
 
 
+# cx_kv_batch of include/cx_sampler.h
+_KV_BATCH = struct.Struct("<QqQqQQ8i")
+KV_BF16, KV_E4M3 = 1, 3
+
+
+def _kv_batch(cache, D, table, kv_len, q_start, T):
+    """(packed cx_kv_batch, page tokens, bf16 pages) of one layer's pages and a batch."""
+    import torch
+    if cache.dim() != 3 or cache.stride(2) != 1 or cache.stride(1) != cache.shape[2]:
+        raise ValueError("cache must be one layer's [n_pages, kv_heads, width] pages, each page "
+                         "contiguous")
+    n, heads, width = cache.shape
+    bf16 = cache.dtype == torch.bfloat16
+    if not bf16 and cache.dtype != torch.uint8:
+        raise ValueError("cache must be bfloat16 pages, or uint8 pages of e4m3 codes and scales")
+    # bf16: 2 P D elements; e4m3: 2 P D codes and 8 P bytes of scales
+    P, rest = divmod(width, 2 * D if bf16 else 2 * D + 8)
+    if rest:
+        raise ValueError(f"a page's width ({width}) does not fit heads of {D}")
+    if table.dim() != 2 or table.stride(1) != 1 or kv_len.dim() != 1 or \
+            not kv_len.is_contiguous() or table.dtype != torch.int32 or \
+            kv_len.dtype != torch.int32:
+        raise ValueError("table [B, pages] and kv_len [B] must be int32 with unit strides")
+    B, M = table.shape
+    if kv_len.shape[0] != B:
+        raise ValueError("table and kv_len differ in B")
+    st = 0
+    if q_start is not None:
+        if q_start.dtype != torch.int32 or tuple(q_start.shape) != (B + 1,) or \
+                not q_start.is_contiguous():
+            raise ValueError("q_start must be a contiguous int32 [B + 1]")
+        st = q_start.data_ptr()
+    elif T != B:
+        raise ValueError("without q_start there is one new token per sequence")
+    for t in (cache, table, kv_len):
+        if not t.is_cuda:
+            raise ValueError("cache, table and kv_len must be cuda tensors")
+    return (_KV_BATCH.pack(cache.data_ptr(), cache.stride(0) * (2 if bf16 else 1),
+                           table.data_ptr(), table.stride(0), kv_len.data_ptr(), st, n, heads, D,
+                           P, KV_BF16 if bf16 else KV_E4M3, B, M, T), P, bf16)
+
+
+def _rows3(name, t):
+    """[tokens, heads, D] bf16 rows on the GPU."""
+    import torch
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.stride(2) != 1 or not t.is_cuda:
+        raise ValueError(f"{name} must be a bfloat16 [tokens, heads, D] cuda tensor with unit "
+                         "element stride")
+    return t.shape
+
+
+def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, interleaved=False,
+                     q_norm=None, k_norm=None, eps=1e-6, q_out=None):
+    """The new tokens' q, k and v made ready for attention, on the current stream.
+
+    q [T, Hq, D], k and v [T, Hkv, D] (bfloat16, any token and head strides that
+    keep rows 16-byte aligned): q and k normed per head (``q_norm`` / ``k_norm``
+    [D] bfloat16 weights, or None), their first dims rotated to the tokens'
+    positions (``rope`` [positions, rotary dim] float32, ``kvcache.rope_table``;
+    None: not at all), k and v written into ``cache``, one layer's pages.
+    ``table`` [B, pages], ``kv_len`` [B] (the new tokens included) and
+    ``q_start`` [B + 1] (None: one new token each) are int32.  Returns q_out
+    [T, Hq, D]."""
+    import torch
+    lib = load()
+    T, Hq, D = _rows3("q", q)
+    kv, P, _ = _kv_batch(cache, D, table, kv_len, q_start, T)
+    heads = cache.shape[1]
+    if _rows3("k", k) != (T, heads, D) or _rows3("v", v) != (T, heads, D):
+        raise ValueError("k and v must be [T, kv_heads, D]")
+    rows = rdim = 0
+    if rope is not None:
+        if rope.dim() != 2 or rope.dtype != torch.float32 or not rope.is_contiguous() or \
+                not rope.is_cuda:
+            raise ValueError("rope must be a contiguous float32 [positions, rotary dim] cuda "
+                             "tensor")
+        rows, rdim = rope.shape
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None and (w.dtype != torch.bfloat16 or tuple(w.shape) != (D,) or
+                              not w.is_contiguous() or not w.is_cuda):
+            raise ValueError(f"{name} must be a contiguous bfloat16 [D] cuda tensor")
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
+    elif _rows3("q_out", q_out) != (T, Hq, D) or not q_out.is_contiguous():
+        raise ValueError("q_out must be a contiguous [T, q_heads, D]")
+    with _on(q.device):
+        _check(lib.cx_kv_append_bf16(
+            kv, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1), Hq,
+            rope.data_ptr() if rope is not None else None, rows, rdim, interleaved,
+            q_norm.data_ptr() if q_norm is not None else None,
+            k_norm.data_ptr() if k_norm is not None else None, eps, q_out.data_ptr(),
+            _stream_ptr(q.device)))
+    return q_out
+
+
+def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, scale=None, window=0,
+                           softcap=0.0, out=None):
+    """Attention of the new tokens over one layer's pages, on the current stream.
+
+    q [T, Hq, D] bfloat16 (as ``kv_append_device`` returns it); ``cache``,
+    ``table``, ``kv_len`` and ``q_start`` as there, the new tokens already
+    appended.  The token at position p attends to the positions up to p, the
+    last ``window`` of them if window > 0; ``scale`` defaults to D ** -0.5;
+    scores are capped to softcap * tanh(score / softcap) if softcap > 0.
+    ``max_new`` is the most new tokens of a sequence (it picks the tile).
+    Returns out [T, Hq, D] bfloat16; a token that attends to nothing gets
+    zeros."""
+    import torch
+    lib = load()
+    T, Hq, D = _rows3("q", q)
+    kv, _, _ = _kv_batch(cache, D, table, kv_len, q_start, T)
+    dev = q.device
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+    elif _rows3("out", out) != (T, Hq, D) or not out.is_contiguous():
+        raise ValueError("out must be a contiguous [T, q_heads, D]")
+    sp = _stream_ptr(dev)
+    ws = _ws_attend.get(lib.cx_paged_attention_workspace_bytes(Hq, cache.shape[1], D, max_new),
+                        dev, sp.value)
+    with _on(dev):
+        _check(lib.cx_paged_attention_bf16(
+            kv, q.data_ptr(), q.stride(0), q.stride(1), Hq, max_new,
+            D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(),
+            ws.data_ptr(), ws.numel(), sp))
+    return out
+
+
+def kv_copy_pages_device(cache, src, dst):
+    """Page dst[i] of every layer becomes a copy of page src[i], on the current
+    stream.  ``cache`` is [layers, n_pages, ...] or, as one layer of it,
+    [n_pages, kv_heads, width]; src and dst are int32 [n].  No page may be the
+    destination of two pairs, or a destination and a source.  Returns cache."""
+    import torch
+    lib = load()
+    if cache.dim() not in (3, 4) or cache.stride(-1) != 1 or cache.stride(-2) != cache.shape[-1]:
+        raise ValueError("cache must be [layers, n_pages, kv_heads, width] or one layer of it, "
+                         "each page contiguous")
+    for t in (src, dst):
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or not t.is_cuda:
+            raise ValueError("src and dst must be contiguous int32 cuda tensors")
+    if src.shape != dst.shape:
+        raise ValueError("src and dst differ in length")
+    if not cache.is_cuda:
+        raise ValueError("cache must be a cuda tensor")
+    el = cache.element_size()
+    layers, stride = (1, 0) if cache.dim() == 3 else (cache.shape[0], cache.stride(0) * el)
+    with _on(cache.device):
+        _check(lib.cx_kv_copy_pages(
+            cache.data_ptr(), stride, cache.stride(-3) * el,
+            cache.shape[-1] * cache.shape[-2] * el, layers, cache.shape[-3], src.data_ptr(),
+            dst.data_ptr(), src.shape[0], _stream_ptr(cache.device)))
+    return cache
+
+
 def header_symbols() -> list[str]:
     """Function names declared in include/cx_sampler.h."""
     import re
@@ -372,8 +548,8 @@ def header_symbols() -> list[str]:
 
 (KERNEL_SAMPLE, KERNEL_SAMPLE_SLOW, KERNEL_VERIFY_STATS, KERNEL_VERIFY_REST,
  KERNEL_SAMPLE_FINISH, KERNEL_PENALTIES, KERNEL_TRUNCATE, KERNEL_LMHEAD,
- KERNEL_LMHEAD_MERGE) = range(9)
-KERNEL_KINDS = 9
+ KERNEL_LMHEAD_MERGE, KERNEL_KV_APPEND, KERNEL_ATTEND, KERNEL_KV_COPY) = range(12)
+KERNEL_KINDS = 12
 
 
 def timing_enable(on: bool = True) -> None:

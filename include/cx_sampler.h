@@ -241,6 +241,113 @@ int cx_lmhead_argmax_bf16(const uint16_t* hidden, int64_t ldh, const uint16_t* w
 
 size_t cx_lmhead_workspace_bytes(int32_t B, int32_t V);
 
+/*
+ * The paged KV cache between two sampling calls: the new tokens' keys and
+ * values written to pages, their attention over the pages, pages copied.  The
+ * reference keeps such a cache, attends over it and rotates positions in numpy
+ * on the host (engine/radix_kv.py, core/attention.py:43-148,
+ * core/tensor.py:36-180).
+ *
+ * A page of one layer holds page_tokens tokens of every kv head.  A head's
+ * part is contiguous, all of it in 16-byte chunks of E elements (E = 8 for
+ * bf16, 16 for e4m3), D = head_dim, P = page_tokens:
+ *   K   chunk (d / E) * P + t holds dims d .. d + E - 1 of token t
+ *   V   chunk (t / E) * D + d holds tokens t .. t + E - 1 of dim d
+ *   e4m3 only: P fp32 scales of the tokens' keys, then P of their values
+ * (2 P D elements, and 8 P bytes of scales).  An e4m3 code stands for its value
+ * times its token's scale.
+ *
+ * One forward pass over a batch of sequences: sequence b's new tokens are rows
+ * q_start[b] .. q_start[b + 1] - 1 of q, k, v and the outputs (q_start from 0 to
+ * T; NULL: one new token each, T = B), and the last ones of its kv_len[b]
+ * tokens; token t lies in page table[b][t / P].  A token whose position is
+ * negative or past the table's pages, or whose page id is outside [0, n_pages),
+ * is neither written nor attended.
+ */
+#define CX_KV_BF16 1
+#define CX_KV_E4M3 3                     /* OCP e4m3: largest value 448 */
+#define CX_KV_MAX_BATCH 4096
+typedef struct cx_kv_batch {
+  void* pages;               /* one layer's pages, 16-byte aligned             */
+  int64_t page_stride;       /* bytes from one page to the next                */
+  const int32_t* table;      /* [B, ld_table] page ids                         */
+  int64_t ld_table;
+  const int32_t* kv_len;     /* [B] tokens, the new ones included              */
+  const int32_t* q_start;    /* [B + 1], or NULL                               */
+  int32_t n_pages, kv_heads;
+  int32_t head_dim;          /* 64, 128 or 256                                 */
+  int32_t page_tokens;       /* 16, 32, 64, 128 or 256                         */
+  int32_t dtype;             /* CX_KV_BF16 or CX_KV_E4M3                       */
+  int32_t B, max_pages, T;   /* max_pages: ids of a table row                  */
+} cx_kv_batch;
+
+/*
+ * The new tokens of a forward pass made ready for attention: q and k normed
+ * per head (optional), rotated to their positions (optional), q written to
+ * q_out, k and v to the pages.  One pass over q, k and v.  fp32 arithmetic,
+ * each result rounded once.
+ *
+ *  q, k, v    bf16 bits, row (token, head) at token * _token + head * _head
+ *             elements, rows 16-byte aligned
+ *  q_norm, k_norm  nullable [D] bf16 bits: x * rsqrt(mean(x^2) + eps) * weight
+ *  rope       nullable [rope_rows, rotary_dim] fp32: the cosines of position p
+ *             (rotary_dim / 2), then the sines; rope_rows at least max_pages *
+ *             page_tokens.  The first rotary_dim dims of a head are rotated (a
+ *             multiple of 16), pairs (j, j + rotary_dim / 2), or (2 j, 2 j + 1)
+ *             if interleaved
+ *  q_out      [T, q_heads, D] bf16 bits
+ * e4m3: a (token, head)'s scale is max|x| / 448, 1 for a row of zeros; a row
+ * holding inf or NaN gets a NaN scale and zero codes.
+ * Device pointers, stream-ordered, no synchronisation, no allocation.
+ */
+int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token, int64_t q_head,
+                      const uint16_t* k, int64_t k_token, int64_t k_head, const uint16_t* v,
+                      int64_t v_token, int64_t v_head, int32_t q_heads, const float* rope,
+                      int32_t rope_rows, int32_t rotary_dim, int32_t interleaved,
+                      const uint16_t* q_norm, const uint16_t* k_norm, double eps,
+                      uint16_t* q_out, void* stream);
+
+/*
+ * Attention of the new tokens over the pages: a decode step's single tokens, a
+ * verify round's gamma + 1, several together.  q head h reads kv head
+ * h / (q_heads / kv_heads).  The token at position p attends to the
+ * positions t <= p, t > p - window (window 0: all), with scores scale * q.k,
+ * capped to softcap * tanh(score / softcap) if softcap > 0.  A token that
+ * attends to nothing gets zeros.  fp32 scores, softmax and sums; out is rounded
+ * once.
+ *
+ *  q          bf16 bits, row (token, head) at token * q_token + head * q_head
+ *             elements, rows 16-byte aligned
+ *  max_new    the most new tokens of a sequence: picks the kernel's tile, and
+ *             any value >= 1 gives right results
+ *  out        [T, q_heads, D] bf16 bits
+ *  workspace  device scratch of cx_paged_attention_workspace_bytes(...) bytes;
+ *             any contents.  One workspace per stream.
+ * Device pointers, stream-ordered, no synchronisation, no allocation.
+ */
+int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
+                            int64_t q_head, int32_t q_heads, int32_t max_new, double scale,
+                            int32_t window, double softcap, uint16_t* out, void* workspace,
+                            size_t ws_bytes, void* stream);
+
+size_t cx_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                          int32_t max_new);
+
+/*
+ * Pages copied in every layer: page dst[i] becomes a copy of page src[i] (a
+ * fork's last page before either sequence appends to it, a compaction's
+ * moves).  A pair with an id outside [0, n_pages) is skipped.  No page may be
+ * the destination of two pairs, or of one pair and the source of another.
+ *
+ *  pages      layer l's page i at l * layer_stride + i * page_stride bytes;
+ *             page_bytes of it are copied (all multiples of 16)
+ *  src, dst   [n] int32
+ * Device pointers, stream-ordered, no synchronisation, no allocation.
+ */
+int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int64_t page_bytes,
+                     int32_t n_layers, int32_t n_pages, const int32_t* src, const int32_t* dst,
+                     int32_t n, void* stream);
+
 /* Kernel timing (measurement only).  While enabled, every library kernel is
  * dispatched with a start / stop event pair recorded by the dispatch itself
  * (hipExtLaunchKernel): the kernel's execution interval on its stream.
@@ -258,7 +365,10 @@ size_t cx_lmhead_workspace_bytes(int32_t B, int32_t V);
 #define CX_KERNEL_TRUNCATE      6  /* _truncate                       */
 #define CX_KERNEL_LMHEAD        7  /* LM head: projection tiles + argmax keys */
 #define CX_KERNEL_LMHEAD_MERGE  8  /* LM head: per-row merge of the keys */
-#define CX_KERNEL_KINDS         9
+#define CX_KERNEL_KV_APPEND     9  /* q, k, v normed, rotated, k and v to the pages */
+#define CX_KERNEL_ATTEND        10 /* paged attention                  */
+#define CX_KERNEL_KV_COPY       11 /* page copies                      */
+#define CX_KERNEL_KINDS         12
 int cx_timing_enable(int on);
 int cx_timing_read(int32_t kernel, double* total_ms, int64_t* launches);
 
