@@ -548,8 +548,9 @@ def header_symbols() -> list[str]:
 
 (KERNEL_SAMPLE, KERNEL_SAMPLE_SLOW, KERNEL_VERIFY_STATS, KERNEL_VERIFY_REST,
  KERNEL_SAMPLE_FINISH, KERNEL_PENALTIES, KERNEL_TRUNCATE, KERNEL_LMHEAD,
- KERNEL_LMHEAD_MERGE, KERNEL_KV_APPEND, KERNEL_ATTEND, KERNEL_KV_COPY) = range(12)
-KERNEL_KINDS = 12
+ KERNEL_LMHEAD_MERGE, KERNEL_KV_APPEND, KERNEL_ATTEND,
+ KERNEL_ATTEND_JOIN, KERNEL_KV_COPY) = range(13)
+KERNEL_KINDS = 13
 
 
 def timing_enable(on: bool = True) -> None:

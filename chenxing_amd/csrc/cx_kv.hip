@@ -17,6 +17,7 @@ int kv_args(const cx_kv_batch* kv, int q_heads, KvArgs* out) {
   if (kv->B < 0 || kv->T < 0 || kv->n_pages < 0 || kv->max_pages < 0 || kv->kv_heads < 1 ||
       kv->ld_table < kv->max_pages)
     return api_fail(CX_EINVAL, "bad shape");
+  if (kv->T > KV_MAX_NEW) return api_fail(CX_EINVAL, "too many new tokens (%d)", kv->T);
   if (kv->B > CX_KV_MAX_BATCH)
     return api_fail(CX_EINVAL, "a call takes at most %d sequences (%d)", CX_KV_MAX_BATCH, kv->B);
   if (D != 64 && D != 128 && D != 256)

@@ -16,6 +16,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float E4M3_MAX = 448.f;
+constexpr int KV_MAX_NEW = 1 << 28;           // new tokens of a call: positions stay above -2^28
 
 // cx_kv_batch with what the kernels derive from it.
 struct KvArgs {

@@ -367,8 +367,9 @@ int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int
 #define CX_KERNEL_LMHEAD_MERGE  8  /* LM head: per-row merge of the keys */
 #define CX_KERNEL_KV_APPEND     9  /* q, k, v normed, rotated, k and v to the pages */
 #define CX_KERNEL_ATTEND        10 /* paged attention                  */
-#define CX_KERNEL_KV_COPY       11 /* page copies                      */
-#define CX_KERNEL_KINDS         12
+#define CX_KERNEL_ATTEND_JOIN   11 /* paged attention: split rows joined */
+#define CX_KERNEL_KV_COPY       12 /* page copies                      */
+#define CX_KERNEL_KINDS         13
 int cx_timing_enable(int on);
 int cx_timing_read(int32_t kernel, double* total_ms, int64_t* launches);
 
