@@ -6,7 +6,7 @@
 // terms: a block of scores raises m to m', and l and the output so far are
 // scaled by exp(m - m').  Two stream-ordered launches:
 //
-//   1. attend_split  workgroups of 4 waves, each with an equal share of all the
+//   1. attend_split  independent waves, each with an equal share of all the
 //                    batch's units (32 tokens of bf16, 64 of e4m3, for one kv
 //                    head and row block); a row block that ends inside the share
 //                    it began in is written out, the others' parts (m, l, sums)
@@ -33,7 +33,6 @@ namespace cx {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ATT_WAVES = 4, ATT_WG = 64 * ATT_WAVES;
-constexpr int ATT_MIN_UNITS = ATT_WAVES;     // of a workgroup's share: one per wave
 constexpr float ATT_LOW = -3e38f;            // running maximum of a row that attends to something
 
 struct AttendArgs {
@@ -45,21 +44,26 @@ struct AttendArgs {
   int cap;                    // the latter
   int window;                 // 0: none
   uint16_t* out;
-  struct AttendJoin* join;    // [grid]
-  float* ml;                  // [2 grid, ROWS, 2]: a part's maxima and sums
-  float* part;                // [2 grid, ROWS, D]
+  struct AttendJoin* join;    // [workers]
+  float* ml;                  // [2 workers, ROWS, 2]: a part's maxima and sums
+  float* part;                // [2 workers, ROWS, D]
 };
 
-// A row block whose units lie in several workgroups' shares: those of
-// workgroups first .. last.  Written by the first; none: last = -1.
+// A row block whose units lie in several workers' shares: those of workers
+// first .. last.  Written by the first; none: last = -1.
 struct AttendJoin {
   int first, last;
   int tok0, row0, rows, head;
   int pad[2];
 };
 
-// What a workgroup needs of a sequence: its rows among the new tokens, the
-// length, and its units of TOK tokens (those in some row's window).
+// 16 bytes of a page, read once: past the caches (131072 tokens 181 -> 161 us)
+__device__ __forceinline__ u32x4 ld_page(const char* p) {
+  return __builtin_nontemporal_load((const u32x4*)p);
+}
+
+// A sequence: its rows among the new tokens, the length, and its units of TOK
+// tokens (those in some row's window).
 struct AttendSeq {
   int tok0, q, len, lim, first, n;
 };
@@ -84,6 +88,63 @@ __device__ __forceinline__ uint64_t scalar64(uint64_t x) {
          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
 
+// Lane groups and registers change places.  Four registers: x[y] of group g
+// becomes x[g] of group y.  Two: the registers of groups 0 1 2 3, [a0 a1 a2 a3]
+// and [b0 b1 b2 b3], become [a0 a2 b0 b2] and [a1 a3 b1 b3].
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+__device__ __forceinline__ void swap_rows(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+// The largest of the four lane groups' values, in every group.
+__device__ __forceinline__ float groups_max(float x) {
+  uint32_t a = __float_as_uint(x), b = a;
+  swap_halves(a, b);
+  x = fmaxf(__uint_as_float(a), __uint_as_float(b));
+  a = b = __float_as_uint(x);
+  swap_rows(a, b);
+  return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+  uint32_t a = __float_as_uint(x), b = a;
+  swap_halves(a, b);
+  x = __uint_as_float(a) + __uint_as_float(b);
+  a = b = __float_as_uint(x);
+  swap_rows(a, b);
+  return __uint_as_float(a) + __uint_as_float(b);
+}
+// A mask of the bf16 or e4m3 elements of x that are NaN or infinite.
+template <bool F8>
+__device__ __forceinline__ uint32_t nonfinite(uint32_t x) {
+  if (F8) {                                  // code 0x7F or 0xFF
+    const uint32_t m = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    return m | (m - (m >> 7));
+  }
+  return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0) |
+         ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0);
+}
+__device__ __forceinline__ void regroup(uint32_t (&x)[4][2]) {
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+    swap_halves(x[0][d], x[2][d]);
+    swap_halves(x[1][d], x[3][d]);
+    swap_rows(x[0][d], x[1][d]);
+    swap_rows(x[2][d], x[3][d]);
+  }
+}
+__device__ __forceinline__ void regroup(uint32_t (&x)[2][2]) {
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+    swap_halves(x[0][d], x[1][d]);
+    swap_rows(x[0][d], x[1][d]);
+  }
+}
+
 __device__ __forceinline__ bf16x8 e4m3x8(uint32_t a, uint32_t b) {
   const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
   const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
@@ -97,26 +158,35 @@ struct AttendShape {
   static constexpr int TOK = F8 ? 64 : 32;   // tokens of a unit
   static constexpr int ROWS = 16 * NT;
   static constexpr int E = F8 ? 16 : 8;      // elements of a 16-byte chunk
-  static constexpr int PAD = D + 4;          // floats of a row of s_o
+  static constexpr int PAD = D + 4;          // floats of a row of a wave's scratch
   static constexpr int WAVES = NT == 1 && D < 256 ? 2 : 1;   // per SIMD
-  static constexpr int OFF_O = ROWS * D * 2;
-  static constexpr int OFF_ML = OFF_O + ATT_WAVES * 16 * PAD * 4;
-  static constexpr int OFF_SCALE = OFF_ML + ATT_WAVES * ROWS * 8;
+  static constexpr int OFF_SCALE = ATT_WAVES * 16 * PAD * 4;
   static constexpr int OFF_PREF = OFF_SCALE + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
   static int lds(int B) { return OFF_PREF + 8 * (B + 1); }
 };
 
-// The lengths are on the device, so each workgroup finds its share itself: the
-// units of every sequence summed up in LDS, and its range of the total.  Its
-// waves take the units of a row block in turn and merge through LDS at its end.
+// Consecutive units of one row block in a worker's share: rows r0 .. r0 + R - 1
+// of (new token, q head of the group) of kv head h of sequence b.
+struct AttendPiece {
+  int b, h, tok0, r0, R, lowest, lim;        // lowest: position of the first new token
+  int unit, cnt;
+  int slot;                                  // of its part, -1: the whole row block
+};
+
+// The lengths are on the device, so each worker (a wave) finds its share itself:
+// the units of every sequence summed up in LDS, and its range of the total.
 //
-//  * S^T = K Q^T, so a lane holds scores of 4 neighbouring tokens a tile for its
-//    row (column) and the softmax's statistics need two shuffles; tile y's row
-//    4 g + j is the unit's token (TOK / 4) g + 4 y + j, which makes a lane's
-//    terms the very operand of O^T = V^T P^T, and its part of V 16 contiguous
-//    bytes of a page: neither passes through LDS.
+//  * S^T = K Q^T, tile y being the unit's tokens 16 y .. 16 y + 15 of one page:
+//    a lane holds scores of tokens 16 y + 4 g + j for its row (column), and the
+//    softmax's statistics need two lane swaps.  O^T = V^T P^T wants a lane's terms
+//    of the TOK / 4 tokens whose V it loaded as 16 contiguous bytes: lane groups
+//    and tiles change places by lane swaps.  Nothing passes through LDS but the
+//    e4m3 scales.
 //  * The next unit's K is requested when this unit's scores are taken, its V
-//    after this unit's products: half of a unit's 16 KB is always in flight.
+//    after this unit's products: half of a unit's 16 KB is always in flight, also
+//    from one piece to the next.  The requests are unconditional (a branch on
+//    them would make the waits of the loop drain them); after the last unit they
+//    all name one place.
 //  * Softmax terms enter the products as two bf16 parts (16 bits): one part's
 //    rounding would add as much error as the result's own.
 template <int D, int NT, bool F8>
@@ -125,22 +195,22 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   constexpr int TOK = Sh::TOK, ROWS = Sh::ROWS, E = Sh::E, PAD = Sh::PAD;
   constexpr int KT = TOK / 16;               // score tiles of a unit, and its 16-token groups
   constexpr int KL = D / (4 * E);            // K loads of a tile
+  constexpr int QL = D / 32;                 // Q loads of 16 rows
   constexpr int DT = D / 16, KH = TOK / 32;
   constexpr int BATCH = 64 / KT;             // units whose page ids a wave holds
+  constexpr uint32_t ALL = (1u << KT) - 1;
   extern __shared__ __align__(16) char lds[];
-  CX_LDS u32x4* const s_q = to_lds((u32x4*)lds);
-  CX_LDS float* const s_o = to_lds((float*)(lds + Sh::OFF_O));
-  CX_LDS float* const s_ml = to_lds((float*)(lds + Sh::OFF_ML));
-  CX_LDS float* const s_scale = to_lds((float*)(lds + Sh::OFF_SCALE)) + wave_id() * 128;
-  CX_LDS uint64_t* const s_sum = to_lds((uint64_t*)(lds + Sh::OFF_PREF)) - ATT_WAVES;
-  CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::OFF_PREF));
   const KvArgs& C = A.kv;
   const int tid = threadIdx.x, w = wave_id(), l = lane_id(), g = l >> 4, c = l & 15;
   const int P = 1 << C.logP;
+  CX_LDS float* const s_o = to_lds((float*)lds) + w * (16 * PAD);
+  CX_LDS float* const s_scale = to_lds((float*)(lds + Sh::OFF_SCALE)) + w * 128;
+  CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::OFF_PREF));
+  CX_LDS uint64_t* const s_sum = s_pref - ATT_WAVES;
 
   // units before each sequence, over its kv heads and row blocks
   if (tid == 0) s_pref[0] = 0;
-  uint64_t run = 0;
+  uint64_t total = 0;
   for (int b0 = 0; b0 < C.B; b0 += ATT_WG) {
     const int b = b0 + tid;
     uint64_t x = 0;
@@ -156,11 +226,11 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     if (l == 63) s_sum[w] = x;
     __syncthreads();
     for (int k = 0; k < w; ++k) x += s_sum[k];
-    if (b < C.B) s_pref[b + 1] = run + x;
+    if (b < C.B) s_pref[b + 1] = total + x;
     __syncthreads();
-    run = s_pref[min(b0 + ATT_WG, C.B)];
+    total = s_pref[min(b0 + ATT_WG, C.B)];
   }
-  const uint64_t total = run;
+  total = scalar64(total);
 
   // tokens that attend to nothing
   for (int b = blockIdx.x; b < C.B; b += gridDim.x)
@@ -171,356 +241,405 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       for (int64_t i = tid; i < n; i += ATT_WG) o[i] = u32x4{0, 0, 0, 0};
     }
 
-  // this workgroup's share of the units: as many workgroups as have
-  // ATT_MIN_UNITS, the first ones with one unit more
-  const uint64_t shares = min((uint64_t)gridDim.x, (total + ATT_MIN_UNITS - 1) / ATT_MIN_UNITS);
+  // this worker's share of the units: a unit at least, the first shares one
+  // more.  Neighbouring workers are on different CUs.
+  const unsigned worker = __builtin_amdgcn_readfirstlane(blockIdx.x + gridDim.x * w);
+  const uint64_t shares = min((uint64_t)gridDim.x * ATT_WAVES, total);
+  if (worker >= shares) {
+    if (l == 0) A.join[worker].last = -1;
+    return;
+  }
+  const uint64_t per = scalar64(total / shares), more = total - per * shares;
+  uint64_t u = worker * per + min((uint64_t)worker, more);
+  const uint64_t end = u + per + (worker < more);
+  int b = 0;
+  for (int hi = C.B - 1; b < hi;) {          // the last b with s_pref[b] <= u
+    const int mid = (b + hi + 1) >> 1;
+    if (s_pref[mid] <= u) b = mid;
+    else hi = mid - 1;
+  }
   bool joined = false;
-  if (blockIdx.x < shares) {
-    const uint64_t per = total / shares, more = total % shares;
-    uint64_t u = scalar64(blockIdx.x * per + min((uint64_t)blockIdx.x, more));
-    const uint64_t end = scalar64(u + per + (blockIdx.x < more));
-    int b = 0;
-    for (int hi = C.B - 1; b < hi;) {        // the last b with s_pref[b] <= u
-      const int mid = (b + hi + 1) >> 1;
-      if (s_pref[mid] <= u) b = mid;
-      else hi = mid - 1;
+  // the piece that begins at unit u; b: the sequence of the one before
+  auto piece = [&]() {
+    while (s_pref[b + 1] <= u) ++b;
+    b = __builtin_amdgcn_readfirstlane(b);
+    const AttendSeq s = attend_seq<TOK>(A, b);
+    const uint64_t rem = scalar64(u - s_pref[b]);
+    const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
+    const unsigned row = rem >> 32 ? (unsigned)(rem / (unsigned)s.n)
+                                   : (unsigned)rem / (unsigned)s.n;
+    const int ua = (int)(rem - (uint64_t)row * (unsigned)s.n);
+    AttendPiece p;
+    p.b = b;
+    p.h = __builtin_amdgcn_readfirstlane((int)(row / (unsigned)blocks));
+    p.tok0 = s.tok0;
+    p.r0 = __builtin_amdgcn_readfirstlane((int)(row % (unsigned)blocks)) * ROWS;
+    p.R = min(ROWS, s.q * A.G - p.r0);
+    p.lowest = s.len - s.q;
+    p.lim = s.lim;
+    p.unit = __builtin_amdgcn_readfirstlane(s.first + ua);
+    p.cnt = __builtin_amdgcn_readfirstlane((int)min((uint64_t)(s.n - ua), end - u));
+    p.slot = ua == 0 && p.cnt == s.n ? -1 : (int)(2 * worker + (ua == 0));
+    p.slot = __builtin_amdgcn_readfirstlane(p.slot);
+    if (ua == 0 && p.cnt < s.n) {
+      joined = true;
+      const uint64_t lastu = u + s.n - 1, cut = more * (per + 1);
+      if (l == 0) {
+        AttendJoin j;
+        j.first = worker;
+        j.last = (int)(lastu < cut ? lastu / (per + 1) : more + (lastu - cut) / per);
+        j.tok0 = p.tok0; j.row0 = p.r0; j.rows = p.R; j.head = p.h;
+        j.pad[0] = j.pad[1] = 0;
+        A.join[worker] = j;
+      }
     }
-    while (u < end) {
-      while (s_pref[b + 1] <= u) ++b;
-      b = __builtin_amdgcn_readfirstlane(b);
-      const AttendSeq s = attend_seq<TOK>(A, b);
-      const uint64_t rem = scalar64(u - s_pref[b]);
-      const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
-      const unsigned row = rem >> 32 ? (unsigned)(rem / (unsigned)s.n)
-                                     : (unsigned)rem / (unsigned)s.n;
-      const int ua = (int)(rem - (uint64_t)row * (unsigned)s.n);
-      const int ub = (int)min((uint64_t)s.n, ua + (end - u));
-      const int h = __builtin_amdgcn_readfirstlane((int)(row / (unsigned)blocks));
-      const int r0 = __builtin_amdgcn_readfirstlane((int)(row % (unsigned)blocks)) * ROWS;
-      const int R = min(ROWS, s.q * A.G - r0);
-      const bool whole = ua == 0 && ub == s.n;
-      const int slot = 2 * blockIdx.x + (ua == 0);
-      if (ua == 0 && !whole) {
-        joined = true;
-        if (tid == 0) {
-          const uint64_t lastu = u + s.n - 1, cut = more * (per + 1);
-          AttendJoin j;
-          j.first = blockIdx.x;
-          j.last = (int)(lastu < cut ? lastu / (per + 1) : more + (lastu - cut) / per);
-          j.tok0 = s.tok0; j.row0 = r0; j.rows = R; j.head = h;
-          j.pad[0] = j.pad[1] = 0;
-          A.join[blockIdx.x] = j;
-        }
+    return p;
+  };
+
+  // ids of BATCH units of a piece from its k-th: lane KT k + group
+  auto load_ids = [&](const AttendPiece& p, int k) {
+    const int t16 = (p.unit + k) * KT + l;
+    return t16 < (p.lim + 15) >> 4 ? C.table[p.b * C.ld_table + (t16 >> (C.logP - 4))] : -1;
+  };
+  u32x4 qr[NT][QL], kr[KT][KL], vr[DT];
+  float ks = 1.f, vs = 1.f;                  // e4m3: the scales of the unit's token l
+  auto load_q = [&](const AttendPiece& p) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = p.r0 + min(16 * nt + c, p.R - 1);
+      const uint16_t* q = A.q + (p.tok0 + row / A.G) * A.q_token + (p.h * A.G + row % A.G) * A.q_head;
+#pragma unroll
+      for (int x = 0; x < QL; ++x)           // e4m3: the dims of a 16-element chunk in two
+        qr[nt][x] = *(const u32x4*)(q + (F8 ? 64 * (x / 2) + 16 * g + 8 * (x % 2) : 32 * x + 8 * g));
+    }
+  };
+  const int vgroup = F8 ? g : g >> 1;        // the group of this lane's tokens of V
+  // place in the page of a unit's 16-token group
+  auto place = [&](int unit, int group) { return ((unit * KT + group) << 4) & (P - 1); };
+  const uint32_t klane = (uint32_t)(c + (g << C.logP)) * 16;
+  // the unit's pages: which are in the pool (bit y: 16-token group y), and where
+  // this lane's V is
+  uint32_t held = 0, hnext = 0;
+  const char* vnext = nullptr;
+  auto load_k = [&](int ids, int k, int unit, int h, bool live) {
+    const char* const head0 = C.pages + (int64_t)h * C.head_bytes;
+    hnext = 0;
+#pragma unroll
+    for (int y = 0; y < KT; ++y) {
+      const int id = lane_read(ids, k * KT + y);
+      const bool in = (unsigned)id < (unsigned)C.n_pages;
+      hnext |= (uint32_t)in << y;
+      const char* p = head0 + (in ? id : 0) * C.page_stride + place(unit, y) * 16;
+#pragma unroll
+      for (int x = 0; x < KL; ++x)
+        kr[y][x] = ld_page(p + ((int64_t)x << (C.logP + 6)) + (live ? klane : 0));
+    }
+    const int id = __shfl(ids, k * KT + vgroup);
+    const char* p = head0 + ((unsigned)id < (unsigned)C.n_pages ? id : 0) * C.page_stride;
+    vnext = p + (live ? v_chunk<E, D>(c, place(unit, vgroup) + (F8 ? 0 : 8 * (g & 1)), C.logP) : 0);
+    if (F8) {
+      const float* sc = (const float*)(p + k_scale<D>(place(unit, g) + c, C.logP));
+      ks = sc[0];
+      vs = sc[P];
+    }
+  };
+  auto load_v = [&]() {
+    held = hnext;
+#pragma unroll
+    for (int n = 0; n < DT; ++n) vr[n] = ld_page(vnext + 256 * n);
+  };
+
+  f32x4 acc[NT][DT];
+  float m[NT], sum[NT];
+  int hi[NT], lo[NT];                        // the row attends to lo < t <= hi
+  int pmin = 0, pmax = 0;                    // positions of the piece's first and last row
+  bool again = false;
+  auto begin = [&](const AttendPiece& p) {
+    pmin = p.lowest + p.r0 / A.G;
+    pmax = p.lowest + (p.r0 + p.R - 1) / A.G;
+    again = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int pos = p.lowest + (p.r0 + min(16 * nt + c, p.R - 1)) / A.G;
+      hi[nt] = min(pos, p.lim - 1);
+      lo[nt] = A.window ? pos - A.window : -1;
+      m[nt] = -INFINITY;
+      sum[nt] = 0;
+#pragma unroll
+      for (int n = 0; n < DT; ++n) acc[nt][n] = f32x4{0, 0, 0, 0};
+    }
+  };
+
+  AttendPiece cur = piece(), nxt;
+  u += cur.cnt;
+  load_q(cur);
+  int ids = load_ids(cur, 0), idn = load_ids(cur, BATCH), idq = -1;
+  load_k(ids, 0, cur.unit, cur.h, true);
+  load_v();
+  bool last = u >= end;
+  nxt = cur;
+  if (!last) nxt = piece();
+  idq = load_ids(nxt, 0);
+  begin(cur);
+  for (int i = 0;;) {
+    const int unit = cur.unit + i, t0 = unit * TOK;
+    // scores: tile y's row 4 g + j is token t0 + 16 y + 4 g + j
+    f32x4 v[NT][KT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int y = 0; y < KT; ++y) v[nt][y] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int x = 0; x < QL; ++x)
+#pragma unroll
+      for (int y = 0; y < KT; ++y) {
+        const bf16x8 ka = F8 ? e4m3x8(kr[y][x / 2][2 * (x % 2)], kr[y][x / 2][2 * (x % 2) + 1])
+                             : __builtin_bit_cast(bf16x8, kr[y][x]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          v[nt][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              ka, __builtin_bit_cast(bf16x8, qr[nt][x]), v[nt][y], 0, 0, 0);
       }
-      u += ub - ua;
-
-      __syncthreads();                       // the last segment's reads of LDS are done
-      for (int i = tid; i < ROWS * (D / 8); i += ATT_WG) {
-        const int r = i % ROWS, ch = i / ROWS;
-        u32x4 x = {0, 0, 0, 0};
-        if (r < R)
-          x = *(const u32x4*)(A.q + (s.tok0 + (r0 + r) / A.G) * A.q_token +
-                              (h * A.G + (r0 + r) % A.G) * A.q_head + 8 * ch);
-        s_q[i] = x;
+    f32x4 vscale[F8 ? KT : 1];
+    if (F8) {
+      s_scale[l] = ks;                       // the wave's own words: no barrier
+      s_scale[64 + l] = vs;
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int y = 0; y < KT; ++y) {
+        const f32x4 kscale = *(const CX_LDS f32x4*)(s_scale + 16 * y + 4 * g);
+        vscale[y] = *(const CX_LDS f32x4*)(s_scale + 64 + 16 * y + 4 * g);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) v[nt][y] *= kscale;
       }
+    }
+    // K and Q are used up: those of the next unit, in this piece or the next
+    const bool turn = i + 1 == cur.cnt;
+    int k = (i + 1) % BATCH;
+    if (turn) {
+      ids = idq;
+      k = 0;
+      load_q(nxt);
+    } else if (k == 0) {
+      ids = idn;
+      idn = load_ids(cur, i + 1 + BATCH);
+    }
+    load_k(ids, k, turn ? nxt.unit : unit + 1, turn ? nxt.h : cur.h, !(turn && last));
 
-      const int lowest = s.len - s.q;
-      int pos[NT];                           // this lane's rows
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) pos[nt] = lowest + min(r0 + 16 * nt + c, r0 + R - 1) / A.G;
-      const int pmin = lowest + r0 / A.G, pmax = lowest + (r0 + R - 1) / A.G;
-
-      const int cnt = (ub - ua - w + ATT_WAVES - 1) / ATT_WAVES;   // this wave's units
-      const int unit0 = s.first + ua + w;
-      // ids of BATCH units from the k-th: lane KT k + group
-      auto load_ids = [&](int k) {
-        const int t16 = (unit0 + ATT_WAVES * (k + l / KT)) * KT + l % KT;
-        int id = -1;
-        if (t16 < (s.lim + 15) >> 4) id = C.table[b * C.ld_table + (t16 >> (C.logP - 4))];
-        return (unsigned)id < (unsigned)C.n_pages ? id : -1;
-      };
-      // this lane's one of a unit's page ids: of its row of K, or of its tokens
-      auto pick = [&](int ids, int k, int group) {
-        int id = lane_read(ids, k * KT);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 1; x < KT; ++x) {
-          const int y = lane_read(ids, k * KT + x);
-          id = group == x ? y : id;
-        }
-        return id;
-      };
-      const int kgroup = F8 ? c >> 2 : c >> 3, vgroup = F8 ? g : g >> 1;
-      // place in the page of a unit's 16-token group
-      auto place = [&](int unit, int group) { return ((unit * KT + group) << 4) & (P - 1); };
-
-      u32x4 kr[KT][KL], vr[DT];
-      float ks = 1.f, vs = 1.f;              // e4m3: the scales of the unit's token l
-      const char* const head0 = C.pages + (int64_t)h * C.head_bytes;
-      const char *vp = nullptr, *vnext = nullptr;
-      bool held = false, hnext = false;
-      auto load_k = [&](int ids, int k, int unit) {
-        const int id = pick(ids, k, kgroup), vid = pick(ids, k, vgroup);
-        const char* p = head0 + max(id, 0) * C.page_stride +
-                        ((place(unit, kgroup) + (F8 ? c & 3 : (c & 3) + 2 * (c & 4))) << 4) +
-                        (g << (C.logP + 4));
+      for (int y = 0; y < KT; ++y) v[nt][y] *= A.s1;
+    if (A.cap) {                             // tanh(z) = 1 - 2 / (exp(2 z) + 1)
 #pragma unroll
-        for (int x = 0; x < KL; ++x)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int y = 0; y < KT; ++y)
-            kr[y][x] = *(const u32x4*)(p + 64 * y + ((int64_t)x << (C.logP + 6)));
-        vnext = head0 + max(vid, 0) * C.page_stride;
-        hnext = vid >= 0;
-        if (F8) ks = *(const float*)(vnext + k_scale<D>(place(unit, g) + c, C.logP));
-      };
-      auto load_v = [&](int unit) {
-        vp = vnext;
-        held = hnext;
-        const char* p = vp + v_chunk<E, D>(c, place(unit, vgroup) + (F8 ? 0 : 8 * (g & 1)), C.logP);
+        for (int y = 0; y < KT; ++y)
 #pragma unroll
-        for (int n = 0; n < DT; ++n) vr[n] = *(const u32x4*)(p + 256 * n);
-        if (F8) vs = *(const float*)(vp + v_scale<D>(place(unit, g) + c, C.logP));
-      };
-
-      f32x4 acc[NT][DT];
-      float m[NT], sum[NT];
+          for (int j = 0; j < 4; ++j)
+            v[nt][y][j] = fmaf(-2.f * A.s2,
+                               __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v[nt][y][j]) + 1.f), A.s2);
+    }
+    // a row's running maximum is at least ATT_LOW once it has attended to a
+    // token, whatever its score: -inf says that it has not
+    float top[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) top[nt] = ATT_LOW;
+    // a unit is open where all its tokens are held, at or before the first row
+    // and inside the last row's window
+    const uint32_t here = held;
+    const bool masked = t0 + TOK - 1 > pmin || t0 + TOK > cur.lim ||
+                        (A.window && t0 <= pmax - A.window) || here != ALL;
+    if (masked) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        m[nt] = -INFINITY;
-        sum[nt] = 0;
+        bool some = false;
 #pragma unroll
-        for (int n = 0; n < DT; ++n) acc[nt][n] = f32x4{0, 0, 0, 0};
-      }
-      int ids = -1, idn = -1;
-      if (cnt > 0) {
-        ids = load_ids(0);
-        idn = load_ids(BATCH);
-        load_k(ids, 0, unit0);
-        load_v(unit0);
-      }
-      __syncthreads();                       // s_q
-      for (int i = 0; i < cnt; ++i) {
-        const int unit = unit0 + ATT_WAVES * i, t0 = unit * TOK;
-        // a unit is open where all its tokens are held, at or before the first
-        // row and inside the last row's window
-        const bool masked = t0 + TOK - 1 > pmin || t0 + TOK > s.lim ||
-                            (A.window && t0 <= pmax - A.window) || __any(!held);
-        const int tl = t0 + (TOK / 4) * g;   // this lane's first token
-        const bool more_units = i + 1 < cnt;
-        u32x4 ph[NT][KH], pl[NT][KH];
+        for (int y = 0; y < KT; ++y) {
+          const int ty = t0 + 16 * y;
+          const bool in = here >> y & 1;
+          some |= in && max(ty, lo[nt] + 1) <= min(ty + 15, hi[nt]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          // scores: tile y's row 4 g + j is token t0 + (TOK / 4) g + 4 y + j
-          f32x4 v[KT];
-#pragma unroll
-          for (int y = 0; y < KT; ++y) v[y] = f32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int x = 0; x < KL; ++x)
-#pragma unroll
-            for (int e = 0; e < (F8 ? 2 : 1); ++e) {
-              const u32x4 qv = s_q[(F8 ? 2 * (4 * x + g) + e : 4 * x + g) * ROWS + 16 * nt + c];
-#pragma unroll
-              for (int y = 0; y < KT; ++y) {
-                const bf16x8 ka = F8 ? e4m3x8(kr[y][x][2 * e], kr[y][x][2 * e + 1])
-                                     : __builtin_bit_cast(bf16x8, kr[y][x]);
-                v[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, __builtin_bit_cast(bf16x8, qv),
-                                                               v[y], 0, 0, 0);
-              }
-            }
-          if (F8) {
-            if (nt == 0) {                   // the wave's own words: no barrier
-              s_scale[l] = ks;
-              s_scale[64 + l] = vs;
-              asm volatile("" ::: "memory");
-            }
-#pragma unroll
-            for (int y = 0; y < KT; ++y) v[y] *= *(const CX_LDS f32x4*)(s_scale + 16 * g + 4 * y);
-          }
-          if (nt == NT - 1 && more_units) {  // K is used up: the next unit's
-            const int k = (i + 1) % BATCH;
-            if (k == 0) {
-              ids = idn;
-              idn = load_ids(i + 1 + BATCH);
-            }
-            load_k(ids, k, unit + ATT_WAVES);
-          }
-#pragma unroll
-          for (int y = 0; y < KT; ++y) v[y] *= A.s1;
-          if (A.cap) {                       // tanh(z) = 1 - 2 / (exp(2 z) + 1)
-#pragma unroll
-            for (int y = 0; y < KT; ++y)
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                v[y][j] = fmaf(-2.f * A.s2,
-                               __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v[y][j]) + 1.f), A.s2);
-          }
-          // a row's running maximum is at least ATT_LOW once it has attended to
-          // a token, whatever its score: -inf says that it has not
-          float top = ATT_LOW;
-          if (masked) {
-            top = -INFINITY;
-#pragma unroll
-            for (int y = 0; y < KT; ++y)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int t = tl + 4 * y + j;
-                const bool in = held && t <= pos[nt] && t < s.lim &&
-                                !(A.window && t <= pos[nt] - A.window);
-                v[y][j] = in ? v[y][j] : -INFINITY;
-                top = in ? ATT_LOW : top;
-              }
-          }
-#pragma unroll
-          for (int y = 0; y < KT; ++y)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(top, v[y][j]);
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const float m1 = fmaxf(m[nt], top);
-          const float base = m1 == -INFINITY ? 0.f : m1;
-          const float alpha = __builtin_amdgcn_exp2f(m[nt] - base);
-          m[nt] = m1;
-          float add = 0;
-#pragma unroll
-          for (int k = 0; k < KH; ++k) {
-            float term[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int y = 2 * k + e / 4, j = e % 4;
-              float p = __builtin_amdgcn_exp2f(v[y][j] - base);
-              add += p;
-              if (F8) p = v[y][j] == -INFINITY ? 0.f : p * s_scale[64 + 16 * g + 4 * y + j];
-              term[e] = p;
-            }
-            // the terms as two bf16 parts each, 16 bits of them.  The first is
-            // cut off and the second kept above 0, so an infinite value keeps
-            // its sign in both products
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              const uint32_t x0 = __float_as_uint(term[2 * d]), x1 = __float_as_uint(term[2 * d + 1]);
-              ph[nt][k][d] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
-              pl[nt][k][d] = pack_bf16(
-                  fmaxf(term[2 * d] - __uint_as_float(x0 & 0xFFFF0000u), term[2 * d] * 0x1p-24f),
-                  fmaxf(term[2 * d + 1] - __uint_as_float(x1 & 0xFFFF0000u),
-                        term[2 * d + 1] * 0x1p-24f));
-            }
-          }
-          sum[nt] = fmaf(sum[nt], alpha, add);
-          if (__any(alpha != 1.f)) {
-#pragma unroll
-            for (int n = 0; n < DT; ++n) acc[nt][n] *= alpha;
+          for (int j = 0; j < 4; ++j) {
+            const int t = ty + 4 * g + j;
+            v[nt][y][j] = in && t <= hi[nt] && t > lo[nt] ? v[nt][y][j] : -INFINITY;
           }
         }
-        // V's tokens from after lo through hi that are held, as a mask of each of
-        // the lane's dwords: the others count as zeros, whatever is there (a
-        // product with a zero term would not)
-        uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-        auto keep_bits = [&](int lo, int hi) {
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            keep[d] = 0;
-#pragma unroll
-            for (int e = 0; e < E / 4; ++e) {
-              const int t = tl + E / 4 * d + e;
-              keep[d] |= held && t < s.lim && t <= hi && t > lo
-                             ? (F8 ? 0xFFu << 8 * e : 0xFFFFu << 16 * e) : 0;
-            }
-          }
-        };
-        // NaN or infinity that only some rows may attend to: one position's rows
-        // after the other, each with its own tokens of V
-        bool fix = false;
-        if (masked) {
-          keep_bits(A.window ? pmin - A.window : -1, pmax);
-          bool bad = false;
-#pragma unroll
-          for (int n = 0; n < DT; ++n)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              const uint32_t x = vr[n][d] & keep[d];
-              if (F8) bad |= (((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
-              else bad |= (x & 0x7F80u) == 0x7F80u || (x & 0x7F800000u) == 0x7F800000u;
-            }
-          fix = pmin != pmax && __any(bad);
-        }
-        int q = fix ? pmin : pmax;
-        do {
-          if (fix) keep_bits(A.window ? q - A.window : -1, q);
-#pragma unroll
-          for (int n = 0; n < DT; ++n)
-#pragma unroll
-            for (int k = 0; k < KH; ++k) {
-              u32x4 x = vr[n];
-#pragma unroll
-              for (int d = 0; d < 4; ++d) x[d] &= keep[d];
-              const bf16x8 va = F8 ? e4m3x8(x[2 * k], x[2 * k + 1]) : __builtin_bit_cast(bf16x8, x);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    va, __builtin_bit_cast(bf16x8, ph[nt][k]), acc[nt][n], 0, 0, 0);
-                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pl[nt][k]), o,
-                                                            0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  acc[nt][n][j] = !fix || pos[nt] == q ? o[j] : acc[nt][n][j];
-              }
-            }
-        } while (++q <= pmax);
-        if (more_units) load_v(unit + ATT_WAVES);
+        top[nt] = some ? ATT_LOW : -INFINITY;
       }
-
-      // the waves' parts added in their order
+    }
+    float alpha[NT];
+    bool moved = false;
+    u32x4 ph[NT][KH], pl[NT][KH];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        sum[nt] += __shfl_xor(sum[nt], 16);
-        sum[nt] += __shfl_xor(sum[nt], 32);
-        if (g == 0) {
-          s_ml[2 * (w * ROWS + 16 * nt + c)] = m[nt];
-          s_ml[2 * (w * ROWS + 16 * nt + c) + 1] = sum[nt];
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int y = 0; y < KT; ++y)
+        top[nt] = fmaxf(top[nt], fmaxf(fmaxf(v[nt][y][0], v[nt][y][1]), fmaxf(v[nt][y][2], v[nt][y][3])));
+      const float m1 = fmaxf(m[nt], groups_max(top[nt]));
+      const float base = m1 == -INFINITY ? 0.f : m1;
+      alpha[nt] = __builtin_amdgcn_exp2f(m[nt] - base);
+      moved |= alpha[nt] != 1.f;
+      m[nt] = m1;
+      uint32_t th[KT][2], tl[KT][2];
+      float add = 0;
+#pragma unroll
+      for (int y = 0; y < KT; ++y) {
+        f32x4 p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(v[nt][y][j] - base);
+        add += (p[0] + p[1]) + (p[2] + p[3]);
+        if (F8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = v[nt][y][j] == -INFINITY ? 0.f : p[j] * vscale[y][j];
+        }
+        // the terms as two bf16 parts each, 16 bits of them.  The first is cut
+        // off and the second kept above 0, so an infinite value keeps its sign
+        // in both products
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const float p0 = p[2 * d], p1 = p[2 * d + 1];
+          const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
+          th[y][d] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
+          tl[y][d] = pack_bf16(fmaxf(p0 - __uint_as_float(x0 & 0xFFFF0000u), p0 * 0x1p-24f),
+                               fmaxf(p1 - __uint_as_float(x1 & 0xFFFF0000u), p1 * 0x1p-24f));
+        }
+      }
+      sum[nt] = fmaf(sum[nt], alpha[nt], add);
+      // lane group G gets the terms of the tokens whose V it holds
+      regroup(th);
+      regroup(tl);
+#pragma unroll
+      for (int x = 0; x < KH; ++x) {
+        ph[nt][x] = u32x4{th[2 * x][0], th[2 * x][1], th[2 * x + 1][0], th[2 * x + 1][1]};
+        pl[nt][x] = u32x4{tl[2 * x][0], tl[2 * x][1], tl[2 * x + 1][0], tl[2 * x + 1][1]};
+      }
+    }
+    if (__any(moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int n = 0; n < DT; ++n) acc[nt][n] *= alpha[nt];
+    }
+    if (masked) {
+      // V of tokens that no row attends to counts as zeros, whatever is there
+      // (a product with a zero term would not)
+      const bool vheld = here >> vgroup & 1;
+      const int tv = t0 + (TOK / 4) * g;     // the first of this lane's tokens of V
+      const int from = A.window ? pmin - A.window : -1, to = min(pmax, cur.lim - 1);
+      uint32_t keep[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        keep[d] = 0;
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) {
+          const int t = tv + E / 4 * d + e;
+          keep[d] |= vheld && t > from && t <= to ? (F8 ? 0xFFu << 8 * e : 0xFFFFu << 16 * e) : 0;
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        __syncthreads();
+      for (int n = 0; n < DT; ++n)
+#pragma unroll
+        for (int d = 0; d < 4; ++d) vr[n][d] &= keep[d];
+      if (pmin != pmax) {
+        // nor may NaN or infinity reach the rows that do not attend to it: left
+        // out here, added row by row at the piece's end
+        bool bad = false;
 #pragma unroll
         for (int n = 0; n < DT; ++n)
-          *(CX_LDS f32x4*)(s_o + (w * 16 + c) * PAD + 16 * n + 4 * g) = acc[nt][n];
-        __syncthreads();
-        for (int i = tid; i < 16 * (D / 8); i += ATT_WG) {
-          const int r = i / (D / 8), d = 8 * (i % (D / 8)), rr = 16 * nt + r;
-          if (rr >= R) continue;
-          float top = -INFINITY, L = 0;
 #pragma unroll
-          for (int k = 0; k < ATT_WAVES; ++k) top = fmaxf(top, s_ml[2 * (k * ROWS + rr)]);
-          const float base = top == -INFINITY ? 0.f : top;
-          f32x4 o0 = {0, 0, 0, 0}, o1 = {0, 0, 0, 0};
-#pragma unroll
-          for (int k = 0; k < ATT_WAVES; ++k) {
-            const float f = __builtin_amdgcn_exp2f(s_ml[2 * (k * ROWS + rr)] - base);
-            L = fmaf(f, s_ml[2 * (k * ROWS + rr) + 1], L);
-            const CX_LDS float* o = s_o + (k * 16 + r) * PAD + d;
-            o0 += f * *(const CX_LDS f32x4*)o;
-            o1 += f * *(const CX_LDS f32x4*)(o + 4);
+          for (int d = 0; d < 4; ++d) {
+            const uint32_t x = nonfinite<F8>(vr[n][d]);
+            bad |= x != 0;
+            vr[n][d] &= ~x;
           }
-          if (whole) {
-            const float f = top == -INFINITY ? 0.f : 1.f / L;
-            const u32x4 x = {pack_bf16(o0[0] * f, o0[1] * f), pack_bf16(o0[2] * f, o0[3] * f),
-                             pack_bf16(o1[0] * f, o1[1] * f), pack_bf16(o1[2] * f, o1[3] * f)};
-            *(u32x4*)(A.out + ((int64_t)(s.tok0 + (r0 + rr) / A.G) * A.q_heads + h * A.G +
-                               (r0 + rr) % A.G) * D + d) = x;
-          } else {
-            float* o = A.part + ((int64_t)slot * ROWS + rr) * D + d;
-            *(f32x4*)o = o0;
-            *(f32x4*)(o + 4) = o1;
-            if (d == 0) {
-              A.ml[2 * (slot * ROWS + rr)] = top;
-              A.ml[2 * (slot * ROWS + rr) + 1] = L;
+        again |= __any(bad);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < DT; ++n)
+#pragma unroll
+      for (int x = 0; x < KH; ++x) {
+        const bf16x8 va = F8 ? e4m3x8(vr[n][2 * x], vr[n][2 * x + 1])
+                             : __builtin_bit_cast(bf16x8, vr[n]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              va, __builtin_bit_cast(bf16x8, ph[nt][x]), acc[nt][n], 0, 0, 0);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              va, __builtin_bit_cast(bf16x8, pl[nt][x]), acc[nt][n], 0, 0, 0);
+      }
+    load_v();
+    if (!turn) {
+      ++i;
+      continue;
+    }
+
+    // the piece ends
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (again) {
+        // each row's own NaN and infinite values (their terms' size does not
+        // matter), token by token
+#pragma unroll
+        for (int n = 0; n < DT; ++n)
+          *(CX_LDS f32x4*)(s_o + c * PAD + 16 * n + 4 * g) = acc[nt][n];
+        asm volatile("" ::: "memory");
+        for (int t = cur.unit * TOK; t < (cur.unit + cur.cnt) * TOK && t < cur.lim; ++t) {
+          const int id = C.table[cur.b * C.ld_table + (t >> C.logP)], o = t & (P - 1);
+          if ((unsigned)id >= (unsigned)C.n_pages) continue;
+          for (int d = l; d < D; d += 64) {
+            const char* p = C.pages + id * C.page_stride + (int64_t)cur.h * C.head_bytes +
+                            v_chunk<E, D>(d, o, C.logP) + o % E * (16 / E);
+            const float x = F8 ? e4m3_value(*(const uint8_t*)p) : bf16_lo(*(const uint16_t*)p);
+            if (fabsf(x) < INFINITY) continue;
+            for (int r = 0; r < 16; ++r) {
+              const int at = cur.lowest + (cur.r0 + min(16 * nt + r, cur.R - 1)) / A.G;
+              if (t <= at && !(A.window && t <= at - A.window)) s_o[r * PAD + d] += x;
             }
+          }
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int n = 0; n < DT; ++n)
+          acc[nt][n] = *(const CX_LDS f32x4*)(s_o + c * PAD + 16 * n + 4 * g);
+      }
+      const int r = 16 * nt + c;
+      const float L = groups_sum(sum[nt]);
+      if (r < cur.R) {
+        if (cur.slot < 0) {
+          const float f = m[nt] == -INFINITY ? 0.f : 1.f / L;
+          const int row = cur.r0 + r;
+          uint16_t* o = A.out + ((int64_t)(cur.tok0 + row / A.G) * A.q_heads + cur.h * A.G +
+                                 row % A.G) * D + 4 * g;
+#pragma unroll
+          for (int n = 0; n < DT; ++n)
+            *(u32x2*)(o + 16 * n) = u32x2{pack_bf16(acc[nt][n][0] * f, acc[nt][n][1] * f),
+                                          pack_bf16(acc[nt][n][2] * f, acc[nt][n][3] * f)};
+        } else {
+          float* o = A.part + ((int64_t)cur.slot * ROWS + r) * D + 4 * g;
+#pragma unroll
+          for (int n = 0; n < DT; ++n) *(f32x4*)(o + 16 * n) = acc[nt][n];
+          if (g == 0) {
+            A.ml[2 * ((int64_t)cur.slot * ROWS + r)] = m[nt];
+            A.ml[2 * ((int64_t)cur.slot * ROWS + r) + 1] = L;
           }
         }
       }
     }
+    if (last) break;
+    cur = nxt;
+    u += cur.cnt;
+    last = u >= end;
+    idn = load_ids(cur, BATCH);
+    if (!last) nxt = piece();
+    idq = load_ids(nxt, 0);
+    begin(cur);
+    i = 0;
   }
-  if (!joined && tid == 0) A.join[blockIdx.x].last = -1;
+  if (!joined && l == 0) A.join[worker].last = -1;
 }
 
 // A row block's parts joined, in the order of its tokens: 256 threads over
@@ -581,19 +700,21 @@ __global__ __launch_bounds__(256) void attend_join(AttendArgs A) {
   }
 }
 
-// The rows of a sequence that share a kv head, at most: the tile of 16, 32 or
-// 64, as far as their sums fit the registers.
+// The tile, in 16 rows, for at most that many rows of a sequence that share a kv
+// head: as few row blocks as the registers allow, of one size.
 static int row_tiles(int64_t rows, int D, int dtype) {
-  if (rows <= 16 || (D == 256 && dtype == CX_KV_E4M3)) return 1;
-  return rows <= 32 || D == 256 || dtype == CX_KV_E4M3 ? 2 : 4;
+  const int most = D == 256 ? 1 : dtype == CX_KV_E4M3 ? 2 : D == 128 ? 3 : 4;
+  const int64_t tiles = (rows + 15) / 16, blocks = (tiles + most - 1) / most;
+  return (int)((tiles + blocks - 1) / blocks);
 }
-static int workgroups(int nt) { return nt == 1 ? 512 : 256; }
+// Workers: as many waves as the chip holds of the tile's kernel.
+static int workgroups(int nt, int D) { return nt == 1 && D < 256 ? 512 : 256; }
 
 struct AttendWork {
   size_t off_ml, off_part, total;
 };
 static AttendWork attend_workspace(int nt, int D) {
-  const size_t W = workgroups(nt), rows = 16 * (size_t)nt;
+  const size_t W = ATT_WAVES * (size_t)workgroups(nt, D), rows = 16 * (size_t)nt;
   AttendWork x;
   x.off_ml = align_up(W * sizeof(AttendJoin), 256);
   x.off_part = x.off_ml + align_up(2 * W * rows * 8, 256);
@@ -611,10 +732,11 @@ static int launch_tile(const AttendArgs& A, hipStream_t s) {
                               hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(CX_KV_MAX_BATCH));
   });
   if (err != hipSuccess) return (int)err;
-  const dim3 grid((unsigned)workgroups(NT));
-  timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8>, grid, dim3(ATT_WG),
+  const unsigned grid = (unsigned)workgroups(NT, D);
+  timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8>, dim3(grid), dim3(ATT_WG),
                (uint32_t)Sh::lds(A.kv.B), s, A);
-  timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join<D, 16 * NT>, grid, dim3(256), 0, s, A);
+  timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join<D, 16 * NT>, dim3(grid * ATT_WAVES), dim3(256),
+               0, s, A);
   return (int)hipGetLastError();
 }
 
@@ -623,10 +745,11 @@ static int launch_attend(const AttendArgs& A, int dtype, int nt, hipStream_t s) 
   const bool f8 = dtype == CX_KV_E4M3;
   if (nt == 1) return f8 ? launch_tile<D, 1, true>(A, s) : launch_tile<D, 1, false>(A, s);
   if constexpr (D < 256) {
-    if (nt == 4) return launch_tile<D, 4, false>(A, s);
-    if (f8) return launch_tile<D, 2, true>(A, s);
+    if (nt == 2) return f8 ? launch_tile<D, 2, true>(A, s) : launch_tile<D, 2, false>(A, s);
+    if (nt == 3 && !f8) return launch_tile<D, 3, false>(A, s);
   }
-  if (nt == 2 && !f8) return launch_tile<D, 2, false>(A, s);
+  if constexpr (D == 64)
+    if (nt == 4 && !f8) return launch_tile<D, 4, false>(A, s);
   return (int)hipErrorInvalidValue;
 }
 
