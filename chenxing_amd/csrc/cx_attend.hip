@@ -642,62 +642,90 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   if (!joined && l == 0) A.join[worker].last = -1;
 }
 
-// A row block's parts joined, in the order of its tokens: 256 threads over
-// (part group, row, 8 dims).
+// A row block's parts joined, in the order of its tokens: workgroup (worker, 16
+// rows).  A wave takes every fourth row, or every fourth group of rows: D / 8
+// lanes a row, the wave's other lane groups on other rows, or on other parts of
+// the row where there are many (their order of adding is fixed all the same).
+// Latency: a round of loads from the other XCDs' parts takes about a microsecond,
+// so 4 parts a lane are requested together, 8 where there are many.
 template <int D, int ROWS>
 __global__ __launch_bounds__(256) void attend_join(AttendArgs A) {
-  __shared__ float s_m[ROWS], s_l[ROWS];
-  __shared__ f32x4 s_acc[256][2];
+  constexpr int LANES = D / 8, GROUPS = 64 / LANES;
   const AttendJoin J = const_load(A.join + blockIdx.x);
   if (J.last < 0) return;
-  const int n = J.last - J.first + 1, tid = threadIdx.x, w = wave_id(), l = lane_id();
-  auto slot = [&](int p) { return 2 * (J.first + p) + (p == 0); };
-  for (int r = w; r < J.rows; r += 4) {
-    float top = -INFINITY, L = 0;
-    for (int p = l; p < n; p += 64) {
-      const float* x = A.ml + 2 * (slot(p) * ROWS + r);
-      const float m1 = fmaxf(top, x[0]), base = m1 == -INFINITY ? 0.f : m1;
-      L = L * __builtin_amdgcn_exp2f(top - base) + x[1] * __builtin_amdgcn_exp2f(x[0] - base);
-      top = m1;
-    }
-    const float all = wave_max(top), base = all == -INFINITY ? 0.f : all;
-    L = wave_sum(L * __builtin_amdgcn_exp2f(top - base));
-    if (l == 0) { s_m[r] = all; s_l[r] = L; }
-  }
-  __syncthreads();
-  const int items = J.rows * (D / 8);
-  int lg = 0;                                // items of a pass: the power of two above, to 256
-  while ((1 << lg) < items && lg < 8) ++lg;
-  const int groups = 256 >> lg, grp = tid >> lg;
-  for (int i0 = 0; i0 < items; i0 += 1 << lg) {
-    const int i = i0 + (tid & ((1 << lg) - 1));
-    const int r = min(i, items - 1) / (D / 8), d = 8 * (i % (D / 8));
-    const float top = s_m[r], base = top == -INFINITY ? 0.f : top;
-    f32x4 o0 = {0, 0, 0, 0}, o1 = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int p = grp; p < n; p += groups) {
-      const float f = __builtin_amdgcn_exp2f(A.ml[2 * (slot(p) * ROWS + r)] - base);
-      const float* x = A.part + ((int64_t)slot(p) * ROWS + r) * D + d;
-      o0 += f * *(const f32x4*)x;
-      o1 += f * *(const f32x4*)(x + 4);
-    }
-    __syncthreads();
-    s_acc[tid][0] = o0;
-    s_acc[tid][1] = o1;
-    __syncthreads();
-    if (grp == 0 && i < items) {
-      for (int k = 1; k < groups; ++k) {
-        o0 += s_acc[tid + (k << lg)][0];
-        o1 += s_acc[tid + (k << lg)][1];
+  const int n = J.last - J.first + 1, w = wave_id(), l = lane_id();
+  const int grp = l / LANES, d = 8 * (l % LANES);
+  const int end = min(J.rows, 16 * (int)blockIdx.y + 16);
+  auto join = [&](auto wide_) {
+    constexpr bool wide = decltype(wide_)::value;
+    constexpr int JOIN_AHEAD = wide ? 8 : 4;
+    constexpr int step = wide ? GROUPS : 1, rows = wide ? 1 : GROUPS;
+    for (int r0 = 16 * blockIdx.y + w * rows; r0 < end; r0 += 4 * rows) {
+      const int r = wide ? r0 : min(r0 + grp, end - 1);
+      float top = -INFINITY, L = 0;
+      f32x4 o0 = {0, 0, 0, 0}, o1 = {0, 0, 0, 0};
+      for (int p0 = wide ? grp : 0; p0 < n; p0 += JOIN_AHEAD * step) {
+        float m[JOIN_AHEAD], s[JOIN_AHEAD];
+        f32x4 x0[JOIN_AHEAD], x1[JOIN_AHEAD];
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k) { // past the last: the last again, with weight 0
+          const int p = p0 + k * step, q = min(p, n - 1);
+          const int64_t at = (int64_t)(2 * (J.first + q) + (q == 0)) * ROWS + r;
+          const float2 ml = *(const float2*)(A.ml + 2 * at);
+          m[k] = p < n ? ml.x : -INFINITY;
+          s[k] = p < n ? ml.y : 0.f;
+          x0[k] = *(const f32x4*)(A.part + at * D + d);
+          x1[k] = *(const f32x4*)(A.part + at * D + d + 4);
+        }
+        float t = top;
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k) t = fmaxf(t, m[k]);
+        const float base = t == -INFINITY ? 0.f : t;
+        const float f0 = __builtin_amdgcn_exp2f(top - base);
+        L *= f0;
+        o0 *= f0;
+        o1 *= f0;
+        top = t;
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k) {
+          // a part without a token has no sums to add (its place may hold anything
+          // where the last part stands in for one past it)
+          if (p0 + k * step >= n) continue;
+          const float f = __builtin_amdgcn_exp2f(m[k] - base);
+          L = fmaf(f, s[k], L);
+          o0 += f * x0[k];
+          o1 += f * x1[k];
+        }
       }
-      const float f = top == -INFINITY ? 0.f : 1.f / s_l[r];
-      const u32x4 x = {pack_bf16(o0[0] * f, o0[1] * f), pack_bf16(o0[2] * f, o0[3] * f),
-                       pack_bf16(o1[0] * f, o1[1] * f), pack_bf16(o1[2] * f, o1[3] * f)};
-      const int row = J.row0 + r;
-      *(u32x4*)(A.out + ((int64_t)(J.tok0 + row / A.G) * A.q_heads + J.head * A.G + row % A.G) * D +
-                d) = x;
+      if (wide) {
+#pragma unroll
+        for (int x = LANES; x < 64; x <<= 1) {
+          const float t = __shfl_xor(top, x), all = fmaxf(top, t);
+          const float base = all == -INFINITY ? 0.f : all;
+          const float fa = __builtin_amdgcn_exp2f(top - base), fb = __builtin_amdgcn_exp2f(t - base);
+          const bool low = (l & x) == 0;       // both add in one order: the lower group's first
+          auto add = [&](float v) {
+            const float u = __shfl_xor(v, x);
+            return low ? fmaf(fa, v, fb * u) : fmaf(fb, u, fa * v);
+          };
+          L = add(L);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { o0[k] = add(o0[k]); o1[k] = add(o1[k]); }
+          top = all;
+        }
+      }
+      if (wide ? grp == 0 : r0 + grp < end) {
+        const float f = top == -INFINITY ? 0.f : 1.f / L;
+        const u32x4 x = {pack_bf16(o0[0] * f, o0[1] * f), pack_bf16(o0[2] * f, o0[3] * f),
+                         pack_bf16(o1[0] * f, o1[1] * f), pack_bf16(o1[2] * f, o1[3] * f)};
+        const int row = J.row0 + r;
+        *(u32x4*)(A.out + ((int64_t)(J.tok0 + row / A.G) * A.q_heads + J.head * A.G + row % A.G) * D +
+                  d) = x;
+      }
     }
-  }
+  };
+  if (n > 8) join(std::true_type());
+  else join(std::false_type());
 }
 
 // The tile, in 16 rows, for at most that many rows of a sequence that share a kv
@@ -735,8 +763,8 @@ static int launch_tile(const AttendArgs& A, hipStream_t s) {
   const unsigned grid = (unsigned)workgroups(NT, D);
   timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8>, dim3(grid), dim3(ATT_WG),
                (uint32_t)Sh::lds(A.kv.B), s, A);
-  timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join<D, 16 * NT>, dim3(grid * ATT_WAVES), dim3(256),
-               0, s, A);
+  timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join<D, 16 * NT>, dim3(grid * ATT_WAVES, NT),
+               dim3(256), 0, s, A);
   return (int)hipGetLastError();
 }
 
