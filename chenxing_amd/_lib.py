@@ -6,8 +6,8 @@ that already live on the GPU and run on the current torch stream.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 import os
 import struct
 import threading
@@ -254,12 +254,16 @@ def _stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def _on(device):
-    """The tensor's device as the current one, where it is not."""
-    import torch
+def _call(torch, device, fn, *args):
+    """fn(*args, the device's current stream), with that device the current one."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc != CX_OK:
+        _check(rc)
 
 
 def sample_device(logits, prm, u, hist=None, hist_len=None, out_id=None, row_status=None,
@@ -387,50 +391,64 @@ _KV_BATCH = struct.Struct("<QqQqQQ8i")
 KV_BF16, KV_E4M3 = 1, 3
 
 
-def _kv_batch(cache, D, table, kv_len, q_start, T):
-    """(packed cx_kv_batch, page tokens, bf16 pages) of one layer's pages and a batch."""
-    import torch
-    if cache.dim() != 3 or cache.stride(2) != 1 or cache.stride(1) != cache.shape[2]:
+def _kv_batch(torch, cache, D, table, kv_len, q_start, T):
+    """cx_kv_batch of one layer's pages and a batch."""
+    n, heads, width = cache.shape if cache.dim() == 3 else (0, 0, 0)
+    stride = cache.stride()
+    if not heads or stride[2] != 1 or (stride[1] != width and heads > 1):
         raise ValueError("cache must be one layer's [n_pages, kv_heads, width] pages, each page "
                          "contiguous")
-    n, heads, width = cache.shape
-    bf16 = cache.dtype == torch.bfloat16
-    if not bf16 and cache.dtype != torch.uint8:
+    if cache.dtype == torch.bfloat16:          # 2 P D elements
+        dtype, (P, rest), page = KV_BF16, divmod(width, 2 * D), 2 * stride[0]
+    elif cache.dtype == torch.uint8:           # 2 P D codes and 8 P bytes of scales
+        dtype, (P, rest), page = KV_E4M3, divmod(width, 2 * D + 8), stride[0]
+    else:
         raise ValueError("cache must be bfloat16 pages, or uint8 pages of e4m3 codes and scales")
-    # bf16: 2 P D elements; e4m3: 2 P D codes and 8 P bytes of scales
-    P, rest = divmod(width, 2 * D if bf16 else 2 * D + 8)
     if rest:
         raise ValueError(f"a page's width ({width}) does not fit heads of {D}")
-    if table.dim() != 2 or table.stride(1) != 1 or kv_len.dim() != 1 or \
-            not kv_len.is_contiguous() or table.dtype != torch.int32 or \
-            kv_len.dtype != torch.int32:
-        raise ValueError("table [B, pages] and kv_len [B] must be int32 with unit strides")
+    i32 = torch.int32
+    if table.dim() != 2 or table.dtype != i32 or kv_len.dtype != i32:
+        raise ValueError("table [B, pages] and kv_len [B] must be int32")
     B, M = table.shape
-    if kv_len.shape[0] != B:
+    if kv_len.shape != (B,):
         raise ValueError("table and kv_len differ in B")
-    st = 0
+    ld, unit = table.stride()
+    if (unit != 1 and M > 1) or not kv_len.is_contiguous():
+        raise ValueError("table and kv_len must have unit strides")
+    start = 0
     if q_start is not None:
-        if q_start.dtype != torch.int32 or tuple(q_start.shape) != (B + 1,) or \
-                not q_start.is_contiguous():
-            raise ValueError("q_start must be a contiguous int32 [B + 1]")
-        st = q_start.data_ptr()
+        if q_start.dtype != i32 or q_start.shape != (B + 1,) or not q_start.is_contiguous() or \
+                not q_start.is_cuda:
+            raise ValueError("q_start must be a contiguous int32 [B + 1] cuda tensor")
+        start = q_start.data_ptr()
     elif T != B:
         raise ValueError("without q_start there is one new token per sequence")
-    for t in (cache, table, kv_len):
-        if not t.is_cuda:
-            raise ValueError("cache, table and kv_len must be cuda tensors")
-    return (_KV_BATCH.pack(cache.data_ptr(), cache.stride(0) * (2 if bf16 else 1),
-                           table.data_ptr(), table.stride(0), kv_len.data_ptr(), st, n, heads, D,
-                           P, KV_BF16 if bf16 else KV_E4M3, B, M, T), P, bf16)
+    if not (cache.is_cuda and table.is_cuda and kv_len.is_cuda):
+        raise ValueError("cache, table and kv_len must be cuda tensors")
+    return _KV_BATCH.pack(cache.data_ptr(), page, table.data_ptr(), max(ld, M), kv_len.data_ptr(),
+                          start, n, heads, D, P, dtype, B, M, T)
 
 
-def _rows3(name, t):
-    """[tokens, heads, D] bf16 rows on the GPU."""
-    import torch
-    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.stride(2) != 1 or not t.is_cuda:
-        raise ValueError(f"{name} must be a bfloat16 [tokens, heads, D] cuda tensor with unit "
-                         "element stride")
-    return t.shape
+def _rows3(torch, name, t, shape=None):
+    """The strides of bf16 rows [tokens, heads, D] on the GPU."""
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or not t.is_cuda or \
+            (shape is not None and t.shape != shape):
+        raise ValueError(f"{name} must be a bfloat16 "
+                         f"{list(shape) if shape is not None else '[tokens, heads, D]'} cuda "
+                         "tensor")
+    st = t.stride()
+    if st[2] != 1:
+        raise ValueError(f"{name} must have unit element stride")
+    return st
+
+
+def _out3(torch, name, t, shape, device):
+    if t is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    _rows3(torch, name, t, shape)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t
 
 
 def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, interleaved=False,
@@ -440,42 +458,42 @@ def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, int
     q [T, Hq, D], k and v [T, Hkv, D] (bfloat16, any token and head strides that
     keep rows 16-byte aligned): q and k normed per head (``q_norm`` / ``k_norm``
     [D] bfloat16 weights, or None), their first dims rotated to the tokens'
-    positions (``rope`` [positions, rotary dim] float32, ``kvcache.rope_table``;
-    None: not at all), k and v written into ``cache``, one layer's pages.
+    positions (``rope`` [positions, rotary dim] float32: the cosines, then the
+    sines; None: not at all), k and v written into ``cache``, one layer's pages.
     ``table`` [B, pages], ``kv_len`` [B] (the new tokens included) and
     ``q_start`` [B + 1] (None: one new token each) are int32.  Returns q_out
     [T, Hq, D]."""
     import torch
-    lib = load()
-    T, Hq, D = _rows3("q", q)
-    kv, P, _ = _kv_batch(cache, D, table, kv_len, q_start, T)
-    heads = cache.shape[1]
-    if _rows3("k", k) != (T, heads, D) or _rows3("v", v) != (T, heads, D):
-        raise ValueError("k and v must be [T, kv_heads, D]")
-    rows = rdim = 0
+    lib = _lib or load()
+    qs = _rows3(torch, "q", q)
+    T, Hq, D = q.shape
+    kv = _kv_batch(torch, cache, D, table, kv_len, q_start, T)
+    shape = (T, cache.shape[1], D)
+    ks, vs = _rows3(torch, "k", k, shape), _rows3(torch, "v", v, shape)
+    rp, rows, rdim = None, 0, 0
     if rope is not None:
         if rope.dim() != 2 or rope.dtype != torch.float32 or not rope.is_contiguous() or \
                 not rope.is_cuda:
             raise ValueError("rope must be a contiguous float32 [positions, rotary dim] cuda "
                              "tensor")
+        rp = rope.data_ptr()
         rows, rdim = rope.shape
+    norms = []
     for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None and (w.dtype != torch.bfloat16 or tuple(w.shape) != (D,) or
+        if w is not None and (w.dtype != torch.bfloat16 or w.shape != (D,) or
                               not w.is_contiguous() or not w.is_cuda):
             raise ValueError(f"{name} must be a contiguous bfloat16 [D] cuda tensor")
-    if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
-    elif _rows3("q_out", q_out) != (T, Hq, D) or not q_out.is_contiguous():
-        raise ValueError("q_out must be a contiguous [T, q_heads, D]")
-    with _on(q.device):
-        _check(lib.cx_kv_append_bf16(
-            kv, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), Hq,
-            rope.data_ptr() if rope is not None else None, rows, rdim, interleaved,
-            q_norm.data_ptr() if q_norm is not None else None,
-            k_norm.data_ptr() if k_norm is not None else None, eps, q_out.data_ptr(),
-            _stream_ptr(q.device)))
+        norms.append(None if w is None else w.data_ptr())
+    q_out = _out3(torch, "q_out", q_out, (T, Hq, D), q.device)
+    _call(torch, q.device, lib.cx_kv_append_bf16, kv, q.data_ptr(), qs[0], qs[1], k.data_ptr(),
+          ks[0], ks[1], v.data_ptr(), vs[0], vs[1], Hq, rp, rows, rdim, interleaved, *norms, eps,
+          q_out.data_ptr())
     return q_out
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(q_heads, kv_heads, D, max_new):
+    return load().cx_paged_attention_workspace_bytes(q_heads, kv_heads, D, max_new)
 
 
 def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, scale=None, window=0,
@@ -491,22 +509,17 @@ def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, sca
     Returns out [T, Hq, D] bfloat16; a token that attends to nothing gets
     zeros."""
     import torch
-    lib = load()
-    T, Hq, D = _rows3("q", q)
-    kv, _, _ = _kv_batch(cache, D, table, kv_len, q_start, T)
+    lib = _lib or load()
+    qs = _rows3(torch, "q", q)
+    T, Hq, D = q.shape
+    kv = _kv_batch(torch, cache, D, table, kv_len, q_start, T)
     dev = q.device
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
-    elif _rows3("out", out) != (T, Hq, D) or not out.is_contiguous():
-        raise ValueError("out must be a contiguous [T, q_heads, D]")
-    sp = _stream_ptr(dev)
-    ws = _ws_attend.get(lib.cx_paged_attention_workspace_bytes(Hq, cache.shape[1], D, max_new),
-                        dev, sp.value)
-    with _on(dev):
-        _check(lib.cx_paged_attention_bf16(
-            kv, q.data_ptr(), q.stride(0), q.stride(1), Hq, max_new,
-            D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(),
-            ws.data_ptr(), ws.numel(), sp))
+    out = _out3(torch, "out", out, (T, Hq, D), dev)
+    ws = _ws_attend.get(_attention_workspace(Hq, cache.shape[1], D, max_new), dev,
+                        torch._C._cuda_getCurrentRawStream(dev.index))
+    _call(torch, dev, lib.cx_paged_attention_bf16, kv, q.data_ptr(), qs[0], qs[1], Hq, max_new,
+          D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(), ws.data_ptr(),
+          ws.numel())
     return out
 
 
@@ -516,24 +529,24 @@ def kv_copy_pages_device(cache, src, dst):
     [n_pages, kv_heads, width]; src and dst are int32 [n].  No page may be the
     destination of two pairs, or a destination and a source.  Returns cache."""
     import torch
-    lib = load()
-    if cache.dim() not in (3, 4) or cache.stride(-1) != 1 or cache.stride(-2) != cache.shape[-1]:
+    lib = _lib or load()
+    dims, st, shape = cache.dim(), cache.stride(), cache.shape
+    if dims not in (3, 4) or st[-1] != 1 or (st[-2] != shape[-1] and shape[-2] > 1):
         raise ValueError("cache must be [layers, n_pages, kv_heads, width] or one layer of it, "
                          "each page contiguous")
-    for t in (src, dst):
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or not t.is_cuda:
-            raise ValueError("src and dst must be contiguous int32 cuda tensors")
+    i32 = torch.int32
+    if src.dtype != i32 or dst.dtype != i32 or src.dim() != 1 or not src.is_contiguous() or \
+            not dst.is_contiguous() or not src.is_cuda or not dst.is_cuda:
+        raise ValueError("src and dst must be contiguous int32 [n] cuda tensors")
     if src.shape != dst.shape:
         raise ValueError("src and dst differ in length")
     if not cache.is_cuda:
         raise ValueError("cache must be a cuda tensor")
     el = cache.element_size()
-    layers, stride = (1, 0) if cache.dim() == 3 else (cache.shape[0], cache.stride(0) * el)
-    with _on(cache.device):
-        _check(lib.cx_kv_copy_pages(
-            cache.data_ptr(), stride, cache.stride(-3) * el,
-            cache.shape[-1] * cache.shape[-2] * el, layers, cache.shape[-3], src.data_ptr(),
-            dst.data_ptr(), src.shape[0], _stream_ptr(cache.device)))
+    layers, stride = (1, 0) if dims == 3 else (shape[0], st[0] * el)
+    _call(torch, cache.device, lib.cx_kv_copy_pages, cache.data_ptr(), stride, st[-3] * el,
+          shape[-1] * shape[-2] * el, layers, shape[-3], src.data_ptr(), dst.data_ptr(),
+          src.shape[0])
     return cache
 
 
