@@ -87,125 +87,315 @@ __device__ __forceinline__ int2 token_place(const KvArgs& A, int t) {
   return make_int2(b, (int)(A.kv_len[b] - (unsigned)n + (unsigned)i));
 }
 
-// One row (token, head) of q, k or v to D / 8 lanes, 8 dims each, every row of
-// the call at once: q heads first, then k, then v.  The mean square and, for
-// e4m3, the largest magnitude go over the row's lanes; the other dim of a
-// rotated pair is in the same lane (interleaved) or rdim / 16 lanes away.
+// A row's lane of 8 dims, d .., as floats.
+struct Row8 {
+  float x[8];
+};
+__device__ __forceinline__ Row8 widen(u32x4 in) {
+  Row8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { r.x[2 * i] = bf16_lo(in[i]); r.x[2 * i + 1] = bf16_hi(in[i]); }
+  return r;
+}
+
+// x * rsqrt(mean(x^2) + eps) * w over the row's D / 8 lanes.
+template <int D>
+__device__ __forceinline__ void norm_row(Row8& r, u32x4 w, float eps) {
+  float ss = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fmaf(r.x[i], r.x[i], ss);
+#pragma unroll
+  for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+  const float f = 1.f / sqrtf(ss * (1.f / D) + eps);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.x[2 * i] = r.x[2 * i] * f * bf16_lo(w[i]);
+    r.x[2 * i + 1] = r.x[2 * i + 1] * f * bf16_hi(w[i]);
+  }
+}
+
+// The cosines and sines of a lane's pairs at one position: of dims d, d + 2 ..
+// where the pair (2 j, 2 j + 1) is in the lane, of dims d .. d + 7 where it is
+// (j, j + rdim / 2), rdim / 16 lanes away.
+struct Turn8 {
+  f32x4 c[2], s[2];
+};
+__device__ __forceinline__ Turn8 load_turn(const AppendArgs& A, int pos, int d) {
+  Turn8 t = {};
+  if (!A.rope || d >= A.rdim) return t;
+  const int half = A.rdim / 2;
+  const float* p = A.rope + (int64_t)pos * A.rdim +
+                   (A.interleaved ? d / 2 : d < half ? d : d - half);
+  t.c[0] = *(const f32x4*)p;
+  t.s[0] = *(const f32x4*)(p + half);
+  if (!A.interleaved) {
+    t.c[1] = *(const f32x4*)(p + 4);
+    t.s[1] = *(const f32x4*)(p + half + 4);
+  }
+  return t;
+}
+__device__ __forceinline__ void turn_row(const AppendArgs& A, Row8& r, const Turn8& t, int d) {
+  if (!A.rope) return;
+  if (A.interleaved) {
+    if (d >= A.rdim) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = r.x[2 * i], b = r.x[2 * i + 1];
+      r.x[2 * i] = a * t.c[0][i] - b * t.s[0][i];
+      r.x[2 * i + 1] = b * t.c[0][i] + a * t.s[0][i];
+    }
+    return;
+  }
+  const int half = A.rdim / 2;
+  const bool low = d < half;
+  const int other = (threadIdx.x + (low ? half / 8 : -(half / 8))) & 63;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = __shfl(r.x[i], other), c = t.c[i / 4][i % 4], s = t.s[i / 4][i % 4];
+    if (d < A.rdim) r.x[i] = low ? r.x[i] * c - y * s : r.x[i] * c + y * s;
+  }
+}
+__device__ __forceinline__ u32x4 narrow(const Row8& r) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = pack_bf16(r.x[2 * i], r.x[2 * i + 1]);
+  return o;
+}
+
+// A lane's 8 e4m3 codes and the row's scale; the largest |x| by its bits: NaN
+// above inf above every number.
+template <int D>
+__device__ __forceinline__ u32x2 encode_row(const Row8& r, float* scale) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(r.x[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = D / 16; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+  const bool fine = m < 0x7F800000u;
+  float f = __uint_as_float(m) / E4M3_MAX;
+  if (f == 0.f) f = 1.f;                     // a row of zeros, or of values whose scale rounds to 0
+  *scale = fine ? f : __builtin_nanf("");
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = fine ? fminf(fmaxf(r.x[i] / f, -E4M3_MAX), E4M3_MAX) : 0.f;
+  u32x2 c;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
+    c[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], p, true);
+  }
+  return c;
+}
+
+// Where a new token goes: byte offset of its page (-1: nowhere) and its place
+// in the page.
+struct Slot {
+  int64_t page;
+  int o, pos;
+};
+__device__ __forceinline__ Slot token_slot(const KvArgs& C, int t) {
+  const int2 at = token_place(C, t);
+  Slot s = {-1, 0, 0};
+  if (at.x < 0 || at.y < 0 || at.y >= (C.M << C.logP)) return s;
+  s.pos = at.y;
+  s.o = at.y & ((1 << C.logP) - 1);
+  const int id = C.table[at.x * C.ld_table + (at.y >> C.logP)];
+  if ((unsigned)id < (unsigned)C.n_pages) s.page = id * C.page_stride;
+  return s;
+}
+
+// A lane's part of a key row, to its page.
+template <int D, bool F8>
+__device__ __forceinline__ void put_key(const KvArgs& C, const Row8& r, const Slot& s, int h, int d) {
+  char* base = C.pages + s.page + (int64_t)h * C.head_bytes;
+  if (F8) {
+    float scale;
+    const u32x2 c = encode_row<D>(r, &scale);
+    if (s.page < 0) return;
+    *(u32x2*)(base + k_chunk<16>(d, s.o, C.logP) + (d & 8)) = c;
+    if (d == 0) *(float*)(base + k_scale<D>(s.o, C.logP)) = scale;
+  } else if (s.page >= 0) {
+    *(u32x4*)(base + k_chunk<8>(d, s.o, C.logP)) = narrow(r);
+  }
+}
+
+// One row (token, head) of q, k or v to D / 8 lanes, every row of the call at
+// once: q heads first, then k, then v.  For few new tokens a sequence, whose rows
+// share no line of the pages.
 template <int D, bool F8>
 __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
   constexpr int LR = D / 8, E = F8 ? 16 : 8;
   const KvArgs& C = A.kv;
-  const int heads = A.q_heads + 2 * C.heads;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LR) + threadIdx.x / LR;
+  const unsigned heads = A.q_heads + 2 * C.heads;
+  const unsigned row = blockIdx.x * (256 / LR) + threadIdx.x / LR;
   const int t = (int)(row / heads), hh = (int)(row % heads);
   if (t >= C.T) return;
-  const int j = threadIdx.x % LR, d = 8 * j;
+  const int d = 8 * (threadIdx.x % LR);
   const int kind = hh < A.q_heads ? 0 : hh < A.q_heads + C.heads ? 1 : 2;
   const int h = kind == 0 ? hh : kind == 1 ? hh - A.q_heads : hh - A.q_heads - C.heads;
   const u32x4 in = *(const u32x4*)(A.x[kind] + t * A.st[kind] + h * A.sh[kind] + d);
-  const int2 place = token_place(C, t);
-  const int pos = place.y;
-  const bool held = place.x >= 0 && pos >= 0 && pos < (C.M << C.logP);
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { x[2 * i] = bf16_lo(in[i]); x[2 * i + 1] = bf16_hi(in[i]); }
   const uint16_t* w = kind < 2 ? A.norm[kind] : nullptr;
-  if (w) {
-    float ss = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int o = LR / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-    const float r = 1.f / sqrtf(ss * (1.f / D) + A.eps);
-    const u32x4 wv = *(const u32x4*)(w + d);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = x[2 * i] * r * bf16_lo(wv[i]);
-      x[2 * i + 1] = x[2 * i + 1] * r * bf16_hi(wv[i]);
-    }
-  }
-  if (kind < 2 && A.rope) {
-    const float* cs = A.rope + (int64_t)(held ? pos : 0) * A.rdim;
-    const int half = A.rdim / 2;
-    if (A.interleaved) {
-      if (d < A.rdim) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float c = cs[d / 2 + i], s = cs[half + d / 2 + i];
-          const float a = x[2 * i], b = x[2 * i + 1];
-          x[2 * i] = a * c - b * s;
-          x[2 * i + 1] = b * c + a * s;
-        }
-      }
-    } else {
-      const bool low = d < half;
-      const int other = threadIdx.x + (low ? half / 8 : -(half / 8));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = __shfl(x[i], other & 63);
-        if (d < A.rdim) {
-          const int p = low ? d + i : d - half + i;
-          const float c = cs[p], s = cs[half + p];
-          x[i] = low ? x[i] * c - y * s : x[i] * c + y * s;
-        }
-      }
-    }
+  u32x4 wv = {};
+  if (w) wv = *(const u32x4*)(w + d);
+  const Slot s = token_slot(C, t);
+  Row8 r = widen(in);
+  if (kind < 2) {
+    const Turn8 turn = load_turn(A, s.pos, d);
+    if (w) norm_row<D>(r, wv, A.eps);
+    turn_row(A, r, turn, d);
   }
   if (kind == 0) {
-    u32x4 o;
+    *(u32x4*)(A.q_out + ((int64_t)t * A.q_heads + h) * D + d) = narrow(r);
+  } else if (kind == 1) {
+    put_key<D, F8>(C, r, s, h, d);
+  } else {
+    char* base = C.pages + s.page + (int64_t)h * C.head_bytes;
+    char* p = base + v_chunk<E, D>(d, s.o, C.logP) + s.o % E * (16 / E);
+    if (F8) {
+      float scale;
+      const u32x2 c = encode_row<D>(r, &scale);
+      if (s.page < 0) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-    *(u32x4*)(A.q_out + ((int64_t)t * A.q_heads + h) * D + d) = o;
+      for (int i = 0; i < 8; ++i) *(uint8_t*)(p + 16 * i) = (uint8_t)(c[i / 4] >> 8 * (i % 4));
+      if (d == 0) *(float*)(base + v_scale<D>(s.o, C.logP)) = scale;
+    } else if (s.page >= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *(uint16_t*)(p + 16 * i) = (uint16_t)(in[i / 2] >> 16 * (i % 2));
+    }
+  }
+}
+
+// Prompts: neighbouring tokens share lines of the pages, so a workgroup takes
+// neighbouring tokens (lines written in part by several XCDs go to memory in
+// part, from each).
+//
+//  * Workgroups 0 .. qk - 1: 2048 / D tokens (a row of D / 8 lanes each) by
+//    APPEND_HEADS heads of q or k, one after the other with the next one's row
+//    requested; a token's cosines and sines are read once for them.
+//  * The others: VT tokens of one head of v.  They pass through LDS, and the
+//    tokens of a chunk that are all here leave as 16 bytes a dim.
+constexpr int APPEND_HEADS = 8, APPEND_VT = 64;
+
+template <int D, bool F8>
+__global__ __launch_bounds__(256) void append_tiles(AppendArgs A, int qk, int groups) {
+  constexpr int LR = D / 8, TT = 256 / LR, E = F8 ? 16 : 8, VT = APPEND_VT;
+  constexpr int EL = F8 ? 1 : 2, PITCH = D * EL + 4;     // bytes of a token's row in LDS
+  __shared__ __align__(16) char s_v[VT * PITCH];
+  __shared__ int64_t s_page[VT];
+  __shared__ int s_o[VT], s_run[VT], s_runs;
+  const KvArgs& C = A.kv;
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < qk) {
+    const int t = (int)(blockIdx.x / (unsigned)groups) * TT + tid / LR, d = 8 * (tid % LR);
+    const int h0 = (int)(blockIdx.x % (unsigned)groups) * APPEND_HEADS;
+    const int heads = A.q_heads + C.heads, end = min(h0 + APPEND_HEADS, heads);
+    if (t >= C.T) return;
+    auto load = [&](int hh) {
+      const bool q = hh < A.q_heads;
+      return *(const u32x4*)(q ? A.x[0] + t * A.st[0] + hh * A.sh[0] + d
+                               : A.x[1] + t * A.st[1] + (hh - A.q_heads) * A.sh[1] + d);
+    };
+    u32x4 next = load(h0);
+    u32x4 wq = {}, wk = {};
+    if (A.norm[0]) wq = *(const u32x4*)(A.norm[0] + d);
+    if (A.norm[1]) wk = *(const u32x4*)(A.norm[1] + d);
+    const Slot s = token_slot(C, t);
+    const Turn8 turn = load_turn(A, s.pos, d);
+    for (int hh = h0; hh < end; ++hh) {
+      Row8 r = widen(next);
+      if (hh + 1 < end) next = load(hh + 1);
+      const bool q = hh < A.q_heads;
+      if (A.norm[q ? 0 : 1]) norm_row<D>(r, q ? wq : wk, A.eps);
+      turn_row(A, r, turn, d);
+      if (q) *(u32x4*)(A.q_out + ((int64_t)t * A.q_heads + hh) * D + d) = narrow(r);
+      else put_key<D, F8>(C, r, s, hh - A.q_heads, d);
+    }
     return;
   }
-  float scale = 1.f;
-  if (F8) {                                   // the largest |x| by its bits: NaN above inf above all
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-#pragma unroll
-    for (int o = LR / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    const bool fine = m < 0x7F800000u;
-    scale = !fine ? __builtin_nanf("") : m == 0 ? 1.f : __uint_as_float(m) / E4M3_MAX;
-    // a row of denormals can round its scale to 0
-    if (scale == 0.f) scale = 1.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = fine ? fminf(fmaxf(x[i] / scale, -E4M3_MAX), E4M3_MAX) : 0.f;
-  }
-  if (!held) return;
-  const int page = C.table[place.x * C.ld_table + (pos >> C.logP)];
-  if ((unsigned)page >= (unsigned)C.n_pages) return;
-  const int o = pos & ((1 << C.logP) - 1);
-  char* base = C.pages + page * C.page_stride + (int64_t)h * C.head_bytes;
-  if (F8) {
-    u32x2 c;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
-      c[i] = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], p, true);
+  const unsigned v = blockIdx.x - (unsigned)qk;
+  const int t0 = (int)(v / (unsigned)C.heads) * VT, h = (int)(v % (unsigned)C.heads);
+  const int n = min(VT, C.T - t0);
+  if (tid < VT) {                            // one wave
+    Slot s = {-1, 0, 0};
+    if (tid < n) s = token_slot(C, t0 + tid);
+    // runs: neighbouring tokens that go to neighbouring places of one chunk
+    const int64_t before = __shfl_up(s.page, 1);
+    const int at = __shfl_up(s.o, 1);
+    const bool in = s.page >= 0;
+    const bool first = in && (tid == 0 || s.page != before || s.o != at + 1 || s.o % E == 0);
+    const uint64_t starts = ballot(first), breaks = starts | ~ballot(in);
+    if (first) {
+      const uint64_t later = tid < 63 ? breaks >> (tid + 1) : 0;
+      const int len = later ? __builtin_ctzll(later) + 1 : 64 - tid;
+      s_run[lanes_below(starts)] = tid | len << 8;
     }
-    if (kind == 1) {
-      *(u32x2*)(base + k_chunk<E>(d, o, C.logP) + (d & 8)) = c;
+    s_page[tid] = s.page;
+    s_o[tid] = s.o;
+    if (tid == 0) s_runs = __builtin_popcountll(starts);
+  }
+  constexpr int LOADS = VT * LR / 256;
+  u32x4 in[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = min(i * TT + tid / LR, n - 1);
+    in[i] = *(const u32x4*)(A.x[2] + (t0 + r) * A.st[2] + h * A.sh[2] + 8 * (tid % LR));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = i * TT + tid / LR, d = 8 * (tid % LR);
+    uint32_t* p = (uint32_t*)(s_v + r * PITCH + d * EL);
+    if (F8) {
+      float scale;
+      const u32x2 c = encode_row<D>(widen(in[i]), &scale);
+      p[0] = c[0];
+      p[1] = c[1];
+      if (d == 0 && r < n && s_page[r] >= 0)
+        *(float*)(C.pages + s_page[r] + (int64_t)h * C.head_bytes + v_scale<D>(s_o[r], C.logP)) = scale;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *(uint8_t*)(base + v_chunk<E, D>(d + i, o, C.logP) + o % E) = (uint8_t)(c[i / 4] >> 8 * (i % 4));
+      for (int k = 0; k < 4; ++k) p[k] = in[i][k];
     }
-    if (j == 0)
-      *(float*)(base + (kind == 1 ? k_scale<D>(o, C.logP) : v_scale<D>(o, C.logP))) = scale;
-    return;
   }
-  if (kind == 1) {
-    u32x4 c;
+  __syncthreads();
+  // (run, 4 / EL dims) to a thread: a dword of each token's row
+  constexpr int DW = D * EL / 4;             // dwords of a row
+  for (int i = tid; i < s_runs * DW; i += 256) {
+    const int run = s_run[i / DW], j = run & 255, len = run >> 8, dw = i % DW;
+    const int d = dw * (4 / EL), o = s_o[j];
+    char* base = C.pages + s_page[j] + (int64_t)h * C.head_bytes;
+    auto word = [&](int k) { return *(const uint32_t*)(s_v + (j + k) * PITCH + 4 * dw); };
+    if (len == E) {
+      uint32_t x[E];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = pack_bf16(x[2 * i], x[2 * i + 1]);
-    *(u32x4*)(base + k_chunk<E>(d, o, C.logP)) = c;
-  } else {
+      for (int k = 0; k < E; ++k) x[k] = word(k);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      *(uint16_t*)(base + v_chunk<E, D>(d + i, o, C.logP) + o % E * 2) =
-          (uint16_t)(in[i / 2] >> 16 * (i % 2));
+      for (int e = 0; e < 4 / EL; ++e) {     // element e of each dword, token by token
+        u32x4 y;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (F8) {
+            const uint32_t sel = 0x0C0C0400u + 0x0101u * e;      // byte e of two words
+            const uint32_t a = __builtin_amdgcn_perm(x[(4 * k + 1) % E], x[4 * k % E], sel);
+            const uint32_t b = __builtin_amdgcn_perm(x[(4 * k + 3) % E], x[(4 * k + 2) % E], sel);
+            y[k] = a | b << 16;
+          } else {
+            y[k] = __builtin_amdgcn_perm(x[2 * k + 1], x[2 * k], e ? 0x07060302u : 0x05040100u);
+          }
+        }
+        *(u32x4*)(base + v_chunk<E, D>(d + e, o, C.logP)) = y;
+      }
+    } else {
+      for (int k = 0; k < len; ++k) {
+        const uint32_t x = word(k);
+        char* p = base + v_chunk<E, D>(d, o + k, C.logP) + (o + k) % E * EL;
+#pragma unroll
+        for (int e = 0; e < 4 / EL; ++e) {
+          if (F8) *(uint8_t*)(p + 16 * e) = (uint8_t)(x >> 8 * e);
+          else *(uint16_t*)(p + 16 * e) = (uint16_t)(x >> 16 * e);
+        }
+      }
+    }
   }
 }
 
@@ -217,29 +407,54 @@ struct CopyArgs {
   const int32_t* dst;
 };
 
-constexpr int COPY_PART = 16384;              // bytes a workgroup copies
+__device__ __forceinline__ u32x4 ld_copy(const char* p) { return *(const u32x4*)p; }
+__device__ __forceinline__ void st_copy(char* p, u32x4 v) { __builtin_nontemporal_store(v, (u32x4*)p); }
 
-// Workgroup (pair, layer, part): 16 KB of the page.
+constexpr int COPY_LOADS = 8;                // 16-byte loads of a thread, all in flight
+constexpr int COPY_PART = COPY_LOADS * 4096; // bytes a workgroup copies
+
+// Workgroup (pair, layer, part): COPY_PART bytes of the page.
 __global__ __launch_bounds__(256) void copy_pages(CopyArgs A) {
   const unsigned part = blockIdx.x % (unsigned)A.parts, x = blockIdx.x / (unsigned)A.parts;
   const unsigned layer = x % (unsigned)A.n_layers, pair = x / (unsigned)A.n_layers;
   const int s = A.src[pair], d = A.dst[pair];
   if ((unsigned)s >= (unsigned)A.n_pages || (unsigned)d >= (unsigned)A.n_pages) return;
   char* base = A.pages + layer * A.layer_stride;
-  const char* from = base + s * A.page_stride;
-  char* to = base + d * A.page_stride;
-  for (int i = 0; i < COPY_PART / 4096; ++i) {
-    const int64_t at = (int64_t)part * COPY_PART + i * 4096 + threadIdx.x * 16;
-    if (at < A.page_bytes) *(u32x4*)(to + at) = *(const u32x4*)(from + at);
+  const int64_t at = (int64_t)part * COPY_PART + threadIdx.x * 16;
+  const char* from = base + s * A.page_stride + at;
+  char* to = base + d * A.page_stride + at;
+  const int64_t left = A.page_bytes - at;
+  u32x4 v[COPY_LOADS];
+  if (left > (COPY_LOADS - 1) * 4096) {
+#pragma unroll
+    for (int i = 0; i < COPY_LOADS; ++i) v[i] = ld_copy(from + i * 4096);
+#pragma unroll
+    for (int i = 0; i < COPY_LOADS; ++i) st_copy(to + i * 4096, v[i]);
+  } else {
+    for (int i = 0; i * 4096 < left; ++i) st_copy(to + i * 4096, ld_copy(from + i * 4096));
   }
 }
 
+template <int D, bool F8>
+static void launch_append(const AppendArgs& A, hipStream_t s) {
+  const unsigned per = 256 / (D / 8), heads = A.q_heads + A.kv.heads;
+  // several new tokens a sequence share the pages' lines
+  if (A.kv.q_start && A.kv.T >= 4 * (int64_t)A.kv.B) {
+    const unsigned groups = (heads + APPEND_HEADS - 1) / APPEND_HEADS;
+    const unsigned qk = (A.kv.T + per - 1) / per * groups;
+    const unsigned v = (A.kv.T + APPEND_VT - 1) / APPEND_VT * A.kv.heads;
+    timed_launch(CX_KERNEL_KV_APPEND, append_tiles<D, F8>, dim3(qk + v), dim3(256), 0, s, A, (int)qk,
+                 (int)groups);
+    return;
+  }
+  const unsigned rows = (unsigned)A.kv.T * (heads + A.kv.heads);
+  timed_launch(CX_KERNEL_KV_APPEND, append_rows<D, F8>, dim3((rows + per - 1) / per), dim3(256), 0,
+               s, A);
+}
 template <int D>
 static void launch_append(const AppendArgs& A, int dtype, hipStream_t s) {
-  const int64_t rows = (int64_t)A.kv.T * (A.q_heads + 2 * A.kv.heads), per = 256 / (D / 8);
-  const dim3 grid((unsigned)((rows + per - 1) / per));
-  timed_launch(CX_KERNEL_KV_APPEND, dtype == CX_KV_BF16 ? append_rows<D, false> : append_rows<D, true>,
-               grid, dim3(256), 0, s, A);
+  if (dtype == CX_KV_BF16) launch_append<D, false>(A, s);
+  else launch_append<D, true>(A, s);
 }
 
 }  // namespace cx
@@ -268,7 +483,7 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
                         (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)rope;
   if ((all & 15) || ((q_token | q_head | k_token | k_head | v_token | v_head) & 7))
     return cx::api_fail(CX_EINVAL, "rows must be 16-byte aligned");
-  if ((int64_t)kv->T * (q_heads + 2 * (int64_t)kv->kv_heads) > ((int64_t)1 << 33))
+  if ((int64_t)kv->T * (q_heads + 2 * (int64_t)kv->kv_heads) >= ((int64_t)1 << 31))
     return cx::api_fail(CX_EINVAL, "too many rows");
   A.x[0] = q; A.x[1] = k; A.x[2] = v;
   A.st[0] = q_token; A.st[1] = k_token; A.st[2] = v_token;
