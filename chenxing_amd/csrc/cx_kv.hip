@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "cx_device.hpp"
 #include "cx_internal.hpp"
 #include "cx_kv.hpp"
@@ -98,15 +100,30 @@ __device__ __forceinline__ Row8 widen(u32x4 in) {
   return r;
 }
 
+// A reduction over the D / 8 lanes of a row, in every one of them: neighbours,
+// pairs, quads of a half row, half rows, and for 32 lanes the two rows.
+template <int D, typename T, typename Op>
+__device__ __forceinline__ T lanes_reduce(T v, Op op) {
+  auto dpp = [](T x, auto ctrl) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x),
+                                                          decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  v = op(v, dpp(v, std::integral_constant<int, 0xB1>()));    // quad_perm 1 0 3 2
+  v = op(v, dpp(v, std::integral_constant<int, 0x4E>()));    // quad_perm 2 3 0 1
+  v = op(v, dpp(v, std::integral_constant<int, 0x141>()));   // row_half_mirror
+  if (D >= 128) v = op(v, dpp(v, std::integral_constant<int, 0x140>()));   // row_mirror
+  if (D == 256) v = op(v, __shfl_xor(v, 16));
+  return v;
+}
+
 // x * rsqrt(mean(x^2) + eps) * w over the row's D / 8 lanes.
 template <int D>
 __device__ __forceinline__ void norm_row(Row8& r, u32x4 w, float eps) {
   float ss = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ss = fmaf(r.x[i], r.x[i], ss);
-#pragma unroll
-  for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-  const float f = 1.f / sqrtf(ss * (1.f / D) + eps);
+  ss = lanes_reduce<D>(ss, [](float a, float b) { return a + b; });
+  const float f = __builtin_amdgcn_rsqf(ss * (1.f / D) + eps);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     r.x[2 * i] = r.x[2 * i] * f * bf16_lo(w[i]);
@@ -141,8 +158,8 @@ __device__ __forceinline__ void turn_row(const AppendArgs& A, Row8& r, const Tur
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float a = r.x[2 * i], b = r.x[2 * i + 1];
-      r.x[2 * i] = a * t.c[0][i] - b * t.s[0][i];
-      r.x[2 * i + 1] = b * t.c[0][i] + a * t.s[0][i];
+      r.x[2 * i] = fmaf(a, t.c[0][i], -(b * t.s[0][i]));
+      r.x[2 * i + 1] = fmaf(b, t.c[0][i], a * t.s[0][i]);
     }
     return;
   }
@@ -152,7 +169,7 @@ __device__ __forceinline__ void turn_row(const AppendArgs& A, Row8& r, const Tur
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float y = __shfl(r.x[i], other), c = t.c[i / 4][i % 4], s = t.s[i / 4][i % 4];
-    if (d < A.rdim) r.x[i] = low ? r.x[i] * c - y * s : r.x[i] * c + y * s;
+    if (d < A.rdim) r.x[i] = fmaf(r.x[i], c, low ? -(y * s) : y * s);
   }
 }
 __device__ __forceinline__ u32x4 narrow(const Row8& r) {
@@ -169,15 +186,16 @@ __device__ __forceinline__ u32x2 encode_row(const Row8& r, float* scale) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(r.x[i]) & 0x7FFFFFFFu);
-#pragma unroll
-  for (int o = D / 16; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+  m = lanes_reduce<D>(m, [](uint32_t a, uint32_t b) { return max(a, b); });
   const bool fine = m < 0x7F800000u;
   float f = __uint_as_float(m) / E4M3_MAX;
   if (f == 0.f) f = 1.f;                     // a row of zeros, or of values whose scale rounds to 0
   *scale = fine ? f : __builtin_nanf("");
+  // times the scale's reciprocal: the quotient within 2 ulp
+  const float inv = fine ? 1.f / f : 0.f;
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fine ? fminf(fmaxf(r.x[i] / f, -E4M3_MAX), E4M3_MAX) : 0.f;
+  for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_fmed3f(fine ? r.x[i] * inv : 0.f, -E4M3_MAX, E4M3_MAX);
   u32x2 c;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
