@@ -88,6 +88,15 @@ __device__ __forceinline__ uint64_t scalar64(uint64_t x) {
          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
 }
 
+// The kernel's arguments in memory (its first, at the segment's start), for the
+// parts of it that run once a piece: what they need is read there again, so the
+// loop keeps its scalar registers.
+__device__ __forceinline__ const AttendArgs& launch_args() {
+  uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttendArgs*)(const CX_CONST AttendArgs*)p;
+}
+
 // Lane groups and registers change places.  Four registers: x[y] of group g
 // becomes x[g] of group y.  Two: the registers of groups 0 1 2 3, [a0 a1 a2 a3]
 // and [b0 b1 b2 b3], become [a0 a2 b0 b2] and [a1 a3 b1 b3].
@@ -261,6 +270,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   bool joined = false;
   // the piece that begins at unit u; b: the sequence of the one before
   auto piece = [&]() {
+    const auto& A = launch_args();
     while (s_pref[b + 1] <= u) ++b;
     b = __builtin_amdgcn_readfirstlane(b);
     const AttendSeq s = attend_seq<TOK>(A, b);
@@ -298,12 +308,14 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
 
   // ids of BATCH units of a piece from its k-th: lane KT k + group
   auto load_ids = [&](const AttendPiece& p, int k) {
+    const auto& C = launch_args().kv;
     const int t16 = (p.unit + k) * KT + l;
     return t16 < (p.lim + 15) >> 4 ? C.table[p.b * C.ld_table + (t16 >> (C.logP - 4))] : -1;
   };
   u32x4 qr[NT][QL], kr[KT][KL], vr[DT];
   float ks = 1.f, vs = 1.f;                  // e4m3: the scales of the unit's token l
   auto load_q = [&](const AttendPiece& p) {
+    const auto& A = launch_args();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = p.r0 + min(16 * nt + c, p.R - 1);
@@ -316,13 +328,16 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   const int vgroup = F8 ? g : g >> 1;        // the group of this lane's tokens of V
   // place in the page of a unit's 16-token group
   auto place = [&](int unit, int group) { return ((unit * KT + group) << 4) & (P - 1); };
-  const uint32_t klane = (uint32_t)(c + (g << C.logP)) * 16;
+  uint32_t koff[KL];                         // this lane's place in K, from chunk 4 x
+#pragma unroll
+  for (int x = 0; x < KL; ++x) koff[x] = (uint32_t)(c + ((4 * x + g) << C.logP)) * 16;
   // the unit's pages: which are in the pool (bit y: 16-token group y), and where
   // this lane's V is
   uint32_t held = 0, hnext = 0;
   const char* vnext = nullptr;
   auto load_k = [&](int ids, int k, int unit, int h, bool live) {
     const char* const head0 = C.pages + (int64_t)h * C.head_bytes;
+    const uint32_t on = live ? ~0u : 0;
     hnext = 0;
 #pragma unroll
     for (int y = 0; y < KT; ++y) {
@@ -332,7 +347,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       const char* p = head0 + (in ? id : 0) * C.page_stride + place(unit, y) * 16;
 #pragma unroll
       for (int x = 0; x < KL; ++x)
-        kr[y][x] = ld_page(p + ((int64_t)x << (C.logP + 6)) + (live ? klane : 0));
+        kr[y][x] = ld_page(p + (koff[x] & on));
     }
     const int id = __shfl(ids, k * KT + vgroup);
     const char* p = head0 + ((unsigned)id < (unsigned)C.n_pages ? id : 0) * C.page_stride;
@@ -342,11 +357,13 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       ks = sc[0];
       vs = sc[P];
     }
+    __builtin_amdgcn_sched_barrier(0);       // the loop's waits count on this order
   };
   auto load_v = [&]() {
     held = hnext;
 #pragma unroll
     for (int n = 0; n < DT; ++n) vr[n] = ld_page(vnext + 256 * n);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
   f32x4 acc[NT][DT];
@@ -355,6 +372,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   int pmin = 0, pmax = 0;                    // positions of the piece's first and last row
   bool again = false;
   auto begin = [&](const AttendPiece& p) {
+    const auto& A = launch_args();
     pmin = p.lowest + p.r0 / A.G;
     pmax = p.lowest + (p.r0 + p.R - 1) / A.G;
     again = false;
@@ -426,10 +444,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     }
     load_k(ids, k, turn ? nxt.unit : unit + 1, turn ? nxt.h : cur.h, !(turn && last));
 
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int y = 0; y < KT; ++y) v[nt][y] *= A.s1;
+    // scores in powers of 2 are to2 * v
+    const float to2 = A.cap ? 1.f : A.s1;
     if (A.cap) {                             // tanh(z) = 1 - 2 / (exp(2 z) + 1)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -438,13 +454,14 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             v[nt][y][j] = fmaf(-2.f * A.s2,
-                               __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v[nt][y][j]) + 1.f), A.s2);
+                               __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(A.s1 * v[nt][y][j]) + 1.f),
+                               A.s2);
     }
     // a row's running maximum is at least ATT_LOW once it has attended to a
     // token, whatever its score: -inf says that it has not
-    float top[NT];
+    float low[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) top[nt] = ATT_LOW;
+    for (int nt = 0; nt < NT; ++nt) low[nt] = ATT_LOW;
     // a unit is open where all its tokens are held, at or before the first row
     // and inside the last row's window
     const uint32_t here = held;
@@ -465,7 +482,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
             v[nt][y][j] = in && t <= hi[nt] && t > lo[nt] ? v[nt][y][j] : -INFINITY;
           }
         }
-        top[nt] = some ? ATT_LOW : -INFINITY;
+        low[nt] = some ? ATT_LOW : -INFINITY;
       }
     }
     float alpha[NT];
@@ -473,10 +490,11 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     u32x4 ph[NT][KH], pl[NT][KH];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      float top = -INFINITY;
 #pragma unroll
       for (int y = 0; y < KT; ++y)
-        top[nt] = fmaxf(top[nt], fmaxf(fmaxf(v[nt][y][0], v[nt][y][1]), fmaxf(v[nt][y][2], v[nt][y][3])));
-      const float m1 = fmaxf(m[nt], groups_max(top[nt]));
+        top = fmaxf(top, fmaxf(fmaxf(v[nt][y][0], v[nt][y][1]), fmaxf(v[nt][y][2], v[nt][y][3])));
+      const float m1 = fmaxf(fmaxf(m[nt], low[nt]), to2 * groups_max(top));
       const float base = m1 == -INFINITY ? 0.f : m1;
       alpha[nt] = __builtin_amdgcn_exp2f(m[nt] - base);
       moved |= alpha[nt] != 1.f;
@@ -487,7 +505,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       for (int y = 0; y < KT; ++y) {
         f32x4 p;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(v[nt][y][j] - base);
+        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(to2, v[nt][y][j], -base));
         add += (p[0] + p[1]) + (p[2] + p[3]);
         if (F8) {
 #pragma unroll
@@ -578,6 +596,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     }
 
     // the piece ends
+    const auto& A = launch_args();
+    const auto& C = A.kv;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       if (again) {
