@@ -168,7 +168,13 @@ struct AttendShape {
   static constexpr int ROWS = 16 * NT;
   static constexpr int E = F8 ? 16 : 8;      // elements of a 16-byte chunk
   static constexpr int PAD = D + 4;          // floats of a row of a wave's scratch
-  static constexpr int WAVES = NT == 1 && D < 256 ? 2 : 1;   // per SIMD
+  // what a row block costs beside its units, in units (64 ragged requests 99, 94
+  // and 93 us with 0, 1 and 2; 32 verify rounds 48, 42, 39 and 35 us with 0 .. 3)
+  static constexpr int PIECE = NT == 1 ? 2 : 4;
+  // waves per SIMD, as many as the registers hold
+  static constexpr int WAVES = D * NT == 64                      ? (F8 ? 3 : 4)
+                               : D * NT < 256 || (NT == 2 && !F8) ? 2
+                                                                  : 1;
   static constexpr int OFF_SCALE = ATT_WAVES * 16 * PAD * 4;
   static constexpr int OFF_PREF = OFF_SCALE + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
   static int lds(int B) { return OFF_PREF + 8 * (B + 1); }
@@ -207,6 +213,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   constexpr int QL = D / 32;                 // Q loads of 16 rows
   constexpr int DT = D / 16, KH = TOK / 32;
   constexpr int BATCH = 64 / KT;             // units whose page ids a wave holds
+  constexpr int PIECE = Sh::PIECE;
   constexpr uint32_t ALL = (1u << KT) - 1;
   extern __shared__ __align__(16) char lds[];
   const KvArgs& C = A.kv;
@@ -225,7 +232,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     uint64_t x = 0;
     if (b < C.B) {
       const AttendSeq s = attend_seq<TOK>(A, b);
-      x = (uint64_t)s.n * C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
+      if (s.n > 0) x = (uint64_t)(s.n + PIECE) * C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -268,7 +275,9 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     else hi = mid - 1;
   }
   bool joined = false;
-  // the piece that begins at unit u; b: the sequence of the one before
+  // the piece that begins at u, and u past it; b: the sequence of the one before.
+  // A row block is PIECE + n long, its units at the end: a share may end before
+  // the first of them (cnt = 0)
   auto piece = [&]() {
     const auto& A = launch_args();
     while (s_pref[b + 1] <= u) ++b;
@@ -276,9 +285,10 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     const AttendSeq s = attend_seq<TOK>(A, b);
     const uint64_t rem = scalar64(u - s_pref[b]);
     const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
-    const unsigned row = rem >> 32 ? (unsigned)(rem / (unsigned)s.n)
-                                   : (unsigned)rem / (unsigned)s.n;
-    const int ua = (int)(rem - (uint64_t)row * (unsigned)s.n);
+    const unsigned cost = s.n + PIECE;
+    const unsigned row = rem >> 32 ? (unsigned)(rem / cost) : (unsigned)rem / cost;
+    const int at = (int)(rem - (uint64_t)row * cost), ua = max(at - PIECE, 0);
+    const int64_t room = (int64_t)(end - u) - max(PIECE - at, 0);
     AttendPiece p;
     p.b = b;
     p.h = __builtin_amdgcn_readfirstlane((int)(row / (unsigned)blocks));
@@ -288,12 +298,12 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     p.lowest = s.len - s.q;
     p.lim = s.lim;
     p.unit = __builtin_amdgcn_readfirstlane(s.first + ua);
-    p.cnt = __builtin_amdgcn_readfirstlane((int)min((uint64_t)(s.n - ua), end - u));
+    p.cnt = __builtin_amdgcn_readfirstlane((int)min((int64_t)(s.n - ua), max(room, (int64_t)0)));
     p.slot = ua == 0 && p.cnt == s.n ? -1 : (int)(2 * worker + (ua == 0));
     p.slot = __builtin_amdgcn_readfirstlane(p.slot);
-    if (ua == 0 && p.cnt < s.n) {
+    if (ua == 0 && p.cnt > 0 && p.cnt < s.n) {
       joined = true;
-      const uint64_t lastu = u + s.n - 1, cut = more * (per + 1);
+      const uint64_t lastu = u - at + cost - 1, cut = more * (per + 1);
       if (l == 0) {
         AttendJoin j;
         j.first = worker;
@@ -303,6 +313,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
         A.join[worker] = j;
       }
     }
+    u = p.cnt > 0 ? u + max(PIECE - at, 0) + p.cnt : end;
     return p;
   };
 
@@ -389,15 +400,26 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   };
 
   AttendPiece cur = piece(), nxt;
-  u += cur.cnt;
+  if (cur.cnt == 0) {
+    if (l == 0) A.join[worker].last = -1;
+    return;
+  }
   load_q(cur);
   int ids = load_ids(cur, 0), idn = load_ids(cur, BATCH), idq = -1;
   load_k(ids, 0, cur.unit, cur.h, true);
   load_v();
-  bool last = u >= end;
-  nxt = cur;
-  if (!last) nxt = piece();
-  idq = load_ids(nxt, 0);
+  bool last = true;
+  // the piece after the current one, if the share holds one
+  auto follow = [&]() {
+    last = true;
+    if (u < end) {
+      nxt = piece();
+      last = nxt.cnt == 0;
+    }
+    if (last) nxt = cur;
+    idq = load_ids(nxt, 0);
+  };
+  follow();
   begin(cur);
   for (int i = 0;;) {
     const int unit = cur.unit + i, t0 = unit * TOK;
@@ -651,11 +673,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     }
     if (last) break;
     cur = nxt;
-    u += cur.cnt;
-    last = u >= end;
     idn = load_ids(cur, BATCH);
-    if (!last) nxt = piece();
-    idq = load_ids(nxt, 0);
+    follow();
     begin(cur);
     i = 0;
   }
@@ -755,14 +774,17 @@ static int row_tiles(int64_t rows, int D, int dtype) {
   const int64_t tiles = (rows + 15) / 16, blocks = (tiles + most - 1) / most;
   return (int)((tiles + blocks - 1) / blocks);
 }
-// Workers: as many waves as the chip holds of the tile's kernel.
-static int workgroups(int nt, int D) { return nt == 1 && D < 256 ? 512 : 256; }
+// Workers: as many waves as the chip's 256 CUs hold of the tile's kernel.
+static int workgroups(int nt, int D, int dtype) {
+  const bool f8 = dtype == CX_KV_E4M3;
+  return 256 * (D * nt == 64 ? (f8 ? 3 : 4) : D * nt < 256 || (nt == 2 && !f8) ? 2 : 1);
+}
 
 struct AttendWork {
   size_t off_ml, off_part, total;
 };
-static AttendWork attend_workspace(int nt, int D) {
-  const size_t W = ATT_WAVES * (size_t)workgroups(nt, D), rows = 16 * (size_t)nt;
+static AttendWork attend_workspace(int nt, int D, int dtype) {
+  const size_t W = ATT_WAVES * (size_t)workgroups(nt, D, dtype), rows = 16 * (size_t)nt;
   AttendWork x;
   x.off_ml = align_up(W * sizeof(AttendJoin), 256);
   x.off_part = x.off_ml + align_up(2 * W * rows * 8, 256);
@@ -780,7 +802,7 @@ static int launch_tile(const AttendArgs& A, hipStream_t s) {
                               hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(CX_KV_MAX_BATCH));
   });
   if (err != hipSuccess) return (int)err;
-  const unsigned grid = (unsigned)workgroups(NT, D);
+  const unsigned grid = 256 * Sh::WAVES;
   timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8>, dim3(grid), dim3(ATT_WG),
                (uint32_t)Sh::lds(A.kv.B), s, A);
   timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join<D, 16 * NT>, dim3(grid * ATT_WAVES, NT),
@@ -809,9 +831,12 @@ size_t cx_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int
                                           int32_t max_new) {
   if (q_heads < 1 || kv_heads < 1 || head_dim < 1 || max_new < 1) return 256;
   const int64_t rows = (int64_t)(q_heads / kv_heads) * max_new;
-  const size_t bf16 = cx::attend_workspace(cx::row_tiles(rows, head_dim, CX_KV_BF16), head_dim).total;
-  const size_t e4m3 = cx::attend_workspace(cx::row_tiles(rows, head_dim, CX_KV_E4M3), head_dim).total;
-  return bf16 > e4m3 ? bf16 : e4m3;
+  size_t most = 0;
+  for (int dtype : {CX_KV_BF16, CX_KV_E4M3}) {
+    const size_t n = cx::attend_workspace(cx::row_tiles(rows, head_dim, dtype), head_dim, dtype).total;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
@@ -843,7 +868,7 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   A.out = out;
   const int64_t rows = (int64_t)A.G * max_new;
   const int D = kv->head_dim, nt = cx::row_tiles(rows, D, kv->dtype);
-  const cx::AttendWork lay = cx::attend_workspace(nt, D);
+  const cx::AttendWork lay = cx::attend_workspace(nt, D, kv->dtype);
   A.join = (cx::AttendJoin*)workspace;
   A.ml = (float*)((char*)workspace + lay.off_ml);
   A.part = (float*)((char*)workspace + lay.off_part);
