@@ -33,6 +33,7 @@ namespace cx {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ATT_WAVES = 4, ATT_WG = 64 * ATT_WAVES;
+constexpr int ATT_SHARE = 2;                 // the least share, in units
 constexpr float ATT_LOW = -3e38f;            // running maximum of a row that attends to something
 
 struct AttendArgs {
@@ -44,13 +45,16 @@ struct AttendArgs {
   int cap;                    // the latter
   int window;                 // 0: none
   uint16_t* out;
+  int* entries;               // number of entries of join
   struct AttendJoin* join;    // [workers]
   float* ml;                  // [2 workers, ROWS, 2]: a part's maxima and sums
   float* part;                // [2 workers, ROWS, D]
 };
 
 // A row block whose units lie in several workers' shares: those of workers
-// first .. last.  Written by the first; none: last = -1.
+// first .. last (last = -1: in one).  Written by the first; there is an entry for
+// every row block, in their order, or, where they are more than the workers, for
+// every worker.
 struct AttendJoin {
   int first, last;
   int tok0, row0, rows, head;
@@ -224,7 +228,11 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::OFF_PREF));
   CX_LDS uint64_t* const s_sum = s_pref - ATT_WAVES;
 
-  // units before each sequence, over its kv heads and row blocks
+  // units before each sequence, over its kv heads and row blocks, and below them
+  // its row blocks (those of a sequence count as at most 4096: more than the
+  // workers all the same)
+  constexpr int RB = 25;
+  constexpr uint64_t RB_MASK = (1u << RB) - 1;
   if (tid == 0) s_pref[0] = 0;
   uint64_t total = 0;
   for (int b0 = 0; b0 < C.B; b0 += ATT_WG) {
@@ -232,7 +240,10 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     uint64_t x = 0;
     if (b < C.B) {
       const AttendSeq s = attend_seq<TOK>(A, b);
-      if (s.n > 0) x = (uint64_t)(s.n + PIECE) * C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
+      if (s.n > 0) {
+        const uint64_t blocks = (uint64_t)C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
+        x = (uint64_t)(s.n + PIECE) * blocks << RB | min(blocks, (uint64_t)4096);
+      }
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -247,6 +258,10 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     total = s_pref[min(b0 + ATT_WG, C.B)];
   }
   total = scalar64(total);
+  const unsigned blocks_all = (unsigned)(total & RB_MASK);
+  const bool by_block = blocks_all <= gridDim.x * ATT_WAVES;
+  total >>= RB;
+  if (blockIdx.x == 0 && tid == 0) *A.entries = by_block ? (int)blocks_all : gridDim.x * ATT_WAVES;
 
   // tokens that attend to nothing
   for (int b = blockIdx.x; b < C.B; b += gridDim.x)
@@ -257,21 +272,21 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       for (int64_t i = tid; i < n; i += ATT_WG) o[i] = u32x4{0, 0, 0, 0};
     }
 
-  // this worker's share of the units: a unit at least, the first shares one
+  // this worker's share of the units: ATT_SHARE at least, the first shares one
   // more.  Neighbouring workers are on different CUs.
   const unsigned worker = __builtin_amdgcn_readfirstlane(blockIdx.x + gridDim.x * w);
-  const uint64_t shares = min((uint64_t)gridDim.x * ATT_WAVES, total);
+  const uint64_t shares = min((uint64_t)gridDim.x * ATT_WAVES, (total + ATT_SHARE - 1) / ATT_SHARE);
   if (worker >= shares) {
-    if (l == 0) A.join[worker].last = -1;
+    if (l == 0 && !by_block) A.join[worker].last = -1;
     return;
   }
   const uint64_t per = scalar64(total / shares), more = total - per * shares;
   uint64_t u = worker * per + min((uint64_t)worker, more);
   const uint64_t end = u + per + (worker < more);
   int b = 0;
-  for (int hi = C.B - 1; b < hi;) {          // the last b with s_pref[b] <= u
+  for (int hi = C.B - 1; b < hi;) {          // the last b with its units at or before u
     const int mid = (b + hi + 1) >> 1;
-    if (s_pref[mid] <= u) b = mid;
+    if (s_pref[mid] >> RB <= u) b = mid;
     else hi = mid - 1;
   }
   bool joined = false;
@@ -280,10 +295,10 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   // the first of them (cnt = 0)
   auto piece = [&]() {
     const auto& A = launch_args();
-    while (s_pref[b + 1] <= u) ++b;
+    while (s_pref[b + 1] >> RB <= u) ++b;
     b = __builtin_amdgcn_readfirstlane(b);
     const AttendSeq s = attend_seq<TOK>(A, b);
-    const uint64_t rem = scalar64(u - s_pref[b]);
+    const uint64_t before = s_pref[b], rem = scalar64(u - (before >> RB));
     const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
     const unsigned cost = s.n + PIECE;
     const unsigned row = rem >> 32 ? (unsigned)(rem / cost) : (unsigned)rem / cost;
@@ -301,16 +316,17 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     p.cnt = __builtin_amdgcn_readfirstlane((int)min((int64_t)(s.n - ua), max(room, (int64_t)0)));
     p.slot = ua == 0 && p.cnt == s.n ? -1 : (int)(2 * worker + (ua == 0));
     p.slot = __builtin_amdgcn_readfirstlane(p.slot);
-    if (ua == 0 && p.cnt > 0 && p.cnt < s.n) {
-      joined = true;
+    if (ua == 0 && p.cnt > 0 && (by_block || p.cnt < s.n)) {
+      joined |= p.cnt < s.n;
       const uint64_t lastu = u - at + cost - 1, cut = more * (per + 1);
       if (l == 0) {
         AttendJoin j;
         j.first = worker;
-        j.last = (int)(lastu < cut ? lastu / (per + 1) : more + (lastu - cut) / per);
+        j.last = p.cnt == s.n ? -1
+                 : (int)(lastu < cut ? lastu / (per + 1) : more + (lastu - cut) / per);
         j.tok0 = p.tok0; j.row0 = p.r0; j.rows = p.R; j.head = p.h;
         j.pad[0] = j.pad[1] = 0;
-        A.join[worker] = j;
+        A.join[by_block ? (unsigned)(before & RB_MASK) + row : worker] = j;
       }
     }
     u = p.cnt > 0 ? u + max(PIECE - at, 0) + p.cnt : end;
@@ -401,7 +417,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
 
   AttendPiece cur = piece(), nxt;
   if (cur.cnt == 0) {
-    if (l == 0) A.join[worker].last = -1;
+    if (l == 0 && !by_block) A.join[worker].last = -1;
     return;
   }
   load_q(cur);
@@ -678,93 +694,122 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     begin(cur);
     i = 0;
   }
-  if (!joined && l == 0) A.join[worker].last = -1;
+  if (!joined && l == 0 && !by_block) A.join[worker].last = -1;
 }
 
-// A row block's parts joined, in the order of its tokens: workgroup (worker, 16
-// rows).  A wave takes every fourth row, or every fourth group of rows: D / 8
-// lanes a row, the wave's other lane groups on other rows, or on other parts of
-// the row where there are many (their order of adding is fixed all the same).
-// Latency: a round of loads from the other XCDs' parts takes about a microsecond,
-// so 4 parts a lane are requested together, 8 where there are many.
-template <int D, int ROWS>
-__global__ __launch_bounds__(256) void attend_join(AttendArgs A) {
-  constexpr int LANES = D / 8, GROUPS = 64 / LANES;
-  const AttendJoin J = const_load(A.join + blockIdx.x);
-  if (J.last < 0) return;
-  const int n = J.last - J.first + 1, w = wave_id(), l = lane_id();
-  const int grp = l / LANES, d = 8 * (l % LANES);
-  const int end = min(J.rows, 16 * (int)blockIdx.y + 16);
-  auto join = [&](auto wide_) {
-    constexpr bool wide = decltype(wide_)::value;
-    constexpr int JOIN_AHEAD = wide ? 8 : 4;
-    constexpr int step = wide ? GROUPS : 1, rows = wide ? 1 : GROUPS;
-    for (int r0 = 16 * blockIdx.y + w * rows; r0 < end; r0 += 4 * rows) {
-      const int r = wide ? r0 : min(r0 + grp, end - 1);
-      float top = -INFINITY, L = 0;
-      f32x4 o0 = {0, 0, 0, 0}, o1 = {0, 0, 0, 0};
-      for (int p0 = wide ? grp : 0; p0 < n; p0 += JOIN_AHEAD * step) {
-        float m[JOIN_AHEAD], s[JOIN_AHEAD];
-        f32x4 x0[JOIN_AHEAD], x1[JOIN_AHEAD];
+// The parts of rows joined, in an order that goes by their number alone.
+struct JoinSum {
+  float top, L;
+  f32x4 o0, o1;
+};
+// Adds parts p, p + step, .. of row r at dims d .. d + 7, AHEAD of them together.
+template <int D, int ROWS, int AHEAD>
+__device__ __forceinline__ JoinSum join_parts(const AttendArgs& A, const AttendJoin& J, int n, int r,
+                                              int d, int p, int step) {
+  JoinSum S = {-INFINITY, 0.f, {0, 0, 0, 0}, {0, 0, 0, 0}};
+  for (int p0 = p; p0 < n; p0 += AHEAD * step) {
+    float m[AHEAD], s[AHEAD];
+    f32x4 x0[AHEAD], x1[AHEAD];
 #pragma unroll
-        for (int k = 0; k < JOIN_AHEAD; ++k) { // past the last: the last again, with weight 0
-          const int p = p0 + k * step, q = min(p, n - 1);
-          const int64_t at = (int64_t)(2 * (J.first + q) + (q == 0)) * ROWS + r;
-          const float2 ml = *(const float2*)(A.ml + 2 * at);
-          m[k] = p < n ? ml.x : -INFINITY;
-          s[k] = p < n ? ml.y : 0.f;
-          x0[k] = *(const f32x4*)(A.part + at * D + d);
-          x1[k] = *(const f32x4*)(A.part + at * D + d + 4);
-        }
-        float t = top;
-#pragma unroll
-        for (int k = 0; k < JOIN_AHEAD; ++k) t = fmaxf(t, m[k]);
-        const float base = t == -INFINITY ? 0.f : t;
-        const float f0 = __builtin_amdgcn_exp2f(top - base);
-        L *= f0;
-        o0 *= f0;
-        o1 *= f0;
-        top = t;
-#pragma unroll
-        for (int k = 0; k < JOIN_AHEAD; ++k) {
-          // a part without a token has no sums to add (its place may hold anything
-          // where the last part stands in for one past it)
-          if (p0 + k * step >= n) continue;
-          const float f = __builtin_amdgcn_exp2f(m[k] - base);
-          L = fmaf(f, s[k], L);
-          o0 += f * x0[k];
-          o1 += f * x1[k];
-        }
-      }
-      if (wide) {
-#pragma unroll
-        for (int x = LANES; x < 64; x <<= 1) {
-          const float t = __shfl_xor(top, x), all = fmaxf(top, t);
-          const float base = all == -INFINITY ? 0.f : all;
-          const float fa = __builtin_amdgcn_exp2f(top - base), fb = __builtin_amdgcn_exp2f(t - base);
-          const bool low = (l & x) == 0;       // both add in one order: the lower group's first
-          auto add = [&](float v) {
-            const float u = __shfl_xor(v, x);
-            return low ? fmaf(fa, v, fb * u) : fmaf(fb, u, fa * v);
-          };
-          L = add(L);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) { o0[k] = add(o0[k]); o1[k] = add(o1[k]); }
-          top = all;
-        }
-      }
-      if (wide ? grp == 0 : r0 + grp < end) {
-        const float f = top == -INFINITY ? 0.f : 1.f / L;
-        const u32x4 x = {pack_bf16(o0[0] * f, o0[1] * f), pack_bf16(o0[2] * f, o0[3] * f),
-                         pack_bf16(o1[0] * f, o1[1] * f), pack_bf16(o1[2] * f, o1[3] * f)};
-        const int row = J.row0 + r;
-        *(u32x4*)(A.out + ((int64_t)(J.tok0 + row / A.G) * A.q_heads + J.head * A.G + row % A.G) * D +
-                  d) = x;
-      }
+    for (int k = 0; k < AHEAD; ++k) {        // past the last: the last again, not added
+      const int q = min(p0 + k * step, n - 1);
+      const int64_t at = (int64_t)(2 * (J.first + q) + (q == 0)) * ROWS + r;
+      const float2 ml = *(const float2*)(A.ml + 2 * at);
+      m[k] = p0 + k * step < n ? ml.x : -INFINITY;
+      s[k] = ml.y;
+      x0[k] = *(const f32x4*)(A.part + at * D + d);
+      x1[k] = *(const f32x4*)(A.part + at * D + d + 4);
     }
-  };
-  if (n > 8) join(std::true_type());
-  else join(std::false_type());
+    float t = S.top;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) t = fmaxf(t, m[k]);
+    const float base = t == -INFINITY ? 0.f : t, f0 = __builtin_amdgcn_exp2f(S.top - base);
+    S.top = t;
+    S.L *= f0;
+    S.o0 *= f0;
+    S.o1 *= f0;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (p0 + k * step >= n) continue;
+      const float f = __builtin_amdgcn_exp2f(m[k] - base);
+      S.L = fmaf(f, s[k], S.L);
+      S.o0 += f * x0[k];
+      S.o1 += f * x1[k];
+    }
+  }
+  return S;
+}
+__device__ __forceinline__ void join_add(JoinSum& a, const JoinSum& b) {
+  const float t = fmaxf(a.top, b.top), base = t == -INFINITY ? 0.f : t;
+  const float fa = __builtin_amdgcn_exp2f(a.top - base), fb = __builtin_amdgcn_exp2f(b.top - base);
+  a.top = t;
+  a.L = fa * a.L + fb * b.L;
+  a.o0 = fa * a.o0 + fb * b.o0;
+  a.o1 = fa * a.o1 + fb * b.o1;
+}
+template <int D>
+__device__ __forceinline__ void join_out(const AttendArgs& A, const AttendJoin& J, const JoinSum& S,
+                                         int r, int d) {
+  const float f = S.top == -INFINITY ? 0.f : 1.f / S.L;
+  const u32x4 x = {pack_bf16(S.o0[0] * f, S.o0[1] * f), pack_bf16(S.o0[2] * f, S.o0[3] * f),
+                   pack_bf16(S.o1[0] * f, S.o1[1] * f), pack_bf16(S.o1[2] * f, S.o1[3] * f)};
+  const int row = J.row0 + r;
+  *(u32x4*)(A.out + ((int64_t)(J.tok0 + row / A.G) * A.q_heads + J.head * A.G + row % A.G) * D + d) = x;
+}
+
+// Few row blocks, so perhaps of many parts: workgroup (entry, row), the row's
+// parts over all its lane groups of D / 8 lanes.
+template <int D, int ROWS>
+__global__ __launch_bounds__(256) void attend_join_row(AttendArgs A) {
+  constexpr int LANES = D / 8, GROUPS = 256 / LANES;
+  __shared__ JoinSum s_sum[GROUPS][LANES];
+  const int count = const_load(A.entries);
+  const AttendJoin J = const_load(A.join + blockIdx.x);
+  const int r = blockIdx.y;
+  if ((int)blockIdx.x >= count || J.last < 0 || r >= J.rows) return;
+  const int n = J.last - J.first + 1, grp = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  JoinSum S = join_parts<D, ROWS, 8>(A, J, n, r, 8 * lane, grp, GROUPS);
+  if (grp > 0) s_sum[grp][lane] = S;
+  __syncthreads();
+  if (grp > 0) return;
+  for (int k = 1; k < min(n, GROUPS); ++k) join_add(S, s_sum[k][lane]);
+  join_out<D>(A, J, S, r, 8 * lane);
+}
+
+// Many row blocks: workgroup (entry, 16 rows).  Each lane group of D / 8 lanes
+// takes a row with all its parts; where there are few rows and many parts, each
+// wave takes one with its groups' shares of them (32 verify rounds, 36 rows: 6 us
+// with groups, 9 with waves; 11 requests of up to 7400 tokens, 8 rows: 20 and 9 us).
+template <int D, int ROWS>
+__global__ __launch_bounds__(256) void attend_join_block(AttendArgs A) {
+  constexpr int LANES = D / 8, GROUPS = 256 / LANES;
+  const int count = const_load(A.entries);
+  const AttendJoin J = const_load(A.join + blockIdx.x);
+  if ((int)blockIdx.x >= count || J.last < 0) return;
+  const int n = J.last - J.first + 1, d = 8 * (threadIdx.x % LANES);
+  const int r0 = 16 * blockIdx.y, end = min(J.rows, r0 + 16);
+  if (n <= 8 || end - r0 > 8) {
+    for (int r = r0 + threadIdx.x / LANES; r < end; r += GROUPS)
+      join_out<D>(A, J, join_parts<D, ROWS, 4>(A, J, n, r, d, 0, 1), r, d);
+    return;
+  }
+  const int l = lane_id();
+  for (int r = r0 + wave_id(); r < end; r += 4) {
+    JoinSum S = join_parts<D, ROWS, 8>(A, J, n, r, d, l / LANES, GROUPS / 4);
+#pragma unroll
+    for (int x = LANES; x < 64; x <<= 1) {
+      JoinSum T;
+      T.top = __shfl_xor(S.top, x);
+      T.L = __shfl_xor(S.L, x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        T.o0[k] = __shfl_xor(S.o0[k], x);
+        T.o1[k] = __shfl_xor(S.o1[k], x);
+      }
+      join_add(S, T);                        // a sum of two: in either order the same
+    }
+    if (l < LANES) join_out<D>(A, J, S, r, d);
+  }
 }
 
 // The tile, in 16 rows, for at most that many rows of a sequence that share a kv
@@ -780,13 +825,18 @@ static int workgroups(int nt, int D, int dtype) {
   return 256 * (D * nt == 64 ? (f8 ? 3 : 4) : D * nt < 256 || (nt == 2 && !f8) ? 2 : 1);
 }
 
+// Workgroups of attend_join_row at most, above attend_join_block (one request of
+// 69773 tokens, heads of 64: 9 and 97 us; 30 of 7007 tokens, 8 kv heads: 8 and 5 us).
+constexpr int ATT_JOIN_ROWS = 1024;
+
 struct AttendWork {
-  size_t off_ml, off_part, total;
+  size_t off_join, off_ml, off_part, total;
 };
 static AttendWork attend_workspace(int nt, int D, int dtype) {
   const size_t W = ATT_WAVES * (size_t)workgroups(nt, D, dtype), rows = 16 * (size_t)nt;
   AttendWork x;
-  x.off_ml = align_up(W * sizeof(AttendJoin), 256);
+  x.off_join = 256;
+  x.off_ml = x.off_join + align_up(W * sizeof(AttendJoin), 256);
   x.off_part = x.off_ml + align_up(2 * W * rows * 8, 256);
   x.total = x.off_part + 2 * W * rows * D * 4;
   return x;
@@ -805,8 +855,16 @@ static int launch_tile(const AttendArgs& A, hipStream_t s) {
   const unsigned grid = 256 * Sh::WAVES;
   timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8>, dim3(grid), dim3(ATT_WG),
                (uint32_t)Sh::lds(A.kv.B), s, A);
-  timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join<D, 16 * NT>, dim3(grid * ATT_WAVES, NT),
-               dim3(256), 0, s, A);
+  // row blocks at most: every sequence's last one may hold fewer rows
+  constexpr int ROWS = 16 * NT;
+  const int64_t blocks = A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B);
+  const int64_t entries = blocks < grid * ATT_WAVES ? blocks : grid * ATT_WAVES;
+  if (entries * ROWS <= ATT_JOIN_ROWS)
+    timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_row<D, ROWS>, dim3((unsigned)entries, ROWS),
+                 dim3(256), 0, s, A);
+  else
+    timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_block<D, ROWS>, dim3((unsigned)entries, NT),
+                 dim3(256), 0, s, A);
   return (int)hipGetLastError();
 }
 
@@ -869,7 +927,8 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   const int64_t rows = (int64_t)A.G * max_new;
   const int D = kv->head_dim, nt = cx::row_tiles(rows, D, kv->dtype);
   const cx::AttendWork lay = cx::attend_workspace(nt, D, kv->dtype);
-  A.join = (cx::AttendJoin*)workspace;
+  A.entries = (int*)workspace;
+  A.join = (cx::AttendJoin*)((char*)workspace + lay.off_join);
   A.ml = (float*)((char*)workspace + lay.off_ml);
   A.part = (float*)((char*)workspace + lay.off_part);
   const hipStream_t s = (hipStream_t)stream;
