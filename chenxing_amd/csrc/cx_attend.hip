@@ -33,6 +33,9 @@ namespace cx {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ATT_WAVES = 4, ATT_WG = 64 * ATT_WAVES;
+// Terms are relative to a maximum that lags by up to this, in powers of 2: they
+// reach 256 instead of 1, and the sums are rarely scaled.
+constexpr float ATT_SLACK = 8.f;
 constexpr int ATT_SHARE = 2;                 // the least share, in units
 constexpr float ATT_LOW = -3e38f;            // running maximum of a row that attends to something
 
@@ -131,15 +134,17 @@ __device__ __forceinline__ float groups_sum(float x) {
   swap_rows(a, b);
   return __uint_as_float(a) + __uint_as_float(b);
 }
-// A mask of the bf16 or e4m3 elements of x that are NaN or infinite.
+// The sign bits of the result say which bf16 or e4m3 elements of x are NaN or
+// infinite (exponent all ones; code 0x7F or 0xFF).
 template <bool F8>
-__device__ __forceinline__ uint32_t nonfinite(uint32_t x) {
-  if (F8) {                                  // code 0x7F or 0xFF
-    const uint32_t m = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-    return m | (m - (m >> 7));
-  }
-  return ((x & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0) |
-         ((x & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0);
+__device__ __forceinline__ uint32_t nonfinite_sign(uint32_t x) {
+  return F8 ? (x & 0x7F7F7F7Fu) + 0x01010101u : (x & 0x7F807F80u) + 0x00800080u;
+}
+// A mask of the other elements.
+template <bool F8>
+__device__ __forceinline__ uint32_t finite_mask(uint32_t x) {
+  const uint32_t m = nonfinite_sign<F8>(x) & (F8 ? 0x80808080u : 0x80008000u);
+  return ~(m | (m - (m >> (F8 ? 7 : 15))));
 }
 __device__ __forceinline__ void regroup(uint32_t (&x)[4][2]) {
 #pragma unroll
@@ -532,11 +537,12 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
 #pragma unroll
       for (int y = 0; y < KT; ++y)
         top = fmaxf(top, fmaxf(fmaxf(v[nt][y][0], v[nt][y][1]), fmaxf(v[nt][y][2], v[nt][y][3])));
-      const float m1 = fmaxf(fmaxf(m[nt], low[nt]), to2 * groups_max(top));
-      const float base = m1 == -INFINITY ? 0.f : m1;
-      alpha[nt] = __builtin_amdgcn_exp2f(m[nt] - base);
-      moved |= alpha[nt] != 1.f;
-      m[nt] = m1;
+      const float m1 = fmaxf(low[nt], to2 * groups_max(top));
+      const bool up = m1 > m[nt] + ATT_SLACK;
+      const float base = up ? m1 : m[nt] == -INFINITY ? 0.f : m[nt];
+      alpha[nt] = up ? __builtin_amdgcn_exp2f(m[nt] - m1) : 1.f;
+      moved |= up;
+      m[nt] = up ? m1 : m[nt];
       uint32_t th[KT][2], tl[KT][2];
       float add = 0;
 #pragma unroll
@@ -600,16 +606,22 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       if (pmin != pmax) {
         // nor may NaN or infinity reach the rows that do not attend to it: left
         // out here, added row by row at the piece's end
-        bool bad = false;
+        uint32_t bad = 0;
 #pragma unroll
         for (int n = 0; n < DT; ++n)
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const uint32_t x = nonfinite<F8>(vr[n][d]);
-            bad |= x != 0;
-            vr[n][d] &= ~x;
-          }
-        again |= __any(bad);
+          for (int d = 0; d < 4; ++d) bad |= nonfinite_sign<F8>(vr[n][d]);
+        if (__any((bad & (F8 ? 0x80808080u : 0x80008000u)) != 0)) {
+          again = true;
+#pragma unroll
+          for (int n = 0; n < DT; ++n)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              // hidden: the sums above are not kept for this
+              asm volatile("" : "+v"(vr[n][d]));
+              vr[n][d] &= finite_mask<F8>(vr[n][d]);
+            }
+        }
       }
     }
 #pragma unroll
