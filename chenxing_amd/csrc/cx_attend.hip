@@ -32,6 +32,7 @@
 namespace cx {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ATT_SEQS = 512;                // sequences whose rows and lengths LDS keeps
 constexpr int ATT_WAVES = 4, ATT_WG = 64 * ATT_WAVES;
 // Terms are relative to a maximum that lags by up to this, in powers of 2: they
 // reach 256 instead of 1, and the sums are rarely scaled.
@@ -75,13 +76,12 @@ struct AttendSeq {
   int tok0, q, len, lim, first, n;
 };
 template <int TOK>
-__device__ __forceinline__ AttendSeq attend_seq(const AttendArgs& A, int b) {
+__device__ __forceinline__ AttendSeq attend_seq(const AttendArgs& A, int2 rows, int len) {
   const KvArgs& C = A.kv;
   AttendSeq s;
-  const int2 r = kv_rows(C, b);
-  s.tok0 = r.x;
-  s.q = r.y - r.x;
-  s.len = max(C.kv_len[b], 0);               // no position is reached by a shorter one
+  s.tok0 = rows.x;
+  s.q = rows.y - rows.x;
+  s.len = max(len, 0);                       // no position is reached by a shorter one
   s.lim = C.n_pages ? min(s.len, C.M << C.logP) : 0;
   const int lowest = s.len - s.q;
   s.first = A.window && lowest >= A.window ? (lowest - A.window + 1) / TOK : 0;
@@ -225,6 +225,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   constexpr int PIECE = Sh::PIECE;
   constexpr uint32_t ALL = (1u << KT) - 1;
   extern __shared__ __align__(16) char lds[];
+  __shared__ int2 s_rows[ATT_SEQS];
+  __shared__ int s_len[ATT_SEQS];
   const KvArgs& C = A.kv;
   const int tid = threadIdx.x, w = wave_id(), l = lane_id(), g = l >> 4, c = l & 15;
   const int P = 1 << C.logP;
@@ -244,7 +246,13 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     const int b = b0 + tid;
     uint64_t x = 0;
     if (b < C.B) {
-      const AttendSeq s = attend_seq<TOK>(A, b);
+      const int2 rows = kv_rows(C, b);
+      const int len = C.kv_len[b];
+      if (b < ATT_SEQS) {
+        s_rows[b] = rows;
+        s_len[b] = len;
+      }
+      const AttendSeq s = attend_seq<TOK>(A, rows, len);
       if (s.n > 0) {
         const uint64_t blocks = (uint64_t)C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
         x = (uint64_t)(s.n + PIECE) * blocks << RB | min(blocks, (uint64_t)4096);
@@ -302,7 +310,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     const auto& A = launch_args();
     while (s_pref[b + 1] >> RB <= u) ++b;
     b = __builtin_amdgcn_readfirstlane(b);
-    const AttendSeq s = attend_seq<TOK>(A, b);
+    const AttendSeq s = b < ATT_SEQS ? attend_seq<TOK>(A, s_rows[b], s_len[b])
+                                     : attend_seq<TOK>(A, kv_rows(A.kv, b), A.kv.kv_len[b]);
     const uint64_t before = s_pref[b], rem = scalar64(u - (before >> RB));
     const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
     const unsigned cost = s.n + PIECE;
