@@ -254,13 +254,13 @@ def _stream_ptr(device):
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def _call(torch, device, fn, *args):
-    """fn(*args, the device's current stream), with that device the current one."""
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
+def _call(torch, dev, fn, *args):
+    """fn(*args, device ``dev``'s current stream), with that device the current one."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch.cuda.current_device():
         rc = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(dev):
             rc = fn(*args, stream)
     if rc != CX_OK:
         _check(rc)
@@ -391,61 +391,67 @@ _KV_BATCH = struct.Struct("<QqQqQQ8i")
 KV_BF16, KV_E4M3 = 1, 3
 
 
-def _kv_batch(torch, cache, D, table, kv_len, q_start, T):
-    """cx_kv_batch of one layer's pages and a batch."""
-    n, heads, width = cache.shape if cache.dim() == 3 else (0, 0, 0)
-    stride = cache.stride()
-    if not heads or stride[2] != 1 or (stride[1] != width and heads > 1):
+def _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T):
+    """(cx_kv_batch of one layer's pages and a batch, its kv heads)."""
+    shape, stride, dtype = cache.shape, cache.stride(), cache.dtype
+    if len(shape) != 3 or stride[2] != 1 or (stride[1] != shape[2] and shape[1] > 1):
         raise ValueError("cache must be one layer's [n_pages, kv_heads, width] pages, each page "
                          "contiguous")
-    if cache.dtype == torch.bfloat16:          # 2 P D elements
-        dtype, (P, rest), page = KV_BF16, divmod(width, 2 * D), 2 * stride[0]
-    elif cache.dtype == torch.uint8:           # 2 P D codes and 8 P bytes of scales
-        dtype, (P, rest), page = KV_E4M3, divmod(width, 2 * D + 8), stride[0]
+    n, heads, width = shape
+    if dtype == torch.bfloat16:                # 2 P D elements
+        code, page = KV_BF16, 2 * stride[0]
+        P, rest = divmod(width, 2 * D)
+    elif dtype == torch.uint8:                 # 2 P D codes and 8 P bytes of scales
+        code, page = KV_E4M3, stride[0]
+        P, rest = divmod(width, 2 * D + 8)
     else:
         raise ValueError("cache must be bfloat16 pages, or uint8 pages of e4m3 codes and scales")
     if rest:
         raise ValueError(f"a page's width ({width}) does not fit heads of {D}")
     i32 = torch.int32
-    if table.dim() != 2 or table.dtype != i32 or kv_len.dtype != i32:
+    shape, stride = table.shape, table.stride()
+    if len(shape) != 2 or table.dtype != i32 or kv_len.dtype != i32:
         raise ValueError("table [B, pages] and kv_len [B] must be int32")
-    B, M = table.shape
+    B, M = shape
     if kv_len.shape != (B,):
         raise ValueError("table and kv_len differ in B")
-    ld, unit = table.stride()
-    if (unit != 1 and M > 1) or not kv_len.is_contiguous():
+    if (stride[1] != 1 and M > 1) or not kv_len.is_contiguous():
         raise ValueError("table and kv_len must have unit strides")
     start = 0
     if q_start is not None:
         if q_start.dtype != i32 or q_start.shape != (B + 1,) or not q_start.is_contiguous() or \
-                not q_start.is_cuda:
-            raise ValueError("q_start must be a contiguous int32 [B + 1] cuda tensor")
+                q_start.get_device() != dev:
+            raise ValueError("q_start must be a contiguous int32 [B + 1] on q's device")
         start = q_start.data_ptr()
     elif T != B:
         raise ValueError("without q_start there is one new token per sequence")
-    if not (cache.is_cuda and table.is_cuda and kv_len.is_cuda):
-        raise ValueError("cache, table and kv_len must be cuda tensors")
-    return _KV_BATCH.pack(cache.data_ptr(), page, table.data_ptr(), max(ld, M), kv_len.data_ptr(),
-                          start, n, heads, D, P, dtype, B, M, T)
+    if cache.get_device() != dev or table.get_device() != dev or kv_len.get_device() != dev:
+        raise ValueError("cache, table and kv_len must be on q's device")
+    return _KV_BATCH.pack(cache.data_ptr(), page, table.data_ptr(), max(stride[0], M),
+                          kv_len.data_ptr(), start, n, heads, D, P, code, B, M, T), heads
 
 
-def _rows3(torch, name, t, shape=None):
-    """The strides of bf16 rows [tokens, heads, D] on the GPU."""
-    if t.dim() != 3 or t.dtype != torch.bfloat16 or not t.is_cuda or \
-            (shape is not None and t.shape != shape):
-        raise ValueError(f"{name} must be a bfloat16 "
-                         f"{list(shape) if shape is not None else '[tokens, heads, D]'} cuda "
-                         "tensor")
+def _rows3(torch, name, t, dev, shape):
+    """The strides of bf16 rows [tokens, heads, D] on device ``dev``."""
     st = t.stride()
-    if st[2] != 1:
-        raise ValueError(f"{name} must have unit element stride")
+    if t.shape != shape or t.dtype != torch.bfloat16 or t.get_device() != dev or st[2] != 1:
+        raise ValueError(f"{name} must be bfloat16 {list(shape)} on q's device (a cuda device), "
+                         "with unit element stride")
     return st
 
 
-def _out3(torch, name, t, shape, device):
+def _q_rows(torch, q):
+    """(device, shape, strides) of the query rows."""
+    dev, shape = q.get_device(), q.shape
+    if dev < 0 or len(shape) != 3:
+        raise ValueError("q must be a bfloat16 [tokens, heads, D] cuda tensor")
+    return dev, shape, _rows3(torch, "q", q, dev, shape)
+
+
+def _out3(torch, name, t, q, dev, shape):
     if t is None:
-        return torch.empty(shape, dtype=torch.bfloat16, device=device)
-    _rows3(torch, name, t, shape)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    _rows3(torch, name, t, dev, shape)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t
@@ -465,28 +471,29 @@ def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, int
     [T, Hq, D]."""
     import torch
     lib = _lib or load()
-    qs = _rows3(torch, "q", q)
-    T, Hq, D = q.shape
-    kv = _kv_batch(torch, cache, D, table, kv_len, q_start, T)
-    shape = (T, cache.shape[1], D)
-    ks, vs = _rows3(torch, "k", k, shape), _rows3(torch, "v", v, shape)
+    dev, shape, qs = _q_rows(torch, q)
+    T, Hq, D = shape
+    kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T)
+    ks = _rows3(torch, "k", k, dev, (T, heads, D))
+    vs = _rows3(torch, "v", v, dev, (T, heads, D))
     rp, rows, rdim = None, 0, 0
     if rope is not None:
-        if rope.dim() != 2 or rope.dtype != torch.float32 or not rope.is_contiguous() or \
-                not rope.is_cuda:
-            raise ValueError("rope must be a contiguous float32 [positions, rotary dim] cuda "
-                             "tensor")
+        if rope.dtype != torch.float32 or rope.dim() != 2 or not rope.is_contiguous() or \
+                rope.get_device() != dev:
+            raise ValueError("rope must be a contiguous float32 [positions, rotary dim] on q's "
+                             "device")
         rp = rope.data_ptr()
         rows, rdim = rope.shape
-    norms = []
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None and (w.dtype != torch.bfloat16 or w.shape != (D,) or
-                              not w.is_contiguous() or not w.is_cuda):
-            raise ValueError(f"{name} must be a contiguous bfloat16 [D] cuda tensor")
-        norms.append(None if w is None else w.data_ptr())
-    q_out = _out3(torch, "q_out", q_out, (T, Hq, D), q.device)
-    _call(torch, q.device, lib.cx_kv_append_bf16, kv, q.data_ptr(), qs[0], qs[1], k.data_ptr(),
-          ks[0], ks[1], v.data_ptr(), vs[0], vs[1], Hq, rp, rows, rdim, interleaved, *norms, eps,
+    norms = [None, None]
+    for i, w in enumerate((q_norm, k_norm)):
+        if w is not None:
+            if w.dtype != torch.bfloat16 or w.shape != (D,) or not w.is_contiguous() or \
+                    w.get_device() != dev:
+                raise ValueError("q_norm and k_norm must be contiguous bfloat16 [D] on q's device")
+            norms[i] = w.data_ptr()
+    q_out = _out3(torch, "q_out", q_out, q, dev, shape)
+    _call(torch, dev, lib.cx_kv_append_bf16, kv, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0],
+          ks[1], v.data_ptr(), vs[0], vs[1], Hq, rp, rows, rdim, interleaved, *norms, eps,
           q_out.data_ptr())
     return q_out
 
@@ -510,13 +517,12 @@ def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, sca
     zeros."""
     import torch
     lib = _lib or load()
-    qs = _rows3(torch, "q", q)
-    T, Hq, D = q.shape
-    kv = _kv_batch(torch, cache, D, table, kv_len, q_start, T)
-    dev = q.device
-    out = _out3(torch, "out", out, (T, Hq, D), dev)
-    ws = _ws_attend.get(_attention_workspace(Hq, cache.shape[1], D, max_new), dev,
-                        torch._C._cuda_getCurrentRawStream(dev.index))
+    dev, shape, qs = _q_rows(torch, q)
+    T, Hq, D = shape
+    kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T)
+    out = _out3(torch, "out", out, q, dev, shape)
+    ws = _ws_attend.get(_attention_workspace(Hq, heads, D, max_new), q.device,
+                        torch._C._cuda_getCurrentRawStream(dev))
     _call(torch, dev, lib.cx_paged_attention_bf16, kv, q.data_ptr(), qs[0], qs[1], Hq, max_new,
           D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(), ws.data_ptr(),
           ws.numel())
@@ -530,21 +536,19 @@ def kv_copy_pages_device(cache, src, dst):
     destination of two pairs, or a destination and a source.  Returns cache."""
     import torch
     lib = _lib or load()
-    dims, st, shape = cache.dim(), cache.stride(), cache.shape
-    if dims not in (3, 4) or st[-1] != 1 or (st[-2] != shape[-1] and shape[-2] > 1):
-        raise ValueError("cache must be [layers, n_pages, kv_heads, width] or one layer of it, "
-                         "each page contiguous")
+    dev, st, shape = cache.get_device(), cache.stride(), cache.shape
+    dims = len(shape)
+    if dims not in (3, 4) or st[-1] != 1 or (st[-2] != shape[-1] and shape[-2] > 1) or dev < 0:
+        raise ValueError("cache must be a cuda tensor [layers, n_pages, kv_heads, width] or one "
+                         "layer of it, each page contiguous")
     i32 = torch.int32
-    if src.dtype != i32 or dst.dtype != i32 or src.dim() != 1 or not src.is_contiguous() or \
-            not dst.is_contiguous() or not src.is_cuda or not dst.is_cuda:
-        raise ValueError("src and dst must be contiguous int32 [n] cuda tensors")
-    if src.shape != dst.shape:
-        raise ValueError("src and dst differ in length")
-    if not cache.is_cuda:
-        raise ValueError("cache must be a cuda tensor")
+    if src.dtype != i32 or dst.dtype != i32 or src.dim() != 1 or src.shape != dst.shape or \
+            not src.is_contiguous() or not dst.is_contiguous() or src.get_device() != dev or \
+            dst.get_device() != dev:
+        raise ValueError("src and dst must be contiguous int32 [n] on cache's device")
     el = cache.element_size()
     layers, stride = (1, 0) if dims == 3 else (shape[0], st[0] * el)
-    _call(torch, cache.device, lib.cx_kv_copy_pages, cache.data_ptr(), stride, st[-3] * el,
+    _call(torch, dev, lib.cx_kv_copy_pages, cache.data_ptr(), stride, st[-3] * el,
           shape[-1] * shape[-2] * el, layers, shape[-3], src.data_ptr(), dst.data_ptr(),
           src.shape[0])
     return cache
