@@ -49,6 +49,9 @@ ATTEND = {
     "prompt": ("bf16", 4, 1, 64, 16, [150, 201], [150, 77], 0, 0.0),
     "prompt_rows": ("bf16", 24, 2, 128, 16, [50, 90], [41, 33], 0, 0.0),
     "more_new_than_tokens": ("bf16", 4, 2, 128, 16, [3, 0, 20], [5, 2, 4], 0, 0.0),
+    "rows_33_narrow": ("bf16", 11, 1, 64, 16, [70, 300], [3, 3], 0, 0.0),
+    "rows_20_narrow_e4m3": ("e4m3", 10, 2, 64, 16, [70, 300, 41], [4, 4, 1], 0, 0.0),
+    "rows_70_e4m3": ("e4m3", 14, 1, 128, 32, [90, 300], [5, 5], 64, 0.0),
 }
 
 
@@ -221,6 +224,96 @@ def test_attention_strides():
     _check(out, want, tol)
 
 
+def _attend_torch(q, k, v, pos, scale, window):
+    """R.attend for one kv head of one sequence on the GPU: q [m, D] at positions
+    pos [m], k and v [t, D], fp64."""
+    import torch
+    t = torch.arange(k.shape[0], device=k.device)
+    ok = t <= pos[:, None]
+    if window:
+        ok &= t > pos[:, None] - window
+    x = (q @ k.T.contiguous() * scale).masked_fill(~ok, -torch.inf)
+    mag = q.abs() @ k.abs().T.contiguous() * scale
+    top = x.amax(1, keepdim=True)
+    p = torch.softmax(x, 1)
+    o = p @ v
+    ds = 2 * (q.shape[1] + 64) * R.U32 * mag + 8 * R.U32 * (x.masked_fill(~ok, 0).abs() + top.abs())
+    rel = 2 * ds + (2 * ok.sum(1, keepdim=True) + 64) * R.U32 + 2.0 ** -16
+    a = (p * rel) @ v.abs() + o.abs() * (p * rel).sum(1, keepdim=True)
+    return o, a + R.U16 * 1.01 * (o.abs() + a) + 1e-38
+
+
+# the lengths spread over the shares in every way: more row blocks than workers,
+# sequences past those kept in LDS, parts joined by group, wave and workgroup
+MANY = {
+    "short_ones": ("bf16", 8, 4, 64, 16, 700, 0, 90, 1, 0),
+    "more_than_lds": ("bf16", 2, 1, 128, 16, 1300, 0, 60, 2, 0),
+    "short_e4m3": ("e4m3", 4, 2, 128, 32, 400, 0, 200, 1, 0),
+    "waves": ("bf16", 4, 2, 128, 16, 45, 800, 4000, 1, 0),
+    "waves_narrow": ("bf16", 6, 3, 64, 32, 40, 800, 4000, 1, 0),
+    "waves_wide": ("bf16", 4, 2, 256, 32, 40, 500, 3000, 1, 0),
+    "groups": ("bf16", 12, 3, 128, 16, 25, 300, 4000, 7, 0),
+    "groups_e4m3": ("e4m3", 12, 3, 128, 16, 25, 300, 4000, 7, 900),
+    "few_long": ("bf16", 8, 2, 64, 64, 3, 20000, 50000, 3, 0),
+    "one_long_e4m3": ("e4m3", 4, 1, 256, 16, 1, 30000, 30000, 1, 0),
+    "window": ("bf16", 8, 4, 128, 16, 90, 1, 6000, 3, 333),
+}
+
+
+@pytest.mark.parametrize("name", MANY)
+def test_attention_many(name):
+    import torch
+    from chenxing_amd._lib import paged_attention_device
+    print(f"[gpu] attention {name}", flush=True)
+    cache, Hq, H, D, P, B, lo, hi, most, window = MANY[name]
+    rng = np.random.default_rng(sum(map(ord, name)))
+    lens = rng.integers(lo, hi + 1, B)
+    new = np.minimum(rng.integers(1 if most == 1 else 0, most + 1, B), np.maximum(lens, 1))
+    table, kv_len, q_start, n = C.batch(rng, lens.tolist(), new.tolist(), P)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(len(name))
+    K, V = (torch.randn(n, H, P, D, generator=g, device="cuda") for _ in range(2))
+    if cache == "bf16":
+        pages = torch.cat([x.bfloat16().view(n, H, P, D // 8, 8).transpose(2, 3).reshape(n, H, -1)
+                           if i == 0 else
+                           x.bfloat16().view(n, H, P // 8, 8, D).transpose(3, 4).reshape(n, H, -1)
+                           for i, x in enumerate((K, V))], 2)
+        K, V = (x.bfloat16().double() for x in (K, V))
+    else:
+        sc = [x.abs().amax(3) / 448 for x in (K, V)]
+        code = [(x / s[..., None]).to(torch.float8_e4m3fn) for x, s in zip((K, V), sc)]
+        K, V = (c.double() * s[..., None].double() for c, s in zip(code, sc))
+        code = [c.view(torch.uint8) for c in code]
+        pages = torch.cat([code[0].view(n, H, P, D // 16, 16).transpose(2, 3).reshape(n, H, -1),
+                           code[1].view(n, H, P // 16, 16, D).transpose(3, 4).reshape(n, H, -1),
+                           torch.cat(sc, 2).view(torch.uint8)], 2)
+    T = int(q_start[-1])
+    q = (2 * torch.randn(T, Hq, D, generator=g, device="cuda")).bfloat16()
+    out = paged_attention_device(q, pages, C.to_gpu(table), C.to_gpu(kv_len),
+                                 C.to_gpu(q_start), max_new=most, window=window).double()
+    tab, G = C.to_gpu(table).long(), Hq // H
+    assert out.isfinite().all()
+    for b in range(B):
+        m, L = int(new[b]), int(lens[b])
+        if not m:
+            continue
+        rows = slice(int(q_start[b]), int(q_start[b]) + m)
+        if L == 0:
+            assert not out[rows].any()
+            continue
+        pg = tab[b, :-(-L // P)]
+        pos = torch.arange(L - m, L, device="cuda").repeat_interleave(G)
+        for h in range(H):
+            k, v = (x[pg, h].reshape(-1, D)[:L] for x in (K, V))
+            qh = q[rows, h * G:(h + 1) * G].reshape(m * G, D).double()
+            keep = pos >= 0
+            want, tol = _attend_torch(qh[keep], k, v, pos[keep], D ** -0.5, window)
+            got = out[rows, h * G:(h + 1) * G].reshape(m * G, D)
+            off = (got[keep] - want).abs()
+            assert (off <= tol).all(), (b, h, L, m, off.max())
+            assert not got[~keep].any()
+
+
 def test_attention_repeats_bit_for_bit():
     print("[gpu] attention repeats", flush=True)
     import torch
@@ -263,6 +356,15 @@ APPEND = {
     "e4m3_wide": ("e4m3", 2, 1, 256, 64, [100, 50], [61, 50], 128, False, False),
     "e4m3_narrow": ("e4m3", 3, 3, 64, 32, [100, 50], [61, 50], 64, False, True),
     "more_new_than_tokens": ("bf16", 2, 2, 64, 16, [2, 0], [5, 3], 64, False, False),
+    # neighbouring tokens of many sequences, with several chunks in a tile
+    "many_few": ("bf16", 2, 1, 64, 16, [3 + 7 * b % 40 for b in range(300)],
+                 [1 + b % 3 for b in range(300)], 64, False, True),
+    "many_some": ("bf16", 2, 1, 128, 16, [12 + 7 * b % 40 for b in range(90)],
+                  [1 + b % 12 for b in range(90)], 32, True, False),
+    "many_some_e4m3": ("e4m3", 2, 1, 128, 32, [20 + 7 * b % 40 for b in range(90)],
+                       [b % 21 for b in range(90)], 128, False, False),
+    "many_wide_e4m3": ("e4m3", 1, 1, 256, 16, [20 + 7 * b % 40 for b in range(60)],
+                       [b % 21 for b in range(60)], 256, True, True),
 }
 
 
