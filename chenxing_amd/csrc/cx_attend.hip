@@ -938,6 +938,10 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
                                                          max_new);
   if (ws_bytes < need)
     return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, need);
+  // the units and row blocks, at most, fit the share arithmetic's 38 bits
+  const double units = (double)kv->max_pages * kv->page_tokens / 32 + 8;
+  const double blocks = kv->kv_heads * ((double)kv->T * (q_heads / kv->kv_heads) / 16 + kv->B);
+  if (units * blocks >= 0x1p38) return cx::api_fail(CX_EINVAL, "too many tokens for one call");
   A.q = q; A.q_token = q_token; A.q_head = q_head;
   A.q_heads = q_heads; A.G = q_heads / kv->kv_heads;
   A.cap = softcap > 0;

@@ -76,6 +76,11 @@ def test_bad_attention_arguments(bad):
     assert _attend(_kv(), **bad) == _lib.CX_EINVAL
 
 
+def test_more_work_than_a_call_takes():
+    kv = _kv(M=1 << 22, ld=1 << 22, T=1 << 22)
+    assert _attend(kv) == _lib.CX_EINVAL and b"too many tokens" in _lib.load().cx_last_error()
+
+
 def test_attention_workspace():
     lib = _lib.load()
     need = lib.cx_paged_attention_workspace_bytes(4, 2, 128, 1)
