@@ -31,7 +31,6 @@
 
 namespace cx {
 
-constexpr float LOG2E = 1.4426950408889634f;
 constexpr int ATT_SEQS = 512;                // sequences whose rows and lengths LDS keeps
 constexpr int ATT_WAVES = 4, ATT_WG = 64 * ATT_WAVES;
 // Terms are relative to a maximum that lags by up to this, in powers of 2: they
@@ -184,6 +183,9 @@ struct AttendShape {
   static constexpr int WAVES = D * NT == 64                      ? (F8 ? 3 : 4)
                                : D * NT < 256 || (NT == 2 && !F8) ? 2
                                                                   : 1;
+  // units of the longest context that BLOCK takes: a unit's time in a wave grows
+  // with D NT (0.8 us at 128, 1.9 at 384; e4m3 twice as many tokens, 1.5 at 128)
+  static constexpr int BLOCK_UNITS = 4096 / (D * NT < 128 ? 128 : D * NT) / (F8 ? 2 : 1);
   static constexpr int OFF_SCALE = ATT_WAVES * 16 * PAD * 4;
   static constexpr int OFF_PREF = OFF_SCALE + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
   static int lds(int B) { return OFF_PREF + 8 * (B + 1); }
@@ -213,7 +215,11 @@ struct AttendPiece {
 //    all name one place.
 //  * Softmax terms enter the products as two bf16 parts (16 bits): one part's
 //    rounding would add as much error as the result's own.
-template <int D, int NT, bool F8>
+//
+// BLOCK: short tables.  A workgroup takes a row block whole, each wave a quarter of
+// its units, and the waves join through LDS: no share to find, no second launch.
+// launch_tile says when.
+template <int D, int NT, bool F8, bool BLOCK>
 __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void attend_split(AttendArgs A) {
   using Sh = AttendShape<D, NT, F8>;
   constexpr int TOK = Sh::TOK, ROWS = Sh::ROWS, E = Sh::E, PAD = Sh::PAD;
@@ -225,8 +231,9 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   constexpr int PIECE = Sh::PIECE;
   constexpr uint32_t ALL = (1u << KT) - 1;
   extern __shared__ __align__(16) char lds[];
-  __shared__ int2 s_rows[ATT_SEQS];
-  __shared__ int s_len[ATT_SEQS];
+  __shared__ int2 s_rows[BLOCK ? 1 : ATT_SEQS];
+  __shared__ int s_len[BLOCK ? 1 : ATT_SEQS];
+  __shared__ float s_ml[BLOCK ? ATT_WAVES * ROWS * 2 : 1];
   const KvArgs& C = A.kv;
   const int tid = threadIdx.x, w = wave_id(), l = lane_id(), g = l >> 4, c = l & 15;
   const int P = 1 << C.logP;
@@ -240,44 +247,46 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   // workers all the same)
   constexpr int RB = 25;
   constexpr uint64_t RB_MASK = (1u << RB) - 1;
-  if (tid == 0) s_pref[0] = 0;
   uint64_t total = 0;
-  for (int b0 = 0; b0 < C.B; b0 += ATT_WG) {
-    const int b = b0 + tid;
-    uint64_t x = 0;
-    if (b < C.B) {
-      const int2 rows = kv_rows(C, b);
-      const int len = C.kv_len[b];
-      if (b < ATT_SEQS) {
-        s_rows[b] = rows;
-        s_len[b] = len;
+  if constexpr (!BLOCK) {
+    if (tid == 0) s_pref[0] = 0;
+    for (int b0 = 0; b0 < C.B; b0 += ATT_WG) {
+      const int b = b0 + tid;
+      uint64_t x = 0;
+      if (b < C.B) {
+        const int2 rows = kv_rows(C, b);
+        const int len = C.kv_len[b];
+        if (b < ATT_SEQS) {
+          s_rows[b] = rows;
+          s_len[b] = len;
+        }
+        const AttendSeq s = attend_seq<TOK>(A, rows, len);
+        if (s.n > 0) {
+          const uint64_t blocks = (uint64_t)C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
+          x = (uint64_t)(s.n + PIECE) * blocks << RB | min(blocks, (uint64_t)4096);
+        }
       }
-      const AttendSeq s = attend_seq<TOK>(A, rows, len);
-      if (s.n > 0) {
-        const uint64_t blocks = (uint64_t)C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
-        x = (uint64_t)(s.n + PIECE) * blocks << RB | min(blocks, (uint64_t)4096);
-      }
-    }
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t y = __shfl_up(x, o);
-      if (l >= o) x += y;
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t y = __shfl_up(x, o);
+        if (l >= o) x += y;
+      }
+      if (l == 63) s_sum[w] = x;
+      __syncthreads();
+      for (int k = 0; k < w; ++k) x += s_sum[k];
+      if (b < C.B) s_pref[b + 1] = total + x;
+      __syncthreads();
+      total = s_pref[min(b0 + ATT_WG, C.B)];
     }
-    if (l == 63) s_sum[w] = x;
-    __syncthreads();
-    for (int k = 0; k < w; ++k) x += s_sum[k];
-    if (b < C.B) s_pref[b + 1] = total + x;
-    __syncthreads();
-    total = s_pref[min(b0 + ATT_WG, C.B)];
   }
   total = scalar64(total);
   const unsigned blocks_all = (unsigned)(total & RB_MASK);
   const bool by_block = blocks_all <= gridDim.x * ATT_WAVES;
   total >>= RB;
-  if (blockIdx.x == 0 && tid == 0) *A.entries = by_block ? (int)blocks_all : gridDim.x * ATT_WAVES;
+  if (!BLOCK && blockIdx.x == 0 && tid == 0) *A.entries = by_block ? (int)blocks_all : gridDim.x * ATT_WAVES;
 
   // tokens that attend to nothing
-  for (int b = blockIdx.x; b < C.B; b += gridDim.x)
+  for (int b = BLOCK ? C.B : blockIdx.x; b < C.B; b += gridDim.x)
     if (s_pref[b + 1] == s_pref[b]) {
       const int2 r = kv_rows(C, b);
       const int64_t n = (int64_t)(r.y - r.x) * A.q_heads * (D / 8);
@@ -289,15 +298,15 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   // more.  Neighbouring workers are on different CUs.
   const unsigned worker = __builtin_amdgcn_readfirstlane(blockIdx.x + gridDim.x * w);
   const uint64_t shares = min((uint64_t)gridDim.x * ATT_WAVES, (total + ATT_SHARE - 1) / ATT_SHARE);
-  if (worker >= shares) {
+  if (!BLOCK && worker >= shares) {
     if (l == 0 && !by_block) A.join[worker].last = -1;
     return;
   }
-  const uint64_t per = scalar64(total / shares), more = total - per * shares;
+  const uint64_t per = BLOCK ? 1 : scalar64(total / shares), more = total - per * shares;
   uint64_t u = worker * per + min((uint64_t)worker, more);
   const uint64_t end = u + per + (worker < more);
   int b = 0;
-  for (int hi = C.B - 1; b < hi;) {          // the last b with its units at or before u
+  for (int hi = BLOCK ? 0 : C.B - 1; b < hi;) {   // the last b with its units at or before u
     const int mid = (b + hi + 1) >> 1;
     if (s_pref[mid] >> RB <= u) b = mid;
     else hi = mid - 1;
@@ -429,15 +438,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     }
   };
 
-  AttendPiece cur = piece(), nxt;
-  if (cur.cnt == 0) {
-    if (l == 0 && !by_block) A.join[worker].last = -1;
-    return;
-  }
-  load_q(cur);
-  int ids = load_ids(cur, 0), idn = load_ids(cur, BATCH), idq = -1;
-  load_k(ids, 0, cur.unit, cur.h, true);
-  load_v();
+  AttendPiece cur, nxt;
+  int ids = -1, idn = -1, idq = -1;
   bool last = true;
   // the piece after the current one, if the share holds one
   auto follow = [&]() {
@@ -449,9 +451,43 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     if (last) nxt = cur;
     idq = load_ids(nxt, 0);
   };
-  follow();
+  int rb = BLOCK ? (int)(blockIdx.x / (unsigned)C.heads) : 0, blocks = 1;
+  do {
+  if constexpr (BLOCK) {
+    // this wave's quarter of row block rb of a sequence and kv head
+    const auto& A = launch_args();
+    const int sb = blockIdx.y;
+    const AttendSeq s = attend_seq<TOK>(A, kv_rows(A.kv, sb), A.kv.kv_len[sb]);
+    blocks = (s.q * A.G + ROWS - 1) / ROWS;
+    if (rb >= blocks) return;
+    const int quarter = (s.n + ATT_WAVES - 1) / ATT_WAVES;
+    cur.b = sb;
+    cur.h = (int)(blockIdx.x % (unsigned)A.kv.heads);
+    cur.tok0 = s.tok0;
+    cur.r0 = rb * ROWS;
+    cur.R = min(ROWS, s.q * A.G - cur.r0);
+    cur.lowest = s.len - s.q;
+    cur.lim = s.lim;
+    cur.unit = __builtin_amdgcn_readfirstlane(s.first + w * quarter);
+    cur.cnt = __builtin_amdgcn_readfirstlane(min(max(s.n - w * quarter, 0), quarter));
+    cur.slot = -1;
+  } else {
+    cur = piece();
+    if (cur.cnt == 0) {
+      if (l == 0 && !by_block) A.join[worker].last = -1;
+      return;
+    }
+  }
+  if (!BLOCK || cur.cnt > 0) {
+    load_q(cur);
+    ids = load_ids(cur, 0);
+    idn = load_ids(cur, BATCH);
+    load_k(ids, 0, cur.unit, cur.h, true);
+    load_v();
+    if (!BLOCK) follow();
+  }
   begin(cur);
-  for (int i = 0;;) {
+  if (!BLOCK || cur.cnt > 0) for (int i = 0;;) {
     const int unit = cur.unit + i, t0 = unit * TOK;
     // scores: tile y's row 4 g + j is token t0 + 16 y + 4 g + j
     f32x4 v[NT][KT];
@@ -487,14 +523,16 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     const bool turn = i + 1 == cur.cnt;
     int k = (i + 1) % BATCH;
     if (turn) {
-      ids = idq;
+      if (!BLOCK) {
+        ids = idq;
+        load_q(nxt);
+      }
       k = 0;
-      load_q(nxt);
     } else if (k == 0) {
       ids = idn;
       idn = load_ids(cur, i + 1 + BATCH);
     }
-    load_k(ids, k, turn ? nxt.unit : unit + 1, turn ? nxt.h : cur.h, !(turn && last));
+    load_k(ids, k, turn && !BLOCK ? nxt.unit : unit + 1, turn && !BLOCK ? nxt.h : cur.h, !(turn && last));
 
     // scores in powers of 2 are to2 * v
     const float to2 = A.cap ? 1.f : A.s1;
@@ -687,7 +725,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       }
       const int r = 16 * nt + c;
       const float L = groups_sum(sum[nt]);
-      if (r < cur.R) {
+      sum[nt] = L;
+      if (!BLOCK && r < cur.R) {
         if (cur.slot < 0) {
           const float f = m[nt] == -INFINITY ? 0.f : 1.f / L;
           const int row = cur.r0 + r;
@@ -708,14 +747,56 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
         }
       }
     }
-    if (last) break;
+    if (BLOCK || last) break;
     cur = nxt;
     idn = load_ids(cur, BATCH);
     follow();
     begin(cur);
     i = 0;
   }
-  if (!joined && l == 0 && !by_block) A.join[worker].last = -1;
+  if constexpr (BLOCK) {
+    // the waves' sums, in their order
+    const auto& A = launch_args();
+    CX_LDS float* const s_all = to_lds((float*)lds);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (g == 0) {
+        s_ml[2 * (w * ROWS + 16 * nt + c)] = m[nt];
+        s_ml[2 * (w * ROWS + 16 * nt + c) + 1] = sum[nt];
+      }
+      if (nt > 0) __syncthreads();
+#pragma unroll
+      for (int n = 0; n < DT; ++n) *(CX_LDS f32x4*)(s_o + c * PAD + 16 * n + 4 * g) = acc[nt][n];
+      __syncthreads();
+      for (int i = tid; i < 16 * (D / 8); i += ATT_WG) {
+        const int r = i / (D / 8), d = 8 * (i % (D / 8)), rr = 16 * nt + r;
+        if (rr >= cur.R) continue;
+        float top = -INFINITY, L = 0;
+#pragma unroll
+        for (int k = 0; k < ATT_WAVES; ++k) top = fmaxf(top, s_ml[2 * (k * ROWS + rr)]);
+        const float base = top == -INFINITY ? 0.f : top;
+        f32x4 o0 = {0, 0, 0, 0}, o1 = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < ATT_WAVES; ++k) {
+          const float f = __builtin_amdgcn_exp2f(s_ml[2 * (k * ROWS + rr)] - base);
+          const CX_LDS float* o = s_all + (k * 16 + r) * PAD + d;
+          L = fmaf(f, s_ml[2 * (k * ROWS + rr) + 1], L);
+          o0 += f * *(const CX_LDS f32x4*)o;
+          o1 += f * *(const CX_LDS f32x4*)(o + 4);
+        }
+        const float f = top == -INFINITY ? 0.f : 1.f / L;
+        const u32x4 x = {pack_bf16(o0[0] * f, o0[1] * f), pack_bf16(o0[2] * f, o0[3] * f),
+                         pack_bf16(o1[0] * f, o1[1] * f), pack_bf16(o1[2] * f, o1[3] * f)};
+        const int row = cur.r0 + rr;
+        *(u32x4*)(A.out + ((int64_t)(cur.tok0 + row / A.G) * A.q_heads + cur.h * A.G + row % A.G) * D +
+                  d) = x;
+      }
+    }
+    rb += (int)(gridDim.x / (unsigned)A.kv.heads);
+    if (rb < blocks) __syncthreads();        // the sums are read
+  }
+  } while (BLOCK && rb < blocks);
+  if (!BLOCK && !joined && l == 0 && !by_block) A.join[worker].last = -1;
 }
 
 // The parts of rows joined, in an order that goes by their number alone.
@@ -864,22 +945,41 @@ static AttendWork attend_workspace(int nt, int D, int dtype) {
 }
 
 template <int D, int NT, bool F8>
-static int launch_tile(const AttendArgs& A, hipStream_t s) {
+static int launch_tile(const AttendArgs& A, int64_t max_new, hipStream_t s) {
   using Sh = AttendShape<D, NT, F8>;
+  constexpr int ROWS = Sh::ROWS;
   static std::once_flag once;
   hipError_t err = hipSuccess;
   std::call_once(once, [&] {
-    err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8>,
+    err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, false>,
                               hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(CX_KV_MAX_BATCH));
+    if (err == hipSuccess)
+      err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, true>,
+                                hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(0));
   });
   if (err != hipSuccess) return (int)err;
   const unsigned grid = 256 * Sh::WAVES;
-  timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8>, dim3(grid), dim3(ATT_WG),
+  const int64_t span = A.window ? std::min<int64_t>(A.window + max_new, (int64_t)A.kv.M << A.kv.logP)
+                                : (int64_t)A.kv.M << A.kv.logP;
+  const int64_t tiles = ((int64_t)A.G * max_new + ROWS - 1) / ROWS;
+  const int64_t blocks = A.kv.heads * std::max(A.kv.B * tiles, (int64_t)A.kv.T * A.G / ROWS);
+  // BLOCK, where a wave's quarter of the longest context takes less than finding
+  // shares and joining them, unless workgroups would queue three deep (heads of 128,
+  // 8 kv heads, 1 and 32 requests, BLOCK and shares: 256 tokens 5.7 and 9.4, 6.3 and
+  // 13.2 us; 1024 tokens 10.4 and 11.2, 21 and 31; 2048 tokens 17 and 12, 43 and 52.
+  // 256 requests of 64 tokens: 21 and 17).  Row blocks that fill half the chip gain
+  // from twice the length; max_new is a hint only, so they are counted by T, too.
+  const int most = Sh::BLOCK_UNITS * (2 * blocks >= grid ? 2 : 1);
+  if (blocks <= 2 * grid && span <= most * Sh::TOK) {
+    timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, true>,
+                 dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds(0), s, A);
+    return (int)hipGetLastError();
+  }
+  timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, false>, dim3(grid), dim3(ATT_WG),
                (uint32_t)Sh::lds(A.kv.B), s, A);
   // row blocks at most: every sequence's last one may hold fewer rows
-  constexpr int ROWS = 16 * NT;
-  const int64_t blocks = A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B);
-  const int64_t entries = blocks < grid * ATT_WAVES ? blocks : grid * ATT_WAVES;
+  const int64_t entries = std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B),
+                                            grid * ATT_WAVES);
   if (entries * ROWS <= ATT_JOIN_ROWS)
     timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_row<D, ROWS>, dim3((unsigned)entries, ROWS),
                  dim3(256), 0, s, A);
@@ -890,15 +990,15 @@ static int launch_tile(const AttendArgs& A, hipStream_t s) {
 }
 
 template <int D>
-static int launch_attend(const AttendArgs& A, int dtype, int nt, hipStream_t s) {
+static int launch_attend(const AttendArgs& A, int dtype, int nt, int64_t max_new, hipStream_t s) {
   const bool f8 = dtype == CX_KV_E4M3;
-  if (nt == 1) return f8 ? launch_tile<D, 1, true>(A, s) : launch_tile<D, 1, false>(A, s);
+  if (nt == 1) return f8 ? launch_tile<D, 1, true>(A, max_new, s) : launch_tile<D, 1, false>(A, max_new, s);
   if constexpr (D < 256) {
-    if (nt == 2) return f8 ? launch_tile<D, 2, true>(A, s) : launch_tile<D, 2, false>(A, s);
-    if (nt == 3 && !f8) return launch_tile<D, 3, false>(A, s);
+    if (nt == 2) return f8 ? launch_tile<D, 2, true>(A, max_new, s) : launch_tile<D, 2, false>(A, max_new, s);
+    if (nt == 3 && !f8) return launch_tile<D, 3, false>(A, max_new, s);
   }
   if constexpr (D == 64)
-    if (nt == 4 && !f8) return launch_tile<D, 4, false>(A, s);
+    if (nt == 4 && !f8) return launch_tile<D, 4, false>(A, max_new, s);
   return (int)hipErrorInvalidValue;
 }
 
@@ -957,9 +1057,9 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   A.ml = (float*)((char*)workspace + lay.off_ml);
   A.part = (float*)((char*)workspace + lay.off_part);
   const hipStream_t s = (hipStream_t)stream;
-  const int e = D == 64    ? cx::launch_attend<64>(A, kv->dtype, nt, s)
-                : D == 128 ? cx::launch_attend<128>(A, kv->dtype, nt, s)
-                           : cx::launch_attend<256>(A, kv->dtype, nt, s);
+  const int e = D == 64    ? cx::launch_attend<64>(A, kv->dtype, nt, max_new, s)
+                : D == 128 ? cx::launch_attend<128>(A, kv->dtype, nt, max_new, s)
+                           : cx::launch_attend<256>(A, kv->dtype, nt, max_new, s);
   if (e != 0) return cx::api_fail(CX_EHIP, "attention launch: %s", hipGetErrorString((hipError_t)e));
   return CX_OK;
 }

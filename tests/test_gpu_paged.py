@@ -67,6 +67,12 @@ def _attend_inputs(name, seed=0):
                 window=window, softcap=cap, new=new)
 
 
+def _widen(x):
+    """A table of 4096 tokens at least: short ones are read by other means."""
+    pad = max(0, 4096 // x["P"] - x["table"].shape[1])
+    return dict(x, table=np.pad(x["table"], ((0, 0), (0, pad)), constant_values=-1))
+
+
 def _attend(x, **kw):
     import torch
     from chenxing_amd._lib import paged_attention_device
@@ -100,10 +106,25 @@ def test_attention(name):
     _check(_attend(x), *_expect(x))
 
 
+@pytest.mark.parametrize("name", ATTEND)
+def test_attention_wide_table(name):
+    print(f"[gpu] attention {name}, wide table", flush=True)
+    x = _widen(_attend_inputs(name))
+    _check(_attend(x), *_expect(x))
+
+
 @pytest.mark.parametrize("max_new", [1, 2, 8, 1000])
 def test_attention_max_new_is_a_hint(max_new):
     print(f"[gpu] attention max_new {max_new}", flush=True)
     x = _attend_inputs("verify")
+    _check(_attend(x, max_new=max_new), *_expect(x))
+
+
+@pytest.mark.parametrize("max_new", [1, 3, 20, 2 ** 28])
+def test_attention_max_new_below_the_rows(max_new):
+    """Prompts of many row blocks under a hint of one, and a hint past any length."""
+    print(f"[gpu] attention prompt rows, max_new {max_new}", flush=True)
+    x = _attend_inputs("prompt_rows")
     _check(_attend(x, max_new=max_new), *_expect(x))
 
 
@@ -129,7 +150,8 @@ def test_attention_large_scores():
 
 @pytest.mark.parametrize("cache", ["bf16", "e4m3"])
 @pytest.mark.parametrize("window", [0, 3])
-def test_attention_masked_nan_and_inf(cache, window):
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_masked_nan_and_inf(cache, window, wide):
     """NaN and inf in the newest tokens' K or V reach the rows that attend to
     them and no other row."""
     print(f"[gpu] attention masked NaN and inf, {cache}, window {window}", flush=True)
@@ -149,6 +171,8 @@ def test_attention_masked_nan_and_inf(cache, window):
     x = dict(q=f32_to_bf16_bits(rng.normal(0, 1, (sum(new), Hq, D)).astype(np.float32)),
              pages=R.pack(K, V, ks, vs), table=table, kv_len=kv_len, q_start=q_start, P=P, D=D,
              window=window, softcap=0.0, new=new)
+    if wide:
+        x = _widen(x)
     want, tol = _expect(x)
     got = _values(C.bits_of(_attend(x)))
     fine = np.isfinite(want)
@@ -158,7 +182,8 @@ def test_attention_masked_nan_and_inf(cache, window):
     assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
 
 
-def test_attention_all_scores_minus_infinity():
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_all_scores_minus_infinity(wide):
     """K of -inf under a positive q: a row without weight is NaN, as its
     formula; a row with one other token is that token."""
     print("[gpu] attention scores of -inf", flush=True)
@@ -170,6 +195,8 @@ def test_attention_all_scores_minus_infinity():
     K[table[1, 1], :, 4] = 0x3F80
     q = f32_to_bf16_bits(np.abs(rng.normal(1, .1, (2, 4, 64))).astype(np.float32) + 0.1)
     x.update(q=q, pages=R.pack(K, V), table=table, kv_len=kv_len, q_start=q_start, new=[1, 1])
+    if wide:
+        x = _widen(x)
     got = _values(C.bits_of(_attend(x)))
     assert np.isnan(got[0]).all()
     v = _values(V[table[1, 1], :, 4])
@@ -257,6 +284,11 @@ MANY = {
     "few_long": ("bf16", 8, 2, 64, 64, 3, 20000, 50000, 3, 0),
     "one_long_e4m3": ("e4m3", 4, 1, 256, 16, 1, 30000, 30000, 1, 0),
     "window": ("bf16", 8, 4, 128, 16, 90, 1, 6000, 3, 333),
+    "window_long": ("bf16", 4, 2, 128, 16, 20, 1, 9000, 4, 2345),
+    "window_many": ("bf16", 8, 4, 64, 16, 600, 0, 500, 2, 33),
+    "window_many_e4m3": ("e4m3", 2, 1, 256, 16, 700, 0, 300, 1, 70),
+    "short_table": ("bf16", 12, 3, 128, 32, 60, 0, 700, 4, 0),
+    "short_table_e4m3": ("e4m3", 6, 3, 64, 64, 130, 0, 900, 2, 0),
 }
 
 
