@@ -878,7 +878,7 @@ __global__ __launch_bounds__(256) void attend_join_row(AttendArgs A) {
   join_out<D>(A, J, S, r, 8 * lane);
 }
 
-// Many row blocks: workgroup (entry, 16 rows).  Each lane group of D / 8 lanes
+// Many row blocks: workgroup (entry, 16 or 4 rows).  Each lane group of D / 8 lanes
 // takes a row with all its parts; where there are few rows and many parts, each
 // wave takes one with its groups' shares of them (32 verify rounds, 36 rows: 6 us
 // with groups, 9 with waves; 11 requests of up to 7400 tokens, 8 rows: 20 and 9 us).
@@ -889,7 +889,7 @@ __global__ __launch_bounds__(256) void attend_join_block(AttendArgs A) {
   const AttendJoin J = const_load(A.join + blockIdx.x);
   if ((int)blockIdx.x >= count || J.last < 0) return;
   const int n = J.last - J.first + 1, d = 8 * (threadIdx.x % LANES);
-  const int r0 = 16 * blockIdx.y, end = min(J.rows, r0 + 16);
+  const int per = ROWS / gridDim.y, r0 = per * blockIdx.y, end = min(J.rows, r0 + per);
   if (n <= 8 || end - r0 > 8) {
     for (int r = r0 + threadIdx.x / LANES; r < end; r += GROUPS)
       join_out<D>(A, J, join_parts<D, ROWS, 4>(A, J, n, r, d, 0, 1), r, d);
@@ -927,9 +927,12 @@ static int workgroups(int nt, int D, int dtype) {
   return 256 * (D * nt == 64 ? (f8 ? 3 : 4) : D * nt < 256 || (nt == 2 && !f8) ? 2 : 1);
 }
 
-// Workgroups of attend_join_row at most, above attend_join_block (one request of
-// 69773 tokens, heads of 64: 9 and 97 us; 30 of 7007 tokens, 8 kv heads: 8 and 5 us).
-constexpr int ATT_JOIN_ROWS = 1024;
+// The join: a workgroup a row where one of attend_join_block's lane groups would add
+// up more than ATT_JOIN_PARTS / 512 parts (one request of 25231 tokens, 2 kv heads of
+// 128: a workgroup a row 9 us, a wave a row 19; 8 of 7489: 5 and 7; 4 of up to 25180,
+// 12 kv heads: 6 and 5); else a wave a row, unless that is many workgroups (4 rounds
+// of 13 rows over 8014 tokens, heads of 64: 6 us, 16 rows a workgroup 15).
+constexpr int64_t ATT_JOIN_PARTS = 6144, ATT_JOIN_ROWS = 8192;
 
 struct AttendWork {
   size_t off_join, off_ml, off_part, total;
@@ -980,12 +983,13 @@ static int launch_tile(const AttendArgs& A, int64_t max_new, hipStream_t s) {
   // row blocks at most: every sequence's last one may hold fewer rows
   const int64_t entries = std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B),
                                             grid * ATT_WAVES);
-  if (entries * ROWS <= ATT_JOIN_ROWS)
+  if (grid * ATT_WAVES * (int64_t)D > ATT_JOIN_PARTS * entries)
     timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_row<D, ROWS>, dim3((unsigned)entries, ROWS),
                  dim3(256), 0, s, A);
   else
-    timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_block<D, ROWS>, dim3((unsigned)entries, NT),
-                 dim3(256), 0, s, A);
+    timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_block<D, ROWS>,
+                 dim3((unsigned)entries, entries * ROWS <= ATT_JOIN_ROWS ? ROWS / 4 : NT), dim3(256), 0, s,
+                 A);
   return (int)hipGetLastError();
 }
 
