@@ -238,8 +238,10 @@ __device__ __forceinline__ void put_key(const KvArgs& C, const Row8& r, const Sl
 }
 
 // One row (token, head) of q, k or v to D / 8 lanes, every row of the call at
-// once: q heads first, then k, then v.  For few new tokens a sequence, whose rows
-// share no line of the pages.
+// once: q heads first, then k, then v.  A small call is one latency, launch and
+// loads (1 token, 48 heads of 128: 3.3 us); a row's v leaves as one element a chunk,
+// so in a large one the stores bound it (256 tokens of as many sequences 6.5 us, 256
+// prompts of 64 tokens 251 us).
 template <int D, bool F8>
 __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
   constexpr int LR = D / 8, E = F8 ? 16 : 8;
@@ -292,6 +294,9 @@ __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
 //    requested; a token's cosines and sines are read once for them.
 //  * The others: VT tokens of one head of v.  They pass through LDS, and the
 //    tokens of a chunk that are all here leave as 16 bytes a dim.
+//
+// Bound: HBM.  5 prompts of 2500 tokens, 48 heads of 128, e4m3: 217 MB in 52 us,
+// 4.2 TB/s where a copy reaches 4.75 (append_rows 125 us).
 constexpr int APPEND_HEADS = 8, APPEND_VT = 64;
 
 template <int D, bool F8>
@@ -431,7 +436,10 @@ __device__ __forceinline__ void st_copy(char* p, u32x4 v) { __builtin_nontempora
 constexpr int COPY_LOADS = 8;                // 16-byte loads of a thread, all in flight
 constexpr int COPY_PART = COPY_LOADS * 4096; // bytes a workgroup copies
 
-// Workgroup (pair, layer, part): COPY_PART bytes of the page.
+// Workgroup (pair, layer, part): COPY_PART bytes of the page.  Bound: HBM.  400
+// pages of 64 KB in 32 layers, 1.68 GB read and written: 334 us, 5.0 TB/s (plain
+// stores 343); 16 such pages, 67 MB: 7.6 us (plain stores 9.2, loads past the caches
+// 10.6).
 __global__ __launch_bounds__(256) void copy_pages(CopyArgs A) {
   const unsigned part = blockIdx.x % (unsigned)A.parts, x = blockIdx.x / (unsigned)A.parts;
   const unsigned layer = x % (unsigned)A.n_layers, pair = x / (unsigned)A.n_layers;
@@ -456,8 +464,13 @@ __global__ __launch_bounds__(256) void copy_pages(CopyArgs A) {
 template <int D, bool F8>
 static void launch_append(const AppendArgs& A, hipStream_t s) {
   const unsigned per = 256 / (D / 8), heads = A.q_heads + A.kv.heads;
-  // several new tokens a sequence share the pages' lines
-  if (A.kv.q_start && A.kv.T >= 4 * (int64_t)A.kv.B) {
+  // New tokens of a sequence share the pages' lines, which pays from 2 or 4 million
+  // elements on; below that append_tiles' three dependent reads cost more (48 heads of
+  // 128, bf16, rows and tiles: 1 sequence of 64 tokens 4.3 and 6.9 us, 32 of 9 7.6 and
+  // 7.8, 256 of 2 10.0 and 9.0, 32 of 64 27 and 12; e4m3: 32 of 16 9.4 and 10.3, 256
+  // of 4 17 and 15; heads of 64: 256 of 4 8.0 and 8.2, 256 of 9 14 and 10)
+  const int64_t work = (int64_t)A.kv.T * (heads + A.kv.heads) * D;
+  if (A.kv.q_start && A.kv.T >= 2 * (int64_t)A.kv.B && work >= (F8 ? 1 << 22 : 1 << 21)) {
     const unsigned groups = (heads + APPEND_HEADS - 1) / APPEND_HEADS;
     const unsigned qk = (A.kv.T + per - 1) / per * groups;
     const unsigned v = (A.kv.T + APPEND_VT - 1) / APPEND_VT * A.kv.heads;

@@ -400,8 +400,9 @@ APPEND = {
 }
 
 
-def _append_inputs(name):
+def _append_inputs(name, more=1):
     cache, Hq, Hkv, D, P, lens, new, r, inter, use_norm = APPEND[name]
+    Hq, Hkv = Hq * more, Hkv * more
     rng = np.random.default_rng(len(name) * 31 + sum(map(ord, name)))
     table, kv_len, q_start, n = C.batch(rng, lens, new, P)
     T = int(q_start[-1])
@@ -465,7 +466,20 @@ def _near_bf16(got_bits, want, err, where=None):
 @pytest.mark.parametrize("name", APPEND)
 def test_append(name):
     print(f"[gpu] append {name}", flush=True)
-    x = _append_inputs(name)
+    _check_append(_append_inputs(name))
+
+
+@pytest.mark.parametrize("name", [n for n, x in APPEND.items() if sum(x[6]) >= 2 * len(x[6]) and
+                                  sum(x[6]) > 10])
+def test_append_many_heads(name):
+    """4 million elements or more: large calls are written by other means."""
+    _, Hq, Hkv, D, _, _, new = APPEND[name][:7]
+    more = -(-2 ** 22 // ((Hq + 2 * Hkv) * D * sum(new)))
+    print(f"[gpu] append {name}, {more} times the heads", flush=True)
+    _check_append(_append_inputs(name, more))
+
+
+def _check_append(x):
     eps = 1e-5
     q, pages = _append(x, eps=eps)
     P, D, n = x["P"], x["D"], len(x["pages"])
