@@ -313,8 +313,11 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
  * h / (q_heads / kv_heads).  The token at position p attends to the
  * positions t <= p, t > p - window (window 0: all), with scores scale * q.k,
  * capped to softcap * tanh(score / softcap) if softcap > 0.  A token that
- * attends to nothing gets zeros.  fp32 scores, softmax and sums; out is rounded
- * once.
+ * attends to nothing gets zeros.  fp32 scores, softmax and sums, the weights
+ * with 16 bits in their products; out is rounded once.  Short tables take one
+ * launch, others two; results do not depend on timing.
+ * T is at most 2^28; calls whose row blocks times table units (16 rows, 32
+ * tokens) reach 2^38 are refused.
  *
  *  q          bf16 bits, row (token, head) at token * q_token + head * q_head
  *             elements, rows 16-byte aligned
