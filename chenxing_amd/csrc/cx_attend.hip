@@ -191,6 +191,47 @@ struct AttendShape {
   static int lds(int B) { return OFF_PREF + 8 * (B + 1); }
 };
 
+// A prompt's row blocks, in groups that span NT units of tokens: a group's n units
+// are those that its last row may attend to, NT more than those of the group before,
+// up to the most that a row's window or the sequence holds.  A sequence of one group
+// (decode, verify) has its n.  Any n that holds a row block's units is right.
+struct AttendGroups {
+  int size, count;                           // row blocks of a group, groups
+  int n0, most;                              // units of the first group, of any
+};
+template <int D, int NT, bool F8>
+__device__ __forceinline__ AttendGroups attend_groups(const AttendArgs& A, const AttendSeq& s,
+                                                      int blocks) {
+  constexpr int TOK = AttendShape<D, NT, F8>::TOK;
+  AttendGroups g;
+  g.size = A.G * (TOK / 16);
+  g.count = (blocks + g.size - 1) / g.size;
+  g.n0 = g.most = s.n;
+  const int lowest = s.len - s.q;
+  if (g.count > 1 && lowest >= 0) {
+    g.n0 = min((lowest + TOK - 1) / TOK + NT - s.first, s.n);
+    if (A.window) g.most = s.first > 0 ? g.n0 : min(s.n, A.window / TOK + NT + 3);
+    g.n0 = min(g.n0, g.most);
+  }
+  return g;
+}
+// What the row blocks of the groups before the j-th cost, / size.
+template <int D, int NT, bool F8>
+__device__ __forceinline__ uint64_t groups_before(const AttendGroups& g, int j) {
+  constexpr int PIECE = AttendShape<D, NT, F8>::PIECE;
+  const int i = min(j, (g.most - g.n0 + NT - 1) / NT);
+  return (uint64_t)i * (g.n0 + PIECE) + (uint64_t)i * (i - 1) / 2 * NT +
+         (uint64_t)(j - i) * (g.most + PIECE);
+}
+// What a head's row blocks cost.
+template <int D, int NT, bool F8>
+__device__ __forceinline__ uint64_t groups_cost(const AttendGroups& g, int blocks) {
+  const int j = g.count - 1;
+  return groups_before<D, NT, F8>(g, j) * g.size +
+         (uint64_t)(blocks - j * g.size) *
+             (min(g.n0 + NT * j, g.most) + AttendShape<D, NT, F8>::PIECE);
+}
+
 // Consecutive units of one row block in a worker's share: rows r0 .. r0 + R - 1
 // of (new token, q head of the group) of kv head h of sequence b.
 struct AttendPiece {
@@ -262,8 +303,9 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
         }
         const AttendSeq s = attend_seq<TOK>(A, rows, len);
         if (s.n > 0) {
-          const uint64_t blocks = (uint64_t)C.heads * ((s.q * A.G + ROWS - 1) / ROWS);
-          x = (uint64_t)(s.n + PIECE) * blocks << RB | min(blocks, (uint64_t)4096);
+          const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
+          x = groups_cost<D, NT, F8>(attend_groups<D, NT, F8>(A, s, blocks), blocks) * C.heads << RB |
+              min((uint64_t)C.heads * blocks, (uint64_t)4096);
         }
       }
 #pragma unroll
@@ -323,9 +365,33 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
                                      : attend_seq<TOK>(A, kv_rows(A.kv, b), A.kv.kv_len[b]);
     const uint64_t before = s_pref[b], rem = scalar64(u - (before >> RB));
     const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
-    const unsigned cost = s.n + PIECE;
-    const unsigned row = rem >> 32 ? (unsigned)(rem / cost) : (unsigned)rem / cost;
-    const int at = (int)(rem - (uint64_t)row * cost), ua = max(at - PIECE, 0);
+    const AttendGroups groups = attend_groups<D, NT, F8>(A, s, blocks);
+    int n = s.n, first = s.first;
+    unsigned row;                            // of the sequence's row blocks by head
+    int at;                                  // place in it
+    if (groups.count == 1) {
+      const unsigned cost = n + PIECE;
+      row = rem >> 32 ? (unsigned)(rem / cost) : (unsigned)rem / cost;
+      at = (int)(rem - (uint64_t)row * cost);
+    } else {
+      const uint64_t head = groups_cost<D, NT, F8>(groups, blocks);
+      const unsigned h = (unsigned)(rem / head);
+      uint64_t r = rem - h * head;
+      int j = 0;
+      for (int hi = groups.count - 1; j < hi;) {
+        const int mid = (j + hi + 1) >> 1;
+        if (groups_before<D, NT, F8>(groups, mid) * groups.size <= r) j = mid;
+        else hi = mid - 1;
+      }
+      r -= groups_before<D, NT, F8>(groups, j) * groups.size;
+      n = min(groups.n0 + NT * j, groups.most);
+      if (A.window) first = max(s.len - s.q + j * NT * TOK - A.window + 1, 0) / TOK;
+      const unsigned cost = n + PIECE, i = r >> 32 ? (unsigned)(r / cost) : (unsigned)r / cost;
+      row = h * (unsigned)blocks + j * groups.size + i;
+      at = (int)(r - (uint64_t)i * cost);
+    }
+    const unsigned cost = n + PIECE;
+    const int ua = max(at - PIECE, 0);
     const int64_t room = (int64_t)(end - u) - max(PIECE - at, 0);
     AttendPiece p;
     p.b = b;
@@ -335,17 +401,17 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     p.R = min(ROWS, s.q * A.G - p.r0);
     p.lowest = s.len - s.q;
     p.lim = s.lim;
-    p.unit = __builtin_amdgcn_readfirstlane(s.first + ua);
-    p.cnt = __builtin_amdgcn_readfirstlane((int)min((int64_t)(s.n - ua), max(room, (int64_t)0)));
-    p.slot = ua == 0 && p.cnt == s.n ? -1 : (int)(2 * worker + (ua == 0));
+    p.unit = __builtin_amdgcn_readfirstlane(first + ua);
+    p.cnt = __builtin_amdgcn_readfirstlane((int)min((int64_t)(n - ua), max(room, (int64_t)0)));
+    p.slot = ua == 0 && p.cnt == n ? -1 : (int)(2 * worker + (ua == 0));
     p.slot = __builtin_amdgcn_readfirstlane(p.slot);
-    if (ua == 0 && p.cnt > 0 && (by_block || p.cnt < s.n)) {
-      joined |= p.cnt < s.n;
+    if (ua == 0 && p.cnt > 0 && (by_block || p.cnt < n)) {
+      joined |= p.cnt < n;
       const uint64_t lastu = u - at + cost - 1, cut = more * (per + 1);
       if (l == 0) {
         AttendJoin j;
         j.first = worker;
-        j.last = p.cnt == s.n ? -1
+        j.last = p.cnt == n ? -1
                  : (int)(lastu < cut ? lastu / (per + 1) : more + (lastu - cut) / per);
         j.tok0 = p.tok0; j.row0 = p.r0; j.rows = p.R; j.head = p.h;
         j.pad[0] = j.pad[1] = 0;
@@ -460,7 +526,6 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     const AttendSeq s = attend_seq<TOK>(A, kv_rows(A.kv, sb), A.kv.kv_len[sb]);
     blocks = (s.q * A.G + ROWS - 1) / ROWS;
     if (rb >= blocks) return;
-    const int quarter = (s.n + ATT_WAVES - 1) / ATT_WAVES;
     cur.b = sb;
     cur.h = (int)(blockIdx.x % (unsigned)A.kv.heads);
     cur.tok0 = s.tok0;
@@ -468,8 +533,13 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     cur.R = min(ROWS, s.q * A.G - cur.r0);
     cur.lowest = s.len - s.q;
     cur.lim = s.lim;
-    cur.unit = __builtin_amdgcn_readfirstlane(s.first + w * quarter);
-    cur.cnt = __builtin_amdgcn_readfirstlane(min(max(s.n - w * quarter, 0), quarter));
+    // the units of its rows' windows, up to its last row
+    const int low = cur.lowest + cur.r0 / A.G, high = cur.lowest + (cur.r0 + cur.R - 1) / A.G;
+    const int first = A.window ? max(low - A.window + 1, 0) / TOK : 0;
+    const int n = max((min(s.lim, high + 1) + TOK - 1) / TOK - first, 0);
+    const int quarter = (n + ATT_WAVES - 1) / ATT_WAVES;
+    cur.unit = __builtin_amdgcn_readfirstlane(first + w * quarter);
+    cur.cnt = __builtin_amdgcn_readfirstlane(min(max(n - w * quarter, 0), quarter));
     cur.slot = -1;
   } else {
     cur = piece();

@@ -287,6 +287,12 @@ MANY = {
     "window_long": ("bf16", 4, 2, 128, 16, 20, 1, 9000, 4, 2345),
     "window_many": ("bf16", 8, 4, 64, 16, 600, 0, 500, 2, 33),
     "window_many_e4m3": ("e4m3", 2, 1, 256, 16, 700, 0, 300, 1, 70),
+    "prompts": ("bf16", 8, 2, 128, 16, 5, 300, 3500, 1700, 0),
+    "prompts_window": ("bf16", 8, 2, 128, 16, 5, 300, 3500, 1700, 500),
+    "prompts_e4m3": ("e4m3", 4, 1, 128, 32, 4, 300, 5000, 1500, 0),
+    "prompts_e4m3_window": ("e4m3", 6, 2, 64, 32, 4, 1000, 3000, 1500, 77),
+    "prompts_wide": ("bf16", 6, 2, 256, 16, 3, 1000, 4000, 900, 700),
+    "prompts_narrow": ("bf16", 14, 2, 64, 16, 3, 1000, 5000, 2000, 0),
     "short_table": ("bf16", 12, 3, 128, 32, 60, 0, 700, 4, 0),
     "short_table_e4m3": ("e4m3", 6, 3, 64, 64, 130, 0, 900, 2, 0),
 }
