@@ -1,4 +1,4 @@
-"""CPU restatement of the paged KV-cache operators in 64 bits: the checker of
+"""CPU restatement of the paged KV-cache operators in 64 bits: the oracle of
 cx_kv_append_bf16, cx_paged_attention_bf16 and cx_kv_copy_pages.  Test
 infrastructure only.
 
