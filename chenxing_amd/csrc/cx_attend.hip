@@ -53,6 +53,7 @@ struct AttendArgs {
   int cap;                    // the latter
   int window;                 // 0: none
   uint16_t* out;
+  int workers;
   int* entries;               // number of entries of join
   struct AttendJoin* join;    // [workers]
   float* ml;                  // [2 workers, ROWS, 2]: a part's maxima and sums
@@ -215,7 +216,7 @@ __device__ __forceinline__ AttendGroups attend_groups(const AttendArgs& A, const
   g.n0 = g.most = s.n;
   const int lowest = s.len - s.q;
   if (g.count > 1 && lowest >= 0) {
-    g.n0 = min((lowest + TOK - 1) / TOK + NT - s.first, s.n);
+    g.n0 = min((int)(((unsigned)lowest + TOK - 1) / TOK) + NT - s.first, s.n);
     if (A.window) g.most = s.first > 0 ? g.n0 : min(s.n, A.window / TOK + NT + 3);
     g.n0 = min(g.n0, g.most);
   }
@@ -290,8 +291,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   CX_LDS uint64_t* const s_sum = s_pref - ATT_WAVES;
 
   // units before each sequence, over its kv heads and row blocks, and below them
-  // its row blocks (those of a sequence count as at most 4096: more than the
-  // workers all the same)
+  // its row blocks (those of a sequence count as at most 4097, one more than there
+  // are workers at most)
   constexpr int RB = 25;
   constexpr uint64_t RB_MASK = (1u << RB) - 1;
   uint64_t total = 0;
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
         if (s.n > 0) {
           const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
           x = groups_cost<D, NT, F8>(attend_groups<D, NT, F8>(A, s, blocks), blocks) * C.heads << RB |
-              min((uint64_t)C.heads * blocks, (uint64_t)4096);
+              min((uint64_t)C.heads * blocks, (uint64_t)4097);
         }
       }
 #pragma unroll
@@ -935,6 +936,15 @@ __device__ __forceinline__ void join_out(const AttendArgs& A, const AttendJoin& 
   *(u32x4*)(A.out + ((int64_t)(J.tok0 + row / A.G) * A.q_heads + J.head * A.G + row % A.G) * D + d) = x;
 }
 
+// An entry in range: those of a call are, unless its lengths change while it runs,
+// when some are not written.
+template <int ROWS>
+__device__ __forceinline__ bool join_holds(const AttendArgs& A, const AttendJoin& J) {
+  return J.first >= 0 && J.last >= J.first && J.last < A.workers && J.rows <= ROWS && J.row0 >= 0 &&
+         (unsigned)J.head < (unsigned)A.kv.heads && J.tok0 >= 0 &&
+         (int64_t)J.row0 + J.rows <= (int64_t)(A.kv.T - J.tok0) * A.G;
+}
+
 // Few row blocks, so perhaps of many parts: workgroup (entry, row), the row's
 // parts over all its lane groups of D / 8 lanes.
 template <int D, int ROWS>
@@ -944,7 +954,7 @@ __global__ __launch_bounds__(256) void attend_join_row(AttendArgs A) {
   const int count = const_load(A.entries);
   const AttendJoin J = const_load(A.join + blockIdx.x);
   const int r = blockIdx.y;
-  if ((int)blockIdx.x >= count || J.last < 0 || r >= J.rows) return;
+  if ((int)blockIdx.x >= count || r >= J.rows || !join_holds<ROWS>(A, J)) return;
   const int n = J.last - J.first + 1, grp = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   JoinSum S = join_parts<D, ROWS, 8>(A, J, n, r, 8 * lane, grp, GROUPS);
   if (grp > 0) s_sum[grp][lane] = S;
@@ -963,7 +973,7 @@ __global__ __launch_bounds__(256) void attend_join_block(AttendArgs A) {
   constexpr int LANES = D / 8, GROUPS = 256 / LANES;
   const int count = const_load(A.entries);
   const AttendJoin J = const_load(A.join + blockIdx.x);
-  if ((int)blockIdx.x >= count || J.last < 0) return;
+  if ((int)blockIdx.x >= count || !join_holds<ROWS>(A, J)) return;
   const int n = J.last - J.first + 1, d = 8 * (threadIdx.x % LANES);
   const int per = ROWS / gridDim.y, r0 = per * blockIdx.y, end = min(J.rows, r0 + per);
   if (n <= 8 || end - r0 > 8) {
@@ -1024,7 +1034,7 @@ static AttendWork attend_workspace(int nt, int D, int dtype) {
 }
 
 template <int D, int NT, bool F8>
-static int launch_tile(const AttendArgs& A, int64_t max_new, hipStream_t s) {
+static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   using Sh = AttendShape<D, NT, F8>;
   constexpr int ROWS = Sh::ROWS;
   static std::once_flag once;
@@ -1038,6 +1048,7 @@ static int launch_tile(const AttendArgs& A, int64_t max_new, hipStream_t s) {
   });
   if (err != hipSuccess) return (int)err;
   const unsigned grid = 256 * Sh::WAVES;
+  A.workers = (int)grid * ATT_WAVES;
   const int64_t span = A.window ? std::min<int64_t>(A.window + max_new, (int64_t)A.kv.M << A.kv.logP)
                                 : (int64_t)A.kv.M << A.kv.logP;
   const int64_t tiles = ((int64_t)A.G * max_new + ROWS - 1) / ROWS;

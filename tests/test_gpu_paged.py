@@ -226,6 +226,20 @@ def test_attention_lengths_past_the_table():
     _check(_attend(x), *_expect(x))
 
 
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_prompts_at_the_last_positions(window, wide):
+    """Prompts whose positions end at 2^31 - 2, past their tables."""
+    print("[gpu] attention of prompts at the last positions", flush=True)
+    x = dict(_attend_inputs("prompt"), window=window)
+    x["kv_len"] = np.array([2 ** 31 - 1, 2 ** 31 - 40], np.int32)
+    x["table"] = np.where(x["table"] < 0, 0, x["table"] % len(x["pages"])).astype(np.int32)
+    x["pages"] = R.pack(*C.dense_pages(np.random.default_rng(2), len(x["pages"]), 1, 16, 64, "bf16")[:2])
+    if wide:
+        x = _widen(x)
+    _check(_attend(x), *_expect(x))
+
+
 def test_attention_strides():
     """q with odd strides, pages inside a wider pool, a table inside a wider one."""
     print("[gpu] attention strides", flush=True)
@@ -300,13 +314,25 @@ MANY = {
 
 @pytest.mark.parametrize("name", MANY)
 def test_attention_many(name):
+    print(f"[gpu] attention {name}", flush=True)
+    _check_many(name, *MANY[name])
+
+
+def test_attention_more_row_blocks_than_workers_under_a_hint_of_one():
+    """Prompts told to be single tokens, heads of 64: 4160 row blocks of 16 rows in
+    a sequence, 4096 workers."""
+    print("[gpu] attention of a prompt, max_new 1", flush=True)
+    _check_many("hint", "bf16", 64, 64, 64, 16, 1, 1030, 1030, 1030, 0, max_new=1)
+
+
+def _check_many(name, cache, Hq, H, D, P, B, lo, hi, most, window, max_new=None):
     import torch
     from chenxing_amd._lib import paged_attention_device
-    print(f"[gpu] attention {name}", flush=True)
-    cache, Hq, H, D, P, B, lo, hi, most, window = MANY[name]
     rng = np.random.default_rng(sum(map(ord, name)))
     lens = rng.integers(lo, hi + 1, B)
     new = np.minimum(rng.integers(1 if most == 1 else 0, most + 1, B), np.maximum(lens, 1))
+    if max_new:
+        new = lens
     table, kv_len, q_start, n = C.batch(rng, lens.tolist(), new.tolist(), P)
     g = torch.Generator(device="cuda")
     g.manual_seed(len(name))
@@ -328,7 +354,8 @@ def test_attention_many(name):
     T = int(q_start[-1])
     q = (2 * torch.randn(T, Hq, D, generator=g, device="cuda")).bfloat16()
     out = paged_attention_device(q, pages, C.to_gpu(table), C.to_gpu(kv_len),
-                                 C.to_gpu(q_start), max_new=most, window=window).double()
+                                 C.to_gpu(q_start), max_new=max_new or most,
+                                 window=window).double()
     tab, G = C.to_gpu(table).long(), Hq // H
     assert out.isfinite().all()
     for b in range(B):
