@@ -1001,9 +1001,12 @@ __global__ __launch_bounds__(256) void attend_join_block(AttendArgs A) {
 }
 
 // The tile, in 16 rows, for at most that many rows of a sequence that share a kv
-// head: as few row blocks as the registers allow, of one size.
+// head: as few row blocks as the registers allow, of one size.  Four tiles of heads of
+// 64 leave one wave a SIMD, three two: where four do not hold all rows, three are
+// faster (28 / 4 heads, prompts of 1024 and 4096 tokens: 29 and 228 us, with four 39
+// and 262; 32 new tokens of 2048, one request: 27 and 19).
 static int row_tiles(int64_t rows, int D, int dtype) {
-  const int most = D == 256 ? 1 : dtype == CX_KV_E4M3 ? 2 : D == 128 ? 3 : 4;
+  const int most = D == 256 ? 1 : dtype == CX_KV_E4M3 ? 2 : D == 128 || rows > 64 ? 3 : 4;
   const int64_t tiles = (rows + 15) / 16, blocks = (tiles + most - 1) / most;
   return (int)((tiles + blocks - 1) / blocks);
 }
