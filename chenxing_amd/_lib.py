@@ -226,7 +226,12 @@ class Workspace:
     streams) must not, since each call's kernels use the buffer for the
     rows' regions and statistics.  A buffer is allocated on the stream it
     serves, so replacing it with a larger one is ordered after the calls
-    already queued there."""
+    already queued there.
+
+    A call that a graph records gets a buffer of the graph's own: the replays
+    write to that address for as long as the graph lives, on whatever stream
+    it is launched, while a buffer kept here goes to the stream's other calls
+    and is let go when one of them needs more."""
 
     def __init__(self):
         self.bufs: dict = {}
@@ -234,6 +239,8 @@ class Workspace:
 
     def get(self, nbytes: int, device, stream_ptr: int):
         import torch
+        if _capturing(torch, device):
+            return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
         key = (device.index, stream_ptr)
         with self.lock:
             buf = self.bufs.get(key)
@@ -241,6 +248,14 @@ class Workspace:
                 buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
                 self.bufs[key] = buf
             return buf
+
+
+def _capturing(torch, device) -> bool:
+    """Whether device's current stream records a graph."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
 
 
 _ws_sample = Workspace()
