@@ -224,9 +224,11 @@ class Workspace:
     demand.  The library's calls on one stream run in order and can share a
     buffer; calls on different streams (or from threads using different
     streams) must not, since each call's kernels use the buffer for the
-    rows' regions and statistics.  A buffer is allocated on the stream it
-    serves, so replacing it with a larger one is ordered after the calls
-    already queued there.
+    rows' regions and statistics.  A call's kernels are launched one by one
+    without the GIL, so a thread holds the buffer (``of``) until all of them
+    are queued: another thread's call on the stream would come between.  A
+    buffer is allocated on the stream it serves, so replacing it with a larger
+    one is ordered after the calls already queued there.
 
     A call that a graph records gets a buffer of the graph's own: the replays
     write to that address for as long as the graph lives, on whatever stream
@@ -235,19 +237,25 @@ class Workspace:
 
     def __init__(self):
         self.bufs: dict = {}
-        self.lock = threading.Lock()
+        self.locks: dict = {}
+
+    def of(self, device, stream_ptr: int):
+        """The lock of the stream's buffer, to be held from ``get`` to the end of
+        the library's call."""
+        key = (device.index, stream_ptr)
+        lock = self.locks.get(key)
+        return self.locks.setdefault(key, threading.Lock()) if lock is None else lock
 
     def get(self, nbytes: int, device, stream_ptr: int):
         import torch
         if _capturing(torch, device):
             return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
         key = (device.index, stream_ptr)
-        with self.lock:
-            buf = self.bufs.get(key)
-            if buf is None or buf.numel() < nbytes:
-                buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
-                self.bufs[key] = buf
-            return buf
+        buf = self.bufs.get(key)
+        if buf is None or buf.numel() < nbytes:
+            buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
+            self.bufs[key] = buf
+        return buf
 
 
 def _capturing(torch, device) -> bool:
@@ -302,19 +310,20 @@ def sample_device(logits, prm, u, hist=None, hist_len=None, out_id=None, row_sta
     ldh = 0 if hist is None else hist.shape[1]
     nbytes = lib.cx_sample_workspace_bytes(B, V, ldh)
     sp = _stream_ptr(dev)
-    ws = _ws_sample.get(nbytes, dev, sp.value)
     fns = {torch.bfloat16: lib.cx_sample_bf16, torch.float32: lib.cx_sample_f32,
            torch.float64: lib.cx_sample_f64}
     if logits.dtype not in fns:
         raise ValueError("logits must be float32, bfloat16 or float64")
     fn = fns[logits.dtype]
-    _check(fn(_P(logits.data_ptr()), logits.stride(0), B, V,
-              _P(hist.data_ptr()) if hist is not None else None,
-              _P(hist_len.data_ptr()) if hist_len is not None else None, ldh,
-              _P(prm.data_ptr()), _P(u.data_ptr()), _P(out_id.data_ptr()),
-              _P(row_status.data_ptr()),
-              _P(out_probs.data_ptr()) if out_probs is not None else None,
-              _P(ws.data_ptr()), ws.numel(), sp))
+    with _ws_sample.of(dev, sp.value):
+        ws = _ws_sample.get(nbytes, dev, sp.value)
+        _check(fn(_P(logits.data_ptr()), logits.stride(0), B, V,
+                  _P(hist.data_ptr()) if hist is not None else None,
+                  _P(hist_len.data_ptr()) if hist_len is not None else None, ldh,
+                  _P(prm.data_ptr()), _P(u.data_ptr()), _P(out_id.data_ptr()),
+                  _P(row_status.data_ptr()),
+                  _P(out_probs.data_ptr()) if out_probs is not None else None,
+                  _P(ws.data_ptr()), ws.numel(), sp))
     return out_id, row_status
 
 
@@ -357,11 +366,12 @@ def spec_verify_device(target, draft, draft_ids, u, temperature, accepted=None, 
             for x in (accepted, next_tok, used, row_status)]
     nbytes = lib.cx_spec_verify_workspace_bytes(B, g, V)
     sp = _stream_ptr(dev)
-    ws = _ws_verify.get(nbytes, dev, sp.value)
-    _check(lib.cx_spec_verify_f32(
-        _P(target.data_ptr()), _P(draft.data_ptr()) if draft is not None else None,
-        _P(draft_ids.data_ptr()), _P(u.data_ptr()), _P(temperature.data_ptr()), B, g, V,
-        *[_P(o.data_ptr()) for o in outs], _P(ws.data_ptr()), ws.numel(), sp))
+    with _ws_verify.of(dev, sp.value):
+        ws = _ws_verify.get(nbytes, dev, sp.value)
+        _check(lib.cx_spec_verify_f32(
+            _P(target.data_ptr()), _P(draft.data_ptr()) if draft is not None else None,
+            _P(draft_ids.data_ptr()), _P(u.data_ptr()), _P(temperature.data_ptr()), B, g, V,
+            *[_P(o.data_ptr()) for o in outs], _P(ws.data_ptr()), ws.numel(), sp))
     return tuple(outs)
 
 
@@ -392,12 +402,13 @@ def lmhead_argmax_device(hidden, weight, out_id=None, out_max=None, out_logits=N
                                    not out_logits.is_contiguous()):
         raise ValueError("out_logits must be a contiguous float32 [B, V] tensor")
     sp = _stream_ptr(dev)
-    ws = _ws_head.get(lib.cx_lmhead_workspace_bytes(B, V), dev, sp.value)
-    _check(lib.cx_lmhead_argmax_bf16(
-        _P(hidden.data_ptr()), hidden.stride(0), _P(weight.data_ptr()), weight.stride(0),
-        B, D, V, _P(out_id.data_ptr()), _P(out_max.data_ptr()),
-        _P(out_logits.data_ptr()) if out_logits is not None else None,
-        _P(ws.data_ptr()), ws.numel(), sp))
+    with _ws_head.of(dev, sp.value):
+        ws = _ws_head.get(lib.cx_lmhead_workspace_bytes(B, V), dev, sp.value)
+        _check(lib.cx_lmhead_argmax_bf16(
+            _P(hidden.data_ptr()), hidden.stride(0), _P(weight.data_ptr()), weight.stride(0),
+            B, D, V, _P(out_id.data_ptr()), _P(out_max.data_ptr()),
+            _P(out_logits.data_ptr()) if out_logits is not None else None,
+            _P(ws.data_ptr()), ws.numel(), sp))
     return out_id, out_max
 
 
@@ -536,11 +547,13 @@ def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, sca
     T, Hq, D = shape
     kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T)
     out = _out3(torch, "out", out, q, dev, shape)
-    ws = _ws_attend.get(_attention_workspace(Hq, heads, D, max_new), q.device,
-                        torch._C._cuda_getCurrentRawStream(dev))
-    _call(torch, dev, lib.cx_paged_attention_bf16, kv, q.data_ptr(), qs[0], qs[1], Hq, max_new,
-          D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(), ws.data_ptr(),
-          ws.numel())
+    nbytes = _attention_workspace(Hq, heads, D, max_new)
+    device, stream = q.device, torch._C._cuda_getCurrentRawStream(dev)
+    with _ws_attend.of(device, stream):
+        ws = _ws_attend.get(nbytes, device, stream)
+        _call(torch, dev, lib.cx_paged_attention_bf16, kv, q.data_ptr(), qs[0], qs[1], Hq, max_new,
+              D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(),
+              ws.data_ptr(), ws.numel())
     return out
 
 

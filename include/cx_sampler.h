@@ -8,6 +8,10 @@
  * the "_host" variants take host memory, run on an internal stream and
  * return when the results are on the host.
  *
+ * A workspace belongs to one stream.  A call queues several kernels that pass
+ * results through it, so threads that share a stream and a workspace call one
+ * at a time; on streams and workspaces of their own they need no order.
+ *
  * Return value: 0 on success; CX_EINVAL (-1) for bad arguments, CX_EHIP (-2)
  * for a HIP runtime error, CX_ENOSPACE (-3) when the workspace is too small.
  * cx_last_error() gives a thread-local message for the last failure.

@@ -3,6 +3,7 @@ which buffer each call is given, and when)."""
 from __future__ import annotations
 
 import contextlib
+import threading
 import time
 
 import pytest
@@ -127,3 +128,47 @@ def test_a_graph_shares_no_buffer_with_later_calls(device, call, warm):
             for b in w.bufs.values()]
     assert recorded not in held
     assert recorded not in {a for a, *_ in device.calls[-2:]}
+
+
+@pytest.mark.parametrize("call", CALLS.values(), ids=CALLS)
+def test_threads_on_one_stream_take_turns(device, call):
+    """A call's kernels are launched one after the other: two calls that are
+    given one buffer do not overlap."""
+    device.seconds = 0.003
+    start = threading.Barrier(4)
+
+    def work():
+        start.wait()
+        for n in (1, 3, 2):
+            call(n)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    calls = sorted(device.calls, key=lambda c: c[2])
+    assert len(calls) == 12
+    for a, b in zip(calls, calls[1:]):
+        assert a[3] <= b[2] or a[0] != b[0]
+
+
+@pytest.mark.parametrize("call", CALLS.values(), ids=CALLS)
+def test_a_refused_call_leaves_the_buffer_to_others(device, call):
+    class Refused(Exception):
+        pass
+
+    def refuse(name):
+        def entry(*a):
+            raise Refused
+        return (lambda *a: 256) if name.endswith("workspace_bytes") else entry
+    device.calls, good = [], _lib._lib
+    _lib._lib = type("L", (), {"__getattr__": lambda self, name: refuse(name)})()
+    try:
+        with pytest.raises(Refused):
+            call(1)
+    finally:
+        _lib._lib = good
+    t = threading.Thread(target=call, args=(1,))
+    t.start()
+    t.join(10)
+    assert not t.is_alive() and len(device.calls) == 1
