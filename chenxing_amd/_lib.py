@@ -239,18 +239,16 @@ class Workspace:
         self.bufs: dict = {}
         self.locks: dict = {}
 
-    def of(self, device, stream_ptr: int):
-        """The lock of the stream's buffer, to be held from ``get`` to the end of
-        the library's call."""
-        key = (device.index, stream_ptr)
+    def of(self, key: tuple):
+        """The lock of the buffer of ``key``, a device's index and its current
+        stream, to be held from ``get`` to the end of the library's call."""
         lock = self.locks.get(key)
         return self.locks.setdefault(key, threading.Lock()) if lock is None else lock
 
-    def get(self, nbytes: int, device, stream_ptr: int):
+    def get(self, key: tuple, nbytes: int, device):
         import torch
-        if _capturing(torch, device):
+        if _capturing(torch, key[0]):
             return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-        key = (device.index, stream_ptr)
         buf = self.bufs.get(key)
         if buf is None or buf.numel() < nbytes:
             buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
@@ -258,11 +256,11 @@ class Workspace:
         return buf
 
 
-def _capturing(torch, device) -> bool:
-    """Whether device's current stream records a graph."""
-    if device.index is None or device.index == torch.cuda.current_device():
+def _capturing(torch, dev) -> bool:
+    """Whether device ``dev``'s current stream records a graph."""
+    if dev is None or dev == torch._C._cuda_getDevice():
         return torch.cuda.is_current_stream_capturing()
-    with torch.cuda.device(device):
+    with torch.cuda.device(dev):
         return torch.cuda.is_current_stream_capturing()
 
 
@@ -280,7 +278,7 @@ def _stream_ptr(device):
 def _call(torch, dev, fn, *args):
     """fn(*args, device ``dev``'s current stream), with that device the current one."""
     stream = torch._C._cuda_getCurrentRawStream(dev)
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
@@ -315,8 +313,9 @@ def sample_device(logits, prm, u, hist=None, hist_len=None, out_id=None, row_sta
     if logits.dtype not in fns:
         raise ValueError("logits must be float32, bfloat16 or float64")
     fn = fns[logits.dtype]
-    with _ws_sample.of(dev, sp.value):
-        ws = _ws_sample.get(nbytes, dev, sp.value)
+    key = dev.index, sp.value
+    with _ws_sample.of(key):
+        ws = _ws_sample.get(key, nbytes, dev)
         _check(fn(_P(logits.data_ptr()), logits.stride(0), B, V,
                   _P(hist.data_ptr()) if hist is not None else None,
                   _P(hist_len.data_ptr()) if hist_len is not None else None, ldh,
@@ -366,8 +365,9 @@ def spec_verify_device(target, draft, draft_ids, u, temperature, accepted=None, 
             for x in (accepted, next_tok, used, row_status)]
     nbytes = lib.cx_spec_verify_workspace_bytes(B, g, V)
     sp = _stream_ptr(dev)
-    with _ws_verify.of(dev, sp.value):
-        ws = _ws_verify.get(nbytes, dev, sp.value)
+    key = dev.index, sp.value
+    with _ws_verify.of(key):
+        ws = _ws_verify.get(key, nbytes, dev)
         _check(lib.cx_spec_verify_f32(
             _P(target.data_ptr()), _P(draft.data_ptr()) if draft is not None else None,
             _P(draft_ids.data_ptr()), _P(u.data_ptr()), _P(temperature.data_ptr()), B, g, V,
@@ -402,8 +402,9 @@ def lmhead_argmax_device(hidden, weight, out_id=None, out_max=None, out_logits=N
                                    not out_logits.is_contiguous()):
         raise ValueError("out_logits must be a contiguous float32 [B, V] tensor")
     sp = _stream_ptr(dev)
-    with _ws_head.of(dev, sp.value):
-        ws = _ws_head.get(lib.cx_lmhead_workspace_bytes(B, V), dev, sp.value)
+    key = dev.index, sp.value
+    with _ws_head.of(key):
+        ws = _ws_head.get(key, lib.cx_lmhead_workspace_bytes(B, V), dev)
         _check(lib.cx_lmhead_argmax_bf16(
             _P(hidden.data_ptr()), hidden.stride(0), _P(weight.data_ptr()), weight.stride(0),
             B, D, V, _P(out_id.data_ptr()), _P(out_max.data_ptr()),
@@ -468,10 +469,11 @@ def _rows3(torch, name, t, dev, shape):
 
 def _q_rows(torch, q):
     """(device, shape, strides) of the query rows."""
-    dev, shape = q.get_device(), q.shape
-    if dev < 0 or len(shape) != 3:
-        raise ValueError("q must be a bfloat16 [tokens, heads, D] cuda tensor")
-    return dev, shape, _rows3(torch, "q", q, dev, shape)
+    dev, shape, st = q.get_device(), q.shape, q.stride()
+    if dev < 0 or len(shape) != 3 or q.dtype != torch.bfloat16 or st[2] != 1:
+        raise ValueError("q must be a bfloat16 [tokens, heads, D] cuda tensor with unit element "
+                         "stride")
+    return dev, shape, st
 
 
 def _out3(torch, name, t, q, dev, shape):
@@ -548,9 +550,9 @@ def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, sca
     kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T)
     out = _out3(torch, "out", out, q, dev, shape)
     nbytes = _attention_workspace(Hq, heads, D, max_new)
-    device, stream = q.device, torch._C._cuda_getCurrentRawStream(dev)
-    with _ws_attend.of(device, stream):
-        ws = _ws_attend.get(nbytes, device, stream)
+    key = dev, torch._C._cuda_getCurrentRawStream(dev)
+    with _ws_attend.of(key):
+        ws = _ws_attend.get(key, nbytes, q.device)
         _call(torch, dev, lib.cx_paged_attention_bf16, kv, q.data_ptr(), qs[0], qs[1], Hq, max_new,
               D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(),
               ws.data_ptr(), ws.numel())

@@ -77,7 +77,7 @@ def device(monkeypatch):
     monkeypatch.setattr(_lib, "_lib", lib)
     monkeypatch.setattr(_lib, "_stream_ptr", lambda dev: _lib._P(lib.stream))
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: lib.stream, raising=False)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: lib.capturing)
     for name in ("_ws_sample", "_ws_verify", "_ws_head", "_ws_attend"):
