@@ -444,6 +444,9 @@ def _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T):
         raise ValueError("table and kv_len differ in B")
     if (stride[1] != 1 and M > 1) or not kv_len.is_contiguous():
         raise ValueError("table and kv_len must have unit strides")
+    ld = stride[0] if B > 1 else M
+    if ld < M:
+        raise ValueError("the table's rows must not overlap (an expanded table: .contiguous())")
     start = 0
     if q_start is not None:
         if q_start.dtype != i32 or q_start.shape != (B + 1,) or not q_start.is_contiguous() or \
@@ -454,7 +457,7 @@ def _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T):
         raise ValueError("without q_start there is one new token per sequence")
     if cache.get_device() != dev or table.get_device() != dev or kv_len.get_device() != dev:
         raise ValueError("cache, table and kv_len must be on q's device")
-    return _KV_BATCH.pack(cache.data_ptr(), page, table.data_ptr(), max(stride[0], M),
+    return _KV_BATCH.pack(cache.data_ptr(), page, table.data_ptr(), ld,
                           kv_len.data_ptr(), start, n, heads, D, P, code, B, M, T), heads
 
 
