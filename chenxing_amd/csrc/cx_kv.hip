@@ -191,11 +191,17 @@ __device__ __forceinline__ u32x2 encode_row(const Row8& r, float* scale) {
   float f = __uint_as_float(m) / E4M3_MAX;
   if (f == 0.f) f = 1.f;                     // a row of zeros, or of values whose scale rounds to 0
   *scale = fine ? f : __builtin_nanf("");
-  // times the scale's reciprocal: the quotient within 2 ulp
-  const float inv = fine ? 1.f / f : 0.f;
+  // The quotient x / f rounded once: times the rounded reciprocal, and what that
+  // left over times it again.  A scale too small for that (below 2^-126 it has no
+  // finite reciprocal) is taken 2^80 times as large, as is x.
+  const float by = f < 0x1p-60f ? 0x1p80f : 1.f, fs = f * by, inv = fine ? 1.f / fs : 0.f;
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = __builtin_amdgcn_fmed3f(fine ? r.x[i] * inv : 0.f, -E4M3_MAX, E4M3_MAX);
+  for (int i = 0; i < 8; ++i) {
+    const float x = fine ? r.x[i] * by : 0.f, a = x * inv;
+    const float z = fmaf(fmaf(-a, fs, x), inv, a);           // without the sign of a zero
+    y[i] = __builtin_amdgcn_fmed3f(__builtin_copysignf(z, x), -E4M3_MAX, E4M3_MAX);
+  }
   u32x2 c;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
