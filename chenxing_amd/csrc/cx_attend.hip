@@ -32,16 +32,16 @@
 #include "cx_internal.hpp"
 #include "cx_kv.hpp"
 #include "cx_sampler.h"
+#include "cx_share.hpp"
 #include "cx_timing.hpp"
 
 namespace cx {
 
 constexpr int ATT_SEQS = 512;                // sequences whose rows and lengths LDS keeps
-constexpr int ATT_WAVES = 4, ATT_WG = 64 * ATT_WAVES;
+constexpr int ATT_WG = 64 * ATT_WAVES;
 // Terms are relative to a maximum that lags by up to this, in powers of 2: they
 // reach 256 instead of 1, and the sums are rarely scaled.
 constexpr float ATT_SLACK = 8.f;
-constexpr int ATT_SHARE = 2;                 // the least share, in units
 constexpr float ATT_LOW = -3e38f;            // running maximum of a row that attends to something
 
 struct AttendArgs {
@@ -55,19 +55,9 @@ struct AttendArgs {
   uint16_t* out;
   int workers;
   int* entries;               // number of entries of join
-  struct AttendJoin* join;    // [workers]
+  AttendJoin* join;           // [workers]
   float* ml;                  // [2 workers, ROWS, 2]: a part's maxima and sums
   float* part;                // [2 workers, ROWS, D]
-};
-
-// A row block whose units lie in several workers' shares: those of workers
-// first .. last (last = -1: in one).  Written by the first; there is an entry for
-// every row block, in their order, or, where they are more than the workers, for
-// every worker.
-struct AttendJoin {
-  int first, last;
-  int tok0, row0, rows, head;
-  int pad[2];
 };
 
 // 16 bytes of a page, read once: past the caches (131072 tokens 181 -> 161 us)
@@ -75,23 +65,9 @@ __device__ __forceinline__ u32x4 ld_page(const char* p) {
   return __builtin_nontemporal_load((const u32x4*)p);
 }
 
-// A sequence: its rows among the new tokens, the length, and its units of TOK
-// tokens (those in some row's window).
-struct AttendSeq {
-  int tok0, q, len, lim, first, n;
-};
-template <int TOK>
-__device__ __forceinline__ AttendSeq attend_seq(const AttendArgs& A, int2 rows, int len) {
-  const KvArgs& C = A.kv;
-  AttendSeq s;
-  s.tok0 = rows.x;
-  s.q = rows.y - rows.x;
-  s.len = max(len, 0);                       // no position is reached by a shorter one
-  s.lim = C.n_pages ? min(s.len, C.M << C.logP) : 0;
-  const int lowest = s.len - s.q;
-  s.first = A.window && lowest >= A.window ? (lowest - A.window + 1) / TOK : 0;
-  s.n = s.q > 0 ? max((s.lim + TOK - 1) / TOK - s.first, 0) : 0;
-  return s;
+// What the split of the work needs of the call.
+__device__ __forceinline__ ShareBatch share_batch(const AttendArgs& A) {
+  return {A.G, A.kv.heads, A.window, A.kv.n_pages ? A.kv.M << A.kv.logP : 0};
 }
 
 // A value that every lane holds, in scalar registers.
@@ -180,11 +156,9 @@ template <int D, int NT, bool F8>
 struct AttendShape {
   static constexpr int TOK = F8 ? 64 : 32;   // tokens of a unit
   static constexpr int ROWS = 16 * NT;
+  using Line = AttendLine<TOK, NT>;
   static constexpr int E = F8 ? 16 : 8;      // elements of a 16-byte chunk
   static constexpr int PAD = D + 4;          // floats of a row of a wave's scratch
-  // what a row block costs beside its units, in units (64 ragged requests 99, 94
-  // and 93 us with 0, 1 and 2; 32 verify rounds 48, 42, 39 and 35 us with 0 .. 3)
-  static constexpr int PIECE = NT == 1 ? 2 : 4;
   // waves per SIMD, as many as the registers hold
   static constexpr int WAVES = D * NT == 64                      ? (F8 ? 3 : 4)
                                : D * NT < 256 || (NT == 2 && !F8) ? 2
@@ -195,56 +169,6 @@ struct AttendShape {
   static constexpr int OFF_SCALE = ATT_WAVES * 16 * PAD * 4;
   static constexpr int OFF_PREF = OFF_SCALE + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
   static int lds(int B) { return OFF_PREF + 8 * (B + 1); }
-};
-
-// A prompt's row blocks, in groups that span NT units of tokens: a group's n units
-// are those that its last row may attend to, NT more than those of the group before,
-// up to the most that a row's window or the sequence holds.  A sequence of one group
-// (decode, verify) has its n.  Any n that holds a row block's units is right.  (All
-// the sequence's units for each instead: 4096 new tokens 1015 us, not 446.)
-struct AttendGroups {
-  int size, count;                           // row blocks of a group, groups
-  int n0, most;                              // units of the first group, of any
-};
-template <int D, int NT, bool F8>
-__device__ __forceinline__ AttendGroups attend_groups(const AttendArgs& A, const AttendSeq& s,
-                                                      int blocks) {
-  constexpr int TOK = AttendShape<D, NT, F8>::TOK;
-  AttendGroups g;
-  g.size = A.G * (TOK / 16);
-  g.count = (blocks + g.size - 1) / g.size;
-  g.n0 = g.most = s.n;
-  const int lowest = s.len - s.q;
-  if (g.count > 1 && lowest >= 0) {
-    g.n0 = min((int)(((unsigned)lowest + TOK - 1) / TOK) + NT - s.first, s.n);
-    if (A.window) g.most = s.first > 0 ? g.n0 : min(s.n, A.window / TOK + NT + 3);
-    g.n0 = min(g.n0, g.most);
-  }
-  return g;
-}
-// What the row blocks of the groups before the j-th cost, / size.
-template <int D, int NT, bool F8>
-__device__ __forceinline__ uint64_t groups_before(const AttendGroups& g, int j) {
-  constexpr int PIECE = AttendShape<D, NT, F8>::PIECE;
-  const int i = min(j, (g.most - g.n0 + NT - 1) / NT);
-  return (uint64_t)i * (g.n0 + PIECE) + (uint64_t)i * (i - 1) / 2 * NT +
-         (uint64_t)(j - i) * (g.most + PIECE);
-}
-// What a head's row blocks cost.
-template <int D, int NT, bool F8>
-__device__ __forceinline__ uint64_t groups_cost(const AttendGroups& g, int blocks) {
-  const int j = g.count - 1;
-  return groups_before<D, NT, F8>(g, j) * g.size +
-         (uint64_t)(blocks - j * g.size) *
-             (min(g.n0 + NT * j, g.most) + AttendShape<D, NT, F8>::PIECE);
-}
-
-// Consecutive units of one row block in a worker's share: rows r0 .. r0 + R - 1
-// of (new token, q head of the group) of kv head h of sequence b.
-struct AttendPiece {
-  int b, h, tok0, r0, R, lowest, lim;        // lowest: position of the first new token
-  int unit, cnt;
-  int slot;                                  // of its part, -1: the whole row block
 };
 
 // The lengths are on the device, so each worker (a wave) finds its share itself:
@@ -276,7 +200,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   constexpr int QL = D / 32;                 // Q loads of 16 rows
   constexpr int DT = D / 16, KH = TOK / 32;
   constexpr int BATCH = 64 / KT;             // units whose page ids a wave holds
-  constexpr int PIECE = Sh::PIECE;
+  using Line = typename Sh::Line;
   constexpr uint32_t ALL = (1u << KT) - 1;
   extern __shared__ __align__(16) char lds[];
   __shared__ int2 s_rows[BLOCK ? 1 : ATT_SEQS];
@@ -290,12 +214,8 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::OFF_PREF));
   CX_LDS uint64_t* const s_sum = s_pref - ATT_WAVES;
 
-  // units before each sequence, over its kv heads and row blocks, and below them
-  // its row blocks (those of a sequence count as at most 4097, one more than there
-  // are workers at most)
-  constexpr int RB = 25;
-  constexpr uint64_t RB_MASK = (1u << RB) - 1;
-  uint64_t total = 0;
+  // the line before each sequence, and its whole
+  uint64_t line = 0;
   if constexpr (!BLOCK) {
     if (tid == 0) s_pref[0] = 0;
     for (int b0 = 0; b0 < C.B; b0 += ATT_WG) {
@@ -308,12 +228,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
           s_rows[b] = rows;
           s_len[b] = len;
         }
-        const AttendSeq s = attend_seq<TOK>(A, rows, len);
-        if (s.n > 0) {
-          const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
-          x = groups_cost<D, NT, F8>(attend_groups<D, NT, F8>(A, s, blocks), blocks) * C.heads << RB |
-              min((uint64_t)C.heads * blocks, (uint64_t)4097);
-        }
+        x = Line::length(share_batch(A), Line::seq(share_batch(A), rows.x, rows.y, len));
       }
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -323,16 +238,18 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       if (l == 63) s_sum[w] = x;
       __syncthreads();
       for (int k = 0; k < w; ++k) x += s_sum[k];
-      if (b < C.B) s_pref[b + 1] = total + x;
+      if (b < C.B) s_pref[b + 1] = line + x;
       __syncthreads();
-      total = s_pref[min(b0 + ATT_WG, C.B)];
+      line = s_pref[min(b0 + ATT_WG, C.B)];
     }
   }
-  total = scalar64(total);
-  const unsigned blocks_all = (unsigned)(total & RB_MASK);
-  const bool by_block = blocks_all <= gridDim.x * ATT_WAVES;
-  total >>= RB;
-  if (!BLOCK && blockIdx.x == 0 && tid == 0) *A.entries = by_block ? (int)blocks_all : gridDim.x * ATT_WAVES;
+  line = scalar64(line);
+  ShareSplit split = share_split(line, gridDim.x * ATT_WAVES);
+  split.per = scalar64(split.per);
+  split.more = scalar64(split.more);
+  const bool by_block = split.by_block;
+  if (!BLOCK && blockIdx.x == 0 && tid == 0)
+    *A.entries = by_block ? (int)line_blocks(line) : gridDim.x * ATT_WAVES;
 
   // tokens that attend to nothing
   for (int b = BLOCK ? C.B : blockIdx.x; b < C.B; b += gridDim.x)
@@ -343,90 +260,34 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       for (int64_t i = tid; i < n; i += ATT_WG) o[i] = u32x4{0, 0, 0, 0};
     }
 
-  // this worker's share of the units: ATT_SHARE at least, the first shares one
-  // more.  Neighbouring workers are on different CUs.
+  // this worker's share; neighbouring workers are on different CUs
   const unsigned worker = __builtin_amdgcn_readfirstlane(blockIdx.x + gridDim.x * w);
-  const uint64_t shares = min((uint64_t)gridDim.x * ATT_WAVES, (total + ATT_SHARE - 1) / ATT_SHARE);
-  if (!BLOCK && worker >= shares) {
+  if (!BLOCK && worker >= split.shares) {
     if (l == 0 && !by_block) A.join[worker].last = -1;
     return;
   }
-  const uint64_t per = BLOCK ? 1 : scalar64(total / shares), more = total - per * shares;
-  uint64_t u = worker * per + min((uint64_t)worker, more);
-  const uint64_t end = u + per + (worker < more);
+  uint64_t u = share_begin(split, worker);
+  const uint64_t end = u + split.per + (worker < split.more);
   int b = 0;
   for (int hi = BLOCK ? 0 : C.B - 1; b < hi;) {   // the last b with its units at or before u
     const int mid = (b + hi + 1) >> 1;
-    if (s_pref[mid] >> RB <= u) b = mid;
+    if (line_units(s_pref[mid]) <= u) b = mid;
     else hi = mid - 1;
   }
   bool joined = false;
-  // the piece that begins at u, and u past it; b: the sequence of the one before.
-  // A row block is PIECE + n long, its units at the end: a share may end before
-  // the first of them (cnt = 0)
+  // the piece that begins at u, and u past it; b: the sequence of the one before
   auto piece = [&]() {
     const auto& A = launch_args();
-    while (s_pref[b + 1] >> RB <= u) ++b;
+    while (line_units(s_pref[b + 1]) <= u) ++b;
     b = __builtin_amdgcn_readfirstlane(b);
-    const AttendSeq s = b < ATT_SEQS ? attend_seq<TOK>(A, s_rows[b], s_len[b])
-                                     : attend_seq<TOK>(A, kv_rows(A.kv, b), A.kv.kv_len[b]);
-    const uint64_t before = s_pref[b], rem = scalar64(u - (before >> RB));
-    const int blocks = (s.q * A.G + ROWS - 1) / ROWS;
-    const AttendGroups groups = attend_groups<D, NT, F8>(A, s, blocks);
-    int n = s.n, first = s.first;
-    unsigned row;                            // of the sequence's row blocks by head
-    int at;                                  // place in it
-    if (groups.count == 1) {
-      const unsigned cost = n + PIECE;
-      row = rem >> 32 ? (unsigned)(rem / cost) : (unsigned)rem / cost;
-      at = (int)(rem - (uint64_t)row * cost);
-    } else {
-      const uint64_t head = groups_cost<D, NT, F8>(groups, blocks);
-      const unsigned h = (unsigned)(rem / head);
-      uint64_t r = rem - h * head;
-      int j = 0;
-      for (int hi = groups.count - 1; j < hi;) {
-        const int mid = (j + hi + 1) >> 1;
-        if (groups_before<D, NT, F8>(groups, mid) * groups.size <= r) j = mid;
-        else hi = mid - 1;
-      }
-      r -= groups_before<D, NT, F8>(groups, j) * groups.size;
-      n = min(groups.n0 + NT * j, groups.most);
-      if (A.window) first = max(s.len - s.q + j * NT * TOK - A.window + 1, 0) / TOK;
-      const unsigned cost = n + PIECE, i = r >> 32 ? (unsigned)(r / cost) : (unsigned)r / cost;
-      row = h * (unsigned)blocks + j * groups.size + i;
-      at = (int)(r - (uint64_t)i * cost);
-    }
-    const unsigned cost = n + PIECE;
-    const int ua = max(at - PIECE, 0);
-    const int64_t room = (int64_t)(end - u) - max(PIECE - at, 0);
-    AttendPiece p;
-    p.b = b;
-    p.h = __builtin_amdgcn_readfirstlane((int)(row / (unsigned)blocks));
-    p.tok0 = s.tok0;
-    p.r0 = __builtin_amdgcn_readfirstlane((int)(row % (unsigned)blocks)) * ROWS;
-    p.R = min(ROWS, s.q * A.G - p.r0);
-    p.lowest = s.len - s.q;
-    p.lim = s.lim;
-    p.unit = __builtin_amdgcn_readfirstlane(first + ua);
-    p.cnt = __builtin_amdgcn_readfirstlane((int)min((int64_t)(n - ua), max(room, (int64_t)0)));
-    p.slot = ua == 0 && p.cnt == n ? -1 : (int)(2 * worker + (ua == 0));
-    p.slot = __builtin_amdgcn_readfirstlane(p.slot);
-    if (ua == 0 && p.cnt > 0 && (by_block || p.cnt < n)) {
-      joined |= p.cnt < n;
-      const uint64_t lastu = u - at + cost - 1, cut = more * (per + 1);
-      if (l == 0) {
-        AttendJoin j;
-        j.first = worker;
-        j.last = p.cnt == n ? -1
-                 : (int)(lastu < cut ? lastu / (per + 1) : more + (lastu - cut) / per);
-        j.tok0 = p.tok0; j.row0 = p.r0; j.rows = p.R; j.head = p.h;
-        j.pad[0] = j.pad[1] = 0;
-        A.join[by_block ? (unsigned)(before & RB_MASK) + row : worker] = j;
-      }
-    }
-    u = p.cnt > 0 ? u + max(PIECE - at, 0) + p.cnt : end;
-    return p;
+    const ShareBatch batch = share_batch(A);
+    auto from = [&](int2 rows, int len) { return Line::seq(batch, rows.x, rows.y, len); };
+    const AttendSeq s = b < ATT_SEQS ? from(s_rows[b], s_len[b]) : from(kv_rows(A.kv, b), A.kv.kv_len[b]);
+    return Line::piece(batch, s, b, s_pref[b], split, worker, end, u,
+                       [&](unsigned entry, const AttendJoin& j) {
+                         joined |= j.last >= 0;
+                         if (l == 0) A.join[entry] = j;
+                       });
   };
 
   // ids of BATCH units of a piece from its k-th: lane KT k + group
@@ -530,8 +391,9 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     // this wave's quarter of row block rb of a sequence and kv head
     const auto& A = launch_args();
     const int sb = blockIdx.y;
-    const AttendSeq s = attend_seq<TOK>(A, kv_rows(A.kv, sb), A.kv.kv_len[sb]);
-    blocks = (s.q * A.G + ROWS - 1) / ROWS;
+    const int2 rows = kv_rows(A.kv, sb);
+    const AttendSeq s = Line::seq(share_batch(A), rows.x, rows.y, A.kv.kv_len[sb]);
+    blocks = Line::row_blocks(share_batch(A), s);
     if (rb >= blocks) return;
     cur.b = sb;
     cur.h = (int)(blockIdx.x % (unsigned)A.kv.heads);
