@@ -37,7 +37,6 @@
 
 namespace cx {
 
-constexpr int ATT_SEQS = 512;                // sequences whose rows and lengths LDS keeps
 constexpr int ATT_WG = 64 * ATT_WAVES;
 // Terms are relative to a maximum that lags by up to this, in powers of 2: they
 // reach 256 instead of 1, and the sums are rarely scaled.
@@ -157,6 +156,7 @@ struct AttendShape {
   static constexpr int TOK = F8 ? 64 : 32;   // tokens of a unit
   static constexpr int ROWS = 16 * NT;
   using Line = AttendLine<TOK, NT>;
+  using Seqs = AttendSeqs<CX_LDS uint64_t*, CX_LDS int*>;
   static constexpr int E = F8 ? 16 : 8;      // elements of a 16-byte chunk
   static constexpr int PAD = D + 4;          // floats of a row of a wave's scratch
   // waves per SIMD, as many as the registers hold
@@ -167,8 +167,8 @@ struct AttendShape {
   // with D NT (0.8 us at 128, 1.9 at 384; e4m3 twice as many tokens, 1.5 at 128)
   static constexpr int BLOCK_UNITS = 4096 / (D * NT < 128 ? 128 : D * NT) / (F8 ? 2 : 1);
   static constexpr int OFF_SCALE = ATT_WAVES * 16 * PAD * 4;
-  static constexpr int OFF_PREF = OFF_SCALE + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
-  static int lds(int B) { return OFF_PREF + 8 * (B + 1); }
+  static constexpr int OFF_SEQS = OFF_SCALE + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
+  static int lds(int B, bool starts) { return OFF_SEQS + Seqs::bytes(B, starts); }
 };
 
 // The lengths are on the device, so each worker (a wave) finds its share itself:
@@ -203,32 +203,29 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   using Line = typename Sh::Line;
   constexpr uint32_t ALL = (1u << KT) - 1;
   extern __shared__ __align__(16) char lds[];
-  __shared__ int2 s_rows[BLOCK ? 1 : ATT_SEQS];
-  __shared__ int s_len[BLOCK ? 1 : ATT_SEQS];
   __shared__ float s_ml[BLOCK ? ATT_WAVES * ROWS * 2 : 1];
   const KvArgs& C = A.kv;
   const int tid = threadIdx.x, w = wave_id(), l = lane_id(), g = l >> 4, c = l & 15;
   const int P = 1 << C.logP;
   CX_LDS float* const s_o = to_lds((float*)lds) + w * (16 * PAD);
   CX_LDS float* const s_scale = to_lds((float*)(lds + Sh::OFF_SCALE)) + w * 128;
-  CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::OFF_PREF));
+  CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::OFF_SEQS));
   CX_LDS uint64_t* const s_sum = s_pref - ATT_WAVES;
+  CX_LDS int* const s_len = (CX_LDS int*)(s_pref + C.B + 1);
+  const typename Sh::Seqs seqs = {s_pref, s_len, s_len + C.B, C.q_start != nullptr};
 
   // the line before each sequence, and its whole
   uint64_t line = 0;
   if constexpr (!BLOCK) {
     if (tid == 0) s_pref[0] = 0;
+    seqs.read(C.kv_len, C.q_start, C.B, C.T, tid, ATT_WG);
+    __syncthreads();
     for (int b0 = 0; b0 < C.B; b0 += ATT_WG) {
       const int b = b0 + tid;
       uint64_t x = 0;
       if (b < C.B) {
-        const int2 rows = kv_rows(C, b);
-        const int len = C.kv_len[b];
-        if (b < ATT_SEQS) {
-          s_rows[b] = rows;
-          s_len[b] = len;
-        }
-        x = Line::length(share_batch(A), Line::seq(share_batch(A), rows.x, rows.y, len));
+        const ShareBatch batch = share_batch(A);
+        x = Line::length(batch, Line::seq(batch, seqs.first(b), seqs.end(b), s_len[b]));
       }
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -254,9 +251,9 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   // tokens that attend to nothing
   for (int b = BLOCK ? C.B : blockIdx.x; b < C.B; b += gridDim.x)
     if (s_pref[b + 1] == s_pref[b]) {
-      const int2 r = kv_rows(C, b);
-      const int64_t n = (int64_t)(r.y - r.x) * A.q_heads * (D / 8);
-      u32x4* o = (u32x4*)(A.out + (int64_t)r.x * A.q_heads * D);
+      const int r0 = seqs.first(b);
+      const int64_t n = (int64_t)(seqs.end(b) - r0) * A.q_heads * (D / 8);
+      u32x4* o = (u32x4*)(A.out + (int64_t)r0 * A.q_heads * D);
       for (int64_t i = tid; i < n; i += ATT_WG) o[i] = u32x4{0, 0, 0, 0};
     }
 
@@ -281,8 +278,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     while (line_units(s_pref[b + 1]) <= u) ++b;
     b = __builtin_amdgcn_readfirstlane(b);
     const ShareBatch batch = share_batch(A);
-    auto from = [&](int2 rows, int len) { return Line::seq(batch, rows.x, rows.y, len); };
-    const AttendSeq s = b < ATT_SEQS ? from(s_rows[b], s_len[b]) : from(kv_rows(A.kv, b), A.kv.kv_len[b]);
+    const AttendSeq s = Line::seq(batch, seqs.first(b), seqs.end(b), s_len[b]);
     return Line::piece(batch, s, b, s_pref[b], split, worker, end, u,
                        [&](unsigned entry, const AttendJoin& j) {
                          joined |= j.last >= 0;
@@ -906,10 +902,10 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   hipError_t err = hipSuccess;
   std::call_once(once, [&] {
     err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, false>,
-                              hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(CX_KV_MAX_BATCH));
+                              hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(CX_KV_MAX_BATCH, true));
     if (err == hipSuccess)
       err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, true>,
-                                hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(0));
+                                hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(0, false));
   });
   if (err != hipSuccess) return (int)err;
   const unsigned grid = 256 * Sh::WAVES;
@@ -927,11 +923,11 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   const int most = Sh::BLOCK_UNITS * (2 * blocks >= grid ? 2 : 1);
   if (blocks <= 2 * grid && span <= most * Sh::TOK) {
     timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, true>,
-                 dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds(0), s, A);
+                 dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds(0, false), s, A);
     return (int)hipGetLastError();
   }
   timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, false>, dim3(grid), dim3(ATT_WG),
-               (uint32_t)Sh::lds(A.kv.B), s, A);
+               (uint32_t)Sh::lds(A.kv.B, A.kv.q_start != nullptr), s, A);
   // row blocks at most: every sequence's last one may hold fewer rows
   const int64_t entries = std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B),
                                             grid * ATT_WAVES);

@@ -94,6 +94,34 @@ __device__ __forceinline__ int share_of(const ShareSplit& s, uint64_t u) {
   return (int)(u < cut ? u / (s.per + 1) : s.more + (u - cut) / s.per);
 }
 
+// The sequences as one workgroup sees them.  They are read once: the lengths may
+// change while the call runs (a graph's next inputs written too early), and a piece
+// is in range only by the values that made its place on the line.
+template <class Word, class Int>
+struct AttendSeqs {
+  Word line;                  // [B + 1] the line before each sequence
+  Int len;                    // [B]
+  Int start;                  // [B + 1] first rows; starts = false: one row each
+  bool starts;
+
+  // Bytes of the three, in this order.
+  static constexpr int bytes(int B, bool starts) {
+    return 8 * (B + 1) + 4 * B + (starts ? 4 * (B + 1) : 0);
+  }
+  // Thread tid's part of lengths and first rows, whatever q_start holds.
+  __device__ __forceinline__ void read(const int32_t* kv_len, const int32_t* q_start, int B, int T,
+                                       int tid, int threads) const {
+    for (int b = tid; b <= B; b += threads) {
+      if (b < B) len[b] = kv_len[b];
+      if (starts) start[b] = min(max(q_start[b], 0), T);
+    }
+  }
+  __device__ __forceinline__ int first(int b) const { return starts ? (int)start[b] : b; }
+  __device__ __forceinline__ int end(int b) const {
+    return starts ? max((int)start[b + 1], (int)start[b]) : b + 1;
+  }
+};
+
 template <int TOK, int NT>
 struct AttendLine {
   static constexpr int ROWS = 16 * NT;
@@ -161,7 +189,8 @@ struct AttendLine {
                                                       Enter enter) {
     AttendPiece p;
     uint64_t rem = u - line_units(line);
-    rem = (uint64_t)(uint32_t)CX_UNIFORM((int)rem) | (uint64_t)(uint32_t)CX_UNIFORM((int)(rem >> 32)) << 32;
+    rem = (uint64_t)(uint32_t)CX_UNIFORM((int)rem) |
+          (uint64_t)(uint32_t)CX_UNIFORM((int)(rem >> 32)) << 32;
     const int blocks = row_blocks(A, s);
     const AttendGroups g = groups(A, s, blocks);
     int n = s.n, first = s.first;

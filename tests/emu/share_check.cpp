@@ -1,7 +1,8 @@
 // The split of attention batches over workers (cx_share.hpp), as attend_split
 // walks it, on random batches: every unit that a row block's rows may attend to is
 // in exactly one piece, in order; the parts of a cut row block are those of
-// consecutive workers, and one join entry in range names them.
+// consecutive workers, and one join entry in range names them.  The lengths and first
+// rows in "device memory" change as soon as the workgroup has read them.
 #define CX_UNIFORM(x) (x)
 #include "cx_share.hpp"
 
@@ -40,11 +41,23 @@ template <int TOK, int NT>
 static bool check(const Batch& x) {
   using Line = AttendLine<TOK, NT>;
   const int B = (int)x.len.size();
-  std::vector<uint64_t> pref(B + 1, 0);
+  std::vector<int> kv_len = x.len, q_start = x.start;
+  bool starts = rng() % 2;
+  for (int b = 0; b <= B; ++b) starts |= x.start[b] != b;
+  std::vector<uint64_t> store(AttendSeqs<uint64_t*, int*>::bytes(B, starts) / 8 + 1);
+  uint64_t* const pref = store.data();
+  int* const len = (int*)(pref + B + 1);
+  const AttendSeqs<uint64_t*, int*> at = {pref, len, len + B, starts};
+  for (int tid = 0; tid < 256; ++tid)
+    at.read(kv_len.data(), starts ? q_start.data() : nullptr, B, x.start.back(), tid, 256);
+  for (int& n : kv_len) n = (int)rng();
+  for (int& n : q_start) n = (int)rng();
+  auto seq = [&](int b) { return Line::seq(x.A, at.first(b), at.end(b), at.len[b]); };
   std::vector<AttendSeq> seqs(B);
+  pref[0] = 0;
   for (int b = 0; b < B; ++b) {
     seqs[b] = Line::seq(x.A, x.start[b], x.start[b + 1], x.len[b]);
-    pref[b + 1] = pref[b] + Line::length(x.A, seqs[b]);
+    pref[b + 1] = pref[b] + Line::length(x.A, seq(b));
   }
   const uint64_t line = pref[B];
   const ShareSplit split = share_split(line, x.workers);
@@ -71,7 +84,7 @@ static bool check(const Batch& x) {
       CHECK(b < B, "sequence %d", b);
       const uint64_t u0 = u;
       bool fine = true;
-      const AttendPiece p = Line::piece(x.A, seqs[b], b, pref[b], split, w, end, u,
+      const AttendPiece p = Line::piece(x.A, seq(b), b, pref[b], split, w, end, u,
                                         [&](unsigned entry, const AttendJoin& j) {
         fine = entry < entries && !written[entry];
         if (!fine) return;
