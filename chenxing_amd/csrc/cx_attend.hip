@@ -158,7 +158,10 @@ struct AttendShape {
   using Line = AttendLine<TOK, NT>;
   using Seqs = AttendSeqs<CX_LDS uint64_t*, CX_LDS int*>;
   static constexpr int E = F8 ? 16 : 8;      // elements of a 16-byte chunk
-  static constexpr int PAD = D + 4;          // floats of a row of a wave's scratch
+  // A wave's scratch: its 16 rows, whole where the waves join their sums (BLOCK),
+  // else a quarter of their dims at a time.
+  static constexpr int PAD = D + 4, FIX = D / 4, FPAD = FIX + 4;   // floats of a row
+  static constexpr int scratch(bool block) { return 16 * (block ? PAD : FPAD); }
   // waves per SIMD, as many as the registers hold
   static constexpr int WAVES = D * NT == 64                      ? (F8 ? 3 : 4)
                                : D * NT < 256 || (NT == 2 && !F8) ? 2
@@ -166,9 +169,12 @@ struct AttendShape {
   // units of the longest context that BLOCK takes: a unit's time in a wave grows
   // with D NT (0.8 us at 128, 1.9 at 384; e4m3 twice as many tokens, 1.5 at 128)
   static constexpr int BLOCK_UNITS = 4096 / (D * NT < 128 ? 128 : D * NT) / (F8 ? 2 : 1);
-  static constexpr int OFF_SCALE = ATT_WAVES * 16 * PAD * 4;
-  static constexpr int OFF_SEQS = OFF_SCALE + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
-  static int lds(int B, bool starts) { return OFF_SEQS + Seqs::bytes(B, starts); }
+  static constexpr int off_scale(bool block) { return ATT_WAVES * scratch(block) * 4; }
+  static constexpr int off_seqs(bool block) {
+    return off_scale(block) + (F8 ? ATT_WAVES * 512 : 0) + ATT_WAVES * 8;
+  }
+  static int lds_shares(int B, bool starts) { return off_seqs(false) + Seqs::bytes(B, starts); }
+  static int lds_block() { return off_seqs(true); }
 };
 
 // The lengths are on the device, so each worker (a wave) finds its share itself:
@@ -207,9 +213,9 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
   const KvArgs& C = A.kv;
   const int tid = threadIdx.x, w = wave_id(), l = lane_id(), g = l >> 4, c = l & 15;
   const int P = 1 << C.logP;
-  CX_LDS float* const s_o = to_lds((float*)lds) + w * (16 * PAD);
-  CX_LDS float* const s_scale = to_lds((float*)(lds + Sh::OFF_SCALE)) + w * 128;
-  CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::OFF_SEQS));
+  CX_LDS float* const s_o = to_lds((float*)lds) + w * Sh::scratch(BLOCK);
+  CX_LDS float* const s_scale = to_lds((float*)(lds + Sh::off_scale(BLOCK))) + w * 128;
+  CX_LDS uint64_t* const s_pref = to_lds((uint64_t*)(lds + Sh::off_seqs(BLOCK)));
   CX_LDS uint64_t* const s_sum = s_pref - ATT_WAVES;
   CX_LDS int* const s_len = (CX_LDS int*)(s_pref + C.B + 1);
   const typename Sh::Seqs seqs = {s_pref, s_len, s_len + C.B, C.q_start != nullptr};
@@ -634,29 +640,32 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     for (int nt = 0; nt < NT; ++nt) {
       if (again) {
         // each row's own NaN and infinite values (their terms' size does not
-        // matter), token by token
+        // matter), token by token, FIX dims of all 16 rows at a time
+        constexpr int FIX = Sh::FIX, FPAD = Sh::FPAD, NQ = FIX / 16;
+        const int fd = l % FIX;
 #pragma unroll
-        for (int n = 0; n < DT; ++n)
-          *(CX_LDS f32x4*)(s_o + c * PAD + 16 * n + 4 * g) = acc[nt][n];
-        asm volatile("" ::: "memory");
-        for (int t = cur.unit * TOK; t < (cur.unit + cur.cnt) * TOK && t < cur.lim; ++t) {
-          const int id = C.table[cur.b * C.ld_table + (t >> C.logP)], o = t & (P - 1);
-          if ((unsigned)id >= (unsigned)C.n_pages) continue;
-          for (int d = l; d < D; d += 64) {
+        for (int x = 0; x < 4; ++x) {
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+            *(CX_LDS f32x4*)(s_o + c * FPAD + 16 * n + 4 * g) = acc[nt][NQ * x + n];
+          asm volatile("" ::: "memory");
+          for (int t = cur.unit * TOK; t < (cur.unit + cur.cnt) * TOK && t < cur.lim; ++t) {
+            const int id = C.table[cur.b * C.ld_table + (t >> C.logP)], o = t & (P - 1);
+            if ((unsigned)id >= (unsigned)C.n_pages) continue;
             const char* p = C.pages + id * C.page_stride + (int64_t)cur.h * C.head_bytes +
-                            v_chunk<E, D>(d, o, C.logP) + o % E * (16 / E);
-            const float x = F8 ? e4m3_value(*(const uint8_t*)p) : bf16_lo(*(const uint16_t*)p);
-            if (fabsf(x) < INFINITY) continue;
-            for (int r = 0; r < 16; ++r) {
+                            v_chunk<E, D>(FIX * x + fd, o, C.logP) + o % E * (16 / E);
+            const float v = F8 ? e4m3_value(*(const uint8_t*)p) : bf16_lo(*(const uint16_t*)p);
+            if (fabsf(v) < INFINITY) continue;
+            for (int r = l / FIX; r < 16; r += 64 / FIX) {
               const int at = cur.lowest + (cur.r0 + min(16 * nt + r, cur.R - 1)) / A.G;
-              if (t <= at && !(A.window && t <= at - A.window)) s_o[r * PAD + d] += x;
+              if (t <= at && !(A.window && t <= at - A.window)) s_o[r * FPAD + fd] += v;
             }
           }
-        }
-        asm volatile("" ::: "memory");
+          asm volatile("" ::: "memory");
 #pragma unroll
-        for (int n = 0; n < DT; ++n)
-          acc[nt][n] = *(const CX_LDS f32x4*)(s_o + c * PAD + 16 * n + 4 * g);
+          for (int n = 0; n < NQ; ++n)
+            acc[nt][NQ * x + n] = *(const CX_LDS f32x4*)(s_o + c * FPAD + 16 * n + 4 * g);
+        }
       }
       const int r = 16 * nt + c;
       const float L = groups_sum(sum[nt]);
@@ -902,10 +911,10 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   hipError_t err = hipSuccess;
   std::call_once(once, [&] {
     err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, false>,
-                              hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(CX_KV_MAX_BATCH, true));
+                              hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds_shares(CX_KV_MAX_BATCH, true));
     if (err == hipSuccess)
       err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, true>,
-                                hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds(0, false));
+                                hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds_block());
   });
   if (err != hipSuccess) return (int)err;
   const unsigned grid = 256 * Sh::WAVES;
@@ -923,11 +932,11 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   const int most = Sh::BLOCK_UNITS * (2 * blocks >= grid ? 2 : 1);
   if (blocks <= 2 * grid && span <= most * Sh::TOK) {
     timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, true>,
-                 dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds(0, false), s, A);
+                 dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds_block(), s, A);
     return (int)hipGetLastError();
   }
   timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, false>, dim3(grid), dim3(ATT_WG),
-               (uint32_t)Sh::lds(A.kv.B, A.kv.q_start != nullptr), s, A);
+               (uint32_t)Sh::lds_shares(A.kv.B, A.kv.q_start != nullptr), s, A);
   // row blocks at most: every sequence's last one may hold fewer rows
   const int64_t entries = std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B),
                                             grid * ATT_WAVES);
