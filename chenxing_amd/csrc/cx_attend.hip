@@ -871,7 +871,7 @@ __global__ __launch_bounds__(256) void attend_join_block(AttendArgs A) {
 // head: as few row blocks as the registers allow, of one size.  Four tiles of heads of
 // 64 leave one wave a SIMD, three two: where four do not hold all rows, three are
 // faster (28 / 4 heads, prompts of 1024 and 4096 tokens: 29 and 228 us, with four 39
-// and 262; 32 new tokens of 2048, one request: 27 and 19).
+// and 262; 32 new tokens of 2048, one request: 19 and 20).
 static int row_tiles(int64_t rows, int D, int dtype) {
   const int most = D == 256 ? 1 : dtype == CX_KV_E4M3 ? 2 : D == 128 || rows > 64 ? 3 : 4;
   const int64_t tiles = (rows + 15) / 16, blocks = (tiles + most - 1) / most;
@@ -883,12 +883,14 @@ static int workgroups(int nt, int D, int dtype) {
   return 256 * (D * nt == 64 ? (f8 ? 3 : 4) : D * nt < 256 || (nt == 2 && !f8) ? 2 : 1);
 }
 
-// The join: a workgroup a row where one of attend_join_block's lane groups would add
-// up more than ATT_JOIN_PARTS / 512 parts (one request of 25231 tokens, 2 kv heads of
-// 128: a workgroup a row 9 us, a wave a row 19; 8 of 7489: 5 and 7; 4 of up to 25180,
-// 12 kv heads: 6 and 5); else a wave a row, unless that is many workgroups (4 rounds
-// of 13 rows over 8014 tokens, heads of 64: 6 us, 16 rows a workgroup 15).
-constexpr int64_t ATT_JOIN_PARTS = 6144, ATT_JOIN_ROWS = 8192;
+// The join: a workgroup a row where a row block may have more than ATT_JOIN_PARTS / D
+// parts, as many as its share of the workers or as the longest context's units make
+// (a workgroup a row and a wave a row, heads of 64: 2 new tokens of 30000, one request
+// of 4 kv heads, 9 and 14 us; 32 of 3000: 12 and 5; 8 requests of 2500: 9 and 5; heads
+// of 128: one of 8000, 8 kv heads, 5 and 8; 32 new of 30000: 8 and 7); else a wave a
+// row, unless that is many workgroups (4 rounds of 13 rows over 8014 tokens, heads of
+// 64: 6 us, 16 rows a workgroup 15).
+constexpr int64_t ATT_JOIN_PARTS = 8192, ATT_JOIN_ROWS = 8192;
 
 struct AttendWork {
   size_t off_join, off_ml, off_part, total;
@@ -940,7 +942,9 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   // row blocks at most: every sequence's last one may hold fewer rows
   const int64_t entries = std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B),
                                             grid * ATT_WAVES);
-  if (grid * ATT_WAVES * (int64_t)D > ATT_JOIN_PARTS * entries)
+  const int64_t parts = std::min<int64_t>(
+      grid * ATT_WAVES / entries, ((span + Sh::TOK - 1) / Sh::TOK + Sh::Line::PIECE) / ATT_SHARE + 1);
+  if (parts * D > ATT_JOIN_PARTS)
     timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_row<D, ROWS>, dim3((unsigned)entries, ROWS),
                  dim3(256), 0, s, A);
   else
