@@ -868,14 +868,29 @@ __global__ __launch_bounds__(256) void attend_join_block(AttendArgs A) {
 }
 
 // The tile, in 16 rows, for at most that many rows of a sequence that share a kv
-// head: as few row blocks as the registers allow, of one size.  Four tiles of heads of
-// 64 leave one wave a SIMD, three two: where four do not hold all rows, three are
-// faster (28 / 4 heads, prompts of 1024 and 4096 tokens: 29 and 228 us, with four 39
-// and 262; 32 new tokens of 2048, one request: 19 and 20).
-static int row_tiles(int64_t rows, int D, int dtype) {
-  const int most = D == 256 ? 1 : dtype == CX_KV_E4M3 ? 2 : D == 128 || rows > 64 ? 3 : 4;
+// head: as few row blocks as the registers allow, of one size.
+static int row_tiles(int64_t rows, int most) {
   const int64_t tiles = (rows + 15) / 16, blocks = (tiles + most - 1) / most;
   return (int)((tiles + blocks - 1) / blocks);
+}
+// Four tiles of heads of 64 leave one wave a SIMD, three two: where four do not hold
+// all rows, three are faster or no slower (28 / 4 heads, prompts of 1024 and 4096
+// tokens: 29 and 228 us, with four 39 and 262; 32 new tokens of 2048, one request: 19
+// and 20; 64 requests of 20 new of 2048, 16 / 2 heads: 58 and 68).  But where three
+// fill at least an eighth more rows than four, calls that have many units are faster
+// with four (64 requests of 32 new tokens of 512, 32 / 8 heads: 47 us, with three 61;
+// of 8192: 506 and 557; 16 requests of 64 new of 512: 30 and 26).  head_units: the
+// units that one row block of each sequence and kv head may have, all together.
+constexpr int64_t ATT_FOUR_UNITS = 24576;
+static int attend_tiles(int64_t rows, int D, int dtype, int64_t head_units) {
+  if (D == 256) return row_tiles(rows, 1);
+  if (dtype == CX_KV_E4M3) return row_tiles(rows, 2);
+  if (D == 128) return row_tiles(rows, 3);
+  if (rows <= 64) return row_tiles(rows, 4);
+  const int nt = row_tiles(rows, 4);
+  const int64_t b3 = (rows + 47) / 48, b4 = (rows + 16 * nt - 1) / (16 * nt);
+  return 8 * 48 * b3 >= 9 * 16 * nt * b4 && head_units * b3 >= ATT_FOUR_UNITS ? nt
+                                                                            : row_tiles(rows, 3);
 }
 // Workers: as many waves as the chip's 256 CUs hold of the tile's kernel.
 static int workgroups(int nt, int D, int dtype) {
@@ -977,7 +992,7 @@ size_t cx_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int
   const int64_t rows = (int64_t)(q_heads / kv_heads) * max_new;
   size_t most = 0;
   for (int dtype : {CX_KV_BF16, CX_KV_E4M3}) {
-    const size_t n = cx::attend_workspace(cx::row_tiles(rows, head_dim, dtype), head_dim, dtype).total;
+    const size_t n = cx::attend_workspace(cx::attend_tiles(rows, head_dim, dtype, 0), head_dim, dtype).total;
     most = n > most ? n : most;
   }
   return most;
@@ -1015,7 +1030,9 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   A.window = window < INT32_MAX - cx::KV_MAX_NEW ? window : INT32_MAX - cx::KV_MAX_NEW;
   A.out = out;
   const int64_t rows = (int64_t)A.G * max_new;
-  const int D = kv->head_dim, nt = cx::row_tiles(rows, D, kv->dtype);
+  const int D = kv->head_dim;
+  const int64_t head_units = (int64_t)kv->B * kv->kv_heads * ((int64_t)kv->max_pages * kv->page_tokens / 32);
+  const int nt = cx::attend_tiles(rows, D, kv->dtype, head_units);
   const cx::AttendWork lay = cx::attend_workspace(nt, D, kv->dtype);
   A.entries = (int*)workspace;
   A.join = (cx::AttendJoin*)((char*)workspace + lay.off_join);
