@@ -928,7 +928,8 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   hipError_t err = hipSuccess;
   std::call_once(once, [&] {
     err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, false>,
-                              hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds_shares(CX_KV_MAX_BATCH, true));
+                              hipFuncAttributeMaxDynamicSharedMemorySize,
+                              Sh::lds_shares(CX_KV_MAX_BATCH, true));
     if (err == hipSuccess)
       err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, true>,
                                 hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds_block());
@@ -949,7 +950,8 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   const int most = Sh::BLOCK_UNITS * (2 * blocks >= grid ? 2 : 1);
   if (blocks <= 2 * grid && span <= most * Sh::TOK) {
     timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, true>,
-                 dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds_block(), s, A);
+                 dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds_block(), s,
+                 A);
     return (int)hipGetLastError();
   }
   timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, false>, dim3(grid), dim3(ATT_WG),
@@ -989,12 +991,16 @@ extern "C" {
 size_t cx_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                           int32_t max_new) {
   if (q_heads < 1 || kv_heads < 1 || head_dim < 1 || max_new < 1) return 256;
-  const int64_t rows = (int64_t)(q_heads / kv_heads) * max_new;
+  // the most of any call of as many rows or fewer, whatever its cache and table;
+  // more than 8 tiles take no tile that fewer do not
+  const int64_t tiles = ((int64_t)(q_heads / kv_heads) * max_new + 15) / 16;
   size_t most = 0;
-  for (int dtype : {CX_KV_BF16, CX_KV_E4M3}) {
-    const size_t n = cx::attend_workspace(cx::attend_tiles(rows, head_dim, dtype, 0), head_dim, dtype).total;
-    most = n > most ? n : most;
-  }
+  for (int64_t t = 1; t <= std::min<int64_t>(tiles, 8); ++t)
+    for (int dtype : {CX_KV_BF16, CX_KV_E4M3})
+      for (int64_t units : {(int64_t)0, cx::ATT_FOUR_UNITS}) {
+        const int nt = cx::attend_tiles(16 * t, head_dim, dtype, units);
+        most = std::max(most, cx::attend_workspace(nt, head_dim, dtype).total);
+      }
   return most;
 }
 
@@ -1014,26 +1020,26 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_token | q_head) & 7))
     return cx::api_fail(CX_EINVAL, "rows must be 16-byte aligned");
   if ((int64_t)kv->T * q_heads > INT32_MAX) return cx::api_fail(CX_EINVAL, "too many rows");
-  const size_t need = cx_paged_attention_workspace_bytes(q_heads, kv->kv_heads, kv->head_dim,
-                                                         max_new);
-  if (ws_bytes < need)
-    return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, need);
+  A.G = q_heads / kv->kv_heads;
+  max_new = std::min(max_new, kv->T);        // no sequence has more
+  const int D = kv->head_dim;
+  const int64_t table_units = (int64_t)kv->max_pages * kv->page_tokens / 32;
+  const int nt = cx::attend_tiles((int64_t)A.G * max_new, D, kv->dtype,
+                                  (int64_t)kv->B * kv->kv_heads * table_units);
+  const cx::AttendWork lay = cx::attend_workspace(nt, D, kv->dtype);
+  if (ws_bytes < lay.total)
+    return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, lay.total);
   // the units and row blocks, at most, fit the share arithmetic's 38 bits
   const double units = (double)kv->max_pages * kv->page_tokens / 32 + 8;
   const double blocks = kv->kv_heads * ((double)kv->T * (q_heads / kv->kv_heads) / 16 + kv->B);
   if (units * blocks >= 0x1p38) return cx::api_fail(CX_EINVAL, "too many tokens for one call");
   A.q = q; A.q_token = q_token; A.q_head = q_head;
-  A.q_heads = q_heads; A.G = q_heads / kv->kv_heads;
+  A.q_heads = q_heads;
   A.cap = softcap > 0;
   A.s1 = (float)((A.cap ? 2 * scale / softcap : scale) * 1.4426950408889634);
   A.s2 = (float)(softcap * 1.4426950408889634);
   A.window = window < INT32_MAX - cx::KV_MAX_NEW ? window : INT32_MAX - cx::KV_MAX_NEW;
   A.out = out;
-  const int64_t rows = (int64_t)A.G * max_new;
-  const int D = kv->head_dim;
-  const int64_t head_units = (int64_t)kv->B * kv->kv_heads * ((int64_t)kv->max_pages * kv->page_tokens / 32);
-  const int nt = cx::attend_tiles(rows, D, kv->dtype, head_units);
-  const cx::AttendWork lay = cx::attend_workspace(nt, D, kv->dtype);
   A.entries = (int*)workspace;
   A.join = (cx::AttendJoin*)((char*)workspace + lay.off_join);
   A.ml = (float*)((char*)workspace + lay.off_ml);
