@@ -25,7 +25,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
 #include <type_traits>
 
 #include "cx_device.hpp"
@@ -924,17 +923,6 @@ template <int D, int NT, bool F8>
 static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   using Sh = AttendShape<D, NT, F8>;
   constexpr int ROWS = Sh::ROWS;
-  static std::once_flag once;
-  hipError_t err = hipSuccess;
-  std::call_once(once, [&] {
-    err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, false>,
-                              hipFuncAttributeMaxDynamicSharedMemorySize,
-                              Sh::lds_shares(CX_KV_MAX_BATCH, true));
-    if (err == hipSuccess)
-      err = hipFuncSetAttribute((const void*)attend_split<D, NT, F8, true>,
-                                hipFuncAttributeMaxDynamicSharedMemorySize, Sh::lds_block());
-  });
-  if (err != hipSuccess) return (int)err;
   const unsigned grid = 256 * Sh::WAVES;
   A.workers = (int)grid * ATT_WAVES;
   const int64_t span = A.window ? std::min<int64_t>(A.window + max_new, (int64_t)A.kv.M << A.kv.logP)
@@ -948,12 +936,18 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   // 256 requests of 64 tokens: 21 and 17).  Row blocks that fill half the chip gain
   // from twice the length; max_new is a hint only, so they are counted by T, too.
   const int most = Sh::BLOCK_UNITS * (2 * blocks >= grid ? 2 : 1);
+  static LdsLimit limit_block, limit;
   if (blocks <= 2 * grid && span <= most * Sh::TOK) {
+    if (int e = limit_block.raise((const void*)attend_split<D, NT, F8, true>, Sh::lds_block()))
+      return e;
     timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, true>,
                  dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds_block(), s,
                  A);
     return (int)hipGetLastError();
   }
+  if (int e = limit.raise((const void*)attend_split<D, NT, F8, false>,
+                          Sh::lds_shares(CX_KV_MAX_BATCH, true)))
+    return e;
   timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, false>, dim3(grid), dim3(ATT_WG),
                (uint32_t)Sh::lds_shares(A.kv.B, A.kv.q_start != nullptr), s, A);
   // row blocks at most: every sequence's last one may hold fewer rows

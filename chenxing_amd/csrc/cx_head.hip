@@ -20,7 +20,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
 
 #include "cx_device.hpp"
 #include "cx_internal.hpp"
@@ -468,14 +467,9 @@ int launch_head(const HeadArgs& A0, hipStream_t s) {
     const int v = A.B > 16;
     static const K tall[2] = {head_tall<1, 3>, head_tall<2, 2>};
     const int kc = min(A.D, v ? tall_chunk<2>() : tall_chunk<1>());
-    // the dynamic-LDS limit raised once per variant to the most any launch takes
-    static std::once_flag once[2];
-    hipError_t err = hipSuccess;
-    std::call_once(once[v], [&] {
-      err = hipFuncSetAttribute((const void*)tall[v], hipFuncAttributeMaxDynamicSharedMemorySize,
-                                TALL_LDS);
-    });
-    if (err != hipSuccess) return (int)err;
+    // the dynamic-LDS limit raised to the most any launch takes
+    static LdsLimit limit[2];
+    if (int e = limit[v].raise((const void*)tall[v], TALL_LDS)) return e;
     timed_launch(CX_KERNEL_LMHEAD, tall[v], dim3((unsigned)A.nvt), dim3(TALL_NW * 64),
                  (uint32_t)(16 * (v + 1) * (kc + 8) * 2), s, A);
     timed_launch(CX_KERNEL_LMHEAD_MERGE, head_merge, dim3(A.B), dim3(HEAD_WG), 0, s, A);

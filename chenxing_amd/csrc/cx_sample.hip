@@ -1756,13 +1756,8 @@ int launch_sample(const SampleArgs& A, hipStream_t s) {
   static const K kern[4] = {sample_kernel<false, false>, sample_kernel<true, false>,
                             sample_kernel<false, true>, sample_kernel<true, true>};
   // Raise the dynamic-LDS limit to what this launch needs (static LDS comes on top).
-  static int attr_set[4] = {0, 0, 0, 0};
-  if (A.lds_bytes > attr_set[v]) {
-    hipError_t e = hipFuncSetAttribute((const void*)kern[v],
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, A.lds_bytes);
-    if (e != hipSuccess) return (int)e;
-    attr_set[v] = A.lds_bytes;
-  }
+  static LdsLimit limit[4];
+  if (int e = limit[v].raise((const void*)kern[v], A.lds_bytes)) return e;
   timed_launch(CX_KERNEL_SAMPLE, kern[v], dim3(A.B * A.nsplit), dim3(WG), A.lds_bytes, s, A);
   return (int)hipGetLastError();
 }

@@ -237,18 +237,12 @@ __global__ __launch_bounds__(WG) void truncate_kernel(SampleArgs A) {
 }
 
 template <typename K>
-static int set_lds(K kernel, int bytes, int& attr) {
-  if (bytes > attr) {
-    hipError_t e = hipFuncSetAttribute((const void*)kernel,
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return (int)e;
-    attr = bytes;
-  }
-  return 0;
+static int set_lds(K kernel, int bytes, LdsLimit& limit) {
+  return limit.raise((const void*)kernel, bytes);
 }
 
 int launch_slow(const SampleArgs& A, hipStream_t s) {
-  static int attr = 0, attr16 = 0;
+  static LdsLimit attr, attr16;
   // the multi-pass layout, or a refined row's finisher region (which also
   // holds the deep-nucleus paths' tables and counters)
   static_assert(DEEP_LDS <= FIN_CAP * 32, "deep-nucleus LDS");
@@ -269,7 +263,7 @@ int launch_slow(const SampleArgs& A, hipStream_t s) {
 }
 
 int launch_penalties(const SampleArgs& A, hipStream_t s) {
-  static int attr = 0;
+  static LdsLimit attr;
   if (int e = set_lds(penalties_kernel, A.slow_lds_bytes, attr)) return e;
   const int nchunk = (A.V + PEN_CHUNK - 1) / PEN_CHUNK;
   timed_launch(CX_KERNEL_PENALTIES, penalties_kernel, dim3(A.B, nchunk), dim3(WG),
@@ -278,7 +272,7 @@ int launch_penalties(const SampleArgs& A, hipStream_t s) {
 }
 
 int launch_truncate(const SampleArgs& A, hipStream_t s) {
-  static int attr = 0;
+  static LdsLimit attr;
   if (int e = set_lds(truncate_kernel, A.slow_lds_bytes, attr)) return e;
   timed_launch(CX_KERNEL_TRUNCATE, truncate_kernel, dim3(A.B), dim3(WG), A.slow_lds_bytes, s, A);
   return (int)hipGetLastError();

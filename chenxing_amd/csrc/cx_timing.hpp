@@ -1,7 +1,8 @@
 // cx_timing.hpp -- opt-in per-launch kernel timing.  While timing is on,
 // every library kernel is launched with hipExtLaunchKernelGGL and a start /
 // stop event pair that the dispatch itself records (the kernel's own
-// execution interval on its stream, not the host's launch overhead).
+// execution interval on its stream, not the host's launch overhead).  The limits
+// that a launch may need raised are in cx_lds.hpp.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
@@ -9,6 +10,7 @@
 #include <mutex>
 #include <vector>
 
+#include "cx_lds.hpp"
 #include "cx_sampler.h"
 
 namespace cx {
