@@ -526,7 +526,9 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
   A.st[0] = q_token; A.st[1] = k_token; A.st[2] = v_token;
   A.sh[0] = q_head; A.sh[1] = k_head; A.sh[2] = v_head;
   A.q_heads = q_heads;
-  A.rope = rope; A.rdim = rope ? rotary_dim : 0;
+  // a rope without rows: no token has a position
+  A.rope = rope_rows > 0 ? rope : nullptr;
+  A.rdim = A.rope ? rotary_dim : 0;
   A.interleaved = interleaved;
   A.norm[0] = q_norm; A.norm[1] = k_norm;
   A.eps = (float)eps;

@@ -299,7 +299,8 @@ typedef struct cx_kv_batch {
  *             page_tokens.  The first rotary_dim dims of a head are rotated (a
  *             multiple of 16), pairs (j, j + rotary_dim / 2), or (2 j, 2 j + 1)
  *             if interleaved
- *  q_out      [T, q_heads, D] bf16 bits
+ *  q_out      [T, q_heads, D] bf16 bits; of a token whose position is outside the
+ *             table's pages, rotated as at position 0
  * e4m3: a (token, head)'s scale is max|x| / 448, 1 for a row of zeros; a row
  * holding inf or NaN gets a NaN scale and zero codes.
  * Device pointers, stream-ordered, no synchronisation, no allocation.
