@@ -25,6 +25,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "cx_device.hpp"
@@ -47,7 +48,8 @@ struct AttendArgs {
   const uint16_t* q;
   int64_t q_token, q_head;
   int q_heads, G;             // G: q heads per kv head
-  float s1, s2;               // score in powers of 2: s1 qk, or s2 tanh(s1 / 2 qk)
+  // score in powers of 2: s1 qk, or s2 tanh(s4 qk), where exp(2 s4 qk) = 2 ^ (s3 qk)
+  float s1, s2, s3, s4;
   int cap;                    // the latter
   int window;                 // 0: none
   uint16_t* out;
@@ -476,16 +478,26 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
 
     // scores in powers of 2 are to2 * v
     const float to2 = A.cap ? 1.f : A.s1;
-    if (A.cap) {                             // tanh(z) = 1 - 2 / (exp(2 z) + 1)
+    if (A.cap) {
+      // tanh(z) = 1 - 2 / (exp(2 z) + 1), off by 2^-23 or so, whose share of a small z
+      // grows with the cap; below 1/8 the series, to z^9 (2^-29 of it)
+      const auto& A = launch_args();
+      const float s1 = A.s1, s2 = A.s2, s3 = A.s3, s4 = A.s4;
+      float c3 = -1.f / 3.f, c5 = 2.f / 15.f, c7 = -17.f / 315.f;
+      asm volatile("" : "+s"(c3), "+s"(c5), "+s"(c7));   // made here, not kept in the loop
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int y = 0; y < KT; ++y)
+        for (int y = 0; y < KT; ++y) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            v[nt][y][j] = fmaf(-2.f * A.s2,
-                               __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(A.s1 * v[nt][y][j]) + 1.f),
-                               A.s2);
+          for (int j = 0; j < 4; ++j) {
+            const float x = v[nt][y][j], z = s4 * x, zz = z * z, sx = s1 * x;
+            const float far = fmaf(-2.f * s2,
+                                   __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s3 * x) + 1.f), s2);
+            const float near = fmaf(sx * zz, fmaf(zz, fmaf(zz, c7, c5), c3), sx);
+            v[nt][y][j] = zz < 1.f / 64.f ? near : far;
+          }
+        }
     }
     // a row's running maximum is at least ATT_LOW once it has attended to a
     // token, whatever its score: -inf says that it has not
@@ -1030,8 +1042,13 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   A.q = q; A.q_token = q_token; A.q_head = q_head;
   A.q_heads = q_heads;
   A.cap = softcap > 0;
-  A.s1 = (float)((A.cap ? 2 * scale / softcap : scale) * 1.4426950408889634);
-  A.s2 = (float)(softcap * 1.4426950408889634);
+  const double log2e = 1.4426950408889634;
+  A.s1 = (float)(scale * log2e);
+  A.s2 = (float)(softcap * log2e);
+  A.s3 = A.cap ? (float)(2 * scale / softcap * log2e) : 0.f;
+  A.s4 = A.cap ? (float)(scale / softcap) : 0.f;
+  if (!std::isfinite(A.s1) || !std::isfinite(A.s3))
+    return cx::api_fail(CX_EINVAL, "scale (%g) and softcap (%g) pass the range of fp32", scale, softcap);
   A.window = window < INT32_MAX - cx::KV_MAX_NEW ? window : INT32_MAX - cx::KV_MAX_NEW;
   A.out = out;
   A.entries = (int*)workspace;

@@ -317,7 +317,8 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
  * verify round's gamma + 1, several together.  q head h reads kv head
  * h / (q_heads / kv_heads).  The token at position p attends to the
  * positions t <= p, t > p - window (window 0: all), with scores scale * q.k,
- * capped to softcap * tanh(score / softcap) if softcap > 0.  A token that
+ * capped to softcap * tanh(score / softcap) if softcap > 0 (infinity: not
+ * capped; the cap adds an error of about 2^-20 of the score).  A token that
  * attends to nothing gets zeros.  fp32 scores, softmax and sums, the weights
  * with 16 bits in their products; out is rounded once.  Short tables take one
  * launch, others two; results do not depend on timing.

@@ -1,5 +1,5 @@
-"""The attention workspace: one of the largest call serves every smaller one
-(CPU)."""
+"""The attention entry point on the host: its workspace (one of the largest call
+serves every smaller one) and its scores' range (CPU)."""
 from __future__ import annotations
 
 import os
@@ -37,3 +37,9 @@ def test_a_workspace_of_the_most_new_tokens_serves_fewer(dtype, stride):
             kv = _kv(dtype=dtype, stride=stride, M=1 << 22, ld=1 << 22, T=1 << 22)
             assert _attend(kv, new=new, nbytes=need) == _lib.CX_EINVAL
             assert b"too many tokens" in lib.cx_last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(scale=float("inf")), dict(scale=1e39), dict(cap=1e-45),
+                                 dict(scale=1e20, cap=1e-20)], ids=str)
+def test_scores_past_the_range_of_fp32_are_refused(bad):
+    assert _attend(_kv(), **bad) == _lib.CX_EINVAL and b"fp32" in _lib.load().cx_last_error()
