@@ -418,7 +418,7 @@ _KV_BATCH = struct.Struct("<QqQqQQ8i")
 KV_BF16, KV_E4M3 = 1, 3
 
 
-def _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T):
+def _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T, page_tokens=None):
     """(cx_kv_batch of one layer's pages and a batch, its kv heads)."""
     shape, stride, dtype = cache.shape, cache.stride(), cache.dtype
     if len(shape) != 3 or stride[2] != 1 or (stride[1] != shape[2] and shape[1] > 1):
@@ -435,6 +435,9 @@ def _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T):
         raise ValueError("cache must be bfloat16 pages, or uint8 pages of e4m3 codes and scales")
     if rest:
         raise ValueError(f"a page's width ({width}) does not fit heads of {D}")
+    if page_tokens is not None and P != page_tokens:
+        raise ValueError(f"a page of {page_tokens} tokens does not hold heads of {D}: its width "
+                         f"({width}) is that of {P} tokens")
     i32 = torch.int32
     shape, stride = table.shape, table.stride()
     if len(shape) != 2 or table.dtype != i32 or kv_len.dtype != i32:
@@ -489,7 +492,7 @@ def _out3(torch, name, t, q, dev, shape):
 
 
 def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, interleaved=False,
-                     q_norm=None, k_norm=None, eps=1e-6, q_out=None):
+                     q_norm=None, k_norm=None, eps=1e-6, q_out=None, page_tokens=None):
     """The new tokens' q, k and v made ready for attention, on the current stream.
 
     q [T, Hq, D], k and v [T, Hkv, D] (bfloat16, any token and head strides that
@@ -498,13 +501,14 @@ def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, int
     positions (``rope`` [positions, rotary dim] float32: the cosines, then the
     sines; None: not at all), k and v written into ``cache``, one layer's pages.
     ``table`` [B, pages], ``kv_len`` [B] (the new tokens included) and
-    ``q_start`` [B + 1] (None: one new token each) are int32.  Returns q_out
-    [T, Hq, D]."""
+    ``q_start`` [B + 1] (None: one new token each) are int32.  A page's tokens
+    follow from its width and D; ``page_tokens``, if given, has to agree.
+    Returns q_out [T, Hq, D]."""
     import torch
     lib = _lib or load()
     dev, shape, qs = _q_rows(torch, q)
     T, Hq, D = shape
-    kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T)
+    kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T, page_tokens)
     ks = _rows3(torch, "k", k, dev, (T, heads, D))
     vs = _rows3(torch, "v", v, dev, (T, heads, D))
     rp, rows, rdim = None, 0, 0
@@ -535,14 +539,15 @@ def _attention_workspace(q_heads, kv_heads, D, max_new):
 
 
 def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, scale=None, window=0,
-                           softcap=0.0, out=None):
+                           softcap=0.0, out=None, page_tokens=None):
     """Attention of the new tokens over one layer's pages, on the current stream.
 
     q [T, Hq, D] bfloat16 (as ``kv_append_device`` returns it); ``cache``,
-    ``table``, ``kv_len`` and ``q_start`` as there, the new tokens already
-    appended.  The token at position p attends to the positions up to p, the
-    last ``window`` of them if window > 0; ``scale`` defaults to D ** -0.5;
-    scores are capped to softcap * tanh(score / softcap) if softcap > 0.
+    ``table``, ``kv_len``, ``q_start`` and ``page_tokens`` as there, the new
+    tokens already appended.  The token at position p attends to the positions
+    up to p, the last ``window`` of them if window > 0; ``scale`` defaults to
+    D ** -0.5; scores are capped to softcap * tanh(score / softcap) if
+    softcap > 0.
     ``max_new`` is the most new tokens of a sequence (it picks the tile).
     Returns out [T, Hq, D] bfloat16; a token that attends to nothing gets
     zeros."""
@@ -550,7 +555,7 @@ def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, sca
     lib = _lib or load()
     dev, shape, qs = _q_rows(torch, q)
     T, Hq, D = shape
-    kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T)
+    kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T, page_tokens)
     out = _out3(torch, "out", out, q, dev, shape)
     nbytes = _attention_workspace(Hq, heads, D, max_new)
     key = dev, torch._C._cuda_getCurrentRawStream(dev)

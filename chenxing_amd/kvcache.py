@@ -179,8 +179,8 @@ class PagedKVCache:
     def batch(self, seqs, new=None) -> dict:
         """The table, kv_len, q_start and most new tokens (``max_new``) of a
         pass over sequences whose last new[i] tokens are new (None: one each),
-        as the device calls' keyword arguments ``table``, ``kv_len`` and
-        ``q_start``, on the pool's device."""
+        as the device calls' keyword arguments ``table``, ``kv_len``,
+        ``q_start`` and ``page_tokens``, on the pool's device."""
         import torch
         B = len(seqs)
         held = [self._seqs[s] for s in seqs]
@@ -194,7 +194,7 @@ class PagedKVCache:
         def up(a):
             return torch.from_numpy(a).to(self.pool.device)
         return dict(table=up(table), kv_len=up(lens), q_start=None if new is None else up(start),
-                    max_new=1 if new is None else max([1, *new]))
+                    page_tokens=self.page_tokens, max_new=1 if new is None else max([1, *new]))
 
     # ---------------------------------------------------------------- pages
     def _take(self) -> int:

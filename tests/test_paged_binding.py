@@ -39,3 +39,26 @@ def test_table_rows_are_where_their_stride_says(table, ld):
 def test_tables_whose_rows_overlap_are_refused(table):
     with pytest.raises(ValueError, match="table"):
         _batch(table())
+
+
+def test_pages_of_another_head_width_are_refused(device):                 # noqa: F811
+    """A pool of heads of 128 in pages of 16 has the width of heads of 64 in pages
+    of 32: what the cache says of itself has to agree."""
+    from chenxing_amd import PagedKVCache
+    cache = PagedKVCache(1, 5, 2, 128, 16, device="cpu")
+    s = cache.add()
+    cache.extend([s], [3])
+    x = cache.batch([s])
+    most = x.pop("max_new")
+    x = {k: v.as_subclass(type(_t(1))) if hasattr(v, "as_subclass") else v for k, v in x.items()}
+    pages = cache.layer(0).as_subclass(type(_t(1)))
+    for D, fits in ((128, True), (64, False)):
+        q, k = _t(1, 4, D, dtype=BF16), _t(1, 2, D, dtype=BF16)
+        for call in (lambda: _lib.kv_append_device(q, k, k, pages, **x),
+                     lambda: _lib.paged_attention_device(q, pages, max_new=most, **x)):
+            if fits:
+                call()
+            else:
+                with pytest.raises(ValueError, match="page of 16 tokens"):
+                    call()
+    assert len(device.calls) == 2
