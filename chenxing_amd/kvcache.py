@@ -30,7 +30,9 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 10000.0, *, linea
                yarn: float = 1.0, original: int = 4096, beta_fast: float = 32.0,
                beta_slow: float = 1.0, device="cuda"):
     """float32 [positions, rotary_dim]: the cosines of every position's angles
-    (rotary_dim / 2 of them), then the sines, computed in float64.
+    (rotary_dim / 2 of them), then the sines, computed in float64.  The append
+    wants a row for every position of its table's pages: a last page counts
+    whole.
 
     Angle j of position p is p * theta ** (-2 j / rotary_dim).  ``linear``
     divides the positions.  ``yarn`` (core/tensor.py:80-121; Peng et al. 2023)

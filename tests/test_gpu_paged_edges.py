@@ -47,3 +47,28 @@ def test_tokens_without_a_position():
     one = torch.ones(T, dtype=torch.int32, device="cuda")
     assert not pool.any()
     assert torch.equal(got, kv_append_device(q, k, k, pool, table, one, rope=rope))
+
+
+def test_a_model_whose_last_position_is_inside_a_page():
+    """37 positions in pages of 16: the rope covers whole pages, a shorter one is
+    refused."""
+    print("[gpu] a rope of 37 positions", flush=True)
+    import torch
+    from chenxing_amd import PagedKVCache, _lib, rope_table
+    T, bf = 37, torch.bfloat16
+    cache = PagedKVCache(2, pages=8, kv_heads=8, head_dim=128)
+    a = cache.add()
+    cache.extend([a], [T])
+    batch = cache.batch([a], [T])
+    most = batch.pop("max_new")
+    q, k, v = (torch.randn(T, h, 128, device="cuda").to(bf) for h in (32, 8, 8))
+    rope = rope_table(-(-T // 16) * 16, 128, theta=500000.0)
+    with pytest.raises(ValueError, match="positions"):
+        _lib.kv_append_device(q, k, v, cache.layer(0), rope=rope[:T], **batch)
+    for i in range(2):
+        q1 = _lib.kv_append_device(q, k, v, cache.layer(i), rope=rope, **batch)
+        o = _lib.paged_attention_device(q1, cache.layer(i), max_new=most, **batch)
+    assert torch.equal(o[0], v[0].repeat_interleave(4, 0)) and o.isfinite().all()
+    b, = cache.fork(a)
+    cache.truncate(a, 20)
+    assert (cache.length(a), cache.length(b)) == (20, T)
