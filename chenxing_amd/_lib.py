@@ -245,13 +245,15 @@ class Workspace:
         lock = self.locks.get(key)
         return self.locks.setdefault(key, threading.Lock()) if lock is None else lock
 
-    def get(self, key: tuple, nbytes: int, device):
+    def get(self, key: tuple, nbytes: int, like, capturing=None):
+        """``nbytes`` or more on tensor ``like``'s device; ``capturing``: whether the
+        stream records a graph (None: to be asked)."""
         import torch
-        if _capturing(torch, key[0]):
-            return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+        if _capturing(torch, key[0]) if capturing is None else capturing:
+            return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=like.device)
         buf = self.bufs.get(key)
         if buf is None or buf.numel() < nbytes:
-            buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
+            buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=like.device)
             self.bufs[key] = buf
         return buf
 
@@ -259,9 +261,9 @@ class Workspace:
 def _capturing(torch, dev) -> bool:
     """Whether device ``dev``'s current stream records a graph."""
     if dev is None or dev == torch._C._cuda_getDevice():
-        return torch.cuda.is_current_stream_capturing()
+        return torch._C._cuda_isCurrentStreamCapturing()
     with torch.cuda.device(dev):
-        return torch.cuda.is_current_stream_capturing()
+        return torch._C._cuda_isCurrentStreamCapturing()
 
 
 _ws_sample = Workspace()
@@ -315,7 +317,7 @@ def sample_device(logits, prm, u, hist=None, hist_len=None, out_id=None, row_sta
     fn = fns[logits.dtype]
     key = dev.index, sp.value
     with _ws_sample.of(key):
-        ws = _ws_sample.get(key, nbytes, dev)
+        ws = _ws_sample.get(key, nbytes, logits)
         _check(fn(_P(logits.data_ptr()), logits.stride(0), B, V,
                   _P(hist.data_ptr()) if hist is not None else None,
                   _P(hist_len.data_ptr()) if hist_len is not None else None, ldh,
@@ -367,7 +369,7 @@ def spec_verify_device(target, draft, draft_ids, u, temperature, accepted=None, 
     sp = _stream_ptr(dev)
     key = dev.index, sp.value
     with _ws_verify.of(key):
-        ws = _ws_verify.get(key, nbytes, dev)
+        ws = _ws_verify.get(key, nbytes, target)
         _check(lib.cx_spec_verify_f32(
             _P(target.data_ptr()), _P(draft.data_ptr()) if draft is not None else None,
             _P(draft_ids.data_ptr()), _P(u.data_ptr()), _P(temperature.data_ptr()), B, g, V,
@@ -404,7 +406,7 @@ def lmhead_argmax_device(hidden, weight, out_id=None, out_max=None, out_logits=N
     sp = _stream_ptr(dev)
     key = dev.index, sp.value
     with _ws_head.of(key):
-        ws = _ws_head.get(key, lib.cx_lmhead_workspace_bytes(B, V), dev)
+        ws = _ws_head.get(key, lib.cx_lmhead_workspace_bytes(B, V), hidden)
         _check(lib.cx_lmhead_argmax_bf16(
             _P(hidden.data_ptr()), hidden.stride(0), _P(weight.data_ptr()), weight.stride(0),
             B, D, V, _P(out_id.data_ptr()), _P(out_max.data_ptr()),
@@ -554,16 +556,23 @@ def paged_attention_device(q, cache, table, kv_len, q_start=None, max_new=1, sca
     import torch
     lib = _lib or load()
     dev, shape, qs = _q_rows(torch, q)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return paged_attention_device(q, cache, table, kv_len, q_start, max_new, scale, window,
+                                          softcap, out, page_tokens)
     T, Hq, D = shape
     kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T, page_tokens)
     out = _out3(torch, "out", out, q, dev, shape)
     nbytes = _attention_workspace(Hq, heads, D, max_new)
-    key = dev, torch._C._cuda_getCurrentRawStream(dev)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    key = dev, stream
     with _ws_attend.of(key):
-        ws = _ws_attend.get(key, nbytes, q.device)
-        _call(torch, dev, lib.cx_paged_attention_bf16, kv, q.data_ptr(), qs[0], qs[1], Hq, max_new,
-              D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(),
-              ws.data_ptr(), ws.numel())
+        ws = _ws_attend.get(key, nbytes, q, torch._C._cuda_isCurrentStreamCapturing())
+        rc = lib.cx_paged_attention_bf16(
+            kv, q.data_ptr(), qs[0], qs[1], Hq, max_new, D ** -0.5 if scale is None else scale,
+            window, softcap, out.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        if rc != CX_OK:
+            _check(rc)
     return out
 
 

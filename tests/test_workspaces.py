@@ -79,7 +79,8 @@ def device(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: lib.stream, raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: lib.capturing)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: lib.capturing,
+                        raising=False)
     for name in ("_ws_sample", "_ws_verify", "_ws_head", "_ws_attend"):
         monkeypatch.setattr(_lib, name, _lib.Workspace())
     _lib._attention_workspace.cache_clear()
