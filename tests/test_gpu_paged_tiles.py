@@ -1,5 +1,6 @@
-"""Many sequences of more rows than a tile of heads of 64 holds: the batches that
-take four tiles of 16 rows, and those one unit short of it."""
+"""Many sequences of more rows than a tile of heads of 64 holds (the batches that
+take four tiles of 16 rows, and those just short of it), and as many sequences as a
+call takes."""
 from __future__ import annotations
 
 import pytest
@@ -17,5 +18,13 @@ pytestmark = pytest.mark.gpu
     # 8 tiles, 7 of them full
     ("four_eight", ("bf16", 8, 1, 64, 16, 160, 600, 2000, 16, 0))])
 def test_attention_of_many_rows(name, args):
+    print(f"[gpu] attention {name}", flush=True)
+    _check_many(name, *args)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("most_e4m3", ("e4m3", 2, 1, 256, 16, 4096, 0, 40, 2, 0)),
+    ("most_singles", ("bf16", 3, 1, 64, 16, 4096, 0, 30, 1, 0))])
+def test_the_most_sequences_of_a_call(name, args):
     print(f"[gpu] attention {name}", flush=True)
     _check_many(name, *args)

@@ -1,4 +1,5 @@
-"""Calls recorded in a HIP graph keep their scratch through later, larger calls."""
+"""Calls recorded in a HIP graph keep their scratch through later, larger calls, and
+threads that share a stream do not share it at once."""
 from __future__ import annotations
 
 import numpy as np
@@ -89,3 +90,28 @@ def test_graph_beside_larger_calls(make, small, large, warm):
         torch.cuda.synchronize()
         for k, t in enumerate(others):
             assert bool((t == k).all()), k
+
+
+@pytest.mark.parametrize("makes", [[(_attention, 1), (_attention, 5), (_attention, 2)],
+                                   [(_lmhead, 8), (_lmhead, 200)], [(_sample, 4), (_sample, 64)],
+                                   [(_verify, 2), (_verify, 16)]])
+def test_threads_on_one_stream(makes):
+    print(f"[gpu] threads on one stream: {makes[0][0].__name__}", flush=True)
+    import threading
+    import torch
+    steps = [f(n) for f, n in makes]
+    want = [s().clone() for s in steps]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        for _ in range(40):
+            got = steps[i]().clone()
+            if not torch.equal(got, want[i]):
+                bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(steps))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
