@@ -19,9 +19,10 @@
 // Bound: HBM, every page read once a row block.  A row block is 16 NT rows of (new
 // token, q head of the kv head's group); 16 rows of one unit are 24 MFMAs (head_dim
 // 128) for 16 KB.  64 ragged requests of up to 8192 tokens, 8 kv heads of 128, 560
-// MB: 92 us and 4 us of join, 6.1 TB/s in the first; 2 of 131072, 1018 MB: 162 and
-// 6 us.  A prompt of 4096 tokens, 32 / 8 heads of 128: 446 us, 309 TFLOP/s, bound by
-// one wave a SIMD (products, softmax and loads of 48 rows one after the other).
+// MB: 95 us and 5 us of join, 5.9 TB/s in the first; 2 of 131072, 1018 MB: 164 and
+// 6.5 us, 6.2 TB/s.  A prompt of 4096 tokens, 32 / 8 heads of 128: 452 us, 304
+// TFLOP/s, bound by one wave a SIMD (products, softmax and loads of 48 rows one after
+// the other) and by its reads: every wave's own, 2.6 GB past the L2s.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

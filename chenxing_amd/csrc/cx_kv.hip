@@ -116,7 +116,8 @@ __device__ __forceinline__ T lanes_reduce(T v, Op op) {
   return v;
 }
 
-// x * rsqrt(mean(x^2) + eps) * w over the row's D / 8 lanes.
+// x * rsqrt(mean(x^2) + eps) * w over the row's D / 8 lanes; the root by v_rsq, within
+// 1 ulp: with the sum's roundings it is not what the result's error comes from.
 template <int D>
 __device__ __forceinline__ void norm_row(Row8& r, u32x4 w, float eps) {
   float ss = 0;
@@ -245,8 +246,8 @@ __device__ __forceinline__ void put_key(const KvArgs& C, const Row8& r, const Sl
 
 // One row (token, head) of q, k or v to D / 8 lanes, every row of the call at
 // once: q heads first, then k, then v.  A small call is one latency, launch and
-// loads (1 token, 48 heads of 128: 3.3 us); a row's v leaves as one element a chunk,
-// so in a large one the stores bound it (256 tokens of as many sequences 6.5 us, 256
+// loads (1 token, 48 heads of 128: 3.7 us); a row's v leaves as one element a chunk,
+// so in a large one the stores bound it (256 tokens of as many sequences 7.0 us, 256
 // prompts of 64 tokens 251 us).
 template <int D, bool F8>
 __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
@@ -301,8 +302,8 @@ __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
 //  * The others: VT tokens of one head of v.  They pass through LDS, and the
 //    tokens of a chunk that are all here leave as 16 bytes a dim.
 //
-// Bound: HBM.  5 prompts of 2500 tokens, 48 heads of 128, e4m3: 217 MB in 52 us,
-// 4.2 TB/s where a copy reaches 4.75 (append_rows 125 us).
+// Bound: HBM.  5 prompts of 2500 tokens, 48 heads of 128, e4m3: 217 MB in 53 us,
+// 4.1 TB/s where a copy reaches 4.75 (append_rows 125 us); bf16: 219 MB in 47 us.
 constexpr int APPEND_HEADS = 8, APPEND_VT = 64;
 
 template <int D, bool F8>
@@ -444,7 +445,7 @@ constexpr int COPY_PART = COPY_LOADS * 4096; // bytes a workgroup copies
 
 // Workgroup (pair, layer, part): COPY_PART bytes of the page.  Bound: HBM.  400
 // pages of 64 KB in 32 layers, 1.68 GB read and written: 334 us, 5.0 TB/s (plain
-// stores 343); 16 such pages, 67 MB: 7.6 us (plain stores 9.2, loads past the caches
+// stores 343); 16 such pages, 67 MB: 7.1 us (plain stores 9.2, loads past the caches
 // 10.6).
 __global__ __launch_bounds__(256) void copy_pages(CopyArgs A) {
   const unsigned part = blockIdx.x % (unsigned)A.parts, x = blockIdx.x / (unsigned)A.parts;

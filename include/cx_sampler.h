@@ -288,8 +288,9 @@ typedef struct cx_kv_batch {
 /*
  * The new tokens of a forward pass made ready for attention: q and k normed
  * per head (optional), rotated to their positions (optional), q written to
- * q_out, k and v to the pages.  One pass over q, k and v.  fp32 arithmetic,
- * each result rounded once.
+ * q_out, k and v to the pages.  One pass over q, k and v.  fp32 arithmetic (the
+ * norm's squares too: a row's largest value between 2^-60 and 2^60, or an eps
+ * that covers smaller ones), each result rounded once.
  *
  *  q, k, v    bf16 bits, row (token, head) at token * _token + head * _head
  *             elements, rows 16-byte aligned
@@ -301,8 +302,9 @@ typedef struct cx_kv_batch {
  *             if interleaved
  *  q_out      [T, q_heads, D] bf16 bits; of a token whose position is outside the
  *             table's pages, rotated as at position 0
- * e4m3: a (token, head)'s scale is max|x| / 448, 1 for a row of zeros; a row
- * holding inf or NaN gets a NaN scale and zero codes.
+ * e4m3: a (token, head)'s scale is the fp32 quotient max|x| / 448, 1 where that
+ * is 0, and a code the nearest of the fp32 quotient x / scale; a row holding inf
+ * or NaN gets a NaN scale and zero codes.
  * Device pointers, stream-ordered, no synchronisation, no allocation.
  */
 int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token, int64_t q_head,
