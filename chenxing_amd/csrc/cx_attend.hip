@@ -1026,6 +1026,8 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   if (!q || !out || !workspace) return cx::api_fail(CX_EINVAL, "null pointer argument");
   if ((((uintptr_t)q | (uintptr_t)out) & 15) || ((q_token | q_head) & 7))
     return cx::api_fail(CX_EINVAL, "rows must be 16-byte aligned");
+  if ((uintptr_t)workspace & 15)
+    return cx::api_fail(CX_EINVAL, "workspace must be 16-byte aligned");
   if ((int64_t)kv->T * q_heads > INT32_MAX) return cx::api_fail(CX_EINVAL, "too many rows");
   A.G = q_heads / kv->kv_heads;
   max_new = std::min(max_new, kv->T);        // no sequence has more

@@ -333,9 +333,10 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
  *             any value >= 1 gives right results
  *  out        [T, q_heads, D] bf16 bits
  *  workspace  device scratch of cx_paged_attention_workspace_bytes(...) bytes;
- *             any contents.  One workspace per stream.  The size grows with
- *             max_new and with the q heads of a kv head: one of the largest
- *             call serves every smaller one, of either cache type.
+ *             16-byte aligned, any contents.  One workspace per stream.  The
+ *             size grows with max_new and with the q heads of a kv head: one
+ *             of the largest call serves every smaller one, of either cache
+ *             type.
  * Device pointers, stream-ordered, no synchronisation, no allocation.
  */
 int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,

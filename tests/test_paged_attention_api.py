@@ -7,7 +7,7 @@ import os
 import pytest
 
 from chenxing_amd import _lib
-from test_paged_api import _attend, _kv
+from test_paged_api import A, _attend, _kv
 
 pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH),
                                 reason="libcx_sampler.so not built")
@@ -43,3 +43,9 @@ def test_a_workspace_of_the_most_new_tokens_serves_fewer(dtype, stride):
                                  dict(scale=1e20, cap=1e-20)], ids=str)
 def test_scores_past_the_range_of_fp32_are_refused(bad):
     assert _attend(_kv(), **bad) == _lib.CX_EINVAL and b"fp32" in _lib.load().cx_last_error()
+
+
+@pytest.mark.parametrize("off", [1, 4, 8])
+def test_a_workspace_off_16_bytes_is_refused(off):
+    assert _attend(_kv(), ws=A + off) == _lib.CX_EINVAL
+    assert b"workspace" in _lib.load().cx_last_error()
