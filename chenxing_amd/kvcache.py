@@ -44,6 +44,8 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 10000.0, *, linea
         raise ValueError("positions must be >= 0 and rotary_dim even")
     if theta <= 0 or linear <= 0 or yarn < 1 or original < 1:
         raise ValueError("theta, linear and original must be positive and yarn >= 1")
+    if yarn > 1 and theta <= 1:
+        raise ValueError("yarn needs pairs that turn slower one after the other: theta > 1")
     j = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
     freq = theta ** (-2.0 * j / rotary_dim) / linear
     size = 1.0

@@ -62,3 +62,11 @@ def test_pages_of_another_head_width_are_refused(device):                 # noqa
                 with pytest.raises(ValueError, match="page of 16 tokens"):
                     call()
     assert len(device.calls) == 2
+
+
+@pytest.mark.parametrize("theta", [1.0, 0.5])
+def test_yarn_needs_angles_that_fall(theta):
+    from chenxing_amd import rope_table
+    with pytest.raises(ValueError, match="theta"):
+        rope_table(4, 8, theta, yarn=2.0, device="cpu")
+    assert rope_table(4, 8, theta, device="cpu").shape == (4, 8)
