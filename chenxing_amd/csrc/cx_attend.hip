@@ -42,6 +42,10 @@ constexpr int ATT_WG = 64 * ATT_WAVES;
 // Terms are relative to a maximum that lags by up to this, in powers of 2: they
 // reach 256 instead of 1, and the sums are rarely scaled.
 constexpr float ATT_SLACK = 8.f;
+// Caps up to this take tanh from the exponential alone: 4e-5 of a score's unit (118
+// requests of 1008..2017 tokens, e4m3, 12 / 4 heads of 64, cap 30: 24.5 us; with the
+// series 27.7).
+constexpr double ATT_CAP = 256;
 constexpr float ATT_LOW = -3e38f;            // running maximum of a row that attends to something
 
 struct AttendArgs {
@@ -51,7 +55,7 @@ struct AttendArgs {
   int q_heads, G;             // G: q heads per kv head
   // score in powers of 2: s1 qk, or s2 tanh(s4 qk), where exp(2 s4 qk) = 2 ^ (s3 qk)
   float s1, s2, s3, s4;
-  int cap;                    // the latter
+  int cap;                    // the latter; 2: above ATT_CAP
   int window;                 // 0: none
   uint16_t* out;
   int workers;
@@ -161,7 +165,7 @@ struct AttendShape {
   using Seqs = AttendSeqs<CX_LDS uint64_t*, CX_LDS int*>;
   static constexpr int E = F8 ? 16 : 8;      // elements of a 16-byte chunk
   // A wave's scratch: its 16 rows, whole where the waves join their sums (BLOCK),
-  // else a quarter of their dims at a time.
+  // else a quarter of their dims (a large batch's lengths take the rest).
   static constexpr int PAD = D + 4, FIX = D / 4, FPAD = FIX + 4;   // floats of a row
   static constexpr int scratch(bool block) { return 16 * (block ? PAD : FPAD); }
   // waves per SIMD, as many as the registers hold
@@ -479,25 +483,30 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
 
     // scores in powers of 2 are to2 * v
     const float to2 = A.cap ? 1.f : A.s1;
-    if (A.cap) {
-      // tanh(z) = 1 - 2 / (exp(2 z) + 1), off by 2^-23 or so, whose share of a small z
-      // grows with the cap; below 1/8 the series, to z^9 (2^-29 of it)
+    if (__builtin_expect(A.cap, 0)) {
+      // tanh(z) = 1 - 2 / (exp(2 z) + 1) is off by 2^-23 of the cap or so, whatever the
+      // score: too much of a large cap.  There below z = 1/16 the series, to z^5
       const auto& A = launch_args();
-      const float s1 = A.s1, s2 = A.s2, s3 = A.s3, s4 = A.s4;
-      float c3 = -1.f / 3.f, c5 = 2.f / 15.f, c7 = -17.f / 315.f;
-      asm volatile("" : "+s"(c3), "+s"(c5), "+s"(c7));   // made here, not kept in the loop
+      const float s2 = A.s2, s3 = A.s3;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int y = 0; y < KT; ++y) {
+          f32x4 far;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = v[nt][y][j], z = s4 * x, zz = z * z, sx = s1 * x;
-            const float far = fmaf(-2.f * s2,
-                                   __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s3 * x) + 1.f), s2);
-            const float near = fmaf(sx * zz, fmaf(zz, fmaf(zz, c7, c5), c3), sx);
-            v[nt][y][j] = zz < 1.f / 64.f ? near : far;
+          for (int j = 0; j < 4; ++j)
+            far[j] = fmaf(-2.f * s2,
+                          __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s3 * v[nt][y][j]) + 1.f), s2);
+          if (A.cap > 1) {
+            float c3 = -1.f / 3.f, c5 = 2.f / 15.f;
+            asm volatile("" : "+s"(c3), "+s"(c5));   // made here, not kept in the loop
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x = v[nt][y][j], z = A.s4 * x, zz = z * z, sx = A.s1 * x;
+              far[j] = zz < 1.f / 256.f ? fmaf(sx * zz, fmaf(zz, c5, c3), sx) : far[j];
+            }
           }
+          v[nt][y] = far;
         }
     }
     // a row's running maximum is at least ATT_LOW once it has attended to a
@@ -653,10 +662,10 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
       if (again) {
         // each row's own NaN and infinite values (their terms' size does not
         // matter), token by token, FIX dims of all 16 rows at a time
-        constexpr int FIX = Sh::FIX, FPAD = Sh::FPAD, NQ = FIX / 16;
+        constexpr int FIX = BLOCK ? 64 : Sh::FIX, FPAD = FIX + 4, NQ = FIX / 16;
         const int fd = l % FIX;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < D / FIX; ++x) {
 #pragma unroll
           for (int n = 0; n < NQ; ++n)
             *(CX_LDS f32x4*)(s_o + c * FPAD + 16 * n + 4 * g) = acc[nt][NQ * x + n];
@@ -668,6 +677,7 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
                             v_chunk<E, D>(FIX * x + fd, o, C.logP) + o % E * (16 / E);
             const float v = F8 ? e4m3_value(*(const uint8_t*)p) : bf16_lo(*(const uint16_t*)p);
             if (fabsf(v) < INFINITY) continue;
+#pragma unroll 1
             for (int r = l / FIX; r < 16; r += 64 / FIX) {
               const int at = cur.lowest + (cur.r0 + min(16 * nt + r, cur.R - 1)) / A.G;
               if (t <= at && !(A.window && t <= at - A.window)) s_o[r * FPAD + fd] += v;
@@ -1044,7 +1054,7 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   if (units * blocks >= 0x1p38) return cx::api_fail(CX_EINVAL, "too many tokens for one call");
   A.q = q; A.q_token = q_token; A.q_head = q_head;
   A.q_heads = q_heads;
-  A.cap = softcap > 0;
+  A.cap = softcap > cx::ATT_CAP ? 2 : softcap > 0;
   const double log2e = 1.4426950408889634;
   A.s1 = (float)(scale * log2e);
   A.s2 = (float)(softcap * log2e);

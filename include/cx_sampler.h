@@ -320,10 +320,11 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
  * h / (q_heads / kv_heads).  The token at position p attends to the
  * positions t <= p, t > p - window (window 0: all), with scores scale * q.k,
  * capped to softcap * tanh(score / softcap) if softcap > 0 (infinity: not
- * capped; the cap adds an error of about 2^-20 of the score).  A token that
- * attends to nothing gets zeros.  fp32 scores, softmax and sums, the weights
- * with 16 bits in their products; out is rounded once.  Short tables take one
- * launch, others two; results do not depend on timing.
+ * capped; the cap adds an error of about 2^-22 of a softcap up to 256, 2^-19 of
+ * the score above).  A token that attends to nothing gets zeros.  fp32
+ * scores, softmax and sums, the weights with 16 bits in their products; out is
+ * rounded once.  Short tables take one launch, others two; results do not
+ * depend on timing.
  * T is at most 2^28; calls whose row blocks times table units (16 rows, 32
  * tokens) reach 2^38 are refused.
  *

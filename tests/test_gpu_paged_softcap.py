@@ -25,6 +25,18 @@ def test_a_cap_far_above_the_scores(name, cap, wide):
     _check(_attend(_widen(x) if wide else x), want, tol)
 
 
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("cap", [30.0, 256.0, 257.0, 600.0, 3000.0])
+@pytest.mark.parametrize("name", ["verify", "long_e4m3"])
+def test_caps_among_large_scores(name, cap, wide):
+    print(f"[gpu] attention {name}, cap {cap}, wide {wide}, large scores", flush=True)
+    x = dict(_attend_inputs(name), softcap=cap)
+    K, V = R.unpack(x["pages"], x["D"])
+    want, tol = R.attend(_values(x["q"]), K, V, x["table"], x["kv_len"], x["q_start"], x["P"],
+                         9.0, x["window"], cap)
+    _check(_attend(_widen(x) if wide else x, scale=9.0), want, tol)
+
+
 @pytest.mark.parametrize("cap", [0.05, 1.0, 5.0])
 def test_caps_below_the_scores(cap):
     print(f"[gpu] attention cap {cap}", flush=True)
