@@ -42,9 +42,9 @@ constexpr int ATT_WG = 64 * ATT_WAVES;
 // Terms are relative to a maximum that lags by up to this, in powers of 2: they
 // reach 256 instead of 1, and the sums are rarely scaled.
 constexpr float ATT_SLACK = 8.f;
-// Caps up to this take tanh from the exponential alone: 4e-5 of a score's unit (118
-// requests of 1008..2017 tokens, e4m3, 12 / 4 heads of 64, cap 30: 24.5 us; with the
-// series 27.7).
+// Caps up to this take tanh from the exponential alone, which is off by 6e-5 at most;
+// larger ones a kernel of their own with tanh's series too (in the one kernel 118
+// requests of 1008..2017 tokens, e4m3, 12 / 4 heads of 64, cap 30: 25.2 -> 25.8 us).
 constexpr double ATT_CAP = 256;
 constexpr float ATT_LOW = -3e38f;            // running maximum of a row that attends to something
 
@@ -55,7 +55,7 @@ struct AttendArgs {
   int q_heads, G;             // G: q heads per kv head
   // score in powers of 2: s1 qk, or s2 tanh(s4 qk), where exp(2 s4 qk) = 2 ^ (s3 qk)
   float s1, s2, s3, s4;
-  int cap;                    // the latter; 2: above ATT_CAP
+  int cap;                    // the latter; 2: by more than ATT_CAP
   int window;                 // 0: none
   uint16_t* out;
   int workers;
@@ -202,8 +202,8 @@ struct AttendShape {
 //
 // BLOCK: short tables.  A workgroup takes a row block whole, each wave a quarter of
 // its units, and the waves join through LDS: no share to find, no second launch.
-// launch_tile says when.
-template <int D, int NT, bool F8, bool BLOCK>
+// launch_tile says when.  WIDE: scores capped by more than ATT_CAP.
+template <int D, int NT, bool F8, bool BLOCK, bool WIDE>
 __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void attend_split(AttendArgs A) {
   using Sh = AttendShape<D, NT, F8>;
   constexpr int TOK = Sh::TOK, ROWS = Sh::ROWS, E = Sh::E, PAD = Sh::PAD;
@@ -482,32 +482,32 @@ __global__ __launch_bounds__(ATT_WG, (AttendShape<D, NT, F8>::WAVES)) void atten
     load_k(ids, k, turn && !BLOCK ? nxt.unit : unit + 1, turn && !BLOCK ? nxt.h : cur.h, !(turn && last));
 
     // scores in powers of 2 are to2 * v
-    const float to2 = A.cap ? 1.f : A.s1;
-    if (__builtin_expect(A.cap, 0)) {
-      // tanh(z) = 1 - 2 / (exp(2 z) + 1) is off by 2^-23 of the cap or so, whatever the
-      // score: too much of a large cap.  There below z = 1/16 the series, to z^5
+    const float to2 = WIDE || A.cap ? 1.f : A.s1;
+    if constexpr (WIDE) {
+      // that is off by 2^-23 of the cap, whatever the score: too much of a large one.
+      // Below z = 1/16 the series, to z^5
       const auto& A = launch_args();
-      const float s2 = A.s2, s3 = A.s3;
+      const float s1 = A.s1, s2 = A.s2, s3 = A.s3, s4 = A.s4;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int y = 0; y < KT; ++y) {
-          f32x4 far;
+        for (int y = 0; y < KT; ++y)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = v[nt][y][j], z = s4 * x, zz = z * z, sx = s1 * x;
+            const float far = fmaf(-2.f * s2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s3 * x) + 1.f), s2);
+            v[nt][y][j] = zz < 1.f / 256.f ? fmaf(sx * zz, fmaf(zz, 2.f / 15.f, -1.f / 3.f), sx) : far;
+          }
+    } else if (A.cap) {                      // tanh(z) = 1 - 2 / (exp(2 z) + 1)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int y = 0; y < KT; ++y)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            far[j] = fmaf(-2.f * s2,
-                          __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s3 * v[nt][y][j]) + 1.f), s2);
-          if (A.cap > 1) {
-            float c3 = -1.f / 3.f, c5 = 2.f / 15.f;
-            asm volatile("" : "+s"(c3), "+s"(c5));   // made here, not kept in the loop
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float x = v[nt][y][j], z = A.s4 * x, zz = z * z, sx = A.s1 * x;
-              far[j] = zz < 1.f / 256.f ? fmaf(sx * zz, fmaf(zz, c5, c3), sx) : far[j];
-            }
-          }
-          v[nt][y] = far;
-        }
+            v[nt][y][j] = fmaf(-2.f * A.s2,
+                               __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(A.s3 * v[nt][y][j]) + 1.f),
+                               A.s2);
     }
     // a row's running maximum is at least ATT_LOW once it has attended to a
     // token, whatever its score: -inf says that it has not
@@ -959,19 +959,24 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
   // 256 requests of 64 tokens: 21 and 17).  Row blocks that fill half the chip gain
   // from twice the length; max_new is a hint only, so they are counted by T, too.
   const int most = Sh::BLOCK_UNITS * (2 * blocks >= grid ? 2 : 1);
-  static LdsLimit limit_block, limit;
+  using Kernel = void (*)(AttendArgs);
+  static const Kernel in_block[2] = {attend_split<D, NT, F8, true, false>,
+                                     attend_split<D, NT, F8, true, true>},
+                      in_shares[2] = {attend_split<D, NT, F8, false, false>,
+                                      attend_split<D, NT, F8, false, true>};
+  static LdsLimit limit_block[2], limit[2];
+  const int wide = A.cap > 1;
   if (blocks <= 2 * grid && span <= most * Sh::TOK) {
-    if (int e = limit_block.raise((const void*)attend_split<D, NT, F8, true>, Sh::lds_block()))
-      return e;
-    timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, true>,
+    if (int e = limit_block[wide].raise((const void*)in_block[wide], Sh::lds_block())) return e;
+    timed_launch(CX_KERNEL_ATTEND, in_block[wide],
                  dim3((unsigned)(A.kv.heads * tiles), A.kv.B), dim3(ATT_WG), (uint32_t)Sh::lds_block(), s,
                  A);
     return (int)hipGetLastError();
   }
-  if (int e = limit.raise((const void*)attend_split<D, NT, F8, false>,
-                          Sh::lds_shares(CX_KV_MAX_BATCH, true)))
+  if (int e = limit[wide].raise((const void*)in_shares[wide],
+                                Sh::lds_shares(CX_KV_MAX_BATCH, true)))
     return e;
-  timed_launch(CX_KERNEL_ATTEND, attend_split<D, NT, F8, false>, dim3(grid), dim3(ATT_WG),
+  timed_launch(CX_KERNEL_ATTEND, in_shares[wide], dim3(grid), dim3(ATT_WG),
                (uint32_t)Sh::lds_shares(A.kv.B, A.kv.q_start != nullptr), s, A);
   // row blocks at most: every sequence's last one may hold fewer rows
   const int64_t entries = std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B),
