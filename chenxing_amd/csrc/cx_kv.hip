@@ -189,25 +189,30 @@ __device__ __forceinline__ u32x2 encode_row(const Row8& r, float* scale) {
   for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(r.x[i]) & 0x7FFFFFFFu);
   m = lanes_reduce<D>(m, [](uint32_t a, uint32_t b) { return max(a, b); });
   const bool fine = m < 0x7F800000u;
-  float f = __uint_as_float(m) / E4M3_MAX;
+  // Quotients as a division rounds them (but perhaps for ties among denormal scales):
+  // times a reciprocal, less what that is too much times it (in this order a zero
+  // keeps its sign).  A scale too small for that (below 2^-126 it has no finite
+  // reciprocal) is taken 2^80 times as large, as is x.
+  auto quotient = [](float x, float f, float inv) {
+    const float a = x * inv;
+    return fmaf(-fmaf(a, f, -x), inv, a);
+  };
+  float f = quotient(__uint_as_float(m), E4M3_MAX, 1.f / E4M3_MAX);
   if (f == 0.f) f = 1.f;                     // a row of zeros, or of values whose scale rounds to 0
   *scale = fine ? f : __builtin_nanf("");
-  // The quotient x / f rounded once: times the rounded reciprocal, and what that
-  // left over times it again.  A scale too small for that (below 2^-126 it has no
-  // finite reciprocal) is taken 2^80 times as large, as is x.
-  const float by = f < 0x1p-60f ? 0x1p80f : 1.f, fs = f * by, inv = fine ? 1.f / fs : 0.f;
+  const float by = f < 0x1p-60f ? 0x1p80f : 1.f, fs = f * by;
+  float inv = __builtin_amdgcn_rcpf(fs);
+  inv = fmaf(fmaf(-inv, fs, 1.f), inv, inv);
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = fine ? r.x[i] * by : 0.f, a = x * inv;
-    const float z = fmaf(fmaf(-a, fs, x), inv, a);           // without the sign of a zero
-    y[i] = __builtin_amdgcn_fmed3f(__builtin_copysignf(z, x), -E4M3_MAX, E4M3_MAX);
+    y[i] = __builtin_amdgcn_fmed3f(quotient(r.x[i] * by, fs, inv), -E4M3_MAX, E4M3_MAX);
   }
   u32x2 c;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int p = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
-    c[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], p, true);
+    c[i] = fine ? __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], p, true) : 0;
   }
   return c;
 }
@@ -229,18 +234,33 @@ __device__ __forceinline__ Slot token_slot(const KvArgs& C, int t) {
   return s;
 }
 
+// A lane's part of a row as the page holds it: 8 elements of bf16, or 8 e4m3 codes
+// and the row's scale.
+struct Part {
+  u32x4 w;
+  float scale;
+};
+template <int D, bool F8>
+__device__ __forceinline__ Part page_part(const Row8& r) {
+  Part p = {};
+  if (F8) {
+    const u32x2 c = encode_row<D>(r, &p.scale);
+    p.w = u32x4{c[0], c[1], 0, 0};
+  } else {
+    p.w = narrow(r);
+  }
+  return p;
+}
 // A lane's part of a key row, to its page.
 template <int D, bool F8>
-__device__ __forceinline__ void put_key(const KvArgs& C, const Row8& r, const Slot& s, int h, int d) {
+__device__ __forceinline__ void put_key(const KvArgs& C, const Part& p, const Slot& s, int h, int d) {
+  if (s.page < 0) return;
   char* base = C.pages + s.page + (int64_t)h * C.head_bytes;
   if (F8) {
-    float scale;
-    const u32x2 c = encode_row<D>(r, &scale);
-    if (s.page < 0) return;
-    *(u32x2*)(base + k_chunk<16>(d, s.o, C.logP) + (d & 8)) = c;
-    if (d == 0) *(float*)(base + k_scale<D>(s.o, C.logP)) = scale;
-  } else if (s.page >= 0) {
-    *(u32x4*)(base + k_chunk<8>(d, s.o, C.logP)) = narrow(r);
+    *(u32x2*)(base + k_chunk<16>(d, s.o, C.logP) + (d & 8)) = u32x2{p.w[0], p.w[1]};
+    if (d == 0) *(float*)(base + k_scale<D>(s.o, C.logP)) = p.scale;
+  } else {
+    *(u32x4*)(base + k_chunk<8>(d, s.o, C.logP)) = p.w;
   }
 }
 
@@ -273,23 +293,23 @@ __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
   }
   if (kind == 0) {
     *(u32x4*)(A.q_out + ((int64_t)t * A.q_heads + h) * D + d) = narrow(r);
-  } else if (kind == 1) {
-    put_key<D, F8>(C, r, s, h, d);
-  } else {
-    char* base = C.pages + s.page + (int64_t)h * C.head_bytes;
-    char* p = base + v_chunk<E, D>(d, s.o, C.logP) + s.o % E * (16 / E);
-    if (F8) {
-      float scale;
-      const u32x2 c = encode_row<D>(r, &scale);
-      if (s.page < 0) return;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) *(uint8_t*)(p + 16 * i) = (uint8_t)(c[i / 4] >> 8 * (i % 4));
-      if (d == 0) *(float*)(base + v_scale<D>(s.o, C.logP)) = scale;
-    } else if (s.page >= 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) *(uint16_t*)(p + 16 * i) = (uint16_t)(in[i / 2] >> 16 * (i % 2));
-    }
+    return;
   }
+  Part y = page_part<D, F8>(r);
+  if (kind == 1) {
+    put_key<D, F8>(C, y, s, h, d);
+    return;
+  }
+  if (s.page < 0) return;
+  if (!F8) y.w = in;                         // as it came, NaN's bits too
+  char* base = C.pages + s.page + (int64_t)h * C.head_bytes;
+  char* p = base + v_chunk<E, D>(d, s.o, C.logP) + s.o % E * (16 / E);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (F8) *(uint8_t*)(p + 16 * i) = (uint8_t)(y.w[i / 4] >> 8 * (i % 4));
+    else *(uint16_t*)(p + 16 * i) = (uint16_t)(y.w[i / 2] >> 16 * (i % 2));
+  }
+  if (F8 && d == 0) *(float*)(base + v_scale<D>(s.o, C.logP)) = y.scale;
 }
 
 // Prompts: neighbouring tokens share lines of the pages, so a workgroup takes
@@ -338,7 +358,7 @@ __global__ __launch_bounds__(256) void append_tiles(AppendArgs A, int qk, int gr
       if (A.norm[q ? 0 : 1]) norm_row<D>(r, q ? wq : wk, A.eps);
       turn_row(A, r, turn, d);
       if (q) *(u32x4*)(A.q_out + ((int64_t)t * A.q_heads + hh) * D + d) = narrow(r);
-      else put_key<D, F8>(C, r, s, hh - A.q_heads, d);
+      else put_key<D, F8>(C, page_part<D, F8>(r), s, hh - A.q_heads, d);
     }
     return;
   }
