@@ -901,8 +901,10 @@ static int row_tiles(int64_t rows, int most) {
 // and 20; 64 requests of 20 new of 2048, 16 / 2 heads: 58 and 68).  But where three
 // fill at least an eighth more rows than four, calls that have many units are faster
 // with four (64 requests of 32 new tokens of 512, 32 / 8 heads: 47 us, with three 61;
-// of 8192: 506 and 557; 16 requests of 64 new of 512: 30 and 26).  head_units: the
-// units that one row block of each sequence and kv head may have, all together.
+// of 8192: 506 and 557; 16 requests of 64 new of 512: 30 and 26), if all sequences have
+// as many rows (42 of 16206 tokens, 1 to 15 new, 24 / 3 heads: 224 and 180).
+// head_units: the units that one row block of each sequence and kv head may have, all
+// together, or 0.
 constexpr int64_t ATT_FOUR_UNITS = 24576;
 static int attend_tiles(int64_t rows, int D, int dtype, int64_t head_units) {
   if (D == 256) return row_tiles(rows, 1);
@@ -1047,9 +1049,10 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   A.G = q_heads / kv->kv_heads;
   max_new = std::min(max_new, kv->T);        // no sequence has more
   const int D = kv->head_dim;
+  const bool even = kv->T >= (int64_t)kv->B * max_new;
   const int64_t table_units = (int64_t)kv->max_pages * kv->page_tokens / 32;
   const int nt = cx::attend_tiles((int64_t)A.G * max_new, D, kv->dtype,
-                                  (int64_t)kv->B * kv->kv_heads * table_units);
+                                  even ? (int64_t)kv->B * kv->kv_heads * table_units : 0);
   const cx::AttendWork lay = cx::attend_workspace(nt, D, kv->dtype);
   if (ws_bytes < lay.total)
     return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, lay.total);
