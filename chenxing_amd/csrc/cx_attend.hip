@@ -922,14 +922,17 @@ static int workgroups(int nt, int D, int dtype) {
   return 256 * (D * nt == 64 ? (f8 ? 3 : 4) : D * nt < 256 || (nt == 2 && !f8) ? 2 : 1);
 }
 
-// The join: a workgroup a row where a row block may have more than ATT_JOIN_PARTS / D
-// parts, as many as its share of the workers or as the longest context's units make
-// (a workgroup a row and a wave a row, heads of 64: 2 new tokens of 30000, one request
-// of 4 kv heads, 9 and 14 us; 32 of 3000: 12 and 5; 8 requests of 2500: 9 and 5; heads
-// of 128: one of 8000, 8 kv heads, 5 and 8; 32 new of 30000: 8 and 7); else a wave a
-// row, unless that is many workgroups (4 rounds of 13 rows over 8014 tokens, heads of
-// 64: 6 us, 16 rows a workgroup 15).
-constexpr int64_t ATT_JOIN_PARTS = 8192, ATT_JOIN_ROWS = 8192;
+// The join: a workgroup a row where a row block may have more than join_parts parts,
+// as many as its share of the workers or as the longest context's units make; else a
+// wave a row, unless that is many workgroups (4 rounds of 13 rows over 8014 tokens,
+// heads of 64: 6 us, 16 rows a workgroup 15).  A wave adds 512 / D parts of 8 dims a
+// lane together; a workgroup a row as many for each of its four waves, but then joins
+// 2048 / D sums one after the other (a workgroup a row and a wave a row, heads of 64: 2
+// new tokens of 30000, one request of 4 kv heads, 9 and 14 us; 32 of 3000: 12 and 5; 8
+// requests of 2500: 9 and 5; of 128: one of 8000, 8 kv heads, 5 and 8; 12 new of 3000:
+// 6.5 and 5.3; of 256: one of 3000, one kv head: 4.4 and 6.1).
+constexpr int join_parts(int D) { return D == 64 ? 192 : D == 128 ? 64 : 20; }
+constexpr int64_t ATT_JOIN_ROWS = 8192;
 
 struct AttendWork {
   size_t off_join, off_ml, off_part, total;
@@ -985,7 +988,7 @@ static int launch_tile(AttendArgs A, int64_t max_new, hipStream_t s) {
                                             grid * ATT_WAVES);
   const int64_t parts = std::min<int64_t>(
       grid * ATT_WAVES / entries, ((span + Sh::TOK - 1) / Sh::TOK + Sh::Line::PIECE) / ATT_SHARE + 1);
-  if (parts * D > ATT_JOIN_PARTS)
+  if (parts > join_parts(D))
     timed_launch(CX_KERNEL_ATTEND_JOIN, attend_join_row<D, ROWS>, dim3((unsigned)entries, ROWS),
                  dim3(256), 0, s, A);
   else
