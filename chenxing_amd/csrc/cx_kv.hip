@@ -267,7 +267,7 @@ __device__ __forceinline__ void put_key(const KvArgs& C, const Part& p, const Sl
 // One row (token, head) of q, k or v to D / 8 lanes, every row of the call at
 // once: q heads first, then k, then v.  A small call is one latency, launch and
 // loads (1 token, 48 heads of 128: 3.7 us); a row's v leaves as one element a chunk,
-// so in a large one the stores bound it (256 tokens of as many sequences 7.0 us, 256
+// so in a large one the stores bound it (256 tokens of as many sequences 6.9 us, 256
 // prompts of 64 tokens 251 us).
 template <int D, bool F8>
 __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
@@ -322,8 +322,8 @@ __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
 //  * The others: VT tokens of one head of v.  They pass through LDS, and the
 //    tokens of a chunk that are all here leave as 16 bytes a dim.
 //
-// Bound: HBM.  5 prompts of 2500 tokens, 48 heads of 128, e4m3: 217 MB in 53 us,
-// 4.1 TB/s where a copy reaches 4.75 (append_rows 125 us); bf16: 219 MB in 47 us.
+// Bound: HBM.  5 prompts of 2500 tokens, 48 heads of 128, e4m3: 217 MB in 52 us,
+// 4.2 TB/s where a copy reaches 4.75 (append_rows 125 us); bf16: 219 MB in 47 us.
 constexpr int APPEND_HEADS = 8, APPEND_VT = 64;
 
 template <int D, bool F8>
