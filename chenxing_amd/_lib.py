@@ -57,6 +57,21 @@ _SIGS = {
     "cx_kv_append_bf16": (C.c_int, [C.c_char_p, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64,
                                     _P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int32, C.c_int32,
                                     C.c_int32, _P, _P, C.c_double, _P, _P]),
+    "cx_kv_append_tree_bf16": (C.c_int, [C.c_char_p, _P, C.c_int64, C.c_int64, _P, C.c_int64,
+                                         C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, _P,
+                                         C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_double, _P,
+                                         _P, _P]),
+    "cx_tree_attention_bf16": (C.c_int, [C.c_char_p, _P, C.c_int64, C.c_int64, C.c_int32, _P,
+                                         C.c_int32, _P, C.c_int32, C.c_double, C.c_int32,
+                                         C.c_double, _P, _P, C.c_size_t, _P]),
+    "cx_tree_attention_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32,
+                                                       C.c_int32]),
+    "cx_tree_masks": (C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, _P, _P]),
+    "cx_tree_accept": (C.c_int, [_P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P,
+                                 _P]),
+    "cx_kv_commit": (C.c_int, [C.c_char_p, C.c_int64, C.c_int32, _P, C.c_int32, _P, _P]),
+    "cx_w4_linear_bf16": (C.c_int, [_P, C.c_int64, _P, _P, C.c_int32, C.c_int32, C.c_int32,
+                                    C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P]),
     "cx_paged_attention_bf16": (C.c_int, [C.c_char_p, _P, C.c_int64, C.c_int64, C.c_int32,
                                           C.c_int32, C.c_double, C.c_int32, C.c_double, _P, _P,
                                           C.c_size_t, _P]),
@@ -270,6 +285,7 @@ _ws_sample = Workspace()
 _ws_verify = Workspace()
 _ws_head = Workspace()
 _ws_attend = Workspace()
+_ws_tree = Workspace()
 
 
 def _stream_ptr(device):
@@ -418,6 +434,7 @@ def lmhead_argmax_device(hidden, weight, out_id=None, out_max=None, out_logits=N
 # cx_kv_batch of include/cx_sampler.h
 _KV_BATCH = struct.Struct("<QqQqQQ8i")
 KV_BF16, KV_E4M3 = 1, 3
+KV_MAX_NEW = 1 << 28
 
 
 def _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T, page_tokens=None):
@@ -493,8 +510,16 @@ def _out3(torch, name, t, q, dev, shape):
     return t
 
 
+def _i32_rows(torch, name, t, dev, shape):
+    """The address of a contiguous int32 tensor of that shape on device ``dev``."""
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{name} must be a contiguous int32 {list(shape)} on the call's device (a "
+                         "cuda device)")
+    return t.data_ptr()
+
+
 def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, interleaved=False,
-                     q_norm=None, k_norm=None, eps=1e-6, q_out=None, page_tokens=None):
+                     q_norm=None, k_norm=None, eps=1e-6, q_out=None, page_tokens=None, depth=None):
     """The new tokens' q, k and v made ready for attention, on the current stream.
 
     q [T, Hq, D], k and v [T, Hkv, D] (bfloat16, any token and head strides that
@@ -505,7 +530,9 @@ def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, int
     ``table`` [B, pages], ``kv_len`` [B] (the new tokens included) and
     ``q_start`` [B + 1] (None: one new token each) are int32.  A page's tokens
     follow from its width and D; ``page_tokens``, if given, has to agree.
-    Returns q_out [T, Hq, D]."""
+    ``depth`` [T] int32: a drafted tree's nodes, rotated to their sequence's first
+    new position plus their depth (``tree_masks_device``) and written to
+    neighbouring places.  Returns q_out [T, Hq, D]."""
     import torch
     lib = _lib or load()
     dev, shape, qs = _q_rows(torch, q)
@@ -529,9 +556,13 @@ def kv_append_device(q, k, v, cache, table, kv_len, q_start=None, rope=None, int
                 raise ValueError("q_norm and k_norm must be contiguous bfloat16 [D] on q's device")
             norms[i] = w.data_ptr()
     q_out = _out3(torch, "q_out", q_out, q, dev, shape)
-    _call(torch, dev, lib.cx_kv_append_bf16, kv, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0],
-          ks[1], v.data_ptr(), vs[0], vs[1], Hq, rp, rows, rdim, interleaved, *norms, eps,
-          q_out.data_ptr())
+    head = (kv, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+            Hq, rp, rows, rdim, interleaved, *norms, eps)
+    if depth is None:
+        _call(torch, dev, lib.cx_kv_append_bf16, *head, q_out.data_ptr())
+    else:
+        _i32_rows(torch, "depth", depth, dev, (T,))
+        _call(torch, dev, lib.cx_kv_append_tree_bf16, *head, depth.data_ptr(), q_out.data_ptr())
     return q_out
 
 
@@ -601,6 +632,173 @@ def kv_copy_pages_device(cache, src, dst):
     return cache
 
 
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(q_heads, kv_heads, D, max_new):
+    return load().cx_tree_attention_workspace_bytes(q_heads, kv_heads, D, max_new)
+
+
+def tree_attention_device(q, cache, table, kv_len, mask, q_start=None, depth=None, max_new=1,
+                          scale=None, window=0, softcap=0.0, out=None, page_tokens=None):
+    """Attention of drafted trees over one layer's pages, on the current stream.
+
+    As ``paged_attention_device``, but a sequence's new tokens are the nodes of a
+    tree: ``mask`` [T, words] int64 says which of them a node attends to (bit i %
+    64 of word i // 64: node i, as ``tree_masks_device`` gives them); all attend
+    to the tokens before them.  A ``window`` > 0 needs ``depth`` [T] int32 and
+    counts from a node's depth, over the tokens before the tree."""
+    import torch
+    lib = _lib or load()
+    dev, shape, qs = _q_rows(torch, q)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return tree_attention_device(q, cache, table, kv_len, mask, q_start, depth, max_new,
+                                         scale, window, softcap, out, page_tokens)
+    T, Hq, D = shape
+    kv, heads = _kv_batch(torch, dev, cache, D, table, kv_len, q_start, T, page_tokens)
+    ms = mask.shape
+    if mask.dtype != torch.int64 or len(ms) != 2 or ms[0] != T or not mask.is_contiguous() or \
+            mask.get_device() != dev:
+        raise ValueError("mask must be a contiguous int64 [tokens, words] on q's device")
+    dp = None if depth is None else _i32_rows(torch, "depth", depth, dev, (T,))
+    out = _out3(torch, "out", out, q, dev, shape)
+    nbytes = _tree_workspace(Hq, heads, D, max_new)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    key = dev, stream
+    with _ws_tree.of(key):
+        ws = _ws_tree.get(key, nbytes, q, torch._C._cuda_isCurrentStreamCapturing())
+        rc = lib.cx_tree_attention_bf16(
+            kv, q.data_ptr(), qs[0], qs[1], Hq, mask.data_ptr(), ms[1], dp, max_new,
+            D ** -0.5 if scale is None else scale, window, softcap, out.data_ptr(), ws.data_ptr(),
+            ws.numel(), stream)
+        if rc != CX_OK:
+            _check(rc)
+    return out
+
+
+def _tree_rows(torch, parents, q_start):
+    """(device, nodes, sequences, q_start's address) of a batch of trees."""
+    dev, T = parents.get_device(), parents.numel()
+    if dev < 0 or parents.dim() != 1:
+        raise ValueError("parents must be an int32 [nodes] cuda tensor")
+    _i32_rows(torch, "parents", parents, dev, (T,))
+    if q_start is None:
+        return dev, T, T, None
+    return dev, T, q_start.numel() - 1, _i32_rows(torch, "q_start", q_start, dev,
+                                                  (max(q_start.numel(), 1),))
+
+
+def tree_masks_device(parents, q_start=None, words=1):
+    """(mask [T, words] int64, depth [T] int32) of drafted trees, on the current
+    stream: the bits of every node and its ancestors, and how many these are.
+
+    ``parents`` [T] int32: a node's parent among the nodes of its sequence, below
+    the node's own index; -1 (or anything else) for a root.  ``q_start`` [B + 1]
+    int32 as for the attention.  ``words``: 64 nodes each."""
+    import torch
+    lib = _lib or load()
+    dev, T, B, start = _tree_rows(torch, parents, q_start)
+    mask = torch.empty(T, words, dtype=torch.int64, device=parents.device)
+    depth = torch.empty(T, dtype=torch.int32, device=parents.device)
+    _call(torch, dev, lib.cx_tree_masks, parents.data_ptr(), start, B, T, mask.data_ptr(), words,
+          depth.data_ptr())
+    return mask, depth
+
+
+def tree_accept_device(parents, tokens, sampled, width, q_start=None):
+    """The path of every tree that the sampled ids follow, on the current stream.
+
+    Node 0, the last confirmed token, is accepted; after a node comes its first
+    child whose token (``tokens`` [T] int32) is the id sampled after it
+    (``sampled`` [T] int32, of any sampler, for instance ``sample_device`` on the
+    nodes' logits), up to ``width`` nodes.  Returns (path [B, width], filled up
+    with -1, count [B], next [B]: the id sampled after the last accepted node),
+    int32."""
+    import torch
+    lib = _lib or load()
+    dev, T, B, start = _tree_rows(torch, parents, q_start)
+    tok = _i32_rows(torch, "tokens", tokens, dev, (T,))
+    ids = _i32_rows(torch, "sampled", sampled, dev, (T,))
+    path = torch.empty(B, width, dtype=torch.int32, device=parents.device)
+    count, nxt = torch.empty(2, B, dtype=torch.int32, device=parents.device)
+    _call(torch, dev, lib.cx_tree_accept, parents.data_ptr(), tok, ids, start, B, T, width,
+          path.data_ptr(), count.data_ptr(), nxt.data_ptr())
+    return path, count, nxt
+
+
+def kv_commit_device(cache, head_dim, table, kv_len, path, count=None, q_start=None,
+                     page_tokens=None):
+    """The accepted nodes' keys and values moved to the first places of their
+    sequence's new tokens in every layer, on the current stream: place j gets what
+    is at place path[b, j], for j < count[b].
+
+    ``cache`` is [layers, n_pages, kv_heads, width] or one layer of it; ``table``,
+    ``kv_len`` (the drafted tokens included) and ``q_start`` are those of the pass
+    that appended them; ``path`` [B, width] and ``count`` [B] int32 come from
+    ``tree_accept_device``.  A row of path ends where it does not rise.  Returns
+    cache."""
+    import torch
+    lib = _lib or load()
+    dev, shape = cache.get_device(), cache.shape
+    if dev < 0 or len(shape) not in (3, 4):
+        raise ValueError("cache must be a cuda tensor [layers, n_pages, kv_heads, width] or one "
+                         "layer of it")
+    layers, stride, layer = 1, 0, cache
+    if len(shape) == 4:
+        layers, stride = shape[0], cache.stride(0) * cache.element_size()
+        if layers == 0:
+            return cache
+        layer = cache[0]
+    B = table.shape[0]
+    if q_start is None:
+        T = B
+    else:
+        T = KV_MAX_NEW                         # any: the rows follow from q_start
+    kv, _ = _kv_batch(torch, dev, layer, head_dim, table, kv_len, q_start, T, page_tokens)
+    if path.dim() != 2:
+        raise ValueError("path must be int32 [B, width]")
+    pp = _i32_rows(torch, "path", path, dev, (B, path.shape[1]))
+    cp = None if count is None else _i32_rows(torch, "count", count, dev, (B,))
+    _call(torch, dev, lib.cx_kv_commit, kv, stride, layers, pp, path.shape[1], cp)
+    return cache
+
+
+def w4_linear_device(x, tiles, scales, N, dtype=None, out=None):
+    """x [M, K] (bfloat16) times 4-bit weights [N, K], on the current stream:
+    [M, N] of ``dtype`` (float32, the default, or bfloat16) or in ``out``.
+
+    ``tiles`` and ``scales`` as ``w4.pack`` lays them out (include/cx_sampler.h
+    has the format); the weights are read once for up to 64 rows of x."""
+    import torch
+    lib = _lib or load()
+    dev = x.get_device()
+    if dev < 0 or x.dim() != 2 or x.dtype != torch.bfloat16 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("x must be a bfloat16 [rows, K] cuda matrix with unit column stride")
+    M, K = x.shape
+    ts, ss = tiles.shape, scales.shape
+    n16, k128 = -(-N // 16), -(-K // 128)
+    if tiles.dtype != torch.int32 or ts != (n16, k128, 64, 4) or not tiles.is_contiguous() or \
+            tiles.get_device() != dev:
+        raise ValueError(f"tiles must be a contiguous int32 [{n16}, {k128}, 64, 4] on x's device")
+    groups = ss[1] if len(ss) > 1 else 0
+    if scales.dtype != torch.float16 or len(ss) not in (3, 4) or ss[0] != n16 or ss[2] != 16 or \
+            ss[3:] not in ((), (2,)) or groups < 1 or K % groups or not scales.is_contiguous() or \
+            scales.get_device() != dev:
+        raise ValueError(f"scales must be a contiguous float16 [{n16}, K / group, 16] or "
+                         f"[{n16}, K / group, 16, 2] on x's device")
+    if out is None:
+        dtype = torch.float32 if dtype is None else dtype
+        out = torch.empty(M, N, dtype=dtype, device=x.device)
+    if out.dtype not in (torch.float32, torch.bfloat16) or dtype not in (None, out.dtype) or \
+            out.shape != (M, N) or (out.stride(1) != 1 and N > 1) or out.get_device() != dev:
+        raise ValueError("out must be float32 or bfloat16 [rows, N] on x's device, with unit column "
+                         "stride")
+    ldx = x.stride(0) if M > 1 else K
+    ldo = out.stride(0) if M > 1 else N
+    _call(torch, dev, lib.cx_w4_linear_bf16, x.data_ptr(), ldx, tiles.data_ptr(), scales.data_ptr(),
+          len(ss) == 4, K // groups, M, N, K, out.data_ptr(), ldo, out.dtype == torch.bfloat16)
+    return out
+
+
 def header_symbols() -> list[str]:
     """Function names declared in include/cx_sampler.h."""
     import re
@@ -613,8 +811,9 @@ def header_symbols() -> list[str]:
 (KERNEL_SAMPLE, KERNEL_SAMPLE_SLOW, KERNEL_VERIFY_STATS, KERNEL_VERIFY_REST,
  KERNEL_SAMPLE_FINISH, KERNEL_PENALTIES, KERNEL_TRUNCATE, KERNEL_LMHEAD,
  KERNEL_LMHEAD_MERGE, KERNEL_KV_APPEND, KERNEL_ATTEND,
- KERNEL_ATTEND_JOIN, KERNEL_KV_COPY) = range(13)
-KERNEL_KINDS = 13
+ KERNEL_ATTEND_JOIN, KERNEL_KV_COPY, KERNEL_TREE, KERNEL_TREE_JOIN, KERNEL_TREE_WALK,
+ KERNEL_KV_COMMIT, KERNEL_W4) = range(18)
+KERNEL_KINDS = 18
 
 
 def timing_enable(on: bool = True) -> None:

@@ -65,13 +65,14 @@ struct AppendArgs {
   int rdim;
   int interleaved;
   const uint16_t* norm[2];    // nullable: q, k
+  const int32_t* depth;       // nullable: positions from the first new one
   float eps;
   uint16_t* q_out;
 };
 
-// The sequence of new token t and its position: the last b with
-// q_start[b] <= t.  -1 for a token outside every sequence.
-__device__ __forceinline__ int2 token_place(const KvArgs& A, int t) {
+// The sequence of new token t, its position and its sequence's first new one: the last
+// b with q_start[b] <= t.  -1 for a token outside every sequence.
+__device__ __forceinline__ int3 token_place(const KvArgs& A, int t) {
   int b = t, i = 0, n = 1;
   if (A.q_start) {
     int lo = 0, hi = A.B;                     // first b with q_start[b + 1] > t
@@ -80,13 +81,14 @@ __device__ __forceinline__ int2 token_place(const KvArgs& A, int t) {
       if (A.q_start[mid + 1] > t) hi = mid;
       else lo = mid + 1;
     }
-    if (lo >= A.B) return make_int2(-1, -1);
+    if (lo >= A.B) return make_int3(-1, -1, -1);
     b = lo;
     const int2 r = kv_rows(A, b);
     i = t - r.x;
     n = r.y - r.x;
   }
-  return make_int2(b, (int)(A.kv_len[b] - (unsigned)n + (unsigned)i));
+  const unsigned first = A.kv_len[b] - (unsigned)n;
+  return make_int3(b, (int)(first + (unsigned)i), (int)first);
 }
 
 // A row's lane of 8 dims, d .., as floats.
@@ -218,16 +220,19 @@ __device__ __forceinline__ u32x2 encode_row(const Row8& r, float* scale) {
 }
 
 // Where a new token goes: byte offset of its page (-1: nowhere) and its place
-// in the page.
+// in the page; pos: the position that it is rotated to.
 struct Slot {
   int64_t page;
   int o, pos;
 };
-__device__ __forceinline__ Slot token_slot(const KvArgs& C, int t) {
-  const int2 at = token_place(C, t);
+__device__ __forceinline__ Slot token_slot(const KvArgs& C, int t, const int32_t* depth) {
+  const int3 at = token_place(C, t);
   Slot s = {-1, 0, 0};
-  if (at.x < 0 || at.y < 0 || at.y >= (C.M << C.logP)) return s;
+  const int held = C.M << C.logP;
+  if (at.x < 0 || at.y < 0 || at.y >= held) return s;
   s.pos = at.y;
+  // (the sum in 64 bits: depths are the caller's)
+  if (depth) s.pos = (int)min(max((int64_t)at.z + depth[t], (int64_t)0), (int64_t)held - 1);
   s.o = at.y & ((1 << C.logP) - 1);
   const int id = C.table[at.x * C.ld_table + (at.y >> C.logP)];
   if ((unsigned)id < (unsigned)C.n_pages) s.page = id * C.page_stride;
@@ -284,7 +289,7 @@ __global__ __launch_bounds__(256) void append_rows(AppendArgs A) {
   const uint16_t* w = kind < 2 ? A.norm[kind] : nullptr;
   u32x4 wv = {};
   if (w) wv = *(const u32x4*)(w + d);
-  const Slot s = token_slot(C, t);
+  const Slot s = token_slot(C, t, A.depth);
   Row8 r = widen(in);
   if (kind < 2) {
     const Turn8 turn = load_turn(A, s.pos, d);
@@ -349,7 +354,7 @@ __global__ __launch_bounds__(256) void append_tiles(AppendArgs A, int qk, int gr
     u32x4 wq = {}, wk = {};
     if (A.norm[0]) wq = *(const u32x4*)(A.norm[0] + d);
     if (A.norm[1]) wk = *(const u32x4*)(A.norm[1] + d);
-    const Slot s = token_slot(C, t);
+    const Slot s = token_slot(C, t, A.depth);
     const Turn8 turn = load_turn(A, s.pos, d);
     for (int hh = h0; hh < end; ++hh) {
       Row8 r = widen(next);
@@ -367,7 +372,7 @@ __global__ __launch_bounds__(256) void append_tiles(AppendArgs A, int qk, int gr
   const int n = min(VT, C.T - t0);
   if (tid < VT) {                            // one wave
     Slot s = {-1, 0, 0};
-    if (tid < n) s = token_slot(C, t0 + tid);
+    if (tid < n) s = token_slot(C, t0 + tid, nullptr);
     // runs: neighbouring tokens that go to neighbouring places of one chunk
     const int64_t before = __shfl_up(s.page, 1);
     const int at = __shfl_up(s.o, 1);
@@ -488,6 +493,63 @@ __global__ __launch_bounds__(256) void copy_pages(CopyArgs A) {
   }
 }
 
+struct CommitArgs {
+  KvArgs kv;
+  int64_t layer_stride;
+  int n_layers, width;
+  const int32_t* path;        // [B, width]
+  const int32_t* count;       // nullable [B]
+};
+
+// Workgroup (sequence, layer, head): a thread a 16-byte chunk of the keys, a dim of the
+// values, or the scales, each token after the other: a path rises, so what a move
+// overwrites has been read.
+template <int D, bool F8>
+__global__ __launch_bounds__(256) void commit_tokens(CommitArgs A) {
+  constexpr int E = F8 ? 16 : 8, KC = D / E;
+  const KvArgs& C = A.kv;
+  const unsigned x = blockIdx.x / (unsigned)C.heads, h = blockIdx.x % (unsigned)C.heads;
+  const int b = (int)(x / (unsigned)A.n_layers);
+  const int2 rows = kv_rows(C, b);
+  const int n = rows.y - rows.x, P = 1 << C.logP;
+  const int64_t s0 = (int64_t)C.kv_len[b] - n;
+  if (s0 < 0) return;
+  char* base = C.pages + (x % (unsigned)A.n_layers) * A.layer_stride + (int64_t)h * C.head_bytes;
+  const int32_t* path = A.path + (int64_t)b * A.width;
+  const int m = A.count ? min(A.count[b], A.width) : A.width;
+  auto place = [&](int64_t slot, int* o) {
+    *o = (int)(slot & (P - 1));
+    const int64_t at = slot >> C.logP;
+    const int id = at < C.M ? C.table[b * C.ld_table + at] : -1;
+    return (unsigned)id < (unsigned)C.n_pages ? base + id * C.page_stride : nullptr;
+  };
+  for (int i = threadIdx.x; i < KC + D + (F8 ? 2 : 0); i += 256) {
+    for (int j = 0, last = -1; j < m; ++j) {
+      const int p = path[j];
+      if (p <= last || p >= n) break;
+      last = p;
+      if (p == j) continue;
+      int so, to;
+      const char* from = place(s0 + p, &so);
+      char* dst = place(s0 + j, &to);
+      if (!from || !dst) continue;
+      if (i < KC) {
+        *(u32x4*)(dst + k_chunk<E>(i * E, to, C.logP)) = *(const u32x4*)(from + k_chunk<E>(i * E, so, C.logP));
+      } else if (i < KC + D) {
+        const int d = i - KC;
+        const char* f = from + v_chunk<E, D>(d, so, C.logP) + so % E * (16 / E);
+        char* t = dst + v_chunk<E, D>(d, to, C.logP) + to % E * (16 / E);
+        if (F8) *(uint8_t*)t = *(const uint8_t*)f;
+        else *(uint16_t*)t = *(const uint16_t*)f;
+      } else if (i == KC + D) {
+        *(uint32_t*)(dst + k_scale<D>(to, C.logP)) = *(const uint32_t*)(from + k_scale<D>(so, C.logP));
+      } else {
+        *(uint32_t*)(dst + v_scale<D>(to, C.logP)) = *(const uint32_t*)(from + v_scale<D>(so, C.logP));
+      }
+    }
+  }
+}
+
 template <int D, bool F8>
 static void launch_append(const AppendArgs& A, hipStream_t s) {
   const unsigned per = 256 / (D / 8), heads = A.q_heads + A.kv.heads;
@@ -525,6 +587,17 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
                       int32_t rope_rows, int32_t rotary_dim, int32_t interleaved,
                       const uint16_t* q_norm, const uint16_t* k_norm, double eps,
                       uint16_t* q_out, void* stream) {
+  return cx_kv_append_tree_bf16(kv, q, q_token, q_head, k, k_token, k_head, v, v_token, v_head,
+                                q_heads, rope, rope_rows, rotary_dim, interleaved, q_norm, k_norm,
+                                eps, nullptr, q_out, stream);
+}
+
+int cx_kv_append_tree_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
+                           int64_t q_head, const uint16_t* k, int64_t k_token, int64_t k_head,
+                           const uint16_t* v, int64_t v_token, int64_t v_head, int32_t q_heads,
+                           const float* rope, int32_t rope_rows, int32_t rotary_dim,
+                           int32_t interleaved, const uint16_t* q_norm, const uint16_t* k_norm,
+                           double eps, const int32_t* depth, uint16_t* q_out, void* stream) {
   cx::AppendArgs A;
   const int rc = cx::kv_args(kv, q_heads, &A.kv);
   if (rc != CX_OK) return rc;
@@ -552,6 +625,7 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
   A.rdim = A.rope ? rotary_dim : 0;
   A.interleaved = interleaved;
   A.norm[0] = q_norm; A.norm[1] = k_norm;
+  A.depth = depth;
   A.eps = (float)eps;
   A.q_out = q_out;
   const hipStream_t s = (hipStream_t)stream;
@@ -587,6 +661,35 @@ int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int
                    dim3(256), 0, (hipStream_t)stream, A);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return cx::api_fail(CX_EHIP, "page copy launch: %s", hipGetErrorString(e));
+  return CX_OK;
+}
+
+int cx_kv_commit(const cx_kv_batch* kv, int64_t layer_stride, int32_t n_layers,
+                 const int32_t* path, int32_t width, const int32_t* count, void* stream) {
+  cx::CommitArgs A;
+  const int rc = cx::kv_args(kv, kv ? kv->kv_heads : 1, &A.kv);
+  if (rc != CX_OK) return rc;
+  if (n_layers < 0 || width < 0 || layer_stride < 0 || layer_stride % 16)
+    return cx::api_fail(CX_EINVAL, "bad shape");
+  if (kv->T == 0 || kv->B == 0 || kv->n_pages == 0 || kv->max_pages == 0 || n_layers == 0 || width == 0)
+    return CX_OK;
+  if (!path) return cx::api_fail(CX_EINVAL, "null pointer argument");
+  if ((int64_t)kv->B * n_layers > INT32_MAX / kv->kv_heads)
+    return cx::api_fail(CX_EINVAL, "too many layers in one call");
+  A.layer_stride = layer_stride;
+  A.n_layers = n_layers;
+  A.width = width;
+  A.path = path;
+  A.count = count;
+  using Kernel = void (*)(cx::CommitArgs);
+  const bool f8 = kv->dtype == CX_KV_E4M3;
+  const Kernel k = kv->head_dim == 64    ? (f8 ? (Kernel)cx::commit_tokens<64, true> : cx::commit_tokens<64, false>)
+                   : kv->head_dim == 128 ? (f8 ? (Kernel)cx::commit_tokens<128, true> : cx::commit_tokens<128, false>)
+                                         : (f8 ? (Kernel)cx::commit_tokens<256, true> : cx::commit_tokens<256, false>);
+  cx::timed_launch(CX_KERNEL_KV_COMMIT, k, dim3((unsigned)(kv->B * n_layers * kv->kv_heads)), dim3(256),
+                   0, (hipStream_t)stream, A);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return cx::api_fail(CX_EHIP, "commit launch: %s", hipGetErrorString(e));
   return CX_OK;
 }
 

@@ -6,6 +6,8 @@ class, over one pool tensor that the device calls take as it is:
 
   ``_lib.kv_append_device``        writes a step's new tokens
   ``_lib.paged_attention_device``  attends over the pages
+  ``_lib.tree_attention_device``   attends for a tree of drafted tokens
+  ``_lib.kv_commit_device``        keeps the accepted ones (``commit``)
   ``_lib.kv_copy_pages_device``    copies pages over all layers
 
 Sequences share pages: ``fork`` copies none, and the first of the sharers to
@@ -82,6 +84,7 @@ class PagedKVCache:
         self.pool = torch.zeros(layers, pages, kv_heads, width, device=device,
                                 dtype=torch.bfloat16 if dtype == "bf16" else torch.uint8)
         self.page_tokens = page_tokens
+        self._head_dim = head_dim
         self._copy = copy
         self._free = list(range(pages))       # a heap: the lowest ids are handed out first
         self._refs = [0] * pages
@@ -156,6 +159,24 @@ class PagedKVCache:
         for p in pages[keep:]:
             self._drop(p)
         self._seqs[seq] = [pages[:keep], length]
+
+    def commit(self, seqs, batch, path, count) -> list[int]:
+        """A round of drafted trees ends: of the last tokens of seqs[i], those that
+        ``batch`` appended, path[i, :count[i]] stay, in that order (``path`` and
+        ``count`` as ``_lib.tree_accept_device`` gives them); how many of each."""
+        from . import _lib
+        start = batch["q_start"]
+        new = [1] * len(seqs) if start is None else start.diff().tolist()
+        kept = count.tolist()
+        if len(set(seqs)) != len(seqs) or len(new) != len(seqs) or len(kept) != len(seqs):
+            raise ValueError("commit takes each sequence of the batch once")
+        if any(not 0 <= c <= n <= self._seqs[s][1] for s, c, n in zip(seqs, kept, new)):
+            raise ValueError("count must be in [0, new tokens of the sequence]")
+        _lib.kv_commit_device(self.pool, self._head_dim, batch["table"], batch["kv_len"], path, count,
+                              start, self.page_tokens)
+        for s, c, n in zip(seqs, kept, new):
+            self.truncate(s, self._seqs[s][1] - n + c)
+        return kept
 
     def free(self, seq: int) -> None:
         self.truncate(seq, 0)

@@ -271,6 +271,7 @@ size_t cx_lmhead_workspace_bytes(int32_t B, int32_t V);
 #define CX_KV_BF16 1
 #define CX_KV_E4M3 3                     /* OCP e4m3: largest value 448 */
 #define CX_KV_MAX_BATCH 4096
+#define CX_TREE_MAX_WORDS 16             /* nodes of a tree that masks reach: 1024 */
 typedef struct cx_kv_batch {
   void* pages;               /* one layer's pages, 16-byte aligned             */
   int64_t page_stride;       /* bytes from one page to the next                */
@@ -315,6 +316,21 @@ int cx_kv_append_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
                       uint16_t* q_out, void* stream);
 
 /*
+ * The same for a tree of drafted tokens: the new token of row t is written to its
+ * place as above, but rotated as at position kv_len[b] - n + depth[t], n the new
+ * tokens of its sequence (siblings stand at one position); clamped to the rows of
+ * the table's pages.
+ *
+ *  depth      [T] int32, or NULL: as above
+ */
+int cx_kv_append_tree_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
+                           int64_t q_head, const uint16_t* k, int64_t k_token, int64_t k_head,
+                           const uint16_t* v, int64_t v_token, int64_t v_head, int32_t q_heads,
+                           const float* rope, int32_t rope_rows, int32_t rotary_dim,
+                           int32_t interleaved, const uint16_t* q_norm, const uint16_t* k_norm,
+                           double eps, const int32_t* depth, uint16_t* q_out, void* stream);
+
+/*
  * Attention of the new tokens over the pages: a decode step's single tokens, a
  * verify round's gamma + 1, several together.  q head h reads kv head
  * h / (q_heads / kv_heads).  The token at position p attends to the
@@ -349,6 +365,81 @@ size_t cx_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int
                                           int32_t max_new);
 
 /*
+ * Attention of a tree of drafted tokens: as cx_paged_attention_bf16, but which of
+ * the new tokens a new token attends to is given.  The n new tokens of sequence b
+ * are its nodes 0 .. n - 1, in the slots kv_len[b] - n ..  A node attends to every
+ * slot before them and to the nodes whose bits its mask has, in any order (its own
+ * bit too, if it attends to itself).  A window w leaves of the slots before them
+ * those whose position is above kv_len[b] - n + depth - w; nodes go by the mask
+ * alone.
+ *
+ *  mask       [T, mask_words], at most CX_TREE_MAX_WORDS: bit i % 64 of word i / 64 of a token's row is node i;
+ *             nodes past the words are not attended to
+ *  depth      [T] int32 >= 0, a node's distance from the first new position; NULL
+ *             where window is 0
+ *  max_new, workspace and the rest: as there, of this call's own workspace size
+ *             (cx_tree_attention_workspace_bytes)
+ * Device pointers, stream-ordered, no synchronisation, no allocation.
+ */
+int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
+                           int64_t q_head, int32_t q_heads, const uint64_t* mask,
+                           int32_t mask_words, const int32_t* depth, int32_t max_new,
+                           double scale, int32_t window, double softcap, uint16_t* out,
+                           void* workspace, size_t ws_bytes, void* stream);
+
+size_t cx_tree_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                         int32_t max_new);
+
+/*
+ * Masks and depths of trees from their parents: a node's mask has the bits of the
+ * node and of its ancestors.  Sequence b's nodes are q_start[b] .. q_start[b + 1] - 1
+ * of T (q_start NULL: one each, T = B).
+ *
+ *  parents    [T] int32: the parent's place among its sequence's nodes, below the
+ *             node's own; anything else is a root
+ *  mask       [T, words] (words >= 1; nodes past 64 words have no bit)
+ *  depth      nullable [T] int32: the number of ancestors
+ * Rows outside every sequence are not written.  Device pointers, stream-ordered, no
+ * synchronisation, no allocation.
+ */
+int cx_tree_masks(const int32_t* parents, const int32_t* q_start, int32_t B, int32_t T,
+                  uint64_t* mask, int32_t words, int32_t* depth, void* stream);
+
+/*
+ * The path of a tree that the sampled ids follow.  Node 0 is the last confirmed
+ * token and always accepted; after node c comes its first child (the lowest index)
+ * whose token is sampled[c], if it has one and the path is shorter than width.
+ * sampled[c], a draw from the model's distribution after node c, may come from any
+ * sampler: the tokens are then distributed as without drafts.
+ *
+ *  parents    [T] int32, as for cx_tree_masks (children have higher indices)
+ *  tokens, sampled  [T] int32
+ *  path       [B, width] int32: the accepted nodes, then -1
+ *  count      [B] int32 accepted nodes, 0 for a sequence without nodes
+ *  next       [B] int32: sampled of the last accepted node, -1 if there is none
+ * Device pointers, stream-ordered, no synchronisation, no allocation.
+ */
+int cx_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t* sampled,
+                   const int32_t* q_start, int32_t B, int32_t T, int32_t width, int32_t* path,
+                   int32_t* count, int32_t* next, void* stream);
+
+/*
+ * Accepted tokens moved to their places in every layer: of sequence b, whose n new
+ * tokens begin in slot s = kv_len[b] - n, slot s + j becomes a copy of slot
+ * s + path[b][j] for j < count[b], as if every slot were read before any is written.
+ * A row of path ends before an entry that is not above the one before it, or not
+ * below n.  A move from or to a slot without a page in the pool is left out.  No
+ * page that is written to may be another sequence's too.
+ *
+ *  kv         pages: layer 0's; layer l's are layer_stride bytes further each
+ *  path       [B, width] int32
+ *  count      [B] int32 (at most width are taken), or NULL: width each
+ * Device pointers, stream-ordered, no synchronisation, no allocation.
+ */
+int cx_kv_commit(const cx_kv_batch* kv, int64_t layer_stride, int32_t n_layers,
+                 const int32_t* path, int32_t width, const int32_t* count, void* stream);
+
+/*
  * Pages copied in every layer: page dst[i] becomes a copy of page src[i] (a
  * fork's last page before either sequence appends to it, a compaction's
  * moves).  A pair with an id outside [0, n_pages) is skipped.  No page may be
@@ -362,6 +453,29 @@ size_t cx_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int
 int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int64_t page_bytes,
                      int32_t n_layers, int32_t n_pages, const int32_t* src, const int32_t* dst,
                      int32_t n, void* stream);
+
+/*
+ * Products of few rows with 4-bit weights: out = x W^T, W [N, K] with
+ * W[n, k] = scale * code + shift of row n and group k / group, or, without shifts,
+ * scale * (code - 8).  fp32 sums (of code / 16 + 1, less what that adds: the error
+ * is about 5 times that of the same sum of W), out rounded once.  A row of x that
+ * holds an infinity or NaN, or values above 2^100, gives NaN.
+ *
+ *  x          [M, ldx] bf16 bits, rows 16-byte aligned
+ *  tiles      codes, 16-byte aligned: [N / 16, K / 128, 64, 4] words of 8 codes, both
+ *             rounded up.  Word s of lane 16 j + r holds row r's codes of k = 128 t +
+ *             32 s + 8 j + e, e = 0 .. 7, at bit 4 (e / 2) + 16 (e % 2)
+ *  scales     fp16 bits, 16-byte aligned: [N / 16 rounded up, K / group, 16], or with
+ *             shifts [.., 16, 2]: scale, shift
+ *  group      32, 64 or 128; K a multiple of it
+ *  out        [M, ldo] fp32, or bf16 bits if out_bf16
+ * Rows of the last tile past N are read and not used.  The weights are read once for
+ * up to 64 rows of x.  Device pointers, stream-ordered, no synchronisation, no
+ * allocation.
+ */
+int cx_w4_linear_bf16(const uint16_t* x, int64_t ldx, const uint32_t* tiles,
+                      const uint16_t* scales, int32_t shifts, int32_t group, int32_t M, int32_t N,
+                      int32_t K, void* out, int64_t ldo, int32_t out_bf16, void* stream);
 
 /* Kernel timing (measurement only).  While enabled, every library kernel is
  * dispatched with a start / stop event pair recorded by the dispatch itself
@@ -384,7 +498,12 @@ int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int
 #define CX_KERNEL_ATTEND        10 /* paged attention                  */
 #define CX_KERNEL_ATTEND_JOIN   11 /* paged attention: split rows joined */
 #define CX_KERNEL_KV_COPY       12 /* page copies                      */
-#define CX_KERNEL_KINDS         13
+#define CX_KERNEL_TREE          13 /* tree attention                   */
+#define CX_KERNEL_TREE_JOIN     14 /* tree attention: split rows joined */
+#define CX_KERNEL_TREE_WALK     15 /* tree masks, accepted paths       */
+#define CX_KERNEL_KV_COMMIT     16 /* accepted tokens moved            */
+#define CX_KERNEL_W4            17 /* products with 4-bit weights      */
+#define CX_KERNEL_KINDS         18
 int cx_timing_enable(int on);
 int cx_timing_read(int32_t kernel, double* total_ms, int64_t* launches);
 
