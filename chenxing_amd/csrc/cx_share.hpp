@@ -26,6 +26,7 @@ struct ShareBatch {
   int G, heads;               // q heads per kv head, kv heads
   int window;                 // 0: none
   int held;                   // tokens that a table row's pages hold
+  bool tree = false;          // new tokens attend to any of the others
 };
 
 // A sequence: its rows among the new tokens, the length, and its units (those in
@@ -38,7 +39,8 @@ struct AttendSeq {
 // are those that its last row may attend to, NT more than those of the group before,
 // up to the most that a row's window or the sequence holds.  A sequence of one group
 // (decode, verify) has its n.  Any n that holds a row block's units is right.  (All
-// the sequence's units for each instead: 4096 new tokens 1015 us, not 446.)
+// the sequence's units for each instead: 4096 new tokens 1015 us, not 446.)  A tree's
+// row blocks have all its units.
 struct AttendGroups {
   int size, count;                           // row blocks of a group, groups
   int n0, most;                              // units of the first group, of any
@@ -70,17 +72,18 @@ __device__ __forceinline__ unsigned line_blocks(uint64_t x) {
   return (unsigned)(x & ((1u << RB) - 1));
 }
 
-// The line's split over the workers: shares of ATT_SHARE units at least, the first
+// The line's split over the workers: shares of ``least`` units at least, the first
 // ones a unit longer.
 struct ShareSplit {
   bool by_block;              // a join entry for every row block
   uint64_t shares, per, more;
 };
-__device__ __forceinline__ ShareSplit share_split(uint64_t line, unsigned workers) {
+__device__ __forceinline__ ShareSplit share_split(uint64_t line, unsigned workers,
+                                                  unsigned least = ATT_SHARE) {
   ShareSplit s;
   const uint64_t total = line_units(line);
   s.by_block = line_blocks(line) <= workers;
-  s.shares = min((uint64_t)workers, (total + ATT_SHARE - 1) / ATT_SHARE);
+  s.shares = min((uint64_t)workers, (total + least - 1) / least);
   s.per = s.shares ? total / s.shares : 0;
   s.more = total - s.per * s.shares;
   return s;
@@ -147,7 +150,7 @@ struct AttendLine {
   static __device__ __forceinline__ AttendGroups groups(const ShareBatch& A, const AttendSeq& s,
                                                         int blocks) {
     AttendGroups g;
-    g.size = A.G * (TOK / 16);
+    g.size = A.tree ? max(blocks, 1) : A.G * (TOK / 16);
     g.count = (blocks + g.size - 1) / g.size;
     g.n0 = g.most = s.n;
     const int lowest = s.len - s.q;

@@ -2,108 +2,870 @@
 // gfx950 (layout: cx_kv.hpp).
 //
 // out[t, h] = sum over the allowed slots s of softmax(scale q.k_s) v_s, in one pass
-// over K and V with the running maximum and sum of the softmax's terms.
+// over K and V with the running maximum m and sum l of the softmax's terms: a block of
+// scores raises m to m', and l and the output so far are scaled by exp(m - m').  Two
+// stream-ordered launches:
+//
+//   1. tree_split  workgroups of 8 waves, each with an equal share of all the batch's
+//                  units (32 slots for one kv head and row block); a row block that
+//                  ends inside the share it began in is written out, the others'
+//                  parts (m, l, sums) go to the workspace.
+//   2. tree_join   a workgroup per split row block and 16 rows: its parts, in the
+//                  order of their slots.
+//
+// or, for short tables, tree_split alone with a workgroup a row block.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "cx_device.hpp"
 #include "cx_internal.hpp"
 #include "cx_kv.hpp"
 #include "cx_sampler.h"
+#include "cx_share.hpp"
 #include "cx_timing.hpp"
 
 namespace cx {
+
+constexpr int TREE_WAVES = 8, TREE_WG = 64 * TREE_WAVES;
+constexpr int TREE_WORKERS = 256;            // a workgroup a CU
+constexpr int TREE_UNIT = 32;                // slots of a unit
+constexpr int TREE_LEAST = 2;                // the least share, in units
+constexpr int TREE_BLOCK_STEPS = 8;          // steps of the longest context in one launch
+constexpr int TREE_BATCH = 512;              // sequences of a launch: their lengths are in LDS
+constexpr float TREE_SLACK = 8.f;            // terms reach 2^8: the sums are rarely scaled
+constexpr float TREE_LOW = -3e38f;           // running maximum of a row that attends to something
 
 struct TreeArgs {
   KvArgs kv;
   const uint16_t* q;
   int64_t q_token, q_head;
   int q_heads, G;             // G: q heads per kv head
-  const uint64_t* mask;       // [T, words]
+  const uint32_t* mask;       // [T, words] of 32 bits
   int words;
   const int32_t* depth;       // nullable
-  float scale, cap;           // cap 0: none
+  // score in powers of 2: s1 qk, or s2 tanh(s4 qk), where exp(2 s4 qk) = 2 ^ (s3 qk)
+  float s1, s2, s3, s4;
+  int cap;                    // the latter
   int window;                 // 0: none
   uint16_t* out;
+  int b0;                     // first sequence of the launch; kv.B: their number
+  int block;                  // a workgroup a row block
+  int* entries;               // number of entries of join
+  AttendJoin* join;           // [TREE_WORKERS]
+  float* ml;                  // [2 TREE_WORKERS, ROWS, 2]: a part's maxima and sums
+  float* part;                // [2 TREE_WORKERS, ROWS, D], in the order of join's lanes
 };
 
-// Wave: a row (node, q head).  64 slots at a time: a lane's slot for the scores, a
-// lane's dims for the sums.
-template <int D, bool F8>
-__global__ __launch_bounds__(64) void tree_rows(TreeArgs A) {
-  constexpr int E = F8 ? 16 : 8, DL = D / 64;
-  __shared__ float s_q[D], s_p[64];
+__device__ __forceinline__ uint64_t tree_scalar(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+// The kernel's arguments in memory (its first, at the segment's start), for the parts
+// that run once a piece: what they need is read there again, so the loop keeps its
+// scalar registers.
+__device__ __forceinline__ const TreeArgs& tree_args() {
+  uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const TreeArgs*)(const CX_CONST TreeArgs*)p;
+}
+// The largest, or the sum, of the four lane groups' values, in every group.
+__device__ __forceinline__ float tree_groups_max(float x) {
+  uint32_t a = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  a = __float_as_uint(x);
+  r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float tree_groups_sum(float x) {
+  uint32_t a = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  a = __float_as_uint(x);
+  r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Eight e4m3 codes as bf16.
+__device__ __forceinline__ bf16x8 tree_e4m3x8(uint32_t a, uint32_t b) {
+  const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
+  const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+  const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
+  const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+  return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+// The sign bits say which of two bf16 are NaN or infinite; a mask of the others.
+__device__ __forceinline__ uint32_t tree_nonfinite(uint32_t x) { return (x & 0x7F807F80u) + 0x00800080u; }
+__device__ __forceinline__ uint32_t tree_finite(uint32_t x) {
+  const uint32_t m = tree_nonfinite(x) & 0x80008000u;
+  return ~(m | (m - (m >> 15)));
+}
+
+// 16 bytes a lane from memory to LDS, lane after lane from `to` on, which wave_vm and a
+// barrier wait for.  (The builtin would make every read of LDS wait for all of them.)
+__device__ __forceinline__ void load_lds16(const char* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(to), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void load_lds4(const char* from, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :: "s"(to), "v"(from) : "memory", "m0");
+}
+// Waits until at most N of the wave's loads are under way, and its LDS writes are done.
+template <int N>
+__device__ __forceinline__ void wave_vm() {
+  constexpr int n = N < 0 ? 0 : N > 63 ? 63 : N;
+  __builtin_amdgcn_s_waitcnt((n & 15) | ((n >> 4) << 14) | (7 << 4));
+}
+
+// 8 waves: WR of them share a unit's K and V, each for 16 NT rows; WT such groups take
+// every WT-th unit.
+template <int D, int NT, int WR, bool F8>
+struct TreeShape {
+  static constexpr int WT = TREE_WAVES / WR, ROWS = 16 * NT * WR;
+  // e4m3: many waves share a unit, so its codes are made bf16 once (CONV), else by
+  // each wave as it reads them
+  static constexpr bool CONV = F8 && WR >= 4 && !(D == 256 && WR == 4);
+  static constexpr int KB = (F8 ? 1 : 2) * TREE_UNIT * D;       // bytes of a unit's K
+  static constexpr int RAW = 2 * KB;
+  static constexpr int LOADS = 2 * KB / 1024;                   // of 1 KB
+  static constexpr int LW = (LOADS + WR - 1) / WR;              // of a wave, at most
+  static constexpr int WIDE = 2 * TREE_UNIT * D * 2;            // a unit in bf16
+  // stages of the ring
+  static constexpr int S = WR == 8 ? (D == 256 ? 4 : 8)
+                           : D == 64 ? 4
+                           : F8      ? 3
+                                     : (D == 128 && WR == 4 ? 3 : 2);
+  // bytes of a group: the ring, e4m3 its scales (256 bytes, kept a step longer), CONV
+  // two units in bf16
+  static constexpr int SCALES = F8 ? 256 * (S + 1) : 0;
+  static constexpr int GROUP = S * RAW + SCALES + (CONV ? 2 * WIDE : 0);
+  // the groups' sums meet DR dims at a time
+  static constexpr int DR = WT == 1 ? D : WR == 2 ? 32 : 64;
+  static constexpr int SCRATCH = WT == 1 ? 0 : (WT - 1) * WR * 16 * (DR + 16) * 4;
+  using Line = AttendLine<TREE_UNIT, NT * WR>;
+  using Seqs = AttendSeqs<CX_LDS uint64_t*, CX_LDS int*>;
+  static constexpr int QUEUE = TREE_WAVES * (S + 1) * 64;       // pieces on their way, by wave
+  static constexpr int off_scratch() { return WT * GROUP; }
+  static constexpr int off_queue() { return off_scratch() + SCRATCH; }
+  static constexpr int off_seqs() { return off_queue() + QUEUE + TREE_WAVES * 8; }
+  static constexpr int lds() { return off_seqs() + Seqs::bytes(TREE_BATCH, true); }
+  static_assert(lds() <= 160 * 1024, "LDS");
+};
+
+//  * S^T = K Q^T: row 4 g + j of score tile y is slot 8 g + 4 y + j of the unit, so a
+//    lane's terms of both tiles are those of the 8 slots whose V is one of its 16-byte
+//    chunks: O^T = V^T P^T takes them as they are.  K's slots stand in LDS in that
+//    order.
+//  * K and V go from the pages to LDS without registers, S - 1 units ahead, from one
+//    piece to the next; a barrier a unit.  Each wave counts its own loads: they are
+//    unconditional, after the last unit all of one place.
+//  * Softmax terms enter the products as two bf16 parts (16 bits): one part's rounding
+//    would add as much error as the result's own.
+template <int D, int NT, int WR, bool F8>
+__global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
+  using Sh = TreeShape<D, NT, WR, F8>;
+  using Line = typename Sh::Line;
+  constexpr int WT = Sh::WT, ROWS = Sh::ROWS, S = Sh::S, KB = Sh::KB, RAW = Sh::RAW;
+  constexpr int E = F8 ? 16 : 8, QL = D / 32, DT = D / 16;
+  constexpr bool CONV = Sh::CONV, NARROW = F8 && !CONV;         // operands from codes
+  extern __shared__ __align__(16) char lds[];
   const KvArgs& C = A.kv;
-  const int l = lane_id();
-  const int t = (int)(blockIdx.x / (unsigned)A.q_heads), h = (int)(blockIdx.x % (unsigned)A.q_heads);
-  int b = t;
-  if (C.q_start) {
-    int lo = 0, hi = C.B;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (C.q_start[mid + 1] > t) hi = mid;
-      else lo = mid + 1;
-    }
-    b = lo;
-    if (b >= C.B) return;
-  }
-  const int2 r = kv_rows(C, b);
-  if (t < r.x || t >= r.y) return;
-  const int P = 1 << C.logP, len = max(C.kv_len[b], 0), base = len - (r.y - r.x);
-  const int lim = min(len, C.M << C.logP);
-  const int lo = A.window ? base + max(A.depth[t], 0) - A.window : -1;
-  for (int d = l; d < D; d += 64) s_q[d] = bf16_lo(A.q[t * A.q_token + h * A.q_head + d]);
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(wave_id()), l = lane_id();
+  const int g = l >> 4, c = l & 15;
+  const int wr = w % WR, wt = w / WR;        // row wave, group
+  const int P = 1 << C.logP;
+  CX_LDS char* const ring = to_lds(lds) + wt * Sh::GROUP;
+  CX_LDS char* const s_scale = ring + S * RAW;
+  CX_LDS char* const wide = s_scale + Sh::SCALES;
+  CX_LDS f32x4* const s_acc = (CX_LDS f32x4*)(to_lds(lds) + Sh::off_scratch());
+  CX_LDS uint64_t* const s_pref = (CX_LDS uint64_t*)(to_lds(lds) + Sh::off_seqs());
+  CX_LDS uint64_t* const s_sum = s_pref - TREE_WAVES;
+  CX_LDS int* const s_len = (CX_LDS int*)(s_pref + C.B + 1);
+  const typename Sh::Seqs seqs = {s_pref, s_len, s_len + C.B, C.q_start != nullptr};
+  CX_LDS int* const s_queue = (CX_LDS int*)(to_lds(lds) + Sh::off_queue()) + w * (S + 1) * 16;
+  auto share_batch = [&]() {
+    const auto& A = tree_args();
+    return ShareBatch{A.G, A.kv.heads, A.window, A.kv.n_pages ? A.kv.M << A.kv.logP : 0, true};
+  };
+  auto first = [&](int b) { return seqs.starts ? seqs.first(b) : tree_args().b0 + b; };
+  auto seq = [&](const ShareBatch& batch, int b) {
+    const int f = first(b);
+    return Line::seq(batch, f, seqs.starts ? seqs.end(b) : f + 1, s_len[b]);
+  };
+
+  // a sequence whose tokens attend to nothing
+  auto nothing = [&](int b) {
+    const int r0 = first(b), rows = (seqs.starts ? seqs.end(b) : r0 + 1) - r0;
+    const int64_t n = (int64_t)rows * A.q_heads * (D / 8);
+    u32x4* o = (u32x4*)(A.out + (int64_t)r0 * A.q_heads * D);
+    for (int64_t i = tid; i < n; i += TREE_WG) o[i] = u32x4{0, 0, 0, 0};
+  };
+
+  // the line before each sequence, and its whole
+  seqs.read(C.kv_len, C.q_start, C.B, C.T, tid, TREE_WG);
+  uint64_t line = 0;
   __syncthreads();
-  float m = -INFINITY, sum = 0, acc[DL] = {};
-  for (int s0 = A.window ? max(min(lo + 1, base), 0) & ~63 : 0; s0 < lim; s0 += 64) {
-    const int s = s0 + l, o = s & (P - 1), node = s - base;
-    const int id = s < lim ? C.table[b * C.ld_table + (s >> C.logP)] : -1;
-    bool in = (unsigned)id < (unsigned)C.n_pages;
-    if (node < 0) in &= s > lo;
-    else in &= node < 64 * A.words && (A.mask[(int64_t)t * A.words + (node >> 6)] >> (node & 63) & 1);
-    const char* base_h = C.pages + (int64_t)(in ? id : 0) * C.page_stride + (int64_t)(h / A.G) * C.head_bytes;
-    float x = -INFINITY;
-    if (in) {
-      x = 0;
-      for (int d = 0; d < D; ++d) {
-        const char* p = base_h + k_chunk<E>(d, o, C.logP) + d % E * (16 / E);
-        x = fmaf(s_q[d], F8 ? e4m3_value(*(const uint8_t*)p) : bf16_lo(*(const uint16_t*)p), x);
-      }
-      if (F8) x *= *(const float*)(base_h + k_scale<D>(o, C.logP));
-      x *= A.scale;
-      if (A.cap > 0) x = A.cap * tanhf(x / A.cap);
-    }
-    const uint64_t some = ballot(in);
-    if (!some) continue;
-    const float top = fmaxf(wave_max(x), -3e38f), m1 = fmaxf(m, top);
-    const float f = expf(m - m1), p = in ? expf(x - m1) : 0.f;
-    m = m1;
-    sum = sum * f + wave_sum(p);
-    s_p[l] = p;
-    __syncthreads();
+  if (!A.block) {
+    const int b = tid;                       // (a launch's sequences are no more)
+    uint64_t x = 0;
+    if (b < C.B) x = Line::length(share_batch(), seq(share_batch(), b));
 #pragma unroll
-    for (int i = 0; i < DL; ++i) acc[i] *= f;
-    for (int k = 0; k < 64; ++k) {
-      if (!(some >> k & 1)) continue;
-      const int sk = s0 + k, ok = sk & (P - 1);
-      const char* bk = C.pages + (int64_t)lane_read(id, k) * C.page_stride + (int64_t)(h / A.G) * C.head_bytes;
-      float pk = s_p[k];
-      if (F8) pk *= *(const float*)(bk + v_scale<D>(ok, C.logP));
-#pragma unroll
-      for (int i = 0; i < DL; ++i) {
-        const char* p = bk + v_chunk<E, D>(l + 64 * i, ok, C.logP) + ok % E * (16 / E);
-        acc[i] = fmaf(pk, F8 ? e4m3_value(*(const uint8_t*)p) : bf16_lo(*(const uint16_t*)p), acc[i]);
-      }
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t y = __shfl_up(x, o);
+      if (l >= o) x += y;
     }
+    if (l == 63) s_sum[w] = x;
     __syncthreads();
+    for (int k = 0; k < w; ++k) x += s_sum[k];
+    if (b < C.B) s_pref[b + 1] = x;
+    if (tid == 0) s_pref[0] = 0;
+    __syncthreads();
+    line = s_pref[C.B];
+  } else if (seq(share_batch(), blockIdx.y).n == 0) {
+    if (blockIdx.x == 0) nothing(blockIdx.y);
+    return;
   }
-  const float f = m == -INFINITY ? 0.f : 1.f / sum;
+  line = tree_scalar(line);
+  ShareSplit split = share_split(line, TREE_WORKERS, TREE_LEAST);
+  split.per = tree_scalar(split.per);
+  split.more = tree_scalar(split.more);
+  const bool by_block = split.by_block;
+  const unsigned worker = blockIdx.x;
+  uint64_t end = 0;
+  if (!A.block) {
+    if (worker == 0 && tid == 0) *A.entries = by_block ? (int)line_blocks(line) : TREE_WORKERS;
+    for (int b = blockIdx.x; b < C.B; b += TREE_WORKERS)
+      if (s_pref[b + 1] == s_pref[b]) nothing(b);
+    if (worker >= split.shares) {
+      if (tid == 0 && !by_block) A.join[worker].last = -1;
+      return;
+    }
+    end = share_begin(split, worker) + split.per + (worker < split.more);
+  }
+
+  // The workgroup's pieces, as they are loaded; what is computed takes them, up to S
+  // later, from the wave's queue.
+  struct {
+    int b, h, lim, unit, cnt;
+  } ahead = {0, 0, 0, 0, 0};
+  int step = 0, steps = 0;                   // of the piece that is loaded
+  uint64_t u = share_begin(split, worker);   // past it
+  int b = 0, rb = (int)(blockIdx.x / (unsigned)C.heads);        // block: the next row block
+  if (!A.block)
+    for (int hi = C.B - 1; b < hi;) {        // the last b with its units at or before u
+      const int mid = (b + hi + 1) >> 1;
+      if (line_units(s_pref[mid]) <= u) b = mid;
+      else hi = mid - 1;
+    }
+  bool joined = false;
+  int pushed = 0;
+  // The next piece, pushed to the queue, and whether there is one.
+  auto next_piece = [&]() {
+    const auto& A = tree_args();
+    const ShareBatch batch = share_batch();
+    AttendPiece p;
+    if (A.block) {
+      const AttendSeq s = seq(batch, blockIdx.y);
+      if (rb >= Line::row_blocks(batch, s)) return false;
+      p.b = blockIdx.y;
+      p.h = (int)(blockIdx.x % (unsigned)A.kv.heads);
+      p.tok0 = s.tok0;
+      p.r0 = rb * ROWS;
+      p.R = min(ROWS, s.q * A.G - p.r0);
+      p.lowest = s.len - s.q;
+      p.lim = s.lim;
+      p.unit = s.first;
+      p.cnt = s.n;
+      p.slot = -1;
+      rb += (int)(gridDim.x / (unsigned)A.kv.heads);
+    } else {
+      if (u >= end) return false;
+      while (line_units(s_pref[b + 1]) <= u) ++b;
+      b = __builtin_amdgcn_readfirstlane(b);
+      p = Line::piece(batch, seq(batch, b), b, s_pref[b], split, worker, end, u,
+                      [&](unsigned entry, const AttendJoin& j) {
+                        joined |= j.last >= 0;
+                        if (tid == 0) A.join[entry] = j;
+                      });
+      u = tree_scalar(u);
+      if (p.cnt == 0) return false;
+    }
+    ahead.b = __builtin_amdgcn_readfirstlane(p.b);
+    ahead.h = __builtin_amdgcn_readfirstlane(p.h);
+    ahead.lim = __builtin_amdgcn_readfirstlane(p.lim);
+    ahead.unit = __builtin_amdgcn_readfirstlane(p.unit);
+    ahead.cnt = __builtin_amdgcn_readfirstlane(p.cnt);
+    const int x = l == 0 ? p.h : l == 1 ? p.tok0 : l == 2 ? p.r0 : l == 3 ? p.R : l == 4 ? p.lowest
+                  : l == 5 ? p.lim : l == 6 ? p.unit : l == 7 ? p.cnt : p.slot;
+    if (l < 9) s_queue[16 * pushed + l] = x;
+    pushed = pushed == S ? 0 : pushed + 1;
+    step = 0;
+    steps = (ahead.cnt + WT - 1) / WT;
+    return true;
+  };
+  // ------------------------------------------------------------------ loads
+  // the ids of a unit's two groups of 16 slots
+  auto page_of = [&](int unit, int half) {
+    const int s16 = 2 * unit + half;
+    const bool in = s16 < (ahead.lim + 15) >> 4;
+    const int64_t at = in ? ahead.b * C.ld_table + (s16 >> (C.logP - 4)) : 0;
+    const int id = const_load(C.table + at);
+    return in && (unsigned)id < (unsigned)C.n_pages ? id : -1;
+  };
+  const int slot16 = 4 * ((c >> 2) & 1) * 2 + (c & 3);          // of 16: 8 (c / 4 % 2) + c % 4
+  const int half_of = c >> 3;                // K: the lane's slot is in group c / 8
+  uint32_t fill = 0, fill_scale = 0;         // the stage that is loaded next, its scales
+  uint32_t held = 0;                         // bits 2 s, 2 s + 1: stage s's groups are in the pool
+  bool more = true;                          // pieces to load
+  auto request = [&]() {
+    if (step >= steps && more) more = next_piece();
+    const int unit = ahead.unit + step * WT + wt;
+    const bool live = more && step * WT + wt < ahead.cnt;
+    int id0 = -1, id1 = -1;
+    if (live) {
+      id0 = page_of(unit, 0);
+      id1 = page_of(unit, 1);
+    }
+    const char* head0 = C.pages + (int64_t)(live ? ahead.h : 0) * C.head_bytes;
+    const char* p0 = head0 + (int64_t)max(id0, 0) * C.page_stride;
+    const char* p1 = head0 + (int64_t)max(id1, 0) * C.page_stride;
+    const int o0 = (unit * 32) & (P - 1), o1 = (unit * 32 + 16) & (P - 1);
+    const uint32_t to = (uint32_t)(uintptr_t)ring + fill * RAW;
+    held = (held & ~(3u << 2 * fill)) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << 2 * fill;
+    const char* const none = (const char*)A.out;                // a place to read without a unit
+    if (F8 && wr == 0) {
+      // natural order of slots: keys' scales, then values'
+      const char* p = (l & 16 ? p1 + 4 * o1 : p0 + 4 * o0) + k_scale<D>(l & 15, C.logP) + (l & 32 ? P * 4 : 0);
+      load_lds4(live ? p : none, (uint32_t)(uintptr_t)s_scale + 256 * fill_scale);
+    }
+    const char* pk = half_of ? p1 + 16 * o1 : p0 + 16 * o0;
 #pragma unroll
-  for (int i = 0; i < DL; ++i)
-    A.out[((int64_t)t * A.q_heads + h) * D + l + 64 * i] = (uint16_t)pack_bf16(acc[i] * f, 0.f);
+    for (int j = 0; j < Sh::LW; ++j) {
+      const int i = wr + WR * j;
+      if (i >= Sh::LOADS) break;             // (uniform)
+      const char* p;
+      if (i < Sh::LOADS / 2) {               // chunk rows 2 i and 2 i + 1 of 32 slots
+        const int y = (l >> 4) & 1;
+        p = pk + (((2 * i + (l >> 5)) << C.logP) + slot16 + 4 * y) * 16;
+      } else {
+        const int f = 64 * (i - Sh::LOADS / 2);                 // the first of its chunks
+        const int row = f / D, d = f % D + l;                   // (D >= 64: one row)
+        const int half = F8 ? row : row >> 1;
+        p = (half ? p1 : p0) + v_chunk<E, D>(d, (half ? o1 : o0) + (F8 ? 0 : 8 * (row & 1)), C.logP);
+      }
+      load_lds16(live ? p : none, to + 1024 * i);
+    }
+    fill = fill + 1 == S ? 0 : fill + 1;
+    if (F8) fill_scale = fill_scale == S ? 0 : fill_scale + 1;
+    ++step;
+  };
+  // until the oldest of the stages under way, all but the N newest, are in LDS
+  auto arrive = [&](auto n) {
+    constexpr int N = decltype(n)::value;
+    if (F8 && wr == 0) wave_vm<N * (Sh::LW + 1)>();
+    else wave_vm<N * Sh::LW>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  uint32_t take = 0;                         // the stage that is computed (CONV: converted) next
+  uint32_t conv = 0;                         // CONV: the bf16 buffer that it goes to
+  auto convert = [&]() {
+    const CX_LDS char* raw = ring + take * RAW;
+    CX_LDS char* to = wide + conv * Sh::WIDE;
+#pragma unroll
+    for (int j = 0; j < (2 * KB / 1024 + WR - 1) / WR; ++j) {
+      if (wr + WR * j >= 2 * KB / 1024) break;                  // (uniform)
+      const int f = (wr + WR * j) * 64 + l;
+      const u32x4 x = *(const CX_LDS u32x4*)(raw + 16 * f);
+      const bf16x8 lo = tree_e4m3x8(x[0], x[1]), hi = tree_e4m3x8(x[2], x[3]);
+      // K: chunk rows of 32 slots; V: of D dims
+      const int fv = f - KB / 16;
+      const int at = fv < 0 ? (f / 32 * 2) * 32 + f % 32 : 2 * KB / 16 + fv / D * 2 * D + fv % D;
+      *(CX_LDS bf16x8*)(to + 16 * at) = lo;
+      *(CX_LDS bf16x8*)(to + 16 * (at + (fv < 0 ? 32 : D))) = hi;
+    }
+    take = take + 1 == S ? 0 : take + 1;
+    conv ^= 1;
+  };
+
+  // ------------------------------------------------------------------ a piece's rows
+  u32x4 qr[NT][QL];
+  f32x4 acc[NT][DT];
+  float m[NT], sum[NT];
+  int lo[NT];                                // of the slots before the tree: those above
+  const uint32_t* mrow[NT];                  // the row's mask
+  uint32_t mlow[NT][2];                      // and its first 64 bits
+  struct {
+    int h, tok0, r0, R, lowest, lim, unit, cnt, slot;
+  } cur;
+  int popped = 0, i = 0, todo = 0;           // the step of the piece, and its steps
+  auto begin = [&]() {
+    const auto& A = tree_args();
+    const int x = s_queue[16 * popped + c];
+    popped = popped == S ? 0 : popped + 1;
+    cur.h = lane_read(x, 0);
+    cur.tok0 = lane_read(x, 1);
+    cur.r0 = lane_read(x, 2);
+    cur.R = lane_read(x, 3);
+    cur.lowest = lane_read(x, 4);
+    cur.lim = lane_read(x, 5);
+    cur.unit = lane_read(x, 6);
+    cur.cnt = lane_read(x, 7);
+    cur.slot = lane_read(x, 8);
+    i = 0;
+    todo = (cur.cnt + WT - 1) / WT;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = cur.r0 + min(16 * (NT * wr + nt) + c, cur.R - 1);
+      const int t = cur.tok0 + row / A.G;
+      const uint16_t* q = A.q + t * A.q_token + (cur.h * A.G + row % A.G) * A.q_head;
+#pragma unroll
+      for (int x = 0; x < QL; ++x) qr[nt][x] = *(const u32x4*)(q + 32 * x + 8 * g);
+      mrow[nt] = A.mask + (int64_t)t * A.words;
+      mlow[nt][0] = mrow[nt][0];
+      mlow[nt][1] = mrow[nt][1];
+      lo[nt] = A.window ? cur.lowest - A.window + min(max(A.depth[t], 0), 1 << 28) : -1;
+      m[nt] = -INFINITY;
+      sum[nt] = 0;
+#pragma unroll
+      for (int n = 0; n < DT; ++n) acc[nt][n] = f32x4{0, 0, 0, 0};
+    }
+  };
+  // the bits of nodes i0 .. i0 + 31
+  auto node_bits = [&](int nt, int i0) {
+    auto word = [&](int k) -> uint32_t {
+      return k < 0 || k >= A.words ? 0 : k == 0 ? mlow[nt][0] : k == 1 ? mlow[nt][1] : mrow[nt][k];
+    };
+    const int k = i0 >> 5, sh = i0 & 31;
+    const uint64_t both = (uint64_t)word(k) | (uint64_t)word(k + 1) << 32;
+    return (uint32_t)(both >> sh);
+  };
+  auto compute = [&](int unit, uint32_t here, const CX_LDS char* kv, const CX_LDS char* scales) {
+    const int t0 = unit * TREE_UNIT;
+    f32x4 v[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) v[nt][0] = v[nt][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int x = 0; x < QL; ++x)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        bf16x8 ka;
+        if (NARROW) {
+          const u32x2 r = *(const CX_LDS u32x2*)(kv + ((2 * x + (g >> 1)) * 32 + 16 * y + c) * 16 + 8 * (g & 1));
+          ka = tree_e4m3x8(r[0], r[1]);
+        } else {
+          ka = *(const CX_LDS bf16x8*)(kv + ((4 * x + g) * 32 + 16 * y + c) * 16);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          v[nt][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, __builtin_bit_cast(bf16x8, qr[nt][x]),
+                                                             v[nt][y], 0, 0, 0);
+      }
+    f32x4 vs[F8 ? 2 : 1];
+    if (F8) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const f32x4 ks = *(const CX_LDS f32x4*)(scales + 4 * (8 * g + 4 * y));
+        vs[y] = *(const CX_LDS f32x4*)(scales + 128 + 4 * (8 * g + 4 * y));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) v[nt][y] *= ks;
+      }
+    }
+    const float to2 = A.cap ? 1.f : A.s1;
+    if (A.cap) {                             // tanh(z) = 1 - 2 / (exp(2 z) + 1), near 0 its series
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = v[nt][y][j], z = A.s4 * x, zz = z * z, sx = A.s1 * x;
+            const float far = fmaf(-2.f * A.s2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(A.s3 * x) + 1.f), A.s2);
+            v[nt][y][j] = zz < 1.f / 256.f ? fmaf(sx * zz, fmaf(zz, 2.f / 15.f, -1.f / 3.f), sx) : far;
+          }
+    }
+    // a unit is open where all its slots are held, before the tree and inside every
+    // row's window
+    bool masked = t0 + TREE_UNIT > min(cur.lowest, cur.lim) || here != 3;
+    if (A.window) {
+      bool out = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) out |= lo[nt] >= t0;
+      masked |= __any(out);
+    }
+    uint32_t valid = ~0u, bits[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) bits[nt] = ~0u;
+    float low[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) low[nt] = TREE_LOW;
+    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+    if (masked) {
+      valid = (here & 1 ? 0xFFFFu : 0u) | (here & 2 ? 0xFFFF0000u : 0u);
+      valid &= below(cur.lim - t0);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t x = below(cur.lowest - t0) & ~below(lo[nt] + 1 - t0);
+        if (t0 + TREE_UNIT > cur.lowest) x |= node_bits(nt, t0 - cur.lowest);
+        bits[nt] = x & valid;
+        low[nt] = bits[nt] ? TREE_LOW : -INFINITY;
+        const uint32_t mine = bits[nt] >> (8 * g);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[nt][y][j] = mine >> (4 * y + j) & 1 ? v[nt][y][j] : -INFINITY;
+      }
+    }
+    float alpha[NT];
+    bool moved = false;
+    u32x4 ph[NT], pl[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float top = fmaxf(fmaxf(fmaxf(v[nt][0][0], v[nt][0][1]), fmaxf(v[nt][0][2], v[nt][0][3])),
+                        fmaxf(fmaxf(v[nt][1][0], v[nt][1][1]), fmaxf(v[nt][1][2], v[nt][1][3])));
+      const float m1 = fmaxf(low[nt], to2 * tree_groups_max(top));
+      const bool up = m1 > m[nt] + TREE_SLACK;
+      const float base = up ? m1 : m[nt] == -INFINITY ? 0.f : m[nt];
+      alpha[nt] = up ? __builtin_amdgcn_exp2f(m[nt] - m1) : 1.f;
+      moved |= up;
+      m[nt] = up ? m1 : m[nt];
+      float add = 0;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        f32x4 p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(to2, v[nt][y][j], -base));
+        add += (p[0] + p[1]) + (p[2] + p[3]);
+        if (F8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = v[nt][y][j] == -INFINITY ? 0.f : p[j] * vs[y][j];
+        }
+        // two bf16 parts: the first cut off, the second never 0, so that an infinite
+        // value keeps its sign in both products (2^-20 of a term too much)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const float p0 = p[2 * d], p1 = p[2 * d + 1];
+          const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
+          ph[nt][2 * y + d] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
+          pl[nt][2 * y + d] = pack_bf16(fmaf(p0, 1.f + 0x1p-20f, -__uint_as_float(x0 & 0xFFFF0000u)),
+                                        fmaf(p1, 1.f + 0x1p-20f, -__uint_as_float(x1 & 0xFFFF0000u)));
+        }
+      }
+      sum[nt] = fmaf(sum[nt], alpha[nt], add);
+    }
+    if (__any(moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int n = 0; n < DT; ++n) acc[nt][n] *= alpha[nt];
+    }
+    const CX_LDS char* vb = kv + (NARROW ? KB : 2 * TREE_UNIT * D);
+    auto value = [&](int n) {
+      if (NARROW) {
+        const u32x2 r = *(const CX_LDS u32x2*)(vb + ((g >> 1) * D + 16 * n + c) * 16 + 8 * (g & 1));
+        return __builtin_bit_cast(u32x4, tree_e4m3x8(r[0], r[1]));
+      }
+      return *(const CX_LDS u32x4*)(vb + (g * D + 16 * n + c) * 16);
+    };
+    if (!masked) {
+#pragma unroll
+      for (int n = 0; n < DT; ++n) {
+        const bf16x8 va = __builtin_bit_cast(bf16x8, value(n));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, ph[nt]),
+                                                               acc[nt][n], 0, 0, 0);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pl[nt]),
+                                                               acc[nt][n], 0, 0, 0);
+      }
+      return;
+    }
+    // V of slots that nobody holds counts as zeros, whatever is there, and NaN and
+    // infinity reach the rows that attend to them only: left out of the products and
+    // added one by one
+    uint32_t keep[4], bad = 0;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const uint32_t two = valid >> (8 * g + 2 * d);
+      keep[d] = (two & 1 ? 0xFFFFu : 0) | (two & 2 ? 0xFFFF0000u : 0);
+    }
+#pragma unroll 1
+    for (int n = 0; n < DT; ++n) {
+      const u32x4 x = value(n);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) bad |= tree_nonfinite(x[d] & keep[d]);
+    }
+    const bool some = __any((bad & 0x80008000u) != 0);
+#pragma unroll
+    for (int n = 0; n < DT; ++n) {
+      u32x4 x = value(n);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) x[d] &= keep[d] & tree_finite(x[d]);
+      const bf16x8 va = __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, ph[nt]),
+                                                             acc[nt][n], 0, 0, 0);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pl[nt]),
+                                                             acc[nt][n], 0, 0, 0);
+    }
+    if (!some) return;
+#pragma unroll 1
+    for (int k = 0; k < TREE_UNIT; ++k) {
+      if (!(valid >> k & 1)) continue;
+#pragma unroll
+      for (int n = 0; n < DT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int d = 16 * n + 4 * g + j;
+          float x;
+          if (NARROW) x = e4m3_value(*(const CX_LDS uint8_t*)(vb + ((k >> 4) * D + d) * 16 + (k & 15)));
+          else x = bf16_lo(*(const CX_LDS uint16_t*)(vb + ((k >> 3) * D + d) * 16 + 2 * (k & 7)));
+          const bool fine = fabsf(x) < INFINITY;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[nt][n][j] += !fine && (bits[nt] >> k & 1) ? x : 0.f;
+        }
+    }
+  };
+
+  // the groups' sums meet in the first one's registers
+  auto meet = [&]() {
+    if constexpr (WT > 1) {
+      constexpr int ND = Sh::DR / 16;
+      CX_LDS f32x4* const mine = s_acc + ((wt - 1) * WR + wr) * (ND + 1) * 64;
+      auto barrier = [&]() {
+        __builtin_amdgcn_s_waitcnt((15 | 3 << 14) | (7 << 4));  // LDS alone
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      };
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f0 = 1.f, f[WT];
+#pragma unroll
+        for (int x = 0; x < DT / ND; ++x) {
+          if (wt > 0) {
+#pragma unroll
+            for (int n = 0; n < ND; ++n) mine[n * 64 + l] = acc[nt][ND * x + n];
+            if (x == 0) mine[ND * 64 + l] = f32x4{m[nt], sum[nt], 0, 0};
+          }
+          barrier();
+          if (wt == 0) {
+            const CX_LDS f32x4* at = s_acc + wr * (ND + 1) * 64;
+            if (x == 0) {
+              float top = m[nt], other[WT];
+#pragma unroll
+              for (int k = 1; k < WT; ++k) {
+                const f32x4 ml = at[((k - 1) * WR * (ND + 1) + ND) * 64 + l];
+                other[k] = ml[0];
+                f[k] = ml[1];
+                top = fmaxf(top, ml[0]);
+              }
+              const float base = top == -INFINITY ? 0.f : top;
+              f0 = __builtin_amdgcn_exp2f(m[nt] - base);
+              sum[nt] *= f0;
+              m[nt] = top;
+#pragma unroll
+              for (int k = 1; k < WT; ++k) {
+                const float e = __builtin_amdgcn_exp2f(other[k] - base);
+                sum[nt] = fmaf(e, f[k], sum[nt]);
+                f[k] = e;
+              }
+            }
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+              f32x4 a = acc[nt][ND * x + n] * f0;
+#pragma unroll
+              for (int k = 1; k < WT; ++k) a += f[k] * at[((k - 1) * WR * (ND + 1) + n) * 64 + l];
+              acc[nt][ND * x + n] = a;
+            }
+          }
+          barrier();
+        }
+      }
+    }
+  };
+  auto finish = [&]() {
+    meet();
+    if (wt > 0) return;
+    const auto& A = tree_args();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float L = tree_groups_sum(sum[nt]);
+      const int r = 16 * (NT * wr + nt) + c;
+      if (cur.slot < 0) {
+        if (r >= cur.R) continue;
+        const float f = m[nt] == -INFINITY ? 0.f : 1.f / L;
+        const int row = cur.r0 + r;
+        uint16_t* o = A.out + ((int64_t)(cur.tok0 + row / A.G) * A.q_heads + cur.h * A.G + row % A.G) * D + 4 * g;
+#pragma unroll
+        for (int n = 0; n < DT; ++n)
+          *(u32x2*)(o + 16 * n) = u32x2{pack_bf16(acc[nt][n][0] * f, acc[nt][n][1] * f),
+                                        pack_bf16(acc[nt][n][2] * f, acc[nt][n][3] * f)};
+      } else if (16 * (NT * wr + nt) < cur.R) {
+        const int64_t tile = (int64_t)cur.slot * (ROWS / 16) + NT * wr + nt;
+        f32x4* o = (f32x4*)(A.part + tile * 16 * D) + l;
+#pragma unroll
+        for (int n = 0; n < DT; ++n) o[64 * n] = acc[nt][n];
+        if (g == 0) *(float2*)(A.ml + 2 * (tile * 16 + c)) = make_float2(m[nt], L);
+      }
+    }
+  };
+
+  // ------------------------------------------------------------------ the steps
+  // FIRST steps load only; then each computes what arrived and loads FIRST steps ahead
+  constexpr int FIRST = CONV ? S : S - 1;
+  uint32_t now = 0;                          // CONV: the bf16 buffer that is computed
+  uint32_t at = 0, at_scale = 0;             // the stage that is computed, its scales
+#pragma unroll 1
+  for (int k = -FIRST;; ++k) {
+    uint32_t here = 0;
+    if (k >= 0) {
+      if (i == todo) {
+        if (k > 0) finish();
+        if (popped == pushed) break;
+        begin();
+      }
+      arrive(std::integral_constant<int, S - 2>());
+      here = held >> 2 * at & 3;
+    }
+    request();
+    if (k >= 0) {
+      const int unit = cur.unit + i * WT + wt;
+      const CX_LDS char* kv = CONV ? wide + now * Sh::WIDE : ring + at * RAW;
+      if (i * WT + wt < cur.cnt) compute(unit, here, kv, s_scale + 256 * at_scale);
+      ++i;
+      now ^= 1;
+      at = at + 1 == S ? 0 : at + 1;
+      if (F8) at_scale = at_scale == S ? 0 : at_scale + 1;
+    }
+    if (CONV && k >= -1) {
+      if (k < 0) arrive(std::integral_constant<int, S - 1>());
+      convert();
+    }
+  }
+  wave_vm<0>();                              // the last loads write LDS: end them first
+  if (!A.block && !joined && tid == 0 && !by_block) A.join[worker].last = -1;
+}
+
+// A row block's parts joined, 16 rows to a workgroup, in the order of their slots.
+template <int D>
+__global__ __launch_bounds__(256) void tree_join(TreeArgs A, int rows) {
+  constexpr int ITEMS = D / 64, AHEAD = 8;   // 16-byte items of a thread
+  const int count = const_load(A.entries);
+  const AttendJoin J = const_load(A.join + blockIdx.x);
+  const int r0 = 16 * blockIdx.y;
+  // (an entry of a call whose lengths change while it runs may not be in range)
+  if ((int)blockIdx.x >= count || J.first < 0 || J.last < J.first || J.last >= TREE_WORKERS ||
+      r0 >= J.rows || J.rows > rows || J.row0 < 0 || (unsigned)J.head >= (unsigned)A.kv.heads ||
+      J.tok0 < 0 || (int64_t)J.row0 + J.rows > (int64_t)(A.kv.T - J.tok0) * A.G)
+    return;
+  const int n = J.last - J.first + 1, l = lane_id(), c = l & 15, g = l >> 4;
+  float top = -INFINITY, L = 0;
+  f32x4 o[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) o[k] = f32x4{0, 0, 0, 0};
+  for (int p0 = 0; p0 < n; p0 += AHEAD) {
+    float m[AHEAD], s[AHEAD];
+    f32x4 x[AHEAD][ITEMS];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {        // past the last: the last again, not added
+      const int q = min(p0 + k, n - 1);
+      const int64_t tile = ((int64_t)(2 * (J.first + q) + (q == 0)) * rows + r0) / 16;
+      const float2 ml = *(const float2*)(A.ml + 2 * (tile * 16 + c));
+      m[k] = p0 + k < n ? ml.x : -INFINITY;
+      s[k] = ml.y;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) x[k][i] = *((const f32x4*)(A.part + tile * 16 * D) + 256 * i + threadIdx.x);
+    }
+    float t = top;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) t = fmaxf(t, m[k]);
+    const float base = t == -INFINITY ? 0.f : t, f0 = __builtin_amdgcn_exp2f(top - base);
+    top = t;
+    L *= f0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) o[i] *= f0;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (p0 + k >= n) continue;
+      const float f = __builtin_amdgcn_exp2f(m[k] - base);
+      L = fmaf(f, s[k], L);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) o[i] += f * x[k][i];
+    }
+  }
+  if (r0 + c >= J.rows) return;
+  const float f = top == -INFINITY ? 0.f : 1.f / L;
+  const int row = J.row0 + r0 + c;
+  uint16_t* out = A.out + ((int64_t)(J.tok0 + row / A.G) * A.q_heads + J.head * A.G + row % A.G) * D + 4 * g;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int d = 16 * (4 * i + wave_id());
+    *(u32x2*)(out + d) = u32x2{pack_bf16(o[i][0] * f, o[i][1] * f), pack_bf16(o[i][2] * f, o[i][3] * f)};
+  }
+}
+
+// Rows of a row block: the least of those that hold a sequence's.
+static int tree_rows(int64_t rows, int D) {
+  if (D == 256) return rows <= 64 ? 64 : 128;
+  return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+}
+
+struct TreeWork {
+  size_t off_join, off_ml, off_part, total;
+};
+static TreeWork tree_workspace(int rows, int D) {
+  TreeWork x;
+  x.off_join = 256;
+  x.off_ml = x.off_join + align_up(TREE_WORKERS * sizeof(AttendJoin), 256);
+  x.off_part = x.off_ml + align_up((size_t)2 * TREE_WORKERS * rows * 8, 256);
+  x.total = x.off_part + (size_t)2 * TREE_WORKERS * rows * D * 4;
+  return x;
+}
+
+template <int D, int NT, int WR, bool F8>
+static int launch_tree(TreeArgs A, int64_t max_new, hipStream_t s) {
+  using Sh = TreeShape<D, NT, WR, F8>;
+  static LdsLimit limit;
+  if (int e = limit.raise((const void*)tree_split<D, NT, WR, F8>, Sh::lds())) return e;
+  const int64_t held = (int64_t)A.kv.M << A.kv.logP;
+  const int64_t span = A.window ? std::min<int64_t>(A.window + max_new, held) : held;
+  const int64_t tiles = (A.G * max_new + Sh::ROWS - 1) / Sh::ROWS;
+  const uint32_t lds = Sh::off_seqs() + Sh::Seqs::bytes(A.kv.B, A.kv.q_start != nullptr);
+  A.block = span <= TREE_BLOCK_STEPS * TREE_UNIT * Sh::WT;
+  if (A.block) {
+    timed_launch(CX_KERNEL_TREE, tree_split<D, NT, WR, F8>, dim3((unsigned)(A.kv.heads * tiles), A.kv.B),
+                 dim3(TREE_WG), lds, s, A);
+    return (int)hipGetLastError();
+  }
+  timed_launch(CX_KERNEL_TREE, tree_split<D, NT, WR, F8>, dim3(TREE_WORKERS), dim3(TREE_WG), lds, s, A);
+  const int64_t entries =
+      std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / Sh::ROWS + A.kv.B), TREE_WORKERS);
+  timed_launch(CX_KERNEL_TREE_JOIN, tree_join<D>, dim3((unsigned)entries, Sh::ROWS / 16), dim3(256), 0, s, A,
+               Sh::ROWS);
+  return (int)hipGetLastError();
+}
+template <int D, bool F8>
+static int launch_tree(const TreeArgs& A, int rows, int64_t max_new, hipStream_t s) {
+  if constexpr (D == 256) {
+    if (rows == 64) return launch_tree<D, 1, 4, F8>(A, max_new, s);
+    return launch_tree<D, 1, 8, F8>(A, max_new, s);
+  } else {
+    if (rows == 32) return launch_tree<D, 1, 2, F8>(A, max_new, s);
+    if (rows == 64) return launch_tree<D, 1, 4, F8>(A, max_new, s);
+    if (rows == 128) return launch_tree<D, 2, 4, F8>(A, max_new, s);
+    return launch_tree<D, 2, 8, F8>(A, max_new, s);
+  }
 }
 
 }  // namespace cx
@@ -112,7 +874,8 @@ extern "C" {
 
 size_t cx_tree_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                          int32_t max_new) {
-  return 256;
+  if (q_heads < 1 || kv_heads < 1 || head_dim < 1 || max_new < 1) return 256;
+  return cx::tree_workspace(cx::tree_rows((int64_t)(q_heads / kv_heads) * max_new, head_dim), head_dim).total;
 }
 
 int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
@@ -140,24 +903,50 @@ int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_t
   A.q = q; A.q_token = q_token; A.q_head = q_head;
   A.q_heads = q_heads;
   A.G = q_heads / kv->kv_heads;
-  A.mask = mask;
-  A.words = mask_words;
+  max_new = std::min(max_new, kv->T);        // no sequence has more
+  const int D = kv->head_dim, rows = cx::tree_rows((int64_t)A.G * max_new, D);
+  const cx::TreeWork lay = cx::tree_workspace(rows, D);
+  if (ws_bytes < lay.total)
+    return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, lay.total);
+  // the units and row blocks, at most, fit the share arithmetic's 38 bits
+  const double units = (double)kv->max_pages * kv->page_tokens / 32 + 8;
+  const double blocks = kv->kv_heads * ((double)kv->T * A.G / 16 + kv->B);
+  if (units * blocks >= 0x1p38) return cx::api_fail(CX_EINVAL, "too many tokens for one call");
+  A.mask = (const uint32_t*)mask;
+  A.words = 2 * mask_words;
   A.depth = depth;
-  A.scale = (float)scale;
-  A.cap = std::isinf(softcap) ? 0.f : (float)softcap;
-  if (!std::isfinite(A.scale) || !std::isfinite(A.cap) ||
-      (A.cap > 0 && !std::isfinite((float)(scale / softcap))) || (softcap > 0 && A.cap == 0 && !std::isinf(softcap)))
+  A.cap = softcap > 0 && !std::isinf(softcap);
+  const double log2e = 1.4426950408889634;
+  A.s1 = (float)(scale * log2e);
+  A.s2 = A.cap ? (float)(softcap * log2e) : 0.f;
+  A.s3 = A.cap ? (float)(2 * scale / softcap * log2e) : 0.f;
+  A.s4 = A.cap ? (float)(scale / softcap) : 0.f;
+  if (!std::isfinite(A.s1) || !std::isfinite(A.s2) || !std::isfinite(A.s3))
     return cx::api_fail(CX_EINVAL, "scale (%g) and softcap (%g) pass the range of fp32", scale, softcap);
-  A.window = window;
+  A.window = std::min(window, INT32_MAX - cx::KV_MAX_NEW);
   A.out = out;
-  using Kernel = void (*)(cx::TreeArgs);
+  A.entries = (int*)workspace;
+  A.join = (cx::AttendJoin*)((char*)workspace + lay.off_join);
+  A.ml = (float*)((char*)workspace + lay.off_ml);
+  A.part = (float*)((char*)workspace + lay.off_part);
   const bool f8 = kv->dtype == CX_KV_E4M3;
-  const Kernel k = kv->head_dim == 64    ? (f8 ? (Kernel)cx::tree_rows<64, true> : cx::tree_rows<64, false>)
-                   : kv->head_dim == 128 ? (f8 ? (Kernel)cx::tree_rows<128, true> : cx::tree_rows<128, false>)
-                                         : (f8 ? (Kernel)cx::tree_rows<256, true> : cx::tree_rows<256, false>);
-  cx::timed_launch(CX_KERNEL_TREE, k, dim3((unsigned)(kv->T * q_heads)), dim3(64), 0, (hipStream_t)stream, A);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return cx::api_fail(CX_EHIP, "tree attention launch: %s", hipGetErrorString(e));
+  const hipStream_t s = (hipStream_t)stream;
+  // one launch after the other where a call has more sequences than a launch takes
+  for (int b0 = 0; b0 < kv->B; b0 += cx::TREE_BATCH) {
+    cx::TreeArgs X = A;
+    X.b0 = b0;
+    X.kv.B = std::min(kv->B - b0, cx::TREE_BATCH);
+    X.kv.table += b0 * kv->ld_table;
+    X.kv.kv_len += b0;
+    if (X.kv.q_start) X.kv.q_start += b0;
+    const int e = D == 64    ? (f8 ? cx::launch_tree<64, true>(X, rows, max_new, s)
+                                   : cx::launch_tree<64, false>(X, rows, max_new, s))
+                  : D == 128 ? (f8 ? cx::launch_tree<128, true>(X, rows, max_new, s)
+                                   : cx::launch_tree<128, false>(X, rows, max_new, s))
+                             : (f8 ? cx::launch_tree<256, true>(X, rows, max_new, s)
+                                   : cx::launch_tree<256, false>(X, rows, max_new, s));
+    if (e != 0) return cx::api_fail(CX_EHIP, "tree attention launch: %s", hipGetErrorString((hipError_t)e));
+  }
   return CX_OK;
 }
 
