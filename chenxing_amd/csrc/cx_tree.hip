@@ -148,7 +148,7 @@ struct TreeShape {
   static constexpr int SCRATCH = WT == 1 ? 0 : (WT - 1) * WR * 16 * (DR + 16) * 4;
   using Line = AttendLine<TREE_UNIT, NT * WR>;
   using Seqs = AttendSeqs<CX_LDS uint64_t*, CX_LDS int*>;
-  static constexpr int QUEUE = TREE_WAVES * (S + 1) * 64;       // pieces on their way, by wave
+  static constexpr int QUEUE = TREE_WAVES * (S + 2) * 64;       // pieces on their way, by wave
   static constexpr int off_scratch() { return WT * GROUP; }
   static constexpr int off_queue() { return off_scratch() + SCRATCH; }
   static constexpr int off_seqs() { return off_queue() + QUEUE + TREE_WAVES * 8; }
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   CX_LDS uint64_t* const s_sum = s_pref - TREE_WAVES;
   CX_LDS int* const s_len = (CX_LDS int*)(s_pref + C.B + 1);
   const typename Sh::Seqs seqs = {s_pref, s_len, s_len + C.B, C.q_start != nullptr};
-  CX_LDS int* const s_queue = (CX_LDS int*)(to_lds(lds) + Sh::off_queue()) + w * (S + 1) * 16;
+  CX_LDS int* const s_queue = (CX_LDS int*)(to_lds(lds) + Sh::off_queue()) + w * (S + 2) * 16;
   auto share_batch = [&]() {
     const auto& A = tree_args();
     return ShareBatch{A.G, A.kv.heads, A.window, A.kv.n_pages ? A.kv.M << A.kv.logP : 0, true};
@@ -247,12 +247,12 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     end = share_begin(split, worker) + split.per + (worker < split.more);
   }
 
-  // The workgroup's pieces, as they are loaded; what is computed takes them, up to S
-  // later, from the wave's queue.
+  // The workgroup's pieces, as they are loaded; what is computed takes them, up to S +
+  // 1 later, from the wave's queue.
   struct {
     int b, h, lim, unit, cnt;
   } ahead = {0, 0, 0, 0, 0};
-  int step = 0, steps = 0;                   // of the piece that is loaded
+  int step = -1, steps = 0;                  // of the piece that is loaded
   uint64_t u = share_begin(split, worker);   // past it
   int b = 0, rb = (int)(blockIdx.x / (unsigned)C.heads);        // block: the next row block
   if (!A.block)
@@ -302,34 +302,34 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     const int x = l == 0 ? p.h : l == 1 ? p.tok0 : l == 2 ? p.r0 : l == 3 ? p.R : l == 4 ? p.lowest
                   : l == 5 ? p.lim : l == 6 ? p.unit : l == 7 ? p.cnt : p.slot;
     if (l < 9) s_queue[16 * pushed + l] = x;
-    pushed = pushed == S ? 0 : pushed + 1;
+    pushed = pushed == S + 1 ? 0 : pushed + 1;
     step = 0;
     steps = (ahead.cnt + WT - 1) / WT;
     return true;
   };
   // ------------------------------------------------------------------ loads
-  // the ids of a unit's two groups of 16 slots
-  auto page_of = [&](int unit, int half) {
-    const int s16 = 2 * unit + half;
-    const bool in = s16 < (ahead.lim + 15) >> 4;
-    const int64_t at = in ? ahead.b * C.ld_table + (s16 >> (C.logP - 4)) : 0;
-    const int id = const_load(C.table + at);
-    return in && (unsigned)id < (unsigned)C.n_pages ? id : -1;
+  // The ids of a unit's two groups of 16 slots, asked for a step before they are used.
+  bool more = true, live = false;            // pieces to load; a unit for this group's next stage
+  int unit = 0, next0 = -1, next1 = -1;
+  auto advance = [&]() {
+    if (++step >= steps && more) more = next_piece();
+    unit = ahead.unit + step * WT + wt;
+    live = more && step * WT + wt < ahead.cnt;
+    auto id = [&](int half) {
+      const int s16 = 2 * unit + half;
+      if (!live || s16 >= (ahead.lim + 15) >> 4) return -1;
+      return const_load(C.table + ahead.b * C.ld_table + (s16 >> (C.logP - 4)));
+    };
+    next0 = id(0);
+    next1 = id(1);
   };
   const int slot16 = 4 * ((c >> 2) & 1) * 2 + (c & 3);          // of 16: 8 (c / 4 % 2) + c % 4
   const int half_of = c >> 3;                // K: the lane's slot is in group c / 8
   uint32_t fill = 0, fill_scale = 0;         // the stage that is loaded next, its scales
   uint32_t held = 0;                         // bits 2 s, 2 s + 1: stage s's groups are in the pool
-  bool more = true;                          // pieces to load
   auto request = [&]() {
-    if (step >= steps && more) more = next_piece();
-    const int unit = ahead.unit + step * WT + wt;
-    const bool live = more && step * WT + wt < ahead.cnt;
-    int id0 = -1, id1 = -1;
-    if (live) {
-      id0 = page_of(unit, 0);
-      id1 = page_of(unit, 1);
-    }
+    const int id0 = (unsigned)next0 < (unsigned)C.n_pages ? next0 : -1;
+    const int id1 = (unsigned)next1 < (unsigned)C.n_pages ? next1 : -1;
     const char* head0 = C.pages + (int64_t)(live ? ahead.h : 0) * C.head_bytes;
     const char* p0 = head0 + (int64_t)max(id0, 0) * C.page_stride;
     const char* p1 = head0 + (int64_t)max(id1, 0) * C.page_stride;
@@ -361,7 +361,6 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     }
     fill = fill + 1 == S ? 0 : fill + 1;
     if (F8) fill_scale = fill_scale == S ? 0 : fill_scale + 1;
-    ++step;
   };
   // until the oldest of the stages under way, all but the N newest, are in LDS
   auto arrive = [&](auto n) {
@@ -407,7 +406,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   auto begin = [&]() {
     const auto& A = tree_args();
     const int x = s_queue[16 * popped + c];
-    popped = popped == S ? 0 : popped + 1;
+    popped = popped == S + 1 ? 0 : popped + 1;
     cur.h = lane_read(x, 0);
     cur.tok0 = lane_read(x, 1);
     cur.r0 = lane_read(x, 2);
@@ -435,6 +434,14 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 #pragma unroll
       for (int n = 0; n < DT; ++n) acc[nt][n] = f32x4{0, 0, 0, 0};
     }
+    // waited for here: at their first use the wait would be part of every step, and drain
+    // the loads under way
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int x = 0; x < QL; ++x) asm volatile("" : "+v"(qr[nt][x]));
+      asm volatile("" : "+v"(lo[nt]), "+v"(mlow[nt][0]), "+v"(mlow[nt][1]));
+    }
   };
   // the bits of nodes i0 .. i0 + 31
   auto node_bits = [&](int nt, int i0) {
@@ -450,22 +457,49 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     f32x4 v[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) v[nt][0] = v[nt][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int x = 0; x < QL; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        bf16x8 ka;
-        if (NARROW) {
-          const u32x2 r = *(const CX_LDS u32x2*)(kv + ((2 * x + (g >> 1)) * 32 + 16 * y + c) * 16 + 8 * (g & 1));
-          ka = tree_e4m3x8(r[0], r[1]);
-        } else {
-          ka = *(const CX_LDS bf16x8*)(kv + ((4 * x + g) * 32 + 16 * y + c) * 16);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          v[nt][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, __builtin_bit_cast(bf16x8, qr[nt][x]),
-                                                             v[nt][y], 0, 0, 0);
+    auto key = [&](int x, int y) {
+      if (NARROW) {
+        const u32x2 r = *(const CX_LDS u32x2*)(kv + ((2 * x + (g >> 1)) * 32 + 16 * y + c) * 16 + 8 * (g & 1));
+        return u32x4{r[0], r[1], 0, 0};
       }
+      return *(const CX_LDS u32x4*)(kv + ((4 * x + g) * 32 + 16 * y + c) * 16);
+    };
+    // (four steps' keys at a time: as many as the registers hold)
+#pragma unroll
+    for (int x0 = 0; x0 < QL; x0 += 4) {
+      constexpr int N = QL < 4 ? QL : 4;
+      u32x4 ka[N][2];
+#pragma unroll
+      for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) ka[x][y] = key(x0 + x, y);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const bf16x8 k = NARROW ? tree_e4m3x8(ka[x][y][0], ka[x][y][1]) : __builtin_bit_cast(bf16x8, ka[x][y]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            v[nt][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, qr[nt][x0 + x]),
+                                                               v[nt][y], 0, 0, 0);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // V, while the scores become terms
+    const CX_LDS char* vb = kv + (NARROW ? KB : 2 * TREE_UNIT * D);
+    auto value = [&](int n) {
+      if (NARROW) {
+        const u32x2 r = *(const CX_LDS u32x2*)(vb + ((g >> 1) * D + 16 * n + c) * 16 + 8 * (g & 1));
+        return u32x4{r[0], r[1], 0, 0};
+      }
+      return *(const CX_LDS u32x4*)(vb + (g * D + 16 * n + c) * 16);
+    };
+    constexpr int EARLY = 4;                 // of V's 16-dim tiles, four together
+    u32x4 va[EARLY];
+#pragma unroll
+    for (int n = 0; n < EARLY; ++n) va[n] = value(n);
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 vs[F8 ? 2 : 1];
     if (F8) {
 #pragma unroll
@@ -564,29 +598,6 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 #pragma unroll
         for (int n = 0; n < DT; ++n) acc[nt][n] *= alpha[nt];
     }
-    const CX_LDS char* vb = kv + (NARROW ? KB : 2 * TREE_UNIT * D);
-    auto value = [&](int n) {
-      if (NARROW) {
-        const u32x2 r = *(const CX_LDS u32x2*)(vb + ((g >> 1) * D + 16 * n + c) * 16 + 8 * (g & 1));
-        return __builtin_bit_cast(u32x4, tree_e4m3x8(r[0], r[1]));
-      }
-      return *(const CX_LDS u32x4*)(vb + (g * D + 16 * n + c) * 16);
-    };
-    if (!masked) {
-#pragma unroll
-      for (int n = 0; n < DT; ++n) {
-        const bf16x8 va = __builtin_bit_cast(bf16x8, value(n));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, ph[nt]),
-                                                               acc[nt][n], 0, 0, 0);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pl[nt]),
-                                                               acc[nt][n], 0, 0, 0);
-      }
-      return;
-    }
     // V of slots that nobody holds counts as zeros, whatever is there, and NaN and
     // infinity reach the rows that attend to them only: left out of the products and
     // added one by one
@@ -596,28 +607,42 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       const uint32_t two = valid >> (8 * g + 2 * d);
       keep[d] = (two & 1 ? 0xFFFFu : 0) | (two & 2 ? 0xFFFF0000u : 0);
     }
-#pragma unroll 1
-    for (int n = 0; n < DT; ++n) {
-      const u32x4 x = value(n);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) bad |= tree_nonfinite(x[d] & keep[d]);
+    for (int n0 = 0; n0 < DT; n0 += EARLY) {
+      u32x4 x[EARLY];
+#pragma unroll
+      for (int n = 0; n < EARLY; ++n) {
+        x[n] = va[n];
+        if (NARROW) x[n] = __builtin_bit_cast(u32x4, tree_e4m3x8(x[n][0], x[n][1]));
+      }
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < EARLY; ++n)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            x[n][d] &= keep[d];
+            bad |= tree_nonfinite(x[n][d]);
+            x[n][d] &= tree_finite(x[n][d]);
+          }
+      }
+      if (n0 + EARLY < DT) {
+#pragma unroll
+        for (int n = 0; n < EARLY; ++n) va[n] = value(n0 + EARLY + n);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int n = 0; n < EARLY; ++n) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[nt][n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8, x[n]), __builtin_bit_cast(bf16x8, ph[nt]), acc[nt][n0 + n], 0, 0, 0);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          acc[nt][n0 + n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(bf16x8, x[n]), __builtin_bit_cast(bf16x8, pl[nt]), acc[nt][n0 + n], 0, 0, 0);
+      }
     }
-    const bool some = __any((bad & 0x80008000u) != 0);
-#pragma unroll
-    for (int n = 0; n < DT; ++n) {
-      u32x4 x = value(n);
-#pragma unroll
-      for (int d = 0; d < 4; ++d) x[d] &= keep[d] & tree_finite(x[d]);
-      const bf16x8 va = __builtin_bit_cast(bf16x8, x);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, ph[nt]),
-                                                             acc[nt][n], 0, 0, 0);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        acc[nt][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(bf16x8, pl[nt]),
-                                                             acc[nt][n], 0, 0, 0);
-    }
+    const bool some = masked && __any((bad & 0x80008000u) != 0);
     if (!some) return;
 #pragma unroll 1
     for (int k = 0; k < TREE_UNIT; ++k) {
@@ -727,7 +752,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   uint32_t now = 0;                          // CONV: the bf16 buffer that is computed
   uint32_t at = 0, at_scale = 0;             // the stage that is computed, its scales
 #pragma unroll 1
-  for (int k = -FIRST;; ++k) {
+  for (int k = -FIRST - 1;; ++k) {           // (before the first there is a piece to find)
     uint32_t here = 0;
     if (k >= 0) {
       if (i == todo) {
@@ -738,7 +763,8 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       arrive(std::integral_constant<int, S - 2>());
       here = held >> 2 * at & 3;
     }
-    request();
+    if (k >= -FIRST) request();
+    advance();
     if (k >= 0) {
       const int unit = cur.unit + i * WT + wt;
       const CX_LDS char* kv = CONV ? wide + now * Sh::WIDE : ring + at * RAW;
