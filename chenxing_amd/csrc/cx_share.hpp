@@ -26,7 +26,6 @@ struct ShareBatch {
   int G, heads;               // q heads per kv head, kv heads
   int window;                 // 0: none
   int held;                   // tokens that a table row's pages hold
-  bool tree = false;          // new tokens attend to any of the others
 };
 
 // A sequence: its rows among the new tokens, the length, and its units (those in
@@ -125,7 +124,8 @@ struct AttendSeqs {
   }
 };
 
-template <int TOK, int NT>
+// TREE: new tokens may attend to any of the others.
+template <int TOK, int NT, bool TREE = false>
 struct AttendLine {
   static constexpr int ROWS = 16 * NT;
   // what a row block costs beside its units, in units (64 ragged requests 99, 94
@@ -150,8 +150,12 @@ struct AttendLine {
   static __device__ __forceinline__ AttendGroups groups(const ShareBatch& A, const AttendSeq& s,
                                                         int blocks) {
     AttendGroups g;
-    g.size = A.tree ? max(blocks, 1) : A.G * (TOK / 16);
+    g.size = A.G * (TOK / 16);
     g.count = (blocks + g.size - 1) / g.size;
+    if (TREE) {
+      g.size = blocks;
+      g.count = 1;
+    }
     g.n0 = g.most = s.n;
     const int lowest = s.len - s.q;
     if (g.count > 1 && lowest >= 0) {

@@ -36,7 +36,9 @@ constexpr int TREE_UNIT = 32;                // slots of a unit
 constexpr int TREE_LEAST = 2;                // the least share, in units
 constexpr int TREE_BLOCK_STEPS = 8;          // steps of the longest context in one launch
 constexpr int TREE_BATCH = 512;              // sequences of a launch: their lengths are in LDS
-constexpr float TREE_SLACK = 8.f;            // terms reach 2^8: the sums are rarely scaled
+// A lane's terms of a unit sum to this before the running maximum is raised: it need not
+// be the largest score, so most units look for none.
+constexpr float TREE_SLACK = 4096.f;
 constexpr float TREE_LOW = -3e38f;           // running maximum of a row that attends to something
 
 struct TreeArgs {
@@ -110,6 +112,10 @@ __device__ __forceinline__ void load_lds16(const char* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(to), "v"(from) : "memory", "m0");
 }
+__device__ __forceinline__ void load_lds16_at(const char* base, uint32_t at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(to), "v"(at), "s"(base) : "memory", "m0");
+}
 __device__ __forceinline__ void load_lds4(const char* from, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                :: "s"(to), "v"(from) : "memory", "m0");
@@ -146,7 +152,7 @@ struct TreeShape {
   // the groups' sums meet DR dims at a time
   static constexpr int DR = WT == 1 ? D : WR == 2 ? 32 : 64;
   static constexpr int SCRATCH = WT == 1 ? 0 : (WT - 1) * WR * 16 * (DR + 16) * 4;
-  using Line = AttendLine<TREE_UNIT, NT * WR>;
+  using Line = AttendLine<TREE_UNIT, NT * WR, true>;
   using Seqs = AttendSeqs<CX_LDS uint64_t*, CX_LDS int*>;
   static constexpr int QUEUE = TREE_WAVES * (S + 2) * 64;       // pieces on their way, by wave
   static constexpr int off_scratch() { return WT * GROUP; }
@@ -189,7 +195,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   CX_LDS int* const s_queue = (CX_LDS int*)(to_lds(lds) + Sh::off_queue()) + w * (S + 2) * 16;
   auto share_batch = [&]() {
     const auto& A = tree_args();
-    return ShareBatch{A.G, A.kv.heads, A.window, A.kv.n_pages ? A.kv.M << A.kv.logP : 0, true};
+    return ShareBatch{A.G, A.kv.heads, A.window, A.kv.n_pages ? A.kv.M << A.kv.logP : 0};
   };
   auto first = [&](int b) { return seqs.starts ? seqs.first(b) : tree_args().b0 + b; };
   auto seq = [&](const ShareBatch& batch, int b) {
@@ -250,9 +256,11 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   // The workgroup's pieces, as they are loaded; what is computed takes them, up to S +
   // 1 later, from the wave's queue.
   struct {
-    int b, h, lim, unit, cnt;
-  } ahead = {0, 0, 0, 0, 0};
-  int step = -1, steps = 0;                  // of the piece that is loaded
+    const int32_t* ids;       // of the sequence's pages
+    const char* head;         // the head's part of page 0
+    int groups, unit, cnt;    // groups of 16 slots
+  } ahead = {nullptr, C.pages, 0, 0, 0};
+  int step = 0, steps = 0;                   // of the piece that is loaded
   uint64_t u = share_begin(split, worker);   // past it
   int b = 0, rb = (int)(blockIdx.x / (unsigned)C.heads);        // block: the next row block
   if (!A.block)
@@ -294,9 +302,9 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       u = tree_scalar(u);
       if (p.cnt == 0) return false;
     }
-    ahead.b = __builtin_amdgcn_readfirstlane(p.b);
-    ahead.h = __builtin_amdgcn_readfirstlane(p.h);
-    ahead.lim = __builtin_amdgcn_readfirstlane(p.lim);
+    ahead.ids = A.kv.table + __builtin_amdgcn_readfirstlane(p.b) * A.kv.ld_table;
+    ahead.head = A.kv.pages + __builtin_amdgcn_readfirstlane(p.h) * (int64_t)A.kv.head_bytes;
+    ahead.groups = (__builtin_amdgcn_readfirstlane(p.lim) + 15) >> 4;
     ahead.unit = __builtin_amdgcn_readfirstlane(p.unit);
     ahead.cnt = __builtin_amdgcn_readfirstlane(p.cnt);
     const int x = l == 0 ? p.h : l == 1 ? p.tok0 : l == 2 ? p.r0 : l == 3 ? p.R : l == 4 ? p.lowest
@@ -311,53 +319,57 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   // The ids of a unit's two groups of 16 slots, asked for a step before they are used.
   bool more = true, live = false;            // pieces to load; a unit for this group's next stage
   int unit = 0, next0 = -1, next1 = -1;
-  auto advance = [&]() {
-    if (++step >= steps && more) more = next_piece();
+  auto ask = [&]() {
     unit = ahead.unit + step * WT + wt;
     live = more && step * WT + wt < ahead.cnt;
     auto id = [&](int half) {
       const int s16 = 2 * unit + half;
-      if (!live || s16 >= (ahead.lim + 15) >> 4) return -1;
-      return const_load(C.table + ahead.b * C.ld_table + (s16 >> (C.logP - 4)));
+      if (!live || s16 >= ahead.groups) return -1;
+      return const_load(ahead.ids + (s16 >> (C.logP - 4)));
     };
     next0 = id(0);
     next1 = id(1);
   };
-  const int slot16 = 4 * ((c >> 2) & 1) * 2 + (c & 3);          // of 16: 8 (c / 4 % 2) + c % 4
-  const int half_of = c >> 3;                // K: the lane's slot is in group c / 8
+  // Load j of the wave is chunks 64 i .. of the stage, i = wr + WR j: of K, chunk rows 2 i
+  // and 2 i + 1 of 32 slots, the lane's in group c / 8; of V (F8: 16 slots a chunk) of D
+  // dims.  The lane's place in its page's part, but for the unit's:
+  constexpr int NK = Sh::LOADS / 2;
+  uint32_t place[Sh::LW];
+#pragma unroll
+  for (int j = 0; j < Sh::LW; ++j) {
+    const int i = wr + WR * j, f = 64 * (i - NK), row = f / D;
+    const int slot = 8 * (c >> 2 & 1) + 4 * (l >> 4 & 1) + (c & 3);
+    place[j] = i < NK ? (((2 * i + (l >> 5)) << C.logP) + slot) * 16
+                      : v_chunk<E, D>(f % D + l, F8 ? 0 : 8 * (row & 1), C.logP);
+  }
+  const uint32_t place_scale = k_scale<D>(l & 15, C.logP) + (l & 32 ? 4 * P : 0);
   uint32_t fill = 0, fill_scale = 0;         // the stage that is loaded next, its scales
   uint32_t held = 0;                         // bits 2 s, 2 s + 1: stage s's groups are in the pool
   auto request = [&]() {
-    const int id0 = (unsigned)next0 < (unsigned)C.n_pages ? next0 : -1;
-    const int id1 = (unsigned)next1 < (unsigned)C.n_pages ? next1 : -1;
-    const char* head0 = C.pages + (int64_t)(live ? ahead.h : 0) * C.head_bytes;
-    const char* p0 = head0 + (int64_t)max(id0, 0) * C.page_stride;
-    const char* p1 = head0 + (int64_t)max(id1, 0) * C.page_stride;
-    const int o0 = (unit * 32) & (P - 1), o1 = (unit * 32 + 16) & (P - 1);
+    const bool in0 = (unsigned)next0 < (unsigned)C.n_pages, in1 = (unsigned)next1 < (unsigned)C.n_pages;
+    held = (held & ~(3u << 2 * fill)) | ((in0 ? 1u : 0u) | (in1 ? 2u : 0u)) << 2 * fill;
+    const char* p0 = ahead.head + (in0 ? next0 : 0) * C.page_stride;
+    const char* p1 = ahead.head + (in1 ? next1 : 0) * C.page_stride;
+    const int o0 = live ? (unit * 32) & (P - 1) : 0, o1 = live ? (unit * 32 + 16) & (P - 1) : 0;
     const uint32_t to = (uint32_t)(uintptr_t)ring + fill * RAW;
-    held = (held & ~(3u << 2 * fill)) | ((id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u)) << 2 * fill;
-    const char* const none = (const char*)A.out;                // a place to read without a unit
+    const uint32_t on = live ? ~0u : 0;      // without a unit: page 0's first bytes, all lanes
     if (F8 && wr == 0) {
-      // natural order of slots: keys' scales, then values'
-      const char* p = (l & 16 ? p1 + 4 * o1 : p0 + 4 * o0) + k_scale<D>(l & 15, C.logP) + (l & 32 ? P * 4 : 0);
-      load_lds4(live ? p : none, (uint32_t)(uintptr_t)s_scale + 256 * fill_scale);
+      // in their slots' order: keys' scales, then values'
+      const char* p = l & 16 ? p1 + 4 * o1 : p0 + 4 * o0;
+      load_lds4(p + (place_scale & on), (uint32_t)(uintptr_t)s_scale + 256 * fill_scale);
     }
-    const char* pk = half_of ? p1 + 16 * o1 : p0 + 16 * o0;
+    const char* pk = c & 8 ? p1 + 16 * o1 : p0 + 16 * o0;
+    constexpr int VS = F8 ? D : 2 * D;       // bytes of V a slot
 #pragma unroll
     for (int j = 0; j < Sh::LW; ++j) {
       const int i = wr + WR * j;
       if (i >= Sh::LOADS) break;             // (uniform)
-      const char* p;
-      if (i < Sh::LOADS / 2) {               // chunk rows 2 i and 2 i + 1 of 32 slots
-        const int y = (l >> 4) & 1;
-        p = pk + (((2 * i + (l >> 5)) << C.logP) + slot16 + 4 * y) * 16;
+      if (NK % WR == 0 ? WR * j < NK : i < NK) {
+        load_lds16(pk + (place[j] & on), to + 1024 * i);
       } else {
-        const int f = 64 * (i - Sh::LOADS / 2);                 // the first of its chunks
-        const int row = f / D, d = f % D + l;                   // (D >= 64: one row)
-        const int half = F8 ? row : row >> 1;
-        p = (half ? p1 : p0) + v_chunk<E, D>(d, (half ? o1 : o0) + (F8 ? 0 : 8 * (row & 1)), C.logP);
+        const int row = 64 * (i - NK) / D, half = F8 ? row : row >> 1;
+        load_lds16_at(half ? p1 + (int64_t)o1 * VS : p0 + (int64_t)o0 * VS, place[j] & on, to + 1024 * i);
       }
-      load_lds16(live ? p : none, to + 1024 * i);
     }
     fill = fill + 1 == S ? 0 : fill + 1;
     if (F8) fill_scale = fill_scale == S ? 0 : fill_scale + 1;
@@ -452,7 +464,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     const uint64_t both = (uint64_t)word(k) | (uint64_t)word(k + 1) << 32;
     return (uint32_t)(both >> sh);
   };
-  auto compute = [&](int unit, uint32_t here, const CX_LDS char* kv, const CX_LDS char* scales) {
+  auto compute = [&](int unit, uint32_t here, const CX_LDS char* kv, const CX_LDS char* scales, auto then) {
     const int t0 = unit * TREE_UNIT;
     f32x4 v[NT][2];
 #pragma unroll
@@ -555,58 +567,81 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
           for (int j = 0; j < 4; ++j) v[nt][y][j] = mine >> (4 * y + j) & 1 ? v[nt][y][j] : -INFINITY;
       }
     }
-    float alpha[NT];
-    bool moved = false;
+    // terms by the maximum so far, unless one is much above it
     u32x4 ph[NT], pl[NT];
+    float add[NT];
+    auto terms = [&](int nt, int y) {
+      const float base = m[nt] == -INFINITY ? 0.f : m[nt];
+      f32x4 p;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(to2, v[nt][y][j], -base));
+      return p;
+    };
+    bool above = false;
+    f32x4 p[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float top = fmaxf(fmaxf(fmaxf(v[nt][0][0], v[nt][0][1]), fmaxf(v[nt][0][2], v[nt][0][3])),
-                        fmaxf(fmaxf(v[nt][1][0], v[nt][1][1]), fmaxf(v[nt][1][2], v[nt][1][3])));
-      const float m1 = fmaxf(low[nt], to2 * tree_groups_max(top));
-      const bool up = m1 > m[nt] + TREE_SLACK;
-      const float base = up ? m1 : m[nt] == -INFINITY ? 0.f : m[nt];
-      alpha[nt] = up ? __builtin_amdgcn_exp2f(m[nt] - m1) : 1.f;
-      moved |= up;
-      m[nt] = up ? m1 : m[nt];
-      float add = 0;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) p[nt][y] = terms(nt, y);
+      add[nt] = ((p[nt][0][0] + p[nt][0][1]) + (p[nt][0][2] + p[nt][0][3])) +
+                ((p[nt][1][0] + p[nt][1][1]) + (p[nt][1][2] + p[nt][1][3]));
+      above |= !(add[nt] < TREE_SLACK) || (m[nt] == -INFINITY && low[nt] != -INFINITY);
+    }
+    if (__any(above)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top = low[nt];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = fmaxf(top, to2 * v[nt][y][j]);
+        const float m1 = fmaxf(m[nt], tree_groups_max(top));
+        const float alpha = m[nt] == m1 ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m1);
+        m[nt] = m1;
+        sum[nt] *= alpha;
+#pragma unroll
+        for (int n = 0; n < DT; ++n) acc[nt][n] *= alpha;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) p[nt][y] = terms(nt, y);
+        add[nt] = ((p[nt][0][0] + p[nt][0][1]) + (p[nt][0][2] + p[nt][0][3])) +
+                  ((p[nt][1][0] + p[nt][1][1]) + (p[nt][1][2] + p[nt][1][3]));
+      }
+    }
+    if (F8) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) p[nt][y] *= vs[y];
+      if (masked) {                          // (0 times a scale that is NaN)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[nt][y][j] = bits[nt] >> (8 * g + 4 * y + j) & 1 ? p[nt][y][j] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      sum[nt] += add[nt];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        f32x4 p;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(to2, v[nt][y][j], -base));
-        add += (p[0] + p[1]) + (p[2] + p[3]);
-        if (F8) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) p[j] = v[nt][y][j] == -INFINITY ? 0.f : p[j] * vs[y][j];
-        }
         // two bf16 parts: the first cut off, the second never 0, so that an infinite
         // value keeps its sign in both products (2^-20 of a term too much)
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
-          const float p0 = p[2 * d], p1 = p[2 * d + 1];
+          const float p0 = p[nt][y][2 * d], p1 = p[nt][y][2 * d + 1];
           const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
           ph[nt][2 * y + d] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
           pl[nt][2 * y + d] = pack_bf16(fmaf(p0, 1.f + 0x1p-20f, -__uint_as_float(x0 & 0xFFFF0000u)),
                                         fmaf(p1, 1.f + 0x1p-20f, -__uint_as_float(x1 & 0xFFFF0000u)));
         }
       }
-      sum[nt] = fmaf(sum[nt], alpha[nt], add);
-    }
-    if (__any(moved)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int n = 0; n < DT; ++n) acc[nt][n] *= alpha[nt];
     }
     // V of slots that nobody holds counts as zeros, whatever is there, and NaN and
     // infinity reach the rows that attend to them only: left out of the products and
     // added one by one
-    uint32_t keep[4], bad = 0;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const uint32_t two = valid >> (8 * g + 2 * d);
-      keep[d] = (two & 1 ? 0xFFFFu : 0) | (two & 2 ? 0xFFFF0000u : 0);
-    }
+    uint32_t bad = 0;
 #pragma unroll
     for (int n0 = 0; n0 < DT; n0 += EARLY) {
       u32x4 x[EARLY];
@@ -620,7 +655,8 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         for (int n = 0; n < EARLY; ++n)
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
-            x[n][d] &= keep[d];
+            const uint32_t two = valid >> (8 * g + 2 * d);
+            x[n][d] &= (two & 1 ? 0xFFFFu : 0) | (two & 2 ? 0xFFFF0000u : 0);
             bad |= tree_nonfinite(x[n][d]);
             x[n][d] &= tree_finite(x[n][d]);
           }
@@ -628,6 +664,11 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       if (n0 + EARLY < DT) {
 #pragma unroll
         for (int n = 0; n < EARLY; ++n) va[n] = value(n0 + EARLY + n);
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+        // its scalar loads would make LDS reads after them wait for all: there are none
+        __builtin_amdgcn_sched_barrier(0);
+        then();
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
@@ -752,7 +793,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   uint32_t now = 0;                          // CONV: the bf16 buffer that is computed
   uint32_t at = 0, at_scale = 0;             // the stage that is computed, its scales
 #pragma unroll 1
-  for (int k = -FIRST - 1;; ++k) {           // (before the first there is a piece to find)
+  for (int k = -FIRST;; ++k) {
     uint32_t here = 0;
     if (k >= 0) {
       if (i == todo) {
@@ -763,16 +804,26 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       arrive(std::integral_constant<int, S - 2>());
       here = held >> 2 * at & 3;
     }
-    if (k >= -FIRST) request();
-    advance();
+    if (step >= steps && more) {
+      more = next_piece();
+      ask();
+    }
+    request();
+    auto next = [&]() {
+      ++step;
+      if (step < steps || !more) ask();
+    };
     if (k >= 0) {
       const int unit = cur.unit + i * WT + wt;
       const CX_LDS char* kv = CONV ? wide + now * Sh::WIDE : ring + at * RAW;
-      if (i * WT + wt < cur.cnt) compute(unit, here, kv, s_scale + 256 * at_scale);
+      if (i * WT + wt < cur.cnt) compute(unit, here, kv, s_scale + 256 * at_scale, next);
+      else next();
       ++i;
       now ^= 1;
       at = at + 1 == S ? 0 : at + 1;
       if (F8) at_scale = at_scale == S ? 0 : at_scale + 1;
+    } else {
+      next();
     }
     if (CONV && k >= -1) {
       if (k < 0) arrive(std::integral_constant<int, S - 1>());
