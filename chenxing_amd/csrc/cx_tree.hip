@@ -34,7 +34,8 @@ constexpr int TREE_WAVES = 8, TREE_WG = 64 * TREE_WAVES;
 constexpr int TREE_WORKERS = 256;            // a workgroup a CU
 constexpr int TREE_UNIT = 32;                // slots of a unit
 constexpr int TREE_LEAST = 2;                // the least share, in units
-constexpr int TREE_BLOCK_STEPS = 8;          // steps of the longest context in one launch
+constexpr int TREE_CHUNK = 24;               // units of a workgroup's chunk at most
+constexpr int64_t TREE_SPREAD = 512;         // workgroups of chunks that are aimed at
 constexpr int TREE_BATCH = 512;              // sequences of a launch: their lengths are in LDS
 // A lane's terms of a unit sum to this before the running maximum is raised: it need not
 // be the largest score, so most units look for none.
@@ -55,11 +56,11 @@ struct TreeArgs {
   int window;                 // 0: none
   uint16_t* out;
   int b0;                     // first sequence of the launch; kv.B: their number
-  int block;                  // a workgroup a row block
+  int tiles, chunks, chunk;   // row blocks of a sequence, their parts, units of a part
   int* entries;               // number of entries of join
   AttendJoin* join;           // [TREE_WORKERS]
-  float* ml;                  // [2 TREE_WORKERS, ROWS, 2]: a part's maxima and sums
-  float* part;                // [2 TREE_WORKERS, ROWS, D], in the order of join's lanes
+  float* ml;                  // [slots, ROWS, 2]: a part's maxima and sums
+  float* part;                // [slots, ROWS, D], in the order of join's lanes
 };
 
 __device__ __forceinline__ uint64_t tree_scalar(uint64_t x) {
@@ -73,6 +74,12 @@ __device__ __forceinline__ const TreeArgs& tree_args() {
   uint64_t p = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
   return *(const TreeArgs*)(const CX_CONST TreeArgs*)p;
+}
+// The lane's number, for rare code: what it makes of it is not kept for the loop.
+__device__ __forceinline__ int rare_lane() {
+  int l = lane_id();
+  asm volatile("" : "+v"(l));
+  return l;
 }
 // The largest, or the sum, of the four lane groups' values, in every group.
 __device__ __forceinline__ float tree_groups_max(float x) {
@@ -90,6 +97,17 @@ __device__ __forceinline__ float tree_groups_sum(float x) {
   a = __float_as_uint(x);
   r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Sequence b of a launch, its lengths by scalar loads.
+template <class Line>
+__device__ __forceinline__ AttendSeq tree_seq(const TreeArgs& A, int b) {
+  int s0 = A.b0 + b, s1 = s0 + 1;
+  if (A.kv.q_start) {
+    s0 = min(max(const_load(A.kv.q_start + b), 0), A.kv.T);
+    s1 = min(max(const_load(A.kv.q_start + b + 1), s0), A.kv.T);
+  }
+  return Line::seq(ShareBatch{A.G, A.kv.heads, A.window, A.kv.n_pages ? A.kv.M << A.kv.logP : 0}, s0, s1,
+                   const_load(A.kv.kv_len + b));
 }
 // Eight e4m3 codes as bf16.
 __device__ __forceinline__ bf16x8 tree_e4m3x8(uint32_t a, uint32_t b) {
@@ -171,7 +189,11 @@ struct TreeShape {
 //    unconditional, after the last unit all of one place.
 //  * Softmax terms enter the products as two bf16 parts (16 bits): one part's rounding
 //    would add as much error as the result's own.
-template <int D, int NT, int WR, bool F8>
+//
+// SHARES: each of TREE_WORKERS workgroups takes an equal stretch of the line of all the
+// batch's units (cx_share.hpp).  Else a workgroup takes A.chunk units of one row block:
+// no lengths to sum up, no places to find (launch_tree says when).
+template <int D, int NT, int WR, bool F8, bool SHARES>
 __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   using Sh = TreeShape<D, NT, WR, F8>;
   using Line = typename Sh::Line;
@@ -202,20 +224,22 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     const int f = first(b);
     return Line::seq(batch, f, seqs.starts ? seqs.end(b) : f + 1, s_len[b]);
   };
-
-  // a sequence whose tokens attend to nothing
-  auto nothing = [&](int b) {
-    const int r0 = first(b), rows = (seqs.starts ? seqs.end(b) : r0 + 1) - r0;
-    const int64_t n = (int64_t)rows * A.q_heads * (D / 8);
+  // tokens r0 .. end - 1 attend to nothing
+  auto nothing = [&](int r0, int end) {
+    const int64_t n = (int64_t)(end - r0) * A.q_heads * (D / 8);
     u32x4* o = (u32x4*)(A.out + (int64_t)r0 * A.q_heads * D);
     for (int64_t i = tid; i < n; i += TREE_WG) o[i] = u32x4{0, 0, 0, 0};
   };
 
-  // the line before each sequence, and its whole
-  seqs.read(C.kv_len, C.q_start, C.B, C.T, tid, TREE_WG);
-  uint64_t line = 0;
-  __syncthreads();
-  if (!A.block) {
+  const unsigned worker = blockIdx.x;
+  ShareSplit split = {};
+  uint64_t end = 0;
+  int blocks = 0;                            // the sequence's row blocks
+  AttendSeq own = {};                        // the sequence
+  if constexpr (SHARES) {
+    // the line before each sequence, and its whole
+    seqs.read(C.kv_len, C.q_start, C.B, C.T, tid, TREE_WG);
+    __syncthreads();
     const int b = tid;                       // (a launch's sequences are no more)
     uint64_t x = 0;
     if (b < C.B) x = Line::length(share_batch(), seq(share_batch(), b));
@@ -230,27 +254,25 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     if (b < C.B) s_pref[b + 1] = x;
     if (tid == 0) s_pref[0] = 0;
     __syncthreads();
-    line = s_pref[C.B];
-  } else if (seq(share_batch(), blockIdx.y).n == 0) {
-    if (blockIdx.x == 0) nothing(blockIdx.y);
-    return;
-  }
-  line = tree_scalar(line);
-  ShareSplit split = share_split(line, TREE_WORKERS, TREE_LEAST);
-  split.per = tree_scalar(split.per);
-  split.more = tree_scalar(split.more);
-  const bool by_block = split.by_block;
-  const unsigned worker = blockIdx.x;
-  uint64_t end = 0;
-  if (!A.block) {
-    if (worker == 0 && tid == 0) *A.entries = by_block ? (int)line_blocks(line) : TREE_WORKERS;
+    const uint64_t line = tree_scalar(s_pref[C.B]);
+    split = share_split(line, TREE_WORKERS, TREE_LEAST);
+    split.per = tree_scalar(split.per);
+    split.more = tree_scalar(split.more);
+    if (worker == 0 && tid == 0) *A.entries = split.by_block ? (int)line_blocks(line) : TREE_WORKERS;
     for (int b = blockIdx.x; b < C.B; b += TREE_WORKERS)
-      if (s_pref[b + 1] == s_pref[b]) nothing(b);
+      if (s_pref[b + 1] == s_pref[b]) nothing(first(b), seqs.starts ? seqs.end(b) : first(b) + 1);
     if (worker >= split.shares) {
-      if (tid == 0 && !by_block) A.join[worker].last = -1;
+      if (tid == 0 && !split.by_block) A.join[worker].last = -1;
       return;
     }
     end = share_begin(split, worker) + split.per + (worker < split.more);
+  } else {
+    own = tree_seq<Line>(A, blockIdx.y);
+    blocks = Line::row_blocks(share_batch(), own);
+    if (own.n == 0) {
+      if (blockIdx.x == 0) nothing(own.tok0, own.tok0 + own.q);
+      return;
+    }
   }
 
   // The workgroup's pieces, as they are loaded; what is computed takes them, up to S +
@@ -261,14 +283,23 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     int groups, unit, cnt;    // groups of 16 slots
   } ahead = {nullptr, C.pages, 0, 0, 0};
   int step = 0, steps = 0;                   // of the piece that is loaded
-  uint64_t u = share_begin(split, worker);   // past it
-  int b = 0, rb = (int)(blockIdx.x / (unsigned)C.heads);        // block: the next row block
-  if (!A.block)
+  uint64_t u = 0;                            // SHARES: past it
+  int b = 0;
+  // else the kv head, the row block and the part of its units
+  const int head = (int)(blockIdx.x % (unsigned)C.heads);
+  int rb = (int)(blockIdx.x / (unsigned)C.heads), chunk = 0;
+  if constexpr (SHARES) {
+    u = share_begin(split, worker);
     for (int hi = C.B - 1; b < hi;) {        // the last b with its units at or before u
       const int mid = (b + hi + 1) >> 1;
       if (line_units(s_pref[mid]) <= u) b = mid;
       else hi = mid - 1;
     }
+  } else {
+    chunk = rb / A.tiles;
+    rb %= A.tiles;
+    if (rb >= blocks || chunk * A.chunk >= own.n) return;
+  }
   bool joined = false;
   int pushed = 0;
   // The next piece, pushed to the queue, and whether there is one.
@@ -276,21 +307,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     const auto& A = tree_args();
     const ShareBatch batch = share_batch();
     AttendPiece p;
-    if (A.block) {
-      const AttendSeq s = seq(batch, blockIdx.y);
-      if (rb >= Line::row_blocks(batch, s)) return false;
-      p.b = blockIdx.y;
-      p.h = (int)(blockIdx.x % (unsigned)A.kv.heads);
-      p.tok0 = s.tok0;
-      p.r0 = rb * ROWS;
-      p.R = min(ROWS, s.q * A.G - p.r0);
-      p.lowest = s.len - s.q;
-      p.lim = s.lim;
-      p.unit = s.first;
-      p.cnt = s.n;
-      p.slot = -1;
-      rb += (int)(gridDim.x / (unsigned)A.kv.heads);
-    } else {
+    if constexpr (SHARES) {
       if (u >= end) return false;
       while (line_units(s_pref[b + 1]) <= u) ++b;
       b = __builtin_amdgcn_readfirstlane(b);
@@ -301,12 +318,32 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
                       });
       u = tree_scalar(u);
       if (p.cnt == 0) return false;
+    } else {
+      // its chunk; then, where a sequence has more new tokens than the caller said, the
+      // first chunk's workgroups take whole row blocks
+      const bool whole = rb >= A.tiles;
+      if (rb >= blocks || (whole && chunk > 0)) return false;
+      p.b = blockIdx.y;
+      p.h = head;
+      p.tok0 = own.tok0;
+      p.r0 = rb * ROWS;
+      p.R = min(ROWS, own.q * A.G - p.r0);
+      p.lowest = own.len - own.q;
+      p.lim = own.lim;
+      p.unit = own.first + (whole ? 0 : chunk * A.chunk);
+      // (the last one what a longer context than the launch counts on has left)
+      p.cnt = whole ? own.n : own.n - chunk * A.chunk;
+      if (!whole && chunk + 1 < A.chunks) p.cnt = min(p.cnt, A.chunk);
+      p.slot = p.cnt == own.n ? -1
+                              : ((int)blockIdx.y * A.kv.heads + head) * A.tiles * A.chunks + rb * A.chunks + chunk;
+      rb += A.tiles;
     }
     ahead.ids = A.kv.table + __builtin_amdgcn_readfirstlane(p.b) * A.kv.ld_table;
     ahead.head = A.kv.pages + __builtin_amdgcn_readfirstlane(p.h) * (int64_t)A.kv.head_bytes;
     ahead.groups = (__builtin_amdgcn_readfirstlane(p.lim) + 15) >> 4;
     ahead.unit = __builtin_amdgcn_readfirstlane(p.unit);
     ahead.cnt = __builtin_amdgcn_readfirstlane(p.cnt);
+    const int l = rare_lane();
     const int x = l == 0 ? p.h : l == 1 ? p.tok0 : l == 2 ? p.r0 : l == 3 ? p.R : l == 4 ? p.lowest
                   : l == 5 ? p.lim : l == 6 ? p.unit : l == 7 ? p.cnt : p.slot;
     if (l < 9) s_queue[16 * pushed + l] = x;
@@ -344,10 +381,11 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   }
   const uint32_t place_scale = k_scale<D>(l & 15, C.logP) + (l & 32 ? 4 * P : 0);
   uint32_t fill = 0, fill_scale = 0;         // the stage that is loaded next, its scales
-  uint32_t held = 0;                         // bits 2 s, 2 s + 1: stage s's groups are in the pool
+  uint32_t held = 0, fill_held = 0;          // two bits a stage: its groups are in the pool
   auto request = [&]() {
     const bool in0 = (unsigned)next0 < (unsigned)C.n_pages, in1 = (unsigned)next1 < (unsigned)C.n_pages;
-    held = (held & ~(3u << 2 * fill)) | ((in0 ? 1u : 0u) | (in1 ? 2u : 0u)) << 2 * fill;
+    held = (held & ~(3u << 2 * fill_held)) | ((in0 ? 1u : 0u) | (in1 ? 2u : 0u)) << 2 * fill_held;
+    fill_held = (fill_held + 1) & 15;
     const char* p0 = ahead.head + (in0 ? next0 : 0) * C.page_stride;
     const char* p1 = ahead.head + (in1 ? next1 : 0) * C.page_stride;
     const int o0 = live ? (unit * 32) & (P - 1) : 0, o1 = live ? (unit * 32 + 16) & (P - 1) : 0;
@@ -415,8 +453,10 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     int h, tok0, r0, R, lowest, lim, unit, cnt, slot;
   } cur;
   int popped = 0, i = 0, todo = 0;           // the step of the piece, and its steps
+  int count = 0;                             // its units, 0 for a wave without rows
   auto begin = [&]() {
     const auto& A = tree_args();
+    const int l = rare_lane(), g = l >> 4, c = l & 15;
     const int x = s_queue[16 * popped + c];
     popped = popped == S + 1 ? 0 : popped + 1;
     cur.h = lane_read(x, 0);
@@ -430,6 +470,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     cur.slot = lane_read(x, 8);
     i = 0;
     todo = (cur.cnt + WT - 1) / WT;
+    count = 16 * NT * wr < cur.R ? cur.cnt : 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = cur.r0 + min(16 * (NT * wr + nt) + c, cur.R - 1);
@@ -464,7 +505,12 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     const uint64_t both = (uint64_t)word(k) | (uint64_t)word(k + 1) << 32;
     return (uint32_t)(both >> sh);
   };
-  auto compute = [&](int unit, uint32_t here, const CX_LDS char* kv, const CX_LDS char* scales, auto then) {
+  // What a unit's products with V need of its scores.
+  u32x4 ph[NT], pl[NT];                      // the terms, in two parts
+  bool masked = false;
+  uint32_t valid = 0, bits[NT];              // slots that are held; that the row attends to
+  const CX_LDS char* vb = nullptr;
+  auto scores = [&](int unit, uint32_t here, const CX_LDS char* kv, const CX_LDS char* scales) {
     const int t0 = unit * TREE_UNIT;
     f32x4 v[NT][2];
 #pragma unroll
@@ -498,20 +544,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         }
       __builtin_amdgcn_sched_barrier(0);
     }
-    // V, while the scores become terms
-    const CX_LDS char* vb = kv + (NARROW ? KB : 2 * TREE_UNIT * D);
-    auto value = [&](int n) {
-      if (NARROW) {
-        const u32x2 r = *(const CX_LDS u32x2*)(vb + ((g >> 1) * D + 16 * n + c) * 16 + 8 * (g & 1));
-        return u32x4{r[0], r[1], 0, 0};
-      }
-      return *(const CX_LDS u32x4*)(vb + (g * D + 16 * n + c) * 16);
-    };
-    constexpr int EARLY = 4;                 // of V's 16-dim tiles, four together
-    u32x4 va[EARLY];
-#pragma unroll
-    for (int n = 0; n < EARLY; ++n) va[n] = value(n);
-    __builtin_amdgcn_sched_barrier(0);
+    vb = kv + (NARROW ? KB : 2 * TREE_UNIT * D);
     f32x4 vs[F8 ? 2 : 1];
     if (F8) {
 #pragma unroll
@@ -537,21 +570,19 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     }
     // a unit is open where all its slots are held, before the tree and inside every
     // row's window
-    bool masked = t0 + TREE_UNIT > min(cur.lowest, cur.lim) || here != 3;
+    masked = t0 + TREE_UNIT > min(cur.lowest, cur.lim) || here != 3;
     if (A.window) {
       bool out = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) out |= lo[nt] >= t0;
       masked |= __any(out);
     }
-    uint32_t valid = ~0u, bits[NT];
+    valid = ~0u;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) bits[nt] = ~0u;
-    float low[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) low[nt] = TREE_LOW;
     auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
     if (masked) {
+      const int g = rare_lane() >> 4;
       valid = (here & 1 ? 0xFFFFu : 0u) | (here & 2 ? 0xFFFF0000u : 0u);
       valid &= below(cur.lim - t0);
 #pragma unroll
@@ -559,7 +590,6 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         uint32_t x = below(cur.lowest - t0) & ~below(lo[nt] + 1 - t0);
         if (t0 + TREE_UNIT > cur.lowest) x |= node_bits(nt, t0 - cur.lowest);
         bits[nt] = x & valid;
-        low[nt] = bits[nt] ? TREE_LOW : -INFINITY;
         const uint32_t mine = bits[nt] >> (8 * g);
 #pragma unroll
         for (int y = 0; y < 2; ++y)
@@ -567,30 +597,26 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
           for (int j = 0; j < 4; ++j) v[nt][y][j] = mine >> (4 * y + j) & 1 ? v[nt][y][j] : -INFINITY;
       }
     }
-    // terms by the maximum so far, unless one is much above it
-    u32x4 ph[NT], pl[NT];
-    float add[NT];
-    auto terms = [&](int nt, int y) {
-      const float base = m[nt] == -INFINITY ? 0.f : m[nt];
-      f32x4 p;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(to2, v[nt][y][j], -base));
-      return p;
-    };
-    bool above = false;
+    // terms by the maximum so far, unless one is much above it (or there is none)
+    float all = 0, add[NT];
     f32x4 p[NT][2];
+    auto terms = [&](int nt, float base) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) p[nt][y] = terms(nt, y);
+        for (int j = 0; j < 4; ++j) p[nt][y][j] = __builtin_amdgcn_exp2f(fmaf(to2, v[nt][y][j], -base));
       add[nt] = ((p[nt][0][0] + p[nt][0][1]) + (p[nt][0][2] + p[nt][0][3])) +
                 ((p[nt][1][0] + p[nt][1][1]) + (p[nt][1][2] + p[nt][1][3]));
-      above |= !(add[nt] < TREE_SLACK) || (m[nt] == -INFINITY && low[nt] != -INFINITY);
+    };
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      terms(nt, m[nt]);
+      all += add[nt];
     }
-    if (__any(above)) {
+    if (masked || __any(!(all < TREE_SLACK))) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float top = low[nt];
+        float top = bits[nt] == 0 ? -INFINITY : TREE_LOW;
 #pragma unroll
         for (int y = 0; y < 2; ++y)
 #pragma unroll
@@ -601,10 +627,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         sum[nt] *= alpha;
 #pragma unroll
         for (int n = 0; n < DT; ++n) acc[nt][n] *= alpha;
-#pragma unroll
-        for (int y = 0; y < 2; ++y) p[nt][y] = terms(nt, y);
-        add[nt] = ((p[nt][0][0] + p[nt][0][1]) + (p[nt][0][2] + p[nt][0][3])) +
-                  ((p[nt][1][0] + p[nt][1][1]) + (p[nt][1][2] + p[nt][1][3]));
+        terms(nt, m1 == -INFINITY ? 0.f : m1);
       }
     }
     if (F8) {
@@ -613,6 +636,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 #pragma unroll
         for (int y = 0; y < 2; ++y) p[nt][y] *= vs[y];
       if (masked) {                          // (0 times a scale that is NaN)
+        const int g = rare_lane() >> 4;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -638,9 +662,22 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         }
       }
     }
-    // V of slots that nobody holds counts as zeros, whatever is there, and NaN and
-    // infinity reach the rows that attend to them only: left out of the products and
-    // added one by one
+  };
+  // The products with V.  V of slots that nobody holds counts as zeros, whatever is there,
+  // and NaN and infinity reach the rows that attend to them only: left out of the
+  // products and added one by one.
+  auto values = [&](auto then) {
+    auto value = [&](int n) {
+      if (NARROW) {
+        const u32x2 r = *(const CX_LDS u32x2*)(vb + ((g >> 1) * D + 16 * n + c) * 16 + 8 * (g & 1));
+        return u32x4{r[0], r[1], 0, 0};
+      }
+      return *(const CX_LDS u32x4*)(vb + (g * D + 16 * n + c) * 16);
+    };
+    constexpr int EARLY = 4;                 // 16-dim tiles that are read together
+    u32x4 va[EARLY];
+#pragma unroll
+    for (int n = 0; n < EARLY; ++n) va[n] = value(n);
     uint32_t bad = 0;
 #pragma unroll
     for (int n0 = 0; n0 < DT; n0 += EARLY) {
@@ -651,6 +688,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         if (NARROW) x[n] = __builtin_bit_cast(u32x4, tree_e4m3x8(x[n][0], x[n][1]));
       }
       if (masked) {
+        const int g = rare_lane() >> 4;
 #pragma unroll
         for (int n = 0; n < EARLY; ++n)
 #pragma unroll
@@ -685,6 +723,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     }
     const bool some = masked && __any((bad & 0x80008000u) != 0);
     if (!some) return;
+    const int lane = rare_lane(), gr = lane >> 4;
 #pragma unroll 1
     for (int k = 0; k < TREE_UNIT; ++k) {
       if (!(valid >> k & 1)) continue;
@@ -692,7 +731,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       for (int n = 0; n < DT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int d = 16 * n + 4 * g + j;
+          const int d = 16 * n + 4 * gr + j;
           float x;
           if (NARROW) x = e4m3_value(*(const CX_LDS uint8_t*)(vb + ((k >> 4) * D + d) * 16 + (k & 15)));
           else x = bf16_lo(*(const CX_LDS uint16_t*)(vb + ((k >> 3) * D + d) * 16 + 2 * (k & 7)));
@@ -764,6 +803,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     meet();
     if (wt > 0) return;
     const auto& A = tree_args();
+    const int l = rare_lane(), g = l >> 4, c = l & 15;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float L = tree_groups_sum(sum[nt]);
@@ -789,12 +829,10 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 
   // ------------------------------------------------------------------ the steps
   // FIRST steps load only; then each computes what arrived and loads FIRST steps ahead
-  constexpr int FIRST = CONV ? S : S - 1;
-  uint32_t now = 0;                          // CONV: the bf16 buffer that is computed
-  uint32_t at = 0, at_scale = 0;             // the stage that is computed, its scales
+  constexpr int FIRST = S - 1 + CONV;
+  uint32_t at = 0, at_scale = 0, at_wide = 0, at_held = 0;      // the stage that is computed
 #pragma unroll 1
   for (int k = -FIRST;; ++k) {
-    uint32_t here = 0;
     if (k >= 0) {
       if (i == todo) {
         if (k > 0) finish();
@@ -802,7 +840,6 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         begin();
       }
       arrive(std::integral_constant<int, S - 2>());
-      here = held >> 2 * at & 3;
     }
     if (step >= steps && more) {
       more = next_piece();
@@ -813,15 +850,11 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       ++step;
       if (step < steps || !more) ask();
     };
-    if (k >= 0) {
-      const int unit = cur.unit + i * WT + wt;
-      const CX_LDS char* kv = CONV ? wide + now * Sh::WIDE : ring + at * RAW;
-      if (i * WT + wt < cur.cnt) compute(unit, here, kv, s_scale + 256 * at_scale, next);
-      else next();
-      ++i;
-      now ^= 1;
-      at = at + 1 == S ? 0 : at + 1;
-      if (F8) at_scale = at_scale == S ? 0 : at_scale + 1;
+    // (a wave without rows, and a group without a unit, only load)
+    if (k >= 0 && i * WT + wt < count) {
+      scores(cur.unit + i * WT + wt, held >> 2 * at_held & 3,
+             CONV ? wide + at_wide * Sh::WIDE : ring + at * RAW, s_scale + 256 * at_scale);
+      values(next);
     } else {
       next();
     }
@@ -829,24 +862,24 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       if (k < 0) arrive(std::integral_constant<int, S - 1>());
       convert();
     }
+    if (k >= 0) {
+      ++i;
+      at = at + 1 == S ? 0 : at + 1;
+      at_held = (at_held + 1) & 15;
+      if (F8) at_scale = at_scale == S ? 0 : at_scale + 1;
+      if (CONV) at_wide ^= 1;
+    }
   }
   wave_vm<0>();                              // the last loads write LDS: end them first
-  if (!A.block && !joined && tid == 0 && !by_block) A.join[worker].last = -1;
+  if (SHARES && !joined && tid == 0 && !split.by_block) A.join[worker].last = -1;
 }
 
-// A row block's parts joined, 16 rows to a workgroup, in the order of their slots.
-template <int D>
-__global__ __launch_bounds__(256) void tree_join(TreeArgs A, int rows) {
+// Part q's slot of a row block's: a thread's ITEMS times 4 of 16 rows' sums.
+template <int D, class Slot>
+__device__ __forceinline__ void tree_join_rows(const TreeArgs& A, int rows, int n, int r0, Slot slot, int R,
+                                               int row0, int tok0, int head) {
   constexpr int ITEMS = D / 64, AHEAD = 8;   // 16-byte items of a thread
-  const int count = const_load(A.entries);
-  const AttendJoin J = const_load(A.join + blockIdx.x);
-  const int r0 = 16 * blockIdx.y;
-  // (an entry of a call whose lengths change while it runs may not be in range)
-  if ((int)blockIdx.x >= count || J.first < 0 || J.last < J.first || J.last >= TREE_WORKERS ||
-      r0 >= J.rows || J.rows > rows || J.row0 < 0 || (unsigned)J.head >= (unsigned)A.kv.heads ||
-      J.tok0 < 0 || (int64_t)J.row0 + J.rows > (int64_t)(A.kv.T - J.tok0) * A.G)
-    return;
-  const int n = J.last - J.first + 1, l = lane_id(), c = l & 15, g = l >> 4;
+  const int l = lane_id(), c = l & 15, g = l >> 4;
   float top = -INFINITY, L = 0;
   f32x4 o[ITEMS];
 #pragma unroll
@@ -856,8 +889,7 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs A, int rows) {
     f32x4 x[AHEAD][ITEMS];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {        // past the last: the last again, not added
-      const int q = min(p0 + k, n - 1);
-      const int64_t tile = ((int64_t)(2 * (J.first + q) + (q == 0)) * rows + r0) / 16;
+      const int64_t tile = ((int64_t)slot(min(p0 + k, n - 1)) * rows + r0) / 16;
       const float2 ml = *(const float2*)(A.ml + 2 * (tile * 16 + c));
       m[k] = p0 + k < n ? ml.x : -INFINITY;
       s[k] = ml.y;
@@ -881,15 +913,42 @@ __global__ __launch_bounds__(256) void tree_join(TreeArgs A, int rows) {
       for (int i = 0; i < ITEMS; ++i) o[i] += f * x[k][i];
     }
   }
-  if (r0 + c >= J.rows) return;
+  if (r0 + c >= R) return;
   const float f = top == -INFINITY ? 0.f : 1.f / L;
-  const int row = J.row0 + r0 + c;
-  uint16_t* out = A.out + ((int64_t)(J.tok0 + row / A.G) * A.q_heads + J.head * A.G + row % A.G) * D + 4 * g;
+  const int row = row0 + r0 + c;
+  uint16_t* out = A.out + ((int64_t)(tok0 + row / A.G) * A.q_heads + head * A.G + row % A.G) * D + 4 * g;
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
     const int d = 16 * (4 * i + wave_id());
     *(u32x2*)(out + d) = u32x2{pack_bf16(o[i][0] * f, o[i][1] * f), pack_bf16(o[i][2] * f, o[i][3] * f)};
   }
+}
+
+// A row block's parts joined, 16 rows to a workgroup, in the order of their slots: of
+// shares, by its entry, ..
+template <int D>
+__global__ __launch_bounds__(256) void tree_join(TreeArgs A, int rows) {
+  const int count = const_load(A.entries);
+  const AttendJoin J = const_load(A.join + blockIdx.x);
+  const int r0 = 16 * blockIdx.y;
+  // (an entry of a call whose lengths change while it runs may not be in range)
+  if ((int)blockIdx.x >= count || J.first < 0 || J.last < J.first || J.last >= TREE_WORKERS ||
+      r0 >= J.rows || J.rows > rows || J.row0 < 0 || (unsigned)J.head >= (unsigned)A.kv.heads ||
+      J.tok0 < 0 || (int64_t)J.row0 + J.rows > (int64_t)(A.kv.T - J.tok0) * A.G)
+    return;
+  tree_join_rows<D>(A, rows, J.last - J.first + 1, r0, [&](int q) { return 2 * (J.first + q) + (q == 0); },
+                    J.rows, J.row0, J.tok0, J.head);
+}
+// .. or of chunks.
+template <int D, class Line>
+__global__ __launch_bounds__(256) void tree_join_chunks(TreeArgs A) {
+  const AttendSeq s = tree_seq<Line>(A, blockIdx.z);
+  const int n = (s.n + A.chunk - 1) / A.chunk, rows = Line::ROWS, r0 = 16 * blockIdx.y;
+  const int head = (int)(blockIdx.x % (unsigned)A.kv.heads), rb = (int)(blockIdx.x / (unsigned)A.kv.heads);
+  const int row0 = rb * rows, R = min(rows, s.q * A.G - row0);
+  if (n < 2 || r0 >= R) return;
+  const int slot0 = (((int)blockIdx.z * A.kv.heads + head) * A.tiles + rb) * A.chunks;
+  tree_join_rows<D>(A, rows, min(n, A.chunks), r0, [&](int q) { return slot0 + q; }, R, row0, s.tok0, head);
 }
 
 // Rows of a row block: the least of those that hold a sequence's.
@@ -898,38 +957,57 @@ static int tree_rows(int64_t rows, int D) {
   return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
+// Parts that the workspace holds: two a worker, and no fewer of the smaller row blocks.
+static int tree_slots(int rows) { return std::max(2 * TREE_WORKERS, 65536 / rows); }
+
 struct TreeWork {
   size_t off_join, off_ml, off_part, total;
 };
 static TreeWork tree_workspace(int rows, int D) {
   TreeWork x;
+  const size_t slots = tree_slots(rows);
   x.off_join = 256;
   x.off_ml = x.off_join + align_up(TREE_WORKERS * sizeof(AttendJoin), 256);
-  x.off_part = x.off_ml + align_up((size_t)2 * TREE_WORKERS * rows * 8, 256);
-  x.total = x.off_part + (size_t)2 * TREE_WORKERS * rows * D * 4;
+  x.off_part = x.off_ml + align_up(slots * rows * 8, 256);
+  x.total = x.off_part + slots * rows * D * 4;
   return x;
 }
 
 template <int D, int NT, int WR, bool F8>
 static int launch_tree(TreeArgs A, int64_t max_new, hipStream_t s) {
   using Sh = TreeShape<D, NT, WR, F8>;
-  static LdsLimit limit;
-  if (int e = limit.raise((const void*)tree_split<D, NT, WR, F8>, Sh::lds())) return e;
+  constexpr int ROWS = Sh::ROWS;
   const int64_t held = (int64_t)A.kv.M << A.kv.logP;
-  const int64_t span = A.window ? std::min<int64_t>(A.window + max_new, held) : held;
-  const int64_t tiles = (A.G * max_new + Sh::ROWS - 1) / Sh::ROWS;
-  const uint32_t lds = Sh::off_seqs() + Sh::Seqs::bytes(A.kv.B, A.kv.q_start != nullptr);
-  A.block = span <= TREE_BLOCK_STEPS * TREE_UNIT * Sh::WT;
-  if (A.block) {
-    timed_launch(CX_KERNEL_TREE, tree_split<D, NT, WR, F8>, dim3((unsigned)(A.kv.heads * tiles), A.kv.B),
-                 dim3(TREE_WG), lds, s, A);
+  const int64_t span = A.window ? std::min<int64_t>(A.window + max_new + TREE_UNIT, held) : held;
+  const int64_t units = (span + TREE_UNIT - 1) / TREE_UNIT;
+  const int64_t tiles = (A.G * max_new + ROWS - 1) / ROWS, blocks = A.kv.B * A.kv.heads * tiles;
+  // Chunks where the longest context is short for the workgroups there are ..
+  const int64_t most = tree_slots(ROWS) / blocks;               // parts of a row block at most
+  int64_t chunks = std::max<int64_t>(std::min({TREE_SPREAD / blocks, most, (units + Sh::WT - 1) / Sh::WT}), 1);
+  const int64_t chunk = (units + chunks - 1) / chunks;
+  if (chunk <= TREE_CHUNK) {
+    chunks = (units + chunk - 1) / chunk;
+    A.tiles = (int)tiles;
+    A.chunks = (int)chunks;
+    A.chunk = (int)chunk;
+    static LdsLimit limit;
+    if (int e = limit.raise((const void*)tree_split<D, NT, WR, F8, false>, Sh::lds())) return e;
+    timed_launch(CX_KERNEL_TREE, tree_split<D, NT, WR, F8, false>,
+                 dim3((unsigned)(A.kv.heads * tiles * chunks), A.kv.B), dim3(TREE_WG),
+                 (uint32_t)Sh::off_seqs(), s, A);
+    if (chunks > 1)
+      timed_launch(CX_KERNEL_TREE_JOIN, tree_join_chunks<D, typename Sh::Line>,
+                   dim3((unsigned)(A.kv.heads * tiles), ROWS / 16, A.kv.B), dim3(256), 0, s, A);
     return (int)hipGetLastError();
   }
-  timed_launch(CX_KERNEL_TREE, tree_split<D, NT, WR, F8>, dim3(TREE_WORKERS), dim3(TREE_WG), lds, s, A);
+  // .. else shares
+  static LdsLimit limit;
+  if (int e = limit.raise((const void*)tree_split<D, NT, WR, F8, true>, Sh::lds())) return e;
+  timed_launch(CX_KERNEL_TREE, tree_split<D, NT, WR, F8, true>, dim3(TREE_WORKERS), dim3(TREE_WG),
+               (uint32_t)(Sh::off_seqs() + Sh::Seqs::bytes(A.kv.B, A.kv.q_start != nullptr)), s, A);
   const int64_t entries =
-      std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / Sh::ROWS + A.kv.B), TREE_WORKERS);
-  timed_launch(CX_KERNEL_TREE_JOIN, tree_join<D>, dim3((unsigned)entries, Sh::ROWS / 16), dim3(256), 0, s, A,
-               Sh::ROWS);
+      std::min<int64_t>(A.kv.heads * ((int64_t)A.kv.T * A.G / ROWS + A.kv.B), TREE_WORKERS);
+  timed_launch(CX_KERNEL_TREE_JOIN, tree_join<D>, dim3((unsigned)entries, ROWS / 16), dim3(256), 0, s, A, ROWS);
   return (int)hipGetLastError();
 }
 template <int D, bool F8>
