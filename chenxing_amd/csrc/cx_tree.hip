@@ -267,10 +267,10 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     }
     end = share_begin(split, worker) + split.per + (worker < split.more);
   } else {
-    own = tree_seq<Line>(A, blockIdx.y);
+    own = tree_seq<Line>(A, blockIdx.z);
     blocks = Line::row_blocks(share_batch(), own);
     if (own.n == 0) {
-      if (blockIdx.x == 0) nothing(own.tok0, own.tok0 + own.q);
+      if (blockIdx.x == 0 && blockIdx.y == 0) nothing(own.tok0, own.tok0 + own.q);
       return;
     }
   }
@@ -285,9 +285,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
   int step = 0, steps = 0;                   // of the piece that is loaded
   uint64_t u = 0;                            // SHARES: past it
   int b = 0;
-  // else the kv head, the row block and the part of its units
-  const int head = (int)(blockIdx.x % (unsigned)C.heads);
-  int rb = (int)(blockIdx.x / (unsigned)C.heads), chunk = 0;
+  int rb = blockIdx.y, chunk = 0;            // else the row block and the part of its units
   if constexpr (SHARES) {
     u = share_begin(split, worker);
     for (int hi = C.B - 1; b < hi;) {        // the last b with its units at or before u
@@ -296,8 +294,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       else hi = mid - 1;
     }
   } else {
-    chunk = rb / A.tiles;
-    rb %= A.tiles;
+    for (; rb >= A.tiles; rb -= A.tiles) ++chunk;               // (a few)
     if (rb >= blocks || chunk * A.chunk >= own.n) return;
   }
   bool joined = false;
@@ -323,8 +320,8 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       // first chunk's workgroups take whole row blocks
       const bool whole = rb >= A.tiles;
       if (rb >= blocks || (whole && chunk > 0)) return false;
-      p.b = blockIdx.y;
-      p.h = head;
+      p.b = blockIdx.z;
+      p.h = blockIdx.x;
       p.tok0 = own.tok0;
       p.r0 = rb * ROWS;
       p.R = min(ROWS, own.q * A.G - p.r0);
@@ -335,7 +332,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       p.cnt = whole ? own.n : own.n - chunk * A.chunk;
       if (!whole && chunk + 1 < A.chunks) p.cnt = min(p.cnt, A.chunk);
       p.slot = p.cnt == own.n ? -1
-                              : ((int)blockIdx.y * A.kv.heads + head) * A.tiles * A.chunks + rb * A.chunks + chunk;
+                              : (p.b * A.kv.heads + p.h) * A.tiles * A.chunks + rb * A.chunks + chunk;
       rb += A.tiles;
     }
     ahead.ids = A.kv.table + __builtin_amdgcn_readfirstlane(p.b) * A.kv.ld_table;
@@ -951,7 +948,7 @@ __global__ __launch_bounds__(256) void tree_join_chunks(TreeArgs A) {
   tree_join_rows<D>(A, rows, min(n, A.chunks), r0, [&](int q) { return slot0 + q; }, R, row0, s.tok0, head);
 }
 
-// Rows of a row block: the least of those that hold a sequence's.
+// Rows of a row block: the least of those that hold a sequence's on average.
 static int tree_rows(int64_t rows, int D) {
   if (D == 256) return rows <= 64 ? 64 : 128;
   return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
@@ -993,7 +990,7 @@ static int launch_tree(TreeArgs A, int64_t max_new, hipStream_t s) {
     static LdsLimit limit;
     if (int e = limit.raise((const void*)tree_split<D, NT, WR, F8, false>, Sh::lds())) return e;
     timed_launch(CX_KERNEL_TREE, tree_split<D, NT, WR, F8, false>,
-                 dim3((unsigned)(A.kv.heads * tiles * chunks), A.kv.B), dim3(TREE_WG),
+                 dim3(A.kv.heads, (unsigned)(tiles * chunks), A.kv.B), dim3(TREE_WG),
                  (uint32_t)Sh::off_seqs(), s, A);
     if (chunks > 1)
       timed_launch(CX_KERNEL_TREE_JOIN, tree_join_chunks<D, typename Sh::Line>,
@@ -1030,7 +1027,12 @@ extern "C" {
 size_t cx_tree_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                          int32_t max_new) {
   if (q_heads < 1 || kv_heads < 1 || head_dim < 1 || max_new < 1) return 256;
-  return cx::tree_workspace(cx::tree_rows((int64_t)(q_heads / kv_heads) * max_new, head_dim), head_dim).total;
+  // the most of any call of as many rows or fewer
+  const int64_t rows = (int64_t)(q_heads / kv_heads) * max_new;
+  size_t most = 0;
+  for (int64_t r : {32, 64, 128, 256})
+    most = std::max(most, cx::tree_workspace(cx::tree_rows(std::min(r, rows), head_dim), head_dim).total);
+  return most;
 }
 
 int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_token,
@@ -1059,7 +1061,9 @@ int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_t
   A.q_heads = q_heads;
   A.G = q_heads / kv->kv_heads;
   max_new = std::min(max_new, kv->T);        // no sequence has more
-  const int D = kv->head_dim, rows = cx::tree_rows((int64_t)A.G * max_new, D);
+  const int D = kv->head_dim;
+  const int64_t each = std::min<int64_t>(max_new, (kv->T + kv->B - 1) / kv->B);
+  const int rows = cx::tree_rows(A.G * each, D);
   const cx::TreeWork lay = cx::tree_workspace(rows, D);
   if (ws_bytes < lay.total)
     return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, lay.total);
