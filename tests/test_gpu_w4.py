@@ -144,3 +144,47 @@ def test_no_rows():
     _, codes, scale, sh = _inputs(1, 20, 64, 32, False)
     w = w4.W4Weight(*(None if t is None else torch.from_numpy(t).cuda() for t in (codes, scale, sh)))
     assert w(torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")).shape == (0, 20)
+
+
+@pytest.mark.parametrize("M", [1, 16, 20, 32, 61, 64])
+@pytest.mark.parametrize("N", [130, 6160, 12300, 24580, 49170])
+@pytest.mark.parametrize("K,group", [(64, 32), (64, 64), (128, 128), (1056, 32), (1216, 64)])
+def test_every_split(M, N, K, group):
+    """Rows of W a wave and waves of a row go by N; K ends in and on a tile of 128."""
+    import torch
+    from chenxing_amd import w4
+    from chenxing_amd._lib import w4_linear_device
+    if K > 128 and N > 20000:
+        K -= 1024 - 128
+    shift = (M + N // 10) % 2 == 0
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    codes = torch.randint(0, 16, (N, K), generator=g, device="cuda", dtype=torch.uint8)
+    scale = ((torch.rand(N, K // group, generator=g, device="cuda") + 0.5) / 16).half()
+    sh = (-7.3 * scale).half() if shift else None
+    x = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    got = w4_linear_device(x, *w4.pack(codes, scale, sh), N, torch.float32)
+    # codes and halves are exact in float64, and R.linear's bound holds for each n: checked
+    # on the rows of W where tiles, waves and workgroups begin and end, all against float64
+    w = codes.double() * scale.double().repeat_interleave(group, 1)
+    w += (sh.double() if shift else -8 * scale.double()).repeat_interleave(group, 1)
+    off = (got.double() - x.double() @ w.T).abs()
+    rows = sorted({r for b in range(0, N, 16 * 64) for r in (b, b + 15, b + 16, b + 31) if r < N} | {N - 1})
+    _, tol = R.linear(x.double().cpu().numpy(), codes[rows].cpu().numpy(), scale[rows].cpu().numpy(),
+                      sh[rows].cpu().numpy() if shift else None, False)
+    assert (off[:, rows].cpu().numpy() <= tol).all()
+    # the others by the largest of their bounds
+    assert (off <= 2 * float(tol.max())).all(), float(off.max())
+
+
+@pytest.mark.parametrize("M", [2, 16])
+def test_rows_far_apart(M):
+    """Rows of x whose distances pass 32 bits."""
+    import torch
+    from chenxing_amd import w4
+    x, codes, scale, sh = _inputs(M, 70, 192, 64, True, 8)
+    w = w4.W4Weight(*(torch.from_numpy(t).cuda() for t in (codes, scale, sh)))
+    for step in (1 << 26, (1 << 28) + 8):
+        wide = torch.empty((M - 1) * step + 192, dtype=torch.bfloat16, device="cuda")
+        rows = wide.as_strided((M, 192), (step, 1))
+        rows.copy_(C.to_gpu(x))
+        _check(x, codes, scale, sh, w(rows), False)
