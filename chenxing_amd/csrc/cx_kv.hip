@@ -496,57 +496,95 @@ __global__ __launch_bounds__(256) void copy_pages(CopyArgs A) {
 struct CommitArgs {
   KvArgs kv;
   int64_t layer_stride;
-  int n_layers, width;
+  int n_layers, width, heads; // heads of a workgroup
   const int32_t* path;        // [B, width]
   const int32_t* count;       // nullable [B]
 };
+constexpr int COMMIT_PASS = 32;              // moves looked up at a time
+constexpr int COMMIT_AHEAD = 8;              // and read before any of them is written
+constexpr int COMMIT_GROUPS = 2048;
 
-// Workgroup (sequence, layer, head): a thread a 16-byte chunk of the keys, a dim of the
-// values, or the scales, each token after the other: a path rises, so what a move
-// overwrites has been read.
+// Workgroup (sequence, layer, a few heads): a thread a 16-byte chunk of the keys, a dim of
+// the values, or a scale.  Values of a token are 16 bytes apart, so that a move touches
+// 16 / E times the lines that hold its bytes.
 template <int D, bool F8>
 __global__ __launch_bounds__(256) void commit_tokens(CommitArgs A) {
-  constexpr int E = F8 ? 16 : 8, KC = D / E;
+  constexpr int E = F8 ? 16 : 8, KC = D / E, ITEMS = KC + D + (F8 ? 2 : 0);
+  __shared__ int64_t s_from[COMMIT_PASS], s_to[COMMIT_PASS];             // pages, in bytes
+  __shared__ int s_slot[COMMIT_PASS], s_moves[2];                        // slots: from << 16 | to
   const KvArgs& C = A.kv;
-  const unsigned x = blockIdx.x / (unsigned)C.heads, h = blockIdx.x % (unsigned)C.heads;
+  const unsigned parts = (C.heads + A.heads - 1) / A.heads, x = blockIdx.x / parts;
+  const int h0 = (int)(blockIdx.x % parts) * A.heads, nh = min(A.heads, C.heads - h0);
   const int b = (int)(x / (unsigned)A.n_layers);
   const int2 rows = kv_rows(C, b);
   const int n = rows.y - rows.x, P = 1 << C.logP;
   const int64_t s0 = (int64_t)C.kv_len[b] - n;
   if (s0 < 0) return;
-  char* base = C.pages + (x % (unsigned)A.n_layers) * A.layer_stride + (int64_t)h * C.head_bytes;
+  char* const base = C.pages + (x % (unsigned)A.n_layers) * A.layer_stride + (int64_t)h0 * C.head_bytes;
   const int32_t* path = A.path + (int64_t)b * A.width;
   const int m = A.count ? min(A.count[b], A.width) : A.width;
-  auto place = [&](int64_t slot, int* o) {
-    *o = (int)(slot & (P - 1));
-    const int64_t at = slot >> C.logP;
-    const int id = at < C.M ? C.table[b * C.ld_table + at] : -1;
-    return (unsigned)id < (unsigned)C.n_pages ? base + id * C.page_stride : nullptr;
-  };
-  for (int i = threadIdx.x; i < KC + D + (F8 ? 2 : 0); i += 256) {
-    for (int j = 0, last = -1; j < m; ++j) {
-      const int p = path[j];
-      if (p <= last || p >= n) break;
-      last = p;
-      if (p == j) continue;
-      int so, to;
-      const char* from = place(s0 + p, &so);
-      char* dst = place(s0 + j, &to);
-      if (!from || !dst) continue;
-      if (i < KC) {
-        *(u32x4*)(dst + k_chunk<E>(i * E, to, C.logP)) = *(const u32x4*)(from + k_chunk<E>(i * E, so, C.logP));
-      } else if (i < KC + D) {
-        const int d = i - KC;
-        const char* f = from + v_chunk<E, D>(d, so, C.logP) + so % E * (16 / E);
-        char* t = dst + v_chunk<E, D>(d, to, C.logP) + to % E * (16 / E);
-        if (F8) *(uint8_t*)t = *(const uint8_t*)f;
-        else *(uint16_t*)t = *(const uint16_t*)f;
-      } else if (i == KC + D) {
-        *(uint32_t*)(dst + k_scale<D>(to, C.logP)) = *(const uint32_t*)(from + k_scale<D>(so, C.logP));
-      } else {
-        *(uint32_t*)(dst + v_scale<D>(to, C.logP)) = *(const uint32_t*)(from + v_scale<D>(so, C.logP));
+  for (int j0 = 0; j0 < m; j0 += COMMIT_PASS) {
+    // the pass's moves: the first wave looks them up, side by side
+    if (wave_id() == 0) {
+      const int j = j0 + lane_id();
+      const int p = lane_id() < COMMIT_PASS && j < m ? path[j] : -1;
+      const int before = j > 0 && p >= 0 ? path[j - 1] : -1;
+      const uint64_t ends = ballot(p <= before || p >= n);
+      const int end = ends ? __builtin_ctzll(ends) : 64;                 // COMMIT_PASS at most
+      int64_t page[2] = {-1, -1};
+      if (lane_id() < end && p != j) {
+        const int64_t slots[2] = {s0 + p, s0 + j};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int64_t at = slots[k] >> C.logP;
+          if (at < C.M) page[k] = C.table[b * C.ld_table + at];
+        }
+      }
+      const bool moves = page[0] >= 0 && page[0] < C.n_pages && page[1] >= 0 && page[1] < C.n_pages;
+      const uint64_t all = ballot(moves);
+      if (moves) {
+        const int at = __builtin_popcountll(all & ((1ull << lane_id()) - 1));
+        s_from[at] = page[0] * C.page_stride;
+        s_to[at] = page[1] * C.page_stride;
+        s_slot[at] = (int)((s0 + p) & (P - 1)) << 16 | (int)((s0 + j) & (P - 1));
+      }
+      if (lane_id() == 0) {
+        s_moves[0] = __builtin_popcountll(all);
+        s_moves[1] = end;
       }
     }
+    __syncthreads();
+    const int moves = s_moves[0], end = s_moves[1];
+    // An element is one thread's for all moves, so that it may read COMMIT_AHEAD of them
+    // before it writes: a path rises, and what is moved to is behind all that is yet to move.
+    for (int i = threadIdx.x; i < nh * ITEMS; i += 256) {
+      char* const head = base + i / ITEMS * C.head_bytes;
+      const int e = i % ITEMS;
+      for (int v0 = 0; v0 < moves; v0 += COMMIT_AHEAD) {
+        auto move = [&](auto zero, auto where) {
+          using T = decltype(zero);
+          T t[COMMIT_AHEAD];
+#pragma unroll
+          for (int u = 0; u < COMMIT_AHEAD; ++u)
+            if (v0 + u < moves) t[u] = *(const T*)(head + s_from[v0 + u] + where(s_slot[v0 + u] >> 16));
+#pragma unroll
+          for (int u = 0; u < COMMIT_AHEAD; ++u)
+            if (v0 + u < moves) *(T*)(head + s_to[v0 + u] + where(s_slot[v0 + u] & 0xFFFF)) = t[u];
+        };
+        if (e < KC) {
+          move(u32x4{}, [&](int slot) { return k_chunk<E>(e * E, slot, C.logP); });
+        } else if (e < KC + D) {
+          using V = typename std::conditional<F8, uint8_t, uint16_t>::type;
+          move(V{}, [&](int slot) { return v_chunk<E, D>(e - KC, slot, C.logP) + slot % E * (16 / E); });
+        } else {
+          move(uint32_t{}, [&](int slot) {
+            return e == KC + D ? k_scale<D>(slot, C.logP) : v_scale<D>(slot, C.logP);
+          });
+        }
+      }
+    }
+    if (end < COMMIT_PASS) break;
+    __syncthreads();
   }
 }
 
@@ -679,6 +717,10 @@ int cx_kv_commit(const cx_kv_batch* kv, int64_t layer_stride, int32_t n_layers,
   A.layer_stride = layer_stride;
   A.n_layers = n_layers;
   A.width = width;
+  // heads together while the chip has workgroups enough
+  A.heads = 1;
+  while (A.heads < kv->kv_heads && (int64_t)kv->B * n_layers * kv->kv_heads >= 2ll * A.heads * cx::COMMIT_GROUPS)
+    A.heads *= 2;
   A.path = path;
   A.count = count;
   using Kernel = void (*)(cx::CommitArgs);
@@ -686,8 +728,8 @@ int cx_kv_commit(const cx_kv_batch* kv, int64_t layer_stride, int32_t n_layers,
   const Kernel k = kv->head_dim == 64    ? (f8 ? (Kernel)cx::commit_tokens<64, true> : cx::commit_tokens<64, false>)
                    : kv->head_dim == 128 ? (f8 ? (Kernel)cx::commit_tokens<128, true> : cx::commit_tokens<128, false>)
                                          : (f8 ? (Kernel)cx::commit_tokens<256, true> : cx::commit_tokens<256, false>);
-  cx::timed_launch(CX_KERNEL_KV_COMMIT, k, dim3((unsigned)(kv->B * n_layers * kv->kv_heads)), dim3(256),
-                   0, (hipStream_t)stream, A);
+  cx::timed_launch(CX_KERNEL_KV_COMMIT, k, dim3((unsigned)(kv->B * n_layers * ((kv->kv_heads + A.heads - 1) / A.heads))),
+                   dim3(256), 0, (hipStream_t)stream, A);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return cx::api_fail(CX_EHIP, "commit launch: %s", hipGetErrorString(e));
   return CX_OK;
