@@ -698,7 +698,7 @@ def tree_masks_device(parents, q_start=None, words=1):
     lib = _lib or load()
     dev, T, B, start = _tree_rows(torch, parents, q_start)
     mask = torch.empty(T, words, dtype=torch.int64, device=parents.device)
-    depth = torch.empty(T, dtype=torch.int32, device=parents.device)
+    depth = torch.empty_like(parents)
     _call(torch, dev, lib.cx_tree_masks, parents.data_ptr(), start, B, T, mask.data_ptr(), words,
           depth.data_ptr())
     return mask, depth
@@ -719,7 +719,8 @@ def tree_accept_device(parents, tokens, sampled, width, q_start=None):
     tok = _i32_rows(torch, "tokens", tokens, dev, (T,))
     ids = _i32_rows(torch, "sampled", sampled, dev, (T,))
     path = torch.empty(B, width, dtype=torch.int32, device=parents.device)
-    count, nxt = torch.empty(2, B, dtype=torch.int32, device=parents.device)
+    count = torch.empty(B, dtype=torch.int32, device=parents.device)
+    nxt = torch.empty_like(count)
     _call(torch, dev, lib.cx_tree_accept, parents.data_ptr(), tok, ids, start, B, T, width,
           path.data_ptr(), count.data_ptr(), nxt.data_ptr())
     return path, count, nxt
@@ -747,7 +748,7 @@ def kv_commit_device(cache, head_dim, table, kv_len, path, count=None, q_start=N
         layers, stride = shape[0], cache.stride(0) * cache.element_size()
         if layers == 0:
             return cache
-        layer = cache[0]
+        layer = cache.select(0, 0)
     B = table.shape[0]
     if q_start is None:
         T = B

@@ -93,6 +93,7 @@ __global__ __launch_bounds__(64) void tree_accept(WalkArgs A) {
     int next = -1;
 #pragma unroll
     for (int c = 0; c < WALK_KEPT; ++c) {
+      if (64 * c >= n) break;
       const uint64_t m = ballot(par[c] == cur && tok[c] == want && 64 * c + l > cur);
       if (next < 0 && m) next = 64 * c + __builtin_ctzll(m);
     }
