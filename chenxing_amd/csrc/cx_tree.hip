@@ -161,7 +161,7 @@ struct TreeShape {
   // stages of the ring
   static constexpr int S = WR == 8 ? (D == 256 ? 4 : 8)
                            : D == 64 ? 4
-                           : F8      ? 3
+                           : F8      ? (D == 256 && WR == 2 ? 2 : 3)
                                      : (D == 128 && WR == 4 ? 3 : 2);
   // bytes of a group: the ring, e4m3 its scales (256 bytes, kept a step longer), CONV
   // two units in bf16
@@ -949,8 +949,8 @@ __global__ __launch_bounds__(256) void tree_join_chunks(TreeArgs A) {
 }
 
 // Rows of a row block: the least of those that hold a sequence's on average.
-static int tree_rows(int64_t rows, int D) {
-  if (D == 256) return rows <= 64 ? 64 : 128;
+static int tree_rows(int64_t rows, int D, bool f8) {
+  if (D == 256) return rows <= 32 && f8 ? 32 : rows <= 64 ? 64 : 128;  // (32 of bf16: the ring passes LDS)
   return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
 }
 
@@ -1010,6 +1010,7 @@ static int launch_tree(TreeArgs A, int64_t max_new, hipStream_t s) {
 template <int D, bool F8>
 static int launch_tree(const TreeArgs& A, int rows, int64_t max_new, hipStream_t s) {
   if constexpr (D == 256) {
+    if constexpr (F8) if (rows == 32) return launch_tree<D, 1, 2, F8>(A, max_new, s);
     if (rows == 64) return launch_tree<D, 1, 4, F8>(A, max_new, s);
     return launch_tree<D, 1, 8, F8>(A, max_new, s);
   } else {
@@ -1031,7 +1032,8 @@ size_t cx_tree_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int3
   const int64_t rows = (int64_t)(q_heads / kv_heads) * max_new;
   size_t most = 0;
   for (int64_t r : {32, 64, 128, 256})
-    most = std::max(most, cx::tree_workspace(cx::tree_rows(std::min(r, rows), head_dim), head_dim).total);
+    for (bool f8 : {false, true})
+      most = std::max(most, cx::tree_workspace(cx::tree_rows(std::min(r, rows), head_dim, f8), head_dim).total);
   return most;
 }
 
@@ -1063,7 +1065,8 @@ int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_t
   max_new = std::min(max_new, kv->T);        // no sequence has more
   const int D = kv->head_dim;
   const int64_t each = std::min<int64_t>(max_new, (kv->T + kv->B - 1) / kv->B);
-  const int rows = cx::tree_rows(A.G * each, D);
+  const bool f8 = kv->dtype == CX_KV_E4M3;
+  const int rows = cx::tree_rows(A.G * each, D, f8);
   const cx::TreeWork lay = cx::tree_workspace(rows, D);
   if (ws_bytes < lay.total)
     return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, lay.total);
@@ -1088,7 +1091,6 @@ int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_t
   A.join = (cx::AttendJoin*)((char*)workspace + lay.off_join);
   A.ml = (float*)((char*)workspace + lay.off_ml);
   A.part = (float*)((char*)workspace + lay.off_part);
-  const bool f8 = kv->dtype == CX_KV_E4M3;
   const hipStream_t s = (hipStream_t)stream;
   // one launch after the other where a call has more sequences than a launch takes
   for (int b0 = 0; b0 < kv->B; b0 += cx::TREE_BATCH) {
