@@ -49,6 +49,19 @@ ATTEND = {
                     "tree"),
 }
 
+EDGES = {
+    "wide_few_e4m3": ("e4m3", 4, 2, 256, 32, [5, 700, 1300, 90], [5, 9, 13, 1], 1, 0, 0.0, "tree"),
+    "wide_few_window": ("e4m3", 4, 2, 256, 32, [5, 700, 1300, 90], [5, 9, 13, 1], 1, 333, 50.0, "tree"),
+    "wide_one_e4m3": ("e4m3", 3, 3, 256, 16, [1, 17, 33, 520], [1, 1, 1, 1], 1, 0, 0.0, "tree"),
+    # more rows than a row block of their average holds
+    "wide_ragged_e4m3": ("e4m3", 4, 2, 256, 16, [60, 700, 30, 90, 40], [60, 3, 2, 1, 1], 1, 0, 0.0, "tree"),
+    "wide_bits_e4m3": ("e4m3", 2, 2, 256, 16, [33, 64, 300], [9, 30, 17], 1, 0, 0.0, "sparse"),
+    # more than a launch's sequences
+    "many": ("bf16", 2, 1, 64, 16, [i % 41 for i in range(1030)], [min(i % 3, i % 41) for i in range(1030)],
+             1, 0, 0.0, "tree"),
+    "far": ("e4m3", 4, 2, 128, 256, [300, 700, 20], [9, 40, 20], 1, 0, 0.0, "tree"),
+}
+
 
 def parents(rng, n, kind="tree"):
     if kind == "chain":
@@ -74,7 +87,7 @@ def trees(rng, new, words, kind):
 
 
 def attend_inputs(name, seed=0):
-    cache, Hq, Hkv, D, P, lens, new, words, window, cap, kind = ATTEND[name]
+    cache, Hq, Hkv, D, P, lens, new, words, window, cap, kind = EDGES.get(name) or ATTEND[name]
     rng = np.random.default_rng(len(name) * 1013 + sum(map(ord, name)) + seed)
     table, kv_len, q_start, n = C.batch(rng, lens, new, P)
     K, V, ks, vs = C.dense_pages(rng, n, Hkv, P, D, cache)
