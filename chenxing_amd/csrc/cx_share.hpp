@@ -129,8 +129,10 @@ template <int TOK, int NT, bool TREE = false>
 struct AttendLine {
   static constexpr int ROWS = 16 * NT;
   // what a row block costs beside its units, in units (64 ragged requests 99, 94
-  // and 93 us with 0, 1 and 2; 32 verify rounds 48, 42, 39 and 35 us with 0 .. 3)
-  static constexpr int PIECE = NT == 1 ? 2 : 4;
+  // and 93 us with 0, 1 and 2; 32 verify rounds 48, 42, 39 and 35 us with 0 .. 3).  Trees,
+  // whose workgroups take a unit or more a step: 32 ragged ones 84, 64, 55, 54 and 58 us
+  // with 2, 4, 6, 9 and 14, 64 full ones in row blocks of 256 484, 456, 439, 443 and 459
+  static constexpr int PIECE = TREE ? (NT < 16 ? 9 : 6) : NT == 1 ? 2 : 4;
 
   // The sequence of new tokens tok0 .. end - 1 and len tokens in all.
   static __device__ __forceinline__ AttendSeq seq(const ShareBatch& A, int tok0, int end, int len) {

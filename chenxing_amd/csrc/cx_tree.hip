@@ -1071,7 +1071,7 @@ int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_t
   if (ws_bytes < lay.total)
     return cx::api_fail(CX_ENOSPACE, "workspace holds %zu bytes, needs %zu", ws_bytes, lay.total);
   // the units and row blocks, at most, fit the share arithmetic's 38 bits
-  const double units = (double)kv->max_pages * kv->page_tokens / 32 + 8;
+  const double units = (double)kv->max_pages * kv->page_tokens / 32 + 16;
   const double blocks = kv->kv_heads * ((double)kv->T * A.G / 16 + kv->B);
   if (units * blocks >= 0x1p38) return cx::api_fail(CX_EINVAL, "too many tokens for one call");
   A.mask = (const uint32_t*)mask;
