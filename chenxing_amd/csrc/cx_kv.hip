@@ -502,11 +502,13 @@ struct CommitArgs {
 };
 constexpr int COMMIT_PASS = 32;              // moves looked up at a time
 constexpr int COMMIT_AHEAD = 8;              // and read before any of them is written
-constexpr int COMMIT_GROUPS = 2048;
+constexpr int COMMIT_GROUPS = 2048;          // workgroups that a call should have
 
 // Workgroup (sequence, layer, a few heads): a thread a 16-byte chunk of the keys, a dim of
-// the values, or a scale.  Values of a token are 16 bytes apart, so that a move touches
-// 16 / E times the lines that hold its bytes.
+// the values, or a scale.  A token's values are 16 bytes apart and its chunks of keys 16 P:
+// bound by the lines that hold them (48 sequences of 32 layers and 8 heads, e4m3: 23 MB of
+// tokens, 118 MB of lines, 31 us; reads and writes in turn 36, a head a workgroup 36; one
+// sequence 3.9 us).
 template <int D, bool F8>
 __global__ __launch_bounds__(256) void commit_tokens(CommitArgs A) {
   constexpr int E = F8 ? 16 : 8, KC = D / E, ITEMS = KC + D + (F8 ? 2 : 0);

@@ -13,7 +13,15 @@
 //   2. tree_join   a workgroup per split row block and 16 rows: its parts, in the
 //                  order of their slots.
 //
-// or, for short tables, tree_split alone with a workgroup a row block.
+// or, for short tables, a workgroup for a chunk of a row block's units, and the join of
+// those that have more than one.
+//
+// K and V are read once for up to 256 rows, so trees of 64 nodes are bound by the matrix
+// cores (with the terms in two parts half as much again as the formula's products) and by
+// the softmax beside them: 2 sequences of 120001 .. 131072 tokens, 32 / 8 heads of 128,
+// bf16, 446 us, 585 TFLOP/s of the formula's; 64 of up to 8192, e4m3, 441 us.  Few rows are
+// bound by the start, a step's latency (1.2 us at D = 128) and a row block's own cost (about
+// 5 us: its rows, the groups' meeting, its part): 32 ragged trees of up to 33 nodes 54 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -34,11 +42,15 @@ constexpr int TREE_WAVES = 8, TREE_WG = 64 * TREE_WAVES;
 constexpr int TREE_WORKERS = 256;            // a workgroup a CU
 constexpr int TREE_UNIT = 32;                // slots of a unit
 constexpr int TREE_LEAST = 2;                // the least share, in units
-constexpr int TREE_CHUNK = 24;               // units of a workgroup's chunk at most
+// Units of a workgroup's chunk at most: one request of 716 tokens 13.5 us in chunks, 17.2
+// in shares; 19 requests in a window of 1024 33 us in shares, 38 and 49 in chunks of 12
+// and 17 units.
+constexpr int TREE_CHUNK = 24;
 constexpr int64_t TREE_SPREAD = 512;         // workgroups of chunks that are aimed at
 constexpr int TREE_BATCH = 512;              // sequences of a launch: their lengths are in LDS
 // A lane's terms of a unit sum to this before the running maximum is raised: it need not
-// be the largest score, so most units look for none.
+// be the largest score, so most units look for none (64 trees of 64 nodes 440 us, with the
+// maximum looked for in every unit 551).
 constexpr float TREE_SLACK = 4096.f;
 constexpr float TREE_LOW = -3e38f;           // running maximum of a row that attends to something
 
@@ -151,7 +163,8 @@ template <int D, int NT, int WR, bool F8>
 struct TreeShape {
   static constexpr int WT = TREE_WAVES / WR, ROWS = 16 * NT * WR;
   // e4m3: many waves share a unit, so its codes are made bf16 once (CONV), else by
-  // each wave as it reads them
+  // each wave as it reads them (64 trees of 64 nodes 440 and 448 us; four waves' two units
+  // of D = 256 in bf16 do not fit beside the ring)
   static constexpr bool CONV = F8 && WR >= 4 && !(D == 256 && WR == 4);
   static constexpr int KB = (F8 ? 1 : 2) * TREE_UNIT * D;       // bytes of a unit's K
   static constexpr int RAW = 2 * KB;
@@ -948,7 +961,9 @@ __global__ __launch_bounds__(256) void tree_join_chunks(TreeArgs A) {
   tree_join_rows<D>(A, rows, min(n, A.chunks), r0, [&](int q) { return slot0 + q; }, R, row0, s.tok0, head);
 }
 
-// Rows of a row block: the least of those that hold a sequence's on average.
+// Rows of a row block: the least of those that hold a sequence's on average (32 ragged
+// trees of 14 nodes, 4 heads a kv head: 64 us with 64 rows, 70 with 128; D = 256, e4m3, 2
+// heads a kv head, 13 nodes: 34.0 us with 32, 38.3 with 64).
 static int tree_rows(int64_t rows, int D, bool f8) {
   if (D == 256) return rows <= 32 && f8 ? 32 : rows <= 64 ? 64 : 128;  // (32 of bf16: the ring passes LDS)
   return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;

@@ -41,7 +41,7 @@ struct W4Args {
 constexpr int W4_AHEAD = 2;
 // The waves that a product should have, of the chip's 8192: two of a SIMD keep enough loads
 // in flight, and each further one has less work for its x and its sums.  16 rows, K = 4096,
-// with 2004 waves, half, twice as many: N = 128256 60, 138, 70 us; N = 14336 with 1792, half,
+// with 2004 and twice as many waves: N = 128256 60 and 70 us; N = 14336 with 1792, half,
 // a quarter: 11.4, 16.4, 26.0 us.
 constexpr int W4_WAVES = 1536;
 // Rows of x so far apart that 16 of them pass 32 bits take the other kernel.
@@ -188,10 +188,9 @@ __device__ __forceinline__ void w4_out(const W4Args& A, const f32x4 (&acc)[MT][N
 // WK waves of the same rows add up through LDS.  All loads go straight to registers,
 // codes and scales two tiles ahead, x (from the caches: a few rows) one.  Every wave
 // reads all of x's part: at 16 rows that is as much as 64 rows of W, so that NTW = 4
-// takes 60 us where 2 and 1 take 81 and 138 (N = 128256, K = 4096, groups of 32 with
-// shifts: 296 MB, 4.6 TB/s); the loads of the group's scales, which hold 64 bytes each, are
-// what is left above the 43 us of its bytes.  One row, N = K = 4096: 5.0 us, of which about 3
-// are a launch's.
+// takes 65 us where 2 and 1 take 81 and 138 (N = 128256, K = 4096, groups of 32 with
+// shifts: 337 MB, 5.2 TB/s, where reads reach 6.9); a lane's loads of the scales bring 4 bytes
+// each.  One row, N = K = 4096: 4.8 us, of which about 3 are a launch's.
 template <int NTW, int STEPS, bool SHIFT>
 __global__ __launch_bounds__(512) void w4_stream(W4Args A) {
   constexpr int GROUPS = 4 / STEPS;          // of a tile
