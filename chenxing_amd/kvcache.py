@@ -163,7 +163,8 @@ class PagedKVCache:
     def commit(self, seqs, batch, path, count) -> list[int]:
         """A round of drafted trees ends: of the last tokens of seqs[i], those that
         ``batch`` appended, path[i, :count[i]] stay, in that order (``path`` and
-        ``count`` as ``_lib.tree_accept_device`` gives them); how many of each."""
+        ``count`` as ``_lib.tree_accept_device`` gives them); how many of each.  A
+        sequence that was forked after the append is refused."""
         from . import _lib
         start = batch["q_start"]
         new = [1] * len(seqs) if start is None else start.diff().tolist()
@@ -172,6 +173,13 @@ class PagedKVCache:
             raise ValueError("commit takes each sequence of the batch once")
         if any(not 0 <= c <= n <= self._seqs[s][1] for s, c, n in zip(seqs, kept, new)):
             raise ValueError("count must be in [0, new tokens of the sequence]")
+        for s, c, n in zip(seqs, kept, new):
+            pages, length = self._seqs[s]
+            first, end = length - n, length - n + c
+            if c and any(self._refs[p] > 1 for p in pages[first // self.page_tokens:
+                                                          -(-end // self.page_tokens)]):
+                raise ValueError("commit moves tokens in pages that another sequence holds too: "
+                                 "commit first, then fork")
         _lib.kv_commit_device(self.pool, self._head_dim, batch["table"], batch["kv_len"], path, count,
                               start, self.page_tokens)
         for s, c, n in zip(seqs, kept, new):

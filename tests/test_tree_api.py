@@ -261,3 +261,26 @@ def test_commit_bookkeeping(monkeypatch):
     with pytest.raises(ValueError):
         c.commit([seqs[0]] * 2, batch, path, count)
     assert len(calls) == 1
+
+
+def test_commit_into_shared_pages_is_refused(monkeypatch):
+    """A fork of the appended tree holds the pages that a commit would write to."""
+    from chenxing_amd import PagedKVCache
+    calls = []
+    monkeypatch.setattr(_lib, "kv_commit_device", lambda *a: calls.append(a))
+    c = PagedKVCache(1, 20, 2, 64, 16, device="cpu", copy=lambda *a: None)
+    s = c.add()
+    c.extend([s], [30])
+    before, = c.fork(s)                        # shares full pages, and one that extend copies
+    c.extend([s], [9])
+    batch = c.batch([s], [9])
+    path, count = torch.tensor([[0, 3, 8]], dtype=I32), torch.tensor([3], dtype=I32)
+    after, = c.fork(s)
+    with pytest.raises(ValueError, match="fork"):
+        c.commit([s], batch, path, count)
+    assert not calls and c.length(s) == 39
+    c.commit([s], batch, path, torch.tensor([0], dtype=I32))
+    assert c.length(s) == 30
+    s = after
+    c.free(before)
+    assert c.commit([s], batch, path, count) == [3] and c.length(s) == 33
