@@ -281,6 +281,8 @@ def test_commit_into_shared_pages_is_refused(monkeypatch):
     assert not calls and c.length(s) == 39
     c.commit([s], batch, path, torch.tensor([0], dtype=I32))
     assert c.length(s) == 30
-    s = after
+    with pytest.raises(ValueError, match="fork"):
+        c.commit([after], batch, path, count)  # slots 30 and 31 are in a page of s
+    c.free(s)
     c.free(before)
-    assert c.commit([s], batch, path, count) == [3] and c.length(s) == 33
+    assert c.commit([after], batch, path, count) == [3] and c.length(after) == 33
