@@ -709,7 +709,8 @@ int cx_kv_commit(const cx_kv_batch* kv, int64_t layer_stride, int32_t n_layers,
   cx::CommitArgs A;
   const int rc = cx::kv_args(kv, kv ? kv->kv_heads : 1, &A.kv);
   if (rc != CX_OK) return rc;
-  if (n_layers < 0 || width < 0 || layer_stride < 0 || layer_stride % 16)
+  if (n_layers < 0 || width < 0 || layer_stride < 0 || layer_stride % 16 ||
+      (layer_stride == 0 && n_layers > 1))   // (all layers would move the same tokens)
     return cx::api_fail(CX_EINVAL, "bad shape");
   if (kv->T == 0 || kv->B == 0 || kv->n_pages == 0 || kv->max_pages == 0 || n_layers == 0 || width == 0)
     return CX_OK;

@@ -14,6 +14,7 @@
 
 #include "cx_device.hpp"
 #include "cx_internal.hpp"
+#include "cx_lds.hpp"
 #include "cx_sampler.h"
 #include "cx_timing.hpp"
 
@@ -358,12 +359,10 @@ static hipError_t launch_tile(const W4Args& A, int group, bool shifts, hipStream
   static const W4Kernel kernels[3][2] = {{w4_tile<MT, NTW, WK, 1, false>, w4_tile<MT, NTW, WK, 1, true>},
                                          {w4_tile<MT, NTW, WK, 2, false>, w4_tile<MT, NTW, WK, 2, true>},
                                          {w4_tile<MT, NTW, WK, 4, false>, w4_tile<MT, NTW, WK, 4, true>}};
+  static LdsLimit limits[3][2];
   constexpr int lds = w4_lds_bytes<MT, NTW, WK>();
   const W4Kernel k = kernels[group / 64][shifts];
-  if (lds > 65536) {
-    const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-  }
+  if (int e = limits[group / 64][shifts].raise((const void*)k, lds)) return (hipError_t)e;
   timed_launch(CX_KERNEL_W4, k, dim3((pairs * (int64_t)WK + 7) / 8, (A.M + 16 * MT - 1) / (16 * MT)), dim3(512), lds, s, A);
   return hipSuccess;
 }
@@ -394,8 +393,8 @@ extern "C" int cx_w4_linear_bf16(const uint16_t* x, int64_t ldx, const uint32_t*
                                  const uint16_t* scales, int32_t shifts, int32_t group, int32_t M,
                                  int32_t N, int32_t K, void* out, int64_t ldo, int32_t out_bf16,
                                  void* stream) {
-  constexpr int most = 1 << 22;              // (65535 workgroups of 64 rows; the kernels' counts are ints)
-  if (M < 0 || N < 1 || K < 1 || M >= most || N >= 1 << 28 || K >= 1 << 28 || ldx < K || ldo < N)
+  // (65535 workgroups of 64 rows; the kernels' counts are ints)
+  if (M < 0 || N < 1 || K < 1 || M >= 1 << 21 || N >= 1 << 28 || K >= 1 << 28 || ldx < K || ldo < N)
     return cx::api_fail(CX_EINVAL, "bad shape (%d, %d, %d)", M, N, K);
   if (group != 32 && group != 64 && group != 128)
     return cx::api_fail(CX_EINVAL, "group (%d) must be 32, 64 or 128", group);

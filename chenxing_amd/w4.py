@@ -55,6 +55,8 @@ def quantize(w, group=64):
     # the codes are those of the scale and shift that are kept
     shift = lo.half()
     scale = ((hi - shift.float()) / 15).half()
+    if not bool(torch.isfinite(scale).all() & torch.isfinite(shift).all()):
+        raise ValueError("weights must be finite, and in the range of float16")
     step = scale.float()[..., None]
     q = torch.where(step > 0, (x - shift.float()[..., None]) / step, 0.0)
     return q.round().clamp(0, 15).byte().view(N, K), scale, shift

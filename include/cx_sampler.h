@@ -431,7 +431,7 @@ int cx_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t*
  * below n.  A move from or to a slot without a page in the pool is left out.  No
  * page that is written to may be another sequence's too.
  *
- *  kv         pages: layer 0's; layer l's are layer_stride bytes further each
+ *  kv         pages: layer 0's; layer l's are layer_stride bytes further each, not 0
  *  path       [B, width] int32
  *  count      [B] int32 (at most width are taken), or NULL: width each
  * Device pointers, stream-ordered, no synchronisation, no allocation.
@@ -467,7 +467,7 @@ int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int
  *             32 s + 8 j + e, e = 0 .. 7, at bit 4 (e / 2) + 16 (e % 2)
  *  scales     fp16 bits, 16-byte aligned: [N / 16 rounded up, K / group, 16], or with
  *             shifts [.., 16, 2]: scale, shift
- *  group      32, 64 or 128; K a multiple of it; N, K < 2^28, M < 2^22
+ *  group      32, 64 or 128; K a multiple of it; N, K < 2^28, M < 2^21
  *  out        [M, ldo] fp32, or bf16 bits if out_bf16
  * Rows of the last tile past N are read and not used.  The weights are read once for
  * up to 64 rows of x.  Device pointers, stream-ordered, no synchronisation, no

@@ -97,7 +97,7 @@ def test_tree_attention_workspace():
 
 @built
 @pytest.mark.parametrize("bad", [dict(stride=-16), dict(stride=8), dict(layers=-1), dict(width=-1),
-                                 dict(path=0), dict(layers=2 ** 31 - 1)], ids=str)
+                                 dict(path=0), dict(layers=2 ** 31 - 1), dict(stride=0)], ids=str)
 def test_bad_commits(bad):
     assert _commit(_kv(), **bad) == _lib.CX_EINVAL and _lib.load().cx_last_error()
 
@@ -118,7 +118,8 @@ def test_bad_accepts(bad):
 
 
 @built
-@pytest.mark.parametrize("bad", [dict(M=-1), dict(N=0), dict(K=0), dict(ldx=255), dict(ldo=19),
+@pytest.mark.parametrize("bad", [dict(M=-1), dict(N=0), dict(K=0), dict(M=1 << 21), dict(N=1 << 28, ldo=1 << 28),
+                                 dict(K=1 << 28, ldx=1 << 28), dict(ldx=255), dict(ldo=19),
                                  dict(group=16), dict(group=0), dict(group=96), dict(K=288, ldx=288),
                                  dict(x=0), dict(tiles=0), dict(scales=0), dict(out=0), dict(x=A + 8),
                                  dict(tiles=A + 4), dict(scales=A + 2), dict(ldx=260), dict(out=A + 2),
@@ -228,6 +229,11 @@ def test_quantize_refuses():
     for group in (16, 48, 128):
         with pytest.raises(ValueError):
             w4.quantize(torch.zeros(4, 64), group)
+    for bad in (float("nan"), float("inf"), 1e6):
+        w = torch.zeros(4, 64)
+        w[2, 5] = bad
+        with pytest.raises(ValueError):
+            w4.quantize(w, 32)
 
 
 def test_oracle_masks_and_paths():
