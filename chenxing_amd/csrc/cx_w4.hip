@@ -247,11 +247,12 @@ __global__ __launch_bounds__(512) void w4_stream(W4Args A) {
 
 // More rows: x passes through LDS, for all waves of a workgroup.  8 / WK waves side by side
 // take 16 NTW rows of W each, WK waves every WK-th tile of K; a step is a tile of each,
-// its x written to LDS a step ahead and asked for two ahead, as are the codes.  A row's 16
-// chunks of 8 k stand in the order of their number ^ the row's, so that the 16 rows that a
-// lane group reads are in different banks.  61 rows, N = 14336, K = 4096: 22 us, 37 with
-// every wave's own loads of x; 30 rows 14 us.  Of a step's time matrix instructions have
-// half, the rest are the codes' conversions and the scales' products.
+// its x sent to LDS a step ahead, past the registers (through them 22.4 us, not 20.1), its
+// codes two ahead.  A row's 16 chunks of 8 k stand in the order of their number ^ the row's,
+// so that the 16 rows that a lane group reads are in different banks.  61 rows, N = 14336, K =
+// 4096: 20.1 us, 37 with every wave's own loads of x; 30 rows 13.9 us.  A step is 2.1 us, with
+// 0.75 of matrix instructions: x in and out of LDS (192 KB a CU), conversions and scales are
+// beside them.
 template <int MT, int NTW, int WK, int STEPS, bool SHIFT>
 __global__ __launch_bounds__(512) void w4_tile(W4Args A) {
   constexpr int GROUPS = 4 / STEPS, ROWS = 16 * MT, CHUNKS = ROWS * 16;  // 16-byte chunks of a tile's x
@@ -269,17 +270,14 @@ __global__ __launch_bounds__(512) void w4_tile(W4Args A) {
   using Tile = W4Tile<NTW, GROUPS>;
   auto load = [&](Tile& t, int it) { t.load(W, it * WK + wk); };
   // this thread's chunks of x: place 512 j + tid is (wave k, row, place in the row)
-  auto load_x = [&](u32x4 (&x)[XL], int it) {
+  auto load_x = [&](int it) {
 #pragma unroll
     for (int j = 0; j < XL; ++j) {
       const int at = 512 * j + tid, row = at / 16 % ROWS, kt = min(it * WK + at / CHUNKS, KT - 1);
       const int k = min(kt * 16 + (at % 16 ^ (row & 15)), chunks - 1);
-      x[j] = *(const u32x4*)(A.x + min(m0 + row, A.M - 1) * A.ldx + 8 * (int64_t)k);
+      load_lds16((const char*)(A.x + min(m0 + row, A.M - 1) * A.ldx + 8 * (int64_t)k),
+                 (uint32_t)(uintptr_t)s_x + 16 * ((it & 1) * WK * CHUNKS + 512 * j + 64 * w));
     }
-  };
-  auto store_x = [&](const u32x4 (&x)[XL], int it) {
-#pragma unroll
-    for (int j = 0; j < XL; ++j) s_x[(it & 1) * WK * CHUNKS + 512 * j + tid] = x[j];
   };
   const W4Constants C = w4_constants<SHIFT>();
   f32x4 acc[MT][NTW];
@@ -287,34 +285,39 @@ __global__ __launch_bounds__(512) void w4_tile(W4Args A) {
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int n = 0; n < NTW; ++n) acc[i][n] = f32x4{0, 0, 0, 0};
-  auto step = [&](int it, Tile& t, const u32x4 (&next)[XL], u32x4 (&later)[XL]) {
-    // the waves' writes of this step's x are done, and their reads of the step's before
-    __builtin_amdgcn_s_waitcnt((15 | 3 << 14) | (7 << 4));
+  auto step = [&](int it, Tile& t) {
+    // this step's x and codes are there (the next codes alone are on their way), in all waves,
+    // and the step before has been read
+    wave_vm<NTW * (1 + GROUPS)>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    load_x(later, it + 2);
+    // (the compiler's own wait for the codes: behind the loads of x it would take in those)
+#pragma unroll
+    for (int n = 0; n < NTW; ++n) {
+      asm volatile("" : "+v"(t.code[n]));
+#pragma unroll
+      for (int q = 0; q < GROUPS; ++q) asm volatile("" : "+v"(t.scale[n][q]));
+    }
+    load_x(it + 1);
     const CX_LDS u32x4* xs = s_x + ((it & 1) * WK + wk) * CHUNKS;
     w4_multiply<MT, NTW, STEPS, SHIFT>(
         C, t, groups - (it * WK + wk) * GROUPS,
         [&](int i, int k) { return xs[(16 * i + c) * 16 + ((4 * k + g) ^ c)]; }, acc);
     load(t, it + W4_AHEAD);
-    store_x(next, it + 1);
   };
   Tile t[W4_AHEAD];
-  u32x4 x[2][XL];
-  load_x(x[0], 0);
   load(t[0], 0);
-  load_x(x[1], 1);
+  load_x(0);
 #pragma unroll
   for (int u = 1; u < W4_AHEAD; ++u) load(t[u], u);
-  store_x(x[0], 0);
   for (int i0 = 0; i0 < iters; i0 += W4_AHEAD)
 #pragma unroll
     for (int u = 0; u < W4_AHEAD; ++u) {
       if (u > 0 && i0 + u >= iters) break;
-      step(i0 + u, t[u], x[(u + 1) & 1], x[u & 1]);
+      step(i0 + u, t[u]);
     }
+  wave_vm<0>();                              // the last loads write LDS
   // the waves' sums, in the order of wk
   if (WK > 1) {
     __syncthreads();
@@ -370,11 +373,14 @@ static hipError_t launch_tile(const W4Args& A, int group, bool shifts, hipStream
 template <int MT>
 static hipError_t launch_tiles(const W4Args& A, int group, bool shifts, hipStream_t s) {
   const int pairs = (A.N + 31) / 32;
-  // 30 and 61 rows, N = 4096, K = 4096: 9.9 and 17.5 us with 16 rows of W a wave, 13.7 and 22.3
-  // with 32; N = 14336: 31.5 and 32.8 with 16, 14.0 and 22.8 with 32
+  // 30 and 61 rows, K = 4096, N = 4096: 8.2 and 14.6 us with 16 rows of W a wave, 9.9 and 19.5
+  // with 32; N = 14336: 26.5 and 27.4 with 16, 13.9 and 20.1 with 32; 30 rows,
+  // N = 50257: 38.9 with 32, 55.8 with 64; N = 128256: 67.2 and 61.2
   if (pairs * 4 < W4_WAVES) return launch_tile<MT, 1, 16 / MT>(A, group, shifts, s);
   if (pairs * 2 < W4_WAVES) return launch_tile<MT, 2, 4>(A, group, shifts, s);
   if (pairs < W4_WAVES) return launch_tile<MT, 2, 2>(A, group, shifts, s);
+  if constexpr (MT == 2)                     // (64 of 64 rows do not fit the registers)
+    if (pairs / 2 >= W4_WAVES) return launch_tile<MT, 4, 1>(A, group, shifts, s);
   return launch_tile<MT, 2, 1>(A, group, shifts, s);
 }
 static hipError_t launch_w4(const W4Args& A, int group, bool shifts, hipStream_t s) {
