@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "cx_device.hpp"
+#include "cx_dma.hpp"
 #include "cx_internal.hpp"
 #include "cx_kv.hpp"
 #include "cx_sampler.h"
@@ -873,10 +874,10 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 }
 
 // Part q's slot of a row block's: a thread's ITEMS times 4 of 16 rows' sums.
-template <int D, class Slot>
-__device__ __forceinline__ void tree_join_rows(const TreeArgs& A, int rows, int n, int r0, Slot slot, int R,
+template <int D, int AHEAD, class Slot>
+__device__ __forceinline__ void tree_join_parts(const TreeArgs& A, int rows, int n, int r0, Slot slot, int R,
                                                int row0, int tok0, int head) {
-  constexpr int ITEMS = D / 64, AHEAD = 8;   // 16-byte items of a thread
+  constexpr int ITEMS = D / 64;              // 16-byte items of a thread
   const int l = lane_id(), c = l & 15, g = l >> 4;
   float top = -INFINITY, L = 0;
   f32x4 o[ITEMS];
@@ -920,6 +921,16 @@ __device__ __forceinline__ void tree_join_rows(const TreeArgs& A, int rows, int 
     const int d = 16 * (4 * i + wave_id());
     *(u32x2*)(out + d) = u32x2{pack_bf16(o[i][0] * f, o[i][1] * f), pack_bf16(o[i][2] * f, o[i][3] * f)};
   }
+}
+
+// AHEAD parts are read at a time: about as many as there are (64 trees in row blocks of 256,
+// two or three parts each: 24 us with 8).
+template <int D, class Slot>
+__device__ __forceinline__ void tree_join_rows(const TreeArgs& A, int rows, int n, int r0, Slot slot, int R,
+                                               int row0, int tok0, int head) {
+  if (n <= 2) tree_join_parts<D, 2>(A, rows, n, r0, slot, R, row0, tok0, head);
+  else if (n <= 4) tree_join_parts<D, 4>(A, rows, n, r0, slot, R, row0, tok0, head);
+  else tree_join_parts<D, 8>(A, rows, n, r0, slot, R, row0, tok0, head);
 }
 
 // A row block's parts joined, 16 rows to a workgroup, in the order of their slots: of

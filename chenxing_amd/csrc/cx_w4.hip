@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include "cx_device.hpp"
+#include "cx_dma.hpp"
 #include "cx_internal.hpp"
 #include "cx_lds.hpp"
 #include "cx_sampler.h"
