@@ -19,9 +19,9 @@
 // K and V are read once for up to 256 rows, so trees of 64 nodes are bound by the matrix
 // cores (with the terms in two parts half as much again as the formula's products) and by
 // the softmax beside them: 2 sequences of 120001 .. 131072 tokens, 32 / 8 heads of 128,
-// bf16, 446 us, 585 TFLOP/s of the formula's; 64 of up to 8192, e4m3, 441 us.  Few rows are
+// bf16, 444 us, 587 TFLOP/s of the formula's; 64 of up to 8192, e4m3, 434 us.  Few rows are
 // bound by the start, a step's latency (1.2 us at D = 128) and a row block's own cost (about
-// 5 us: its rows, the groups' meeting, its part): 32 ragged trees of up to 33 nodes 54 us.
+// 5 us: its rows, the groups' meeting, its part): 32 ragged trees of up to 33 nodes 52 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -924,7 +924,7 @@ __device__ __forceinline__ void tree_join_parts(const TreeArgs& A, int rows, int
 }
 
 // AHEAD parts are read at a time: about as many as there are (64 trees in row blocks of 256,
-// two or three parts each: 24 us with 8).
+// two or three parts each: 16.7 us, 24 with 8 at all times).
 template <int D, class Slot>
 __device__ __forceinline__ void tree_join_rows(const TreeArgs& A, int rows, int n, int r0, Slot slot, int R,
                                                int row0, int tok0, int head) {
