@@ -173,6 +173,8 @@ class PagedKVCache:
             raise ValueError("commit takes each sequence of the batch once")
         if any(not 0 <= c <= n <= self._seqs[s][1] for s, c, n in zip(seqs, kept, new)):
             raise ValueError("count must be in [0, new tokens of the sequence]")
+        if batch["kv_len"].tolist() != [self._seqs[s][1] for s in seqs]:
+            raise ValueError("the sequences are not as long as when the batch was made")
         for s, c, n in zip(seqs, kept, new):
             pages, length = self._seqs[s]
             first, end = length - n, length - n + c

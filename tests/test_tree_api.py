@@ -269,6 +269,26 @@ def test_commit_bookkeeping(monkeypatch):
     assert len(calls) == 1
 
 
+def test_commit_of_a_batch_of_other_lengths_is_refused(monkeypatch):
+    from chenxing_amd import PagedKVCache
+    calls = []
+    monkeypatch.setattr(_lib, "kv_commit_device", lambda *a: calls.append(a))
+    c = PagedKVCache(1, 20, 2, 64, 16, device="cpu")
+    seqs = [c.add(), c.add()]
+    c.extend(seqs, [25, 20])
+    batch = c.batch(seqs, [9, 4])
+    path, count = torch.tensor([[0, 3], [0, 1]], dtype=I32), torch.tensor([2, 2], dtype=I32)
+    with pytest.raises(ValueError):
+        c.commit(seqs[::-1], batch, path, count)
+    c.extend([seqs[1]], [1])
+    with pytest.raises(ValueError):
+        c.commit(seqs, batch, path, count)
+    c.truncate(seqs[1], 20)
+    assert c.commit(seqs, batch, path, count) == [2, 2] and len(calls) == 1
+    with pytest.raises(ValueError):            # twice
+        c.commit(seqs, batch, path, count)
+
+
 def test_commit_into_shared_pages_is_refused(monkeypatch):
     """A fork of the appended tree holds the pages that a commit would write to."""
     from chenxing_amd import PagedKVCache
