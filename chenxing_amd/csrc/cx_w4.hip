@@ -46,6 +46,7 @@ constexpr int W4_AHEAD = 2;
 // with 2004 and twice as many waves: N = 128256 60 and 70 us; N = 14336 with 1792, half,
 // a quarter: 11.4, 16.4, 26.0 us.
 constexpr int W4_WAVES = 1536;
+constexpr int W4_CUS = 256;
 // Rows of x so far apart that 16 of them pass 32 bits take the other kernel.
 constexpr int64_t W4_STRIDE = 1 << 26;
 
@@ -370,14 +371,19 @@ static hipError_t launch_tile(const W4Args& A, int group, bool shifts, hipStream
   timed_launch(CX_KERNEL_W4, k, dim3((pairs * (int64_t)WK + 7) / 8, (A.M + 16 * MT - 1) / (16 * MT)), dim3(512), lds, s, A);
   return hipSuccess;
 }
-// Rows of W a wave, waves of a row: as many rows as leave W4_WAVES waves.
+// Rows of W a wave, waves that share them: few and many while the workgroups are on the chip
+// at once, then as many rows as leave W4_WAVES waves.  K = 4096, 30 and 61 rows, with 16
+// rows of W a wave and with 32: N = 4096 8.2 and 14.6, 9.9 and 19.5 us; N = 14336 26.5 and
+// 27.4, 13.9 and 20.1 us; N = 6144, 32 rows, 15.2 and 11.0 us.  30 rows with 32 and with 64:
+// N = 50257 38.9 and 55.8 us, N = 128256 67.2 and 61.2.
 template <int MT>
 static hipError_t launch_tiles(const W4Args& A, int group, bool shifts, hipStream_t s) {
   const int pairs = (A.N + 31) / 32;
-  // 30 and 61 rows, K = 4096, N = 4096: 8.2 and 14.6 us with 16 rows of W a wave, 9.9 and 19.5
-  // with 32; N = 14336: 26.5 and 27.4 with 16, 13.9 and 20.1 with 32; 30 rows,
-  // N = 50257: 38.9 with 32, 55.8 with 64; N = 128256: 67.2 and 61.2
-  if (pairs * 4 < W4_WAVES) return launch_tile<MT, 1, 16 / MT>(A, group, shifts, s);
+  if (pairs <= W4_CUS) {
+    if constexpr (MT == 2)
+      if (pairs * 2 > W4_CUS) return launch_tile<MT, 2, 8>(A, group, shifts, s);
+    return launch_tile<MT, 1, 16 / MT>(A, group, shifts, s);
+  }
   if (pairs * 2 < W4_WAVES) return launch_tile<MT, 2, 4>(A, group, shifts, s);
   if (pairs < W4_WAVES) return launch_tile<MT, 2, 2>(A, group, shifts, s);
   if constexpr (MT == 2)                     // (64 of 64 rows do not fit the registers)
@@ -385,9 +391,11 @@ static hipError_t launch_tiles(const W4Args& A, int group, bool shifts, hipStrea
   return launch_tile<MT, 2, 1>(A, group, shifts, s);
 }
 static hipError_t launch_w4(const W4Args& A, int group, bool shifts, hipStream_t s) {
-  if (A.M > 32) return launch_tiles<4>(A, group, shifts, s);
-  if (A.M > 16 || A.ldx > W4_STRIDE) return launch_tiles<2>(A, group, shifts, s);
   const int tiles = (A.N + 15) / 16;
+  // 32 rows a workgroup also where these are all on the chip at once (64 rows, N = 512, K =
+  // 14336: 18 us, 45 with 64 rows a workgroup; 128 rows, N = 1024, K = 4096: 8.0 and 15.8)
+  if (A.M > 32 && tiles * (int64_t)((A.M + 31) / 32) > W4_CUS) return launch_tiles<4>(A, group, shifts, s);
+  if (A.M > 16 || A.ldx > W4_STRIDE) return launch_tiles<2>(A, group, shifts, s);
   if (tiles * (8 / 4) >= W4_WAVES) launch_stream<4>(A, group, shifts, s);
   else if (tiles * (8 / 2) >= W4_WAVES) launch_stream<2>(A, group, shifts, s);
   else launch_stream<1>(A, group, shifts, s);
