@@ -990,7 +990,8 @@ static int launch_tree(TreeArgs A, int64_t max_new, hipStream_t s) {
   constexpr int ROWS = Sh::ROWS;
   const int64_t held = (int64_t)A.kv.M << A.kv.logP;
   const int64_t span = A.window ? std::min<int64_t>(A.window + max_new + TREE_UNIT, held) : held;
-  const int64_t units = (span + TREE_UNIT - 1) / TREE_UNIT;
+  // (a table without columns: one empty chunk, whose rows are 0)
+  const int64_t units = std::max<int64_t>((span + TREE_UNIT - 1) / TREE_UNIT, 1);
   const int64_t tiles = (A.G * max_new + ROWS - 1) / ROWS, blocks = A.kv.B * A.kv.heads * tiles;
   // Chunks where the longest context is short for the workgroups there are ..
   const int64_t most = tree_slots(ROWS) / blocks;               // parts of a row block at most
