@@ -164,17 +164,28 @@ class PagedKVCache:
         """A round of drafted trees ends: of the last tokens of seqs[i], those that
         ``batch`` appended, path[i, :count[i]] stay, in that order (``path`` and
         ``count`` as ``_lib.tree_accept_device`` gives them); how many of each.  A
-        sequence that was forked after the append is refused."""
+        sequence that was forked after the append is refused, and so is a batch whose
+        lengths or pages are no longer the sequences' (after ``compact``, make it
+        again: the tokens have moved with their pages)."""
         from . import _lib
-        start = batch["q_start"]
-        new = [1] * len(seqs) if start is None else start.diff().tolist()
-        kept = count.tolist()
-        if len(set(seqs)) != len(seqs) or len(new) != len(seqs) or len(kept) != len(seqs):
-            raise ValueError("commit takes each sequence of the batch once")
+        import torch
+        table, start = batch["table"], batch["q_start"]
+        B, M = len(seqs), table.shape[1]
+        if len(set(seqs)) != B or table.shape[0] != B or count.shape != (B,) or \
+                count.device != table.device or not (start is None or start.shape == (B + 1,)):
+            raise ValueError("commit takes each sequence of the batch once, and count [sequences] on "
+                             "the pool's device")
+        # in one copy to the host, what the moves go by
+        parts = [count, batch["kv_len"], table.flatten(), *([] if start is None else [start])]
+        host = torch.cat(parts).cpu().numpy()
+        kept, lens, held = host[:B].tolist(), host[B:2 * B], host[2 * B:(2 + M) * B].reshape(B, M)
+        new = [1] * B if start is None else np.diff(host[(2 + M) * B:]).tolist()
         if any(not 0 <= c <= n <= self._seqs[s][1] for s, c, n in zip(seqs, kept, new)):
             raise ValueError("count must be in [0, new tokens of the sequence]")
-        if batch["kv_len"].tolist() != [self._seqs[s][1] for s in seqs]:
-            raise ValueError("the sequences are not as long as when the batch was made")
+        for s, n, row in zip(seqs, lens, held):
+            pages, length = self._seqs[s]
+            if n != length or row[:len(pages)].tolist() != pages:
+                raise ValueError("the sequences' lengths or pages are not those of the batch")
         for s, c, n in zip(seqs, kept, new):
             pages, length = self._seqs[s]
             first, end = length - n, length - n + c

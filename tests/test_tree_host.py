@@ -8,8 +8,10 @@ import sys
 
 import pytest
 
-from chenxing_amd import _lib
-from conftest import ROOT
+torch = pytest.importorskip("torch")
+
+from chenxing_amd import _lib                                        # noqa: E402
+from conftest import ROOT                                            # noqa: E402
 
 built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libcx_sampler.so not built")
 
@@ -36,3 +38,86 @@ def _alone(call):
 def test_a_table_without_columns_is_no_fault(start, window):
     """Every row then attends to nothing: there are no units to divide among workgroups."""
     assert _alone(f"_tree(T._kv(M=0, ld=0, table=0{start}), window={window})") == _lib.CX_EHIP
+
+
+# ------------------------------------------------------------------ PagedKVCache.commit
+@pytest.fixture
+def moved(monkeypatch):
+    """The calls that commit makes of the device."""
+    calls = []
+    monkeypatch.setattr(_lib, "kv_commit_device", lambda *a: calls.append(a))
+    return calls
+
+
+def _cache():
+    from chenxing_amd import PagedKVCache
+    return PagedKVCache(1, 20, 2, 64, 16, device="cpu", copy=lambda *a: None)
+
+
+def _ids(*rows):
+    return torch.tensor(rows, dtype=torch.int32)
+
+
+def test_commit_after_a_compaction_is_refused(moved):
+    """The batch's pages are then another sequence's; a new batch commits."""
+    c = _cache()
+    a, b = c.add(), c.add()
+    c.extend([a, b], [20, 20])
+    c.extend([b], [9])
+    batch = c.batch([b], [9])
+    assert batch["table"].tolist() == [[2, 3]]
+    c.free(a)
+    c.compact()
+    other = c.add()
+    c.extend([other], [40])
+    assert c.length(b) == 29 and not {2, 3}.isdisjoint(c.pages_of(other))
+    path, count = _ids([0, 4, 8]), _ids(3)
+    with pytest.raises(ValueError, match="pages"):
+        c.commit([b], batch, path, count)
+    assert not moved and c.length(b) == 29
+    again = c.batch([b], [9])
+    assert c.commit([b], again, path, count) == [3] and c.length(b) == 23
+    assert moved[0][2].tolist() == [[0, 1]]
+
+
+def test_commit_after_a_sequence_left_its_pages_is_refused(moved):
+    """A fork, an extend and a truncate lead to the same length in a copied page."""
+    c = _cache()
+    s = c.add()
+    c.extend([s], [20])
+    c.extend([s], [6])
+    batch = c.batch([s], [6])
+    c.fork(s)
+    c.extend([s], [1])
+    c.truncate(s, 26)
+    path, count = _ids([0, 4]), _ids(2)
+    with pytest.raises(ValueError, match="pages"):
+        c.commit([s], batch, path, count)
+    assert not moved and c.length(s) == 26
+    assert c.commit([s], c.batch([s], [6]), path, count) == [2] and c.length(s) == 22
+
+
+def test_commit_of_sequences_in_another_order_is_refused(moved):
+    c = _cache()
+    a, b = c.add(), c.add()
+    c.extend([a, b], [30, 30])
+    batch = c.batch([a, b], [9, 9])
+    path, count = _ids([0, 3], [0, 1]), _ids(2, 2)
+    with pytest.raises(ValueError, match="pages"):
+        c.commit([b, a], batch, path, count)
+    with pytest.raises(ValueError):
+        c.commit([a], batch, path, count)
+    assert not moved
+    assert c.commit([a, b], batch, path, count) == [2, 2] and len(moved) == 1
+
+
+def test_commit_of_batches_of_single_tokens(moved):
+    """Without q_start every sequence has one new token; sequences without pages."""
+    c = _cache()
+    a, b = c.add(), c.add()
+    c.extend([a, b], [17, 1])
+    batch = c.batch([a, b])
+    assert c.commit([a, b], batch, _ids([0], [-1]), _ids(1, 0)) == [1, 0]
+    assert [c.length(a), c.length(b)] == [17, 0] and len(moved) == 1
+    empty = c.batch([b], [0])
+    assert c.commit([b], empty, _ids([-1]), _ids(0)) == [0] and c.length(b) == 0
