@@ -735,8 +735,8 @@ def kv_commit_device(cache, head_dim, table, kv_len, path, count=None, q_start=N
     ``cache`` is [layers, n_pages, kv_heads, width] or one layer of it; ``table``,
     ``kv_len`` (the drafted tokens included) and ``q_start`` are those of the pass
     that appended them; ``path`` [B, width] and ``count`` [B] int32 come from
-    ``tree_accept_device``.  A row of path ends where it does not rise.  Returns
-    cache."""
+    ``tree_accept_device``.  A row of path ends where it does not rise; an entry that
+    ends it before its count becomes -1.  Returns cache."""
     import torch
     lib = _lib or load()
     dev, shape = cache.get_device(), cache.shape

@@ -497,7 +497,7 @@ struct CommitArgs {
   KvArgs kv;
   int64_t layer_stride;
   int n_layers, width, heads; // heads of a workgroup
-  const int32_t* path;        // [B, width]
+  int32_t* path;              // [B, width]
   const int32_t* count;       // nullable [B]
 };
 constexpr int COMMIT_PASS = 32;              // moves looked up at a time
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256) void commit_tokens(CommitArgs A) {
   const int64_t s0 = (int64_t)C.kv_len[b] - n;
   if (s0 < 0) return;
   char* const base = C.pages + (x % (unsigned)A.n_layers) * A.layer_stride + (int64_t)h0 * C.head_bytes;
-  const int32_t* path = A.path + (int64_t)b * A.width;
+  int32_t* path = A.path + (int64_t)b * A.width;
   const int m = A.count ? min(A.count[b], A.width) : A.width;
   for (int j0 = 0; j0 < m; j0 += COMMIT_PASS) {
     // the pass's moves: the first wave looks them up, side by side
@@ -553,6 +553,8 @@ __global__ __launch_bounds__(256) void commit_tokens(CommitArgs A) {
       if (lane_id() == 0) {
         s_moves[0] = __builtin_popcountll(all);
         s_moves[1] = end;
+        // a row that ends too early says where; for those that read it later it ends there too
+        if (blockIdx.x % (A.n_layers * parts) == 0 && end < min(m - j0, COMMIT_PASS)) path[j0 + end] = -1;
       }
     }
     __syncthreads();
@@ -705,7 +707,7 @@ int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int
 }
 
 int cx_kv_commit(const cx_kv_batch* kv, int64_t layer_stride, int32_t n_layers,
-                 const int32_t* path, int32_t width, const int32_t* count, void* stream) {
+                 int32_t* path, int32_t width, const int32_t* count, void* stream) {
   cx::CommitArgs A;
   const int rc = cx::kv_args(kv, kv ? kv->kv_heads : 1, &A.kv);
   if (rc != CX_OK) return rc;

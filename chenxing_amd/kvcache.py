@@ -163,25 +163,29 @@ class PagedKVCache:
     def commit(self, seqs, batch, path, count) -> list[int]:
         """A round of drafted trees ends: of the last tokens of seqs[i], those that
         ``batch`` appended, path[i, :count[i]] stay, in that order (``path`` and
-        ``count`` as ``_lib.tree_accept_device`` gives them); how many of each.  A
-        sequence that was forked after the append is refused, and so is a batch whose
-        lengths or pages are no longer the sequences' (after ``compact``, make it
-        again: the tokens have moved with their pages)."""
+        ``count`` as ``_lib.tree_accept_device`` gives them); how many of each.  Of a
+        row of path that does not rise, or reaches past the new tokens, those before
+        that stay, and path holds -1 there afterwards.  A sequence that was forked
+        after the append is refused, and so is a batch whose lengths or pages are no
+        longer the sequences' (after ``compact``, make it again: the tokens have moved
+        with their pages)."""
         from . import _lib
         import torch
         table, start = batch["table"], batch["q_start"]
-        B, M = len(seqs), table.shape[1]
-        if len(set(seqs)) != B or table.shape[0] != B or count.shape != (B,) or \
-                count.device != table.device or not (start is None or start.shape == (B + 1,)):
-            raise ValueError("commit takes each sequence of the batch once, and count [sequences] on "
-                             "the pool's device")
+        B, M, width = len(seqs), table.shape[1], path.shape[-1]
+        if len(set(seqs)) != B or table.shape[0] != B or count.shape != (B,) or path.shape != (B, width) or \
+                count.device != table.device or path.device != table.device or \
+                not (start is None or start.shape == (B + 1,)):
+            raise ValueError("commit takes each sequence of the batch once, and path [sequences, width] "
+                             "and count [sequences] on the pool's device")
         # in one copy to the host, what the moves go by
-        parts = [count, batch["kv_len"], table.flatten(), *([] if start is None else [start])]
-        host = torch.cat(parts).cpu().numpy()
-        kept, lens, held = host[:B].tolist(), host[B:2 * B], host[2 * B:(2 + M) * B].reshape(B, M)
-        new = [1] * B if start is None else np.diff(host[(2 + M) * B:]).tolist()
-        if any(not 0 <= c <= n <= self._seqs[s][1] for s, c, n in zip(seqs, kept, new)):
-            raise ValueError("count must be in [0, new tokens of the sequence]")
+        parts = [count, batch["kv_len"], table, path, *([] if start is None else [start])]
+        host = torch.cat([t.flatten() for t in parts]).cpu().numpy()
+        kept, lens, held, way, first = np.split(host, np.cumsum([B, B, B * M, B * width]))
+        kept, held, way = kept.tolist(), held.reshape(B, M), way.reshape(B, width)
+        new = [1] * B if start is None else np.diff(first).tolist()
+        if any(not 0 <= c <= min(n, width, self._seqs[s][1]) for s, c, n in zip(seqs, kept, new)):
+            raise ValueError("count must be in [0, new tokens of the sequence], and path that wide")
         for s, n, row in zip(seqs, lens, held):
             pages, length = self._seqs[s]
             if n != length or row[:len(pages)].tolist() != pages:
@@ -193,8 +197,11 @@ class PagedKVCache:
                                                           -(-end // self.page_tokens)]):
                 raise ValueError("commit moves tokens in pages that another sequence holds too: "
                                  "commit first, then fork")
-        _lib.kv_commit_device(self.pool, self._head_dim, batch["table"], batch["kv_len"], path, count,
-                              start, self.page_tokens)
+        _lib.kv_commit_device(self.pool, self._head_dim, table, batch["kv_len"], path, count, start,
+                              self.page_tokens)
+        rises = (np.diff(way, axis=1, prepend=-1) > 0) & (way < np.reshape(new, (B, 1)))
+        if not (rises | (np.arange(width) >= np.reshape(kept, (B, 1)))).all():
+            kept = [min(c, [*row, -1].index(-1)) for row, c in zip(path.tolist(), kept)]
         for s, c, n in zip(seqs, kept, new):
             self.truncate(s, self._seqs[s][1] - n + c)
         return kept

@@ -428,7 +428,7 @@ int cx_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t*
  * tokens begin in slot s = kv_len[b] - n, slot s + j becomes a copy of slot
  * s + path[b][j] for j < count[b], as if every slot were read before any is written.
  * A row of path ends before an entry that is not above the one before it, or not
- * below n.  A move from or to a slot without a page in the pool is left out.  No
+ * below n; where that is before j reaches count[b], the entry becomes -1.  A move from or to a slot without a page in the pool is left out.  No
  * page that is written to may be another sequence's too.
  *
  *  kv         pages: layer 0's; layer l's are layer_stride bytes further each, not 0
@@ -437,7 +437,7 @@ int cx_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t*
  * Device pointers, stream-ordered, no synchronisation, no allocation.
  */
 int cx_kv_commit(const cx_kv_batch* kv, int64_t layer_stride, int32_t n_layers,
-                 const int32_t* path, int32_t width, const int32_t* count, void* stream);
+                 int32_t* path, int32_t width, const int32_t* count, void* stream);
 
 /*
  * Pages copied in every layer: page dst[i] becomes a copy of page src[i] (a

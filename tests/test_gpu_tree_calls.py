@@ -1,5 +1,5 @@
 """Calls of the tree operators that their documentation allows at its edges: tables
-without columns."""
+without columns, paths that stop."""
 from __future__ import annotations
 
 import numpy as np
@@ -7,7 +7,8 @@ import pytest
 
 import paged_cases as C
 import tree_cases as X
-from test_gpu_tree import _mask
+from oracle import paged_ref as R
+from test_gpu_tree import _commit_inputs, _mask
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +35,72 @@ def test_tables_without_columns(cache, D, new, window):
                           C.to_gpu(np.array([5, 0, 90], np.int32)), _mask(mask), start, C.to_gpu(depth),
                           max(new), window=window, out=out)
     assert (out[:T] == 0).all() and (out[T:] == 7.0).all()
+
+
+ROWS = [([0, 4, 2, 8], 2), ([0, 3, 3, 5], 2), ([1, 4, 9, 7], 2), ([-1, 4, 5, 6], 0), ([9, 1, 2, 3], 0),
+        ([2, 5, 6, 8], 4), ([0, 4, 8, 1], 3)]
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_paths_that_stop_are_marked(cache):
+    """The entry that ends a row before its count becomes -1, for one layer and several;
+    a row that ends with its count, or by it, stays as it is."""
+    import torch
+    from chenxing_amd._lib import kv_commit_device
+    B = len(ROWS)
+    _, table, kv_len, q_start, dense, _, _ = _commit_inputs(cache, 64, 16, 3, 2, [30] * B, [9] * B, 4)
+    path = np.array([r for r, _ in ROWS], np.int32)
+    for count in ([4] * B, None, [2] * B):
+        for layers in (1, 2):
+            pool = torch.stack([C.to_gpu(R.pack(*x)) for x in dense[:layers]])
+            p = C.to_gpu(path)
+            kv_commit_device(pool, 64, C.to_gpu(table), C.to_gpu(kv_len), p,
+                             None if count is None else C.to_gpu(np.array(count, np.int32)),
+                             C.to_gpu(q_start))
+            want = path.copy()
+            for b, (_, n) in enumerate(ROWS):
+                if n < (4 if count is None else count[b]):
+                    want[b, n] = -1
+            assert (p.cpu().numpy() == want).all()
+
+
+def test_long_paths_that_stop_are_marked():
+    """In the second and the third pass of moves."""
+    from chenxing_amd._lib import kv_commit_device
+    _, table, kv_len, q_start, dense, _, _ = _commit_inputs("bf16", 64, 16, 2, 1, [200] * 4, [150] * 4, 90)
+    path = np.tile(np.arange(1, 91, dtype=np.int32), (4, 1))
+    for b, at in enumerate((31, 32, 64, 89)):
+        path[b, at] = path[b, at - 1]
+    p = C.to_gpu(path)
+    kv_commit_device(C.to_gpu(R.pack(*dense[0])), 64, C.to_gpu(table), C.to_gpu(kv_len), p,
+                     q_start=C.to_gpu(q_start))
+    for b, at in enumerate((31, 32, 64, 89)):
+        path[b, at] = -1
+    assert (p.cpu().numpy() == path).all()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_a_cache_keeps_what_was_moved(cache):
+    """PagedKVCache.commit of rows that do not rise: the sequence holds the nodes before
+    that, in their order, and nothing behind them."""
+    import torch
+    from chenxing_amd import PagedKVCache
+    c = PagedKVCache(2, 40, 3, 64, 16, dtype=cache)
+    seqs = [c.add() for _ in ROWS]
+    c.extend(seqs, [21] * len(seqs))
+    c.extend(seqs, [9] * len(seqs))
+    c.pool.view(torch.uint8).random_(0, 120)
+    before = [R.unpack(C.bits_of(x), 64) for x in c.pool]
+    batch = c.batch(seqs, [9] * len(seqs))
+    path = C.to_gpu(np.array([r for r, _ in ROWS], np.int32))
+    count = torch.full((len(seqs),), 4, dtype=torch.int32, device="cuda")
+    assert c.commit(seqs, batch, path, count) == [n for _, n in ROWS]
+    assert [c.length(s) for s in seqs] == [21 + n for _, n in ROWS]
+    for old, x in zip(before, c.pool):
+        now = R.unpack(C.bits_of(x), 64)
+        for s, (row, n) in zip(seqs, ROWS):
+            pages, had = c.pages_of(s), batch["table"][seqs.index(s)].tolist()
+            for j in range(n):
+                at, frm = 21 + j, 21 + row[j]
+                for a, b in zip(now, old):
+                    assert (a[pages[at // 16], :, at % 16] == b[had[frm // 16], :, frm % 16]).all()

@@ -121,3 +121,38 @@ def test_commit_of_batches_of_single_tokens(moved):
     assert [c.length(a), c.length(b)] == [17, 0] and len(moved) == 1
     empty = c.batch([b], [0])
     assert c.commit([b], empty, _ids([-1]), _ids(0)) == [0] and c.length(b) == 0
+
+
+def test_commit_of_more_than_the_path_is_refused(moved):
+    c = _cache()
+    s = c.add()
+    c.extend([s], [20])
+    c.extend([s], [9])
+    batch = c.batch([s], [9])
+    with pytest.raises(ValueError, match="count"):
+        c.commit([s], batch, _ids([0, 4]), _ids(6))
+    for path in (_ids([0, 4], [0, 4]), _ids(0, 4)):
+        with pytest.raises(ValueError):
+            c.commit([s], batch, path, _ids(2))
+    assert not moved and c.length(s) == 29
+
+
+@pytest.mark.parametrize("row,stays", [([0, 4, 2], 2), ([0, 4, 4], 2), ([0, 4, 9], 2), ([-1, 4, 5], 0),
+                                       ([9, 4, 5], 0), ([0, 4, 8], 3)], ids=str)
+def test_commit_keeps_what_was_moved(monkeypatch, row, stays):
+    """Of a row that stops rising, or passes the nodes, the tokens before that: the
+    device call ends there, and marks the place."""
+    calls = []
+
+    def device(pool, D, table, kv_len, path, count, *rest):
+        calls.append(path.tolist())
+        if stays < 3:
+            path[1, stays] = -1
+    monkeypatch.setattr(_lib, "kv_commit_device", device)
+    c = _cache()
+    a, b = c.add(), c.add()
+    c.extend([a, b], [20, 30])
+    batch = c.batch([a, b], [6, 9])
+    path = _ids([0, 5, -1], row)
+    assert c.commit([a, b], batch, path, _ids(2, 3)) == [2, stays]
+    assert len(calls) == 1 and [c.length(a), c.length(b)] == [16, 21 + stays]
