@@ -67,6 +67,8 @@ _SIGS = {
     "cx_tree_attention_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32,
                                                        C.c_int32]),
     "cx_tree_masks": (C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, _P, _P]),
+    "cx_tree_masks_window": (C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, _P,
+                                       C.c_int32, _P]),
     "cx_tree_accept": (C.c_int, [_P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P,
                                  _P]),
     "cx_kv_commit": (C.c_int, [C.c_char_p, C.c_int64, C.c_int32, _P, C.c_int32, _P, _P]),
@@ -645,7 +647,8 @@ def tree_attention_device(q, cache, table, kv_len, mask, q_start=None, depth=Non
     tree: ``mask`` [T, words] int64 says which of them a node attends to (bit i %
     64 of word i // 64: node i, as ``tree_masks_device`` gives them); all attend
     to the tokens before them.  A ``window`` > 0 needs ``depth`` [T] int32 and
-    counts from a node's depth, over the tokens before the tree."""
+    counts from a node's depth, over the tokens before the tree; nodes that it has
+    passed are for the mask to leave out (``tree_masks_device``'s ``window``)."""
     import torch
     lib = _lib or load()
     dev, shape, qs = _q_rows(torch, q)
@@ -687,20 +690,21 @@ def _tree_rows(torch, parents, q_start):
                                                   (max(q_start.numel(), 1),))
 
 
-def tree_masks_device(parents, q_start=None, words=1):
+def tree_masks_device(parents, q_start=None, words=1, window=0):
     """(mask [T, words] int64, depth [T] int32) of drafted trees, on the current
     stream: the bits of every node and its ancestors, and how many these are.
 
     ``parents`` [T] int32: a node's parent among the nodes of its sequence, below
     the node's own index; -1 (or anything else) for a root.  ``q_start`` [B + 1]
-    int32 as for the attention.  ``words``: 64 nodes each."""
+    int32 as for the attention.  ``words``: 64 nodes each.  ``window`` > 0, as for
+    the attention: only ancestors less than ``window`` above the node."""
     import torch
     lib = _lib or load()
     dev, T, B, start = _tree_rows(torch, parents, q_start)
     mask = torch.empty(T, words, dtype=torch.int64, device=parents.device)
     depth = torch.empty_like(parents)
-    _call(torch, dev, lib.cx_tree_masks, parents.data_ptr(), start, B, T, mask.data_ptr(), words,
-          depth.data_ptr())
+    _call(torch, dev, lib.cx_tree_masks_window, parents.data_ptr(), start, B, T, mask.data_ptr(), words,
+          depth.data_ptr(), window)
     return mask, depth
 
 

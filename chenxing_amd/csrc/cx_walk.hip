@@ -20,6 +20,7 @@ struct WalkArgs {
   const int32_t* sampled;
   const int32_t* q_start;     // nullable
   int B, T, words, width;
+  int window;                 // 0: none
   uint64_t* mask;
   int32_t* depth;             // nullable
   int32_t* path;
@@ -53,8 +54,8 @@ __global__ __launch_bounds__(256) void tree_masks(WalkArgs A) {
     uint64_t m = 0;
     int d = -1;
     for (int a = i; a >= 0;) {               // parents lie below their children: it ends
-      if (a >> 6 == w) m |= 1ull << (a & 63);
       ++d;
+      if (a >> 6 == w && (A.window == 0 || d < A.window)) m |= 1ull << (a & 63);
       const int p = kept ? s_parent[a] : A.parents[r.x + a];
       a = p < a ? p : -1;
     }
@@ -119,7 +120,14 @@ extern "C" {
 
 int cx_tree_masks(const int32_t* parents, const int32_t* q_start, int32_t B, int32_t T,
                   uint64_t* mask, int32_t words, int32_t* depth, void* stream) {
+  return cx_tree_masks_window(parents, q_start, B, T, mask, words, depth, 0, stream);
+}
+
+int cx_tree_masks_window(const int32_t* parents, const int32_t* q_start, int32_t B, int32_t T,
+                         uint64_t* mask, int32_t words, int32_t* depth, int32_t window,
+                         void* stream) {
   if (B < 0 || T < 0 || words < 1) return cx::api_fail(CX_EINVAL, "bad shape");
+  if (window < 0) return cx::api_fail(CX_EINVAL, "window must be >= 0");
   if (!q_start && T != B)
     return cx::api_fail(CX_EINVAL, "without q_start there is one node per sequence");
   if (B == 0 || T == 0) return CX_OK;
@@ -130,6 +138,7 @@ int cx_tree_masks(const int32_t* parents, const int32_t* q_start, int32_t B, int
   A.B = B; A.T = T; A.words = words;
   A.mask = mask;
   A.depth = depth;
+  A.window = window;
   cx::timed_launch(CX_KERNEL_TREE_WALK, cx::tree_masks, dim3(B), dim3(256), 0, (hipStream_t)stream, A);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return cx::api_fail(CX_EHIP, "tree masks launch: %s", hipGetErrorString(e));

@@ -371,7 +371,7 @@ size_t cx_paged_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int
  * slot before them and to the nodes whose bits its mask has, in any order (its own
  * bit too, if it attends to itself).  A window w leaves of the slots before them
  * those whose position is above kv_len[b] - n + depth - w; nodes go by the mask
- * alone.
+ * alone (cx_tree_masks_window leaves out those that the window has passed).
  *
  *  mask       [T, mask_words], at most CX_TREE_MAX_WORDS: bit i % 64 of word i / 64 of a token's row is node i;
  *             nodes past the words are not attended to
@@ -404,6 +404,15 @@ size_t cx_tree_attention_workspace_bytes(int32_t q_heads, int32_t kv_heads, int3
  */
 int cx_tree_masks(const int32_t* parents, const int32_t* q_start, int32_t B, int32_t T,
                   uint64_t* mask, int32_t words, int32_t* depth, void* stream);
+
+/*
+ * The same for attention with a window: a mask has the bits of the node and of its
+ * window - 1 nearest ancestors, those whose positions are above its own less window
+ * (0: of all).  Depths count all ancestors.
+ */
+int cx_tree_masks_window(const int32_t* parents, const int32_t* q_start, int32_t B, int32_t T,
+                         uint64_t* mask, int32_t words, int32_t* depth, int32_t window,
+                         void* stream);
 
 /*
  * The path of a tree that the sampled ids follow.  Node 0 is the last confirmed

@@ -13,16 +13,19 @@ import numpy as np
 from .paged_ref import U16, U32
 
 
-def masks(parents, words: int):
-    """(mask [n, words] uint64, depth [n]) of one tree."""
+def masks(parents, words: int, window: int = 0):
+    """(mask [n, words] uint64, depth [n]) of one tree: the bits of a node and of its
+    ancestors, with a window of those whose depth is above the node's less the window."""
     n = len(parents)
     m, d = np.zeros((n, words), np.uint64), np.zeros(n, np.int64)
+    way = []
     for i, p in enumerate(parents):
-        if 0 <= p < i:
-            m[i] = m[p]
-            d[i] = d[p] + 1
-        if i < 64 * words:
-            m[i, i // 64] |= np.uint64(1) << np.uint64(i % 64)
+        up = way[p] if 0 <= p < i else []
+        way.append([*up, i])
+        d[i] = len(up)
+        for j in way[i]:
+            if j < 64 * words and (not window or d[j] > d[i] - window):
+                m[i, j // 64] |= np.uint64(1) << np.uint64(j % 64)
     return m, d
 
 

@@ -1,5 +1,5 @@
 """Calls of the tree operators that their documentation allows at its edges: tables
-without columns, paths that stop."""
+without columns, paths that stop, windows."""
 from __future__ import annotations
 
 import numpy as np
@@ -8,6 +8,8 @@ import pytest
 import paged_cases as C
 import tree_cases as X
 from oracle import paged_ref as R
+from oracle import tree_ref as Q
+from oracle.bf16 import bf16_bits_to_f32
 from test_gpu_tree import _commit_inputs, _mask
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +106,40 @@ def test_a_cache_keeps_what_was_moved(cache):
                 at, frm = 21 + j, 21 + row[j]
                 for a, b in zip(now, old):
                     assert (a[pages[at // 16], :, at % 16] == b[had[frm // 16], :, frm % 16]).all()
+
+
+@pytest.mark.parametrize("new,words,kind", [([1], 1, "tree"), ([64, 65, 0, 63], 2, "tree"), ([130], 1, "chain"),
+                                            ([2100, 5], 33, "tree"), ([70, 200], 4, "chain")])
+@pytest.mark.parametrize("window", [1, 2, 7, 64, 65, 1 << 30])
+def test_masks_of_a_window(new, words, kind, window):
+    from chenxing_amd._lib import tree_masks_device
+    rng = np.random.default_rng(sum(new) + window % 97)
+    par = [X.parents(rng, n, kind) for n in new]
+    want = [Q.masks(p, words, window) for p in par]
+    start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    m, d = tree_masks_device(C.to_gpu(np.array(sum(par, []), np.int32)), C.to_gpu(start), words, window)
+    assert (m.cpu().numpy().view(np.uint64) == np.concatenate([a for a, _ in want])).all()
+    assert (d.cpu().numpy() == np.concatenate([a for _, a in want])).all()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("wide", [0, 4096], ids=["short_table", "long_table"])
+@pytest.mark.parametrize("window", [1, 7, 33, 64])
+def test_chains_deeper_than_their_window(cache, wide, window):
+    """A chain is the causal operator's round, window and all."""
+    from chenxing_amd._lib import paged_attention_device, tree_attention_device, tree_masks_device
+    X.ATTEND["tmp"] = (cache, 8, 2, 128, 16, [60, 200, 64, 40], [50, 64, 64, 1], 1, window, 0.0, "chain")
+    x = X.attend_inputs("tmp", window)
+    del X.ATTEND["tmp"]
+    x = X.widen(x, wide)
+    par = C.to_gpu(np.concatenate([np.arange(-1, n - 1) for n in x["new"]]).astype(np.int32))
+    args = [C.to_gpu(x[k]) for k in ("q", "pages", "table", "kv_len")]
+    start = C.to_gpu(x["q_start"])
+    mask, depth = tree_masks_device(par, start, window=window)
+    got = tree_attention_device(*args, mask, start, depth, 64, window=window)
+    causal = paged_attention_device(*args, start, 64, window=window)
+    K, V = R.unpack(x["pages"], 128)
+    want, tol = R.attend(bf16_bits_to_f32(x["q"]).astype(np.float64), K, V, x["table"], x["kv_len"],
+                         x["q_start"], 16, 128 ** -0.5, window)
+    for o in (got, causal):
+        assert (np.abs(bf16_bits_to_f32(C.bits_of(o)) - want) <= tol).all()

@@ -12,6 +12,7 @@ torch = pytest.importorskip("torch")
 
 from chenxing_amd import _lib                                        # noqa: E402
 from conftest import ROOT                                            # noqa: E402
+from oracle import tree_ref as Q                                     # noqa: E402
 
 built = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libcx_sampler.so not built")
 
@@ -156,3 +157,22 @@ def test_commit_keeps_what_was_moved(monkeypatch, row, stays):
     path = _ids([0, 5, -1], row)
     assert c.commit([a, b], batch, path, _ids(2, 3)) == [2, stays]
     assert len(calls) == 1 and [c.length(a), c.length(b)] == [16, 21 + stays]
+
+
+# ------------------------------------------------------------------ masks of a window
+@built
+@pytest.mark.parametrize("bad", [dict(window=-1), dict(B=-1), dict(words=0), dict(parents=0), dict(start=0)],
+                         ids=str)
+def test_bad_window_masks(bad):
+    d = dict(parents=1 << 20, start=1 << 20, B=2, T=9, mask=1 << 20, words=1, depth=1 << 20, window=3)
+    d.update(bad)
+    assert _lib.load().cx_tree_masks_window(*d.values(), None) == _lib.CX_EINVAL
+
+
+def test_oracle_window_masks():
+    m, d = Q.masks([-1, 0, 0, 1, 3, 2, 4], 1, 3)
+    assert m[:, 0].tolist() == [1, 3, 5, 11, 2 + 8 + 16, 1 + 4 + 32, 8 + 16 + 64]
+    assert d.tolist() == [0, 1, 1, 2, 3, 2, 4]
+    for w in (0, 5, 100):
+        assert (Q.masks([-1, 0, 0, 1, 3, 2, 4], 1, w)[0] == Q.masks([-1, 0, 0, 1, 3, 2, 4], 1)[0]).all()
+    assert (Q.masks([-1, 0, 1], 1, 1)[0][:, 0] == [1, 2, 4]).all()
