@@ -40,15 +40,33 @@ def weights(codes, scale, shift=None):
 
 
 def linear(x, codes, scale, shift=None, bf16=False):
-    """(y [M, N], bound on a device result's error): fp32 sums, in any order, of the
-    terms 16 s (1 + q / 16) x and (t - 16 s) x."""
+    """(y [M, N], bound on a device result's error).
+
+    y / 16 = sum over groups g of s_g P_g + t_g H_g, with P_g = sum x (1 + q / 16) - c
+    sum x and H_g = sum x / 16 of the group's k; c = 1, without shifts 1.5 and t = 0.
+    The products of bf16 are exact in fp32.  In whatever order a group's are summed,
+    each of them passes through one addition at least, so that at most 2 group
+    additions' roundings, of partial sums below A_g = sum |x| (1 + q / 16 + c), are in
+    P_g, and group, below sum |x| / 16, in H_g.  Each group enters the sum of groups with
+    two roundings, and that may be split into 8 which add up with 7 more: of partial
+    sums below the sum of the groups' |s P| + |t H|, which do not grow as the sums of
+    magnitudes do.  (1.01: the roundings' own products.)"""
     N, K = codes.shape
+    M, groups = x.shape[0], scale.shape[1]
+    g = K // groups
     y = x @ weights(codes, scale, shift).T
-    s = np.repeat(np.abs(scale.astype(np.float64)), K // scale.shape[1], 1)
-    t = 8 * s if shift is None else np.repeat(np.abs(shift.astype(np.float64)), K // scale.shape[1], 1)
-    mag = np.abs(x) @ (s * (codes + 16.0) + t + 16 * s).T
-    # K products (exact) and their sums, a group's two scalings and sums
-    tol = (K + 2 * scale.shape[1] + 8) * U32 * mag + 1e-38
+    s = np.abs(scale.astype(np.float64)).T
+    t = np.zeros_like(s) if shift is None else np.abs(shift.astype(np.float64)).T
+    c = 1.5 if shift is None else 1.0
+    inside, between = np.zeros((M, N)), np.zeros((M, N))
+    for i in range(groups):                    # (a group at a time: M N K values are many)
+        xg = x[:, i * g:(i + 1) * g]
+        v = 1 + codes[:, i * g:(i + 1) * g].T / 16.0
+        mag = np.abs(xg)
+        inside += 2 * g * s[i] * (mag @ (v + c)) + g * t[i] * mag.sum(1, keepdims=True) / 16
+        between += s[i] * np.abs(xg @ (v - c)) + t[i] * np.abs(xg.sum(1, keepdims=True)) / 16
+    between += U32 * 1.01 * inside
+    tol = 16 * U32 * 1.01 * (inside + (2 * groups + 7) * between) + 1e-38
     if bf16:
         tol = tol + U16 * 1.01 * (np.abs(y) + tol)
     return y, tol
