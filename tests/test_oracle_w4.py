@@ -8,6 +8,7 @@ import pytest
 from oracle import w4_ref as R
 from oracle.bf16 import bf16_bits_to_f32
 from test_gpu_w4 import SIZES, _inputs
+from test_gpu_w4_depths import DEEP
 
 
 def _case(M, N, K, group, shift):
@@ -17,7 +18,7 @@ def _case(M, N, K, group, shift):
 
 
 @pytest.mark.parametrize("shift", [False, True])
-@pytest.mark.parametrize("M,N,K,group", SIZES)
+@pytest.mark.parametrize("M,N,K,group", sorted({*SIZES, *DEEP}))
 def test_a_lost_piece_passes_the_bound(M, N, K, group, shift):
     """32 k of one group, or a tile of 128, left out or taken twice: more than half of all
     results are further off than the bound, in fp32 and in bf16."""
