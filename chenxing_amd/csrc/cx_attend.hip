@@ -26,7 +26,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "cx_device.hpp"
@@ -1067,7 +1069,8 @@ int cx_paged_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_
   A.q_heads = q_heads;
   A.cap = softcap > cx::ATT_CAP ? 2 : softcap > 0;
   const double log2e = 1.4426950408889634;
-  A.s1 = (float)(scale * log2e);
+  // (0 times a masked score's infinity would be NaN)
+  A.s1 = std::max((float)(scale * log2e), std::numeric_limits<float>::min());
   A.s2 = (float)(softcap * log2e);
   A.s3 = A.cap ? (float)(2 * scale / softcap * log2e) : 0.f;
   A.s4 = A.cap ? (float)(scale / softcap) : 0.f;

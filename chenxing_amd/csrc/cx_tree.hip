@@ -27,6 +27,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "cx_device.hpp"
@@ -1094,7 +1095,8 @@ int cx_tree_attention_bf16(const cx_kv_batch* kv, const uint16_t* q, int64_t q_t
   A.depth = depth;
   A.cap = softcap > 0 && !std::isinf(softcap);
   const double log2e = 1.4426950408889634;
-  A.s1 = (float)(scale * log2e);
+  // (0 times a masked score's infinity would be NaN)
+  A.s1 = std::max((float)(scale * log2e), std::numeric_limits<float>::min());
   A.s2 = A.cap ? (float)(softcap * log2e) : 0.f;
   A.s3 = A.cap ? (float)(2 * scale / softcap * log2e) : 0.f;
   A.s4 = A.cap ? (float)(scale / softcap) : 0.f;

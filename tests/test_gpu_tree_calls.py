@@ -1,5 +1,5 @@
 """Calls of the tree operators that their documentation allows at its edges: tables
-without columns, paths that stop, windows."""
+without columns, paths that stop, windows, scales that vanish."""
 from __future__ import annotations
 
 import numpy as np
@@ -9,8 +9,8 @@ import paged_cases as C
 import tree_cases as X
 from oracle import paged_ref as R
 from oracle import tree_ref as Q
-from oracle.bf16 import bf16_bits_to_f32
-from test_gpu_tree import _commit_inputs, _mask
+from oracle.bf16 import bf16_bits_to_f32, f32_to_bf16_bits
+from test_gpu_tree import _attend, _commit_inputs, _mask
 
 pytestmark = pytest.mark.gpu
 
@@ -142,4 +142,25 @@ def test_chains_deeper_than_their_window(cache, wide, window):
     want, tol = R.attend(bf16_bits_to_f32(x["q"]).astype(np.float64), K, V, x["table"], x["kv_len"],
                          x["q_start"], 16, 128 ** -0.5, window)
     for o in (got, causal):
+        assert (np.abs(bf16_bits_to_f32(C.bits_of(o)) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("wide", [0, 4096], ids=["short_table", "long_table"])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_scales_below_the_range_of_fp32(wide, softcap):
+    """All scores are alike then: a row is the mean of what it attends to."""
+    from chenxing_amd._lib import paged_attention_device
+    x = X.widen(X.attend_inputs("edges", 4), wide)
+    x["softcap"] = softcap
+    K, V = R.unpack(x["pages"], x["D"])
+    q = bf16_bits_to_f32(x["q"]).astype(np.float64)
+    for scale in (1e-46, 1e-60):
+        want, tol = Q.attend(q, K, V, x["table"], x["kv_len"], x["q_start"], x["mask"], x["depth"], x["P"],
+                             scale, 0, softcap)
+        got = bf16_bits_to_f32(_attend(x, scale=scale))
+        assert (np.abs(got - want) <= tol).all()
+        o = paged_attention_device(C.to_gpu(x["q"]), C.to_gpu(x["pages"]), C.to_gpu(x["table"]),
+                                   C.to_gpu(x["kv_len"]), C.to_gpu(x["q_start"]), max(x["new"]),
+                                   scale=scale, softcap=softcap)
+        want, tol = R.attend(q, K, V, x["table"], x["kv_len"], x["q_start"], x["P"], scale, 0, softcap)
         assert (np.abs(bf16_bits_to_f32(C.bits_of(o)) - want) <= tol).all()
