@@ -651,14 +651,14 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         // two bf16 parts: the first cut off, the second never 0, so that an infinite
-        // value keeps its sign in both products (2^-20 of a term too much)
+        // value keeps its sign in both products (2^-23 of a term too much)
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
           const float p0 = p[nt][y][2 * d], p1 = p[nt][y][2 * d + 1];
           const uint32_t x0 = __float_as_uint(p0), x1 = __float_as_uint(p1);
           ph[nt][2 * y + d] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
-          pl[nt][2 * y + d] = pack_bf16(fmaf(p0, 1.f + 0x1p-20f, -__uint_as_float(x0 & 0xFFFF0000u)),
-                                        fmaf(p1, 1.f + 0x1p-20f, -__uint_as_float(x1 & 0xFFFF0000u)));
+          pl[nt][2 * y + d] = pack_bf16(fmaf(p0, 1.f + 0x1p-23f, -__uint_as_float(x0 & 0xFFFF0000u)),
+                                        fmaf(p1, 1.f + 0x1p-23f, -__uint_as_float(x1 & 0xFFFF0000u)));
         }
       }
     }

@@ -164,3 +164,40 @@ def test_scales_below_the_range_of_fp32(wide, softcap):
                                    scale=scale, softcap=softcap)
         want, tol = R.attend(q, K, V, x["table"], x["kv_len"], x["q_start"], x["P"], scale, 0, softcap)
         assert (np.abs(bf16_bits_to_f32(C.bits_of(o)) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("wide", [1, 1 << 16], ids=["short_table", "long_table"])
+@pytest.mark.parametrize("heads", [2, 40], ids=["few_rows", "many_rows"])
+def test_terms_are_not_too_large(cache, D, wide, heads):
+    """Terms of 1 and 2^-13 and values of 1 and 33: (1 + 33 2^-13) / (1 + 2^-13) lies 2^-21
+    below the middle of 1 and 1 + 2^-7, neighbours in bf16, and goes to 1.  Both sums are
+    exact in fp32, the division and the product with it round by 2^-25 and 2^-24: a result
+    goes elsewhere only where the terms are more than 2^-22 too large."""
+    import torch
+    from chenxing_amd._lib import tree_attention_device
+    P, nodes = 16, 16
+    E = 8 if cache == "bf16" else 16
+    ka, va = R._at(P, D, E, 1, np.arange(D))
+    _, v0 = R._at(P, D, E, 0, np.arange(D))
+    pages = np.zeros((2, 1, 2 * P * D if cache == "bf16" else 2 * P * D + 8 * P),
+                     np.uint16 if cache == "bf16" else np.uint8)
+    if cache == "bf16":
+        bits = f32_to_bf16_bits(np.array([1, 33], np.float32))
+        pages[0, 0, ka[0]], pages[0, 0, v0], pages[0, 0, va] = bits[0], bits[0], bits[1]
+    else:                                          # codes of 1, and scales
+        pages[0, 0, ka[0]] = pages[0, 0, v0] = pages[0, 0, va] = 0x38
+        scales = np.ones(2 * P, np.float32)
+        scales[P + 1] = 33
+        pages[0, 0, 2 * P * D:] = scales.view(np.uint8)
+    table = np.full((1, max(2, wide // P)), -1, np.int32)
+    table[0, :2] = [0, 1]
+    q = torch.zeros(nodes, heads, D, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = -13
+    o = tree_attention_device(q, C.to_gpu(pages), C.to_gpu(table),
+                              torch.tensor([2 + nodes], dtype=torch.int32, device="cuda"),
+                              torch.zeros(nodes, 1, dtype=torch.int64, device="cuda"),
+                              torch.tensor([0, nodes], dtype=torch.int32, device="cuda"), max_new=nodes,
+                              scale=1 / 1.4426950408889634)
+    assert (o == 1).all()
