@@ -36,7 +36,9 @@ def pack(codes, scale, shift=None):
         # [tile, row, k tile, word, lane group, pair, odd]; no two codes share a bit
         x = (x.view(n, 16, k128, 4, 4, 4, 2) << at).sum((5, 6), dtype=torch.int32)
         tiles[i // 16:i // 16 + n] = x.permute(0, 2, 4, 1, 3).reshape(n, k128, 64, 4)
-    both = scale[..., None] if shift is None else torch.stack([scale, shift.to(scale.dtype)], 2)
+    both = scale.half()[..., None] if shift is None else torch.stack([scale.half(), shift.half()], 2)
+    if not bool(torch.isfinite(both).all()):
+        raise ValueError("scale and shift must be finite, and in the range of float16")
     laid = torch.zeros(16 * n16, *both.shape[1:], dtype=torch.float16, device=codes.device)
     laid[:N] = both
     laid = laid.view(n16, 16, *both.shape[1:]).transpose(1, 2).contiguous()

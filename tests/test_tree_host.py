@@ -176,3 +176,28 @@ def test_oracle_window_masks():
     for w in (0, 5, 100):
         assert (Q.masks([-1, 0, 0, 1, 3, 2, 4], 1, w)[0] == Q.masks([-1, 0, 0, 1, 3, 2, 4], 1)[0]).all()
     assert (Q.masks([-1, 0, 1], 1, 1)[0][:, 0] == [1, 2, 4]).all()
+
+
+# ------------------------------------------------------------------ 4-bit weights
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf"), 65520.0, -1e30])
+@pytest.mark.parametrize("which", ["scale", "shift"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+def test_pack_refuses_what_float16_does_not_hold(value, which, dtype):
+    """Scales and shifts are kept as float16: one beyond it would make a row of W infinite."""
+    from chenxing_amd import w4
+    d = dict(scale=torch.ones(20, 2, dtype=dtype), shift=torch.ones(20, 2, dtype=dtype))
+    w4.pack(torch.zeros(20, 64, dtype=torch.uint8), **d)
+    d[which][17, 1] = value
+    with pytest.raises(ValueError, match="float16"):
+        w4.pack(torch.zeros(20, 64, dtype=torch.uint8), **d)
+
+
+def test_pack_takes_the_largest_of_float16():
+    from chenxing_amd import w4
+    scale = torch.full((1, 1), -65504.0)
+    _, laid = w4.pack(torch.zeros(1, 32, dtype=torch.uint8), scale, -scale)
+    assert laid[0, 0, 0].tolist() == [-65504.0, 65504.0]
+    # a wider shift is rounded once, not to the scale's type first
+    _, laid = w4.pack(torch.zeros(1, 32, dtype=torch.uint8), torch.ones(1, 1, dtype=torch.bfloat16),
+                      torch.full((1, 1), 1 + 2.0 ** -9))
+    assert laid[0, 0, 0].tolist() == [1.0, 1 + 2.0 ** -9]
