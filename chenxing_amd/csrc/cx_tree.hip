@@ -41,14 +41,18 @@
 namespace cx {
 
 constexpr int TREE_WAVES = 8, TREE_WG = 64 * TREE_WAVES;
-constexpr int TREE_WORKERS = 256;            // a workgroup a CU
+constexpr int TREE_WORKERS = 256;            // a workgroup a CU: they are on the chip at once
 constexpr int TREE_UNIT = 32;                // slots of a unit
 constexpr int TREE_LEAST = 2;                // the least share, in units
-// Units of a workgroup's chunk at most: one request of 716 tokens 13.5 us in chunks, 17.2
-// in shares; 19 requests in a window of 1024 33 us in shares, 38 and 49 in chunks of 12
-// and 17 units.
-constexpr int TREE_CHUNK = 24;
-constexpr int64_t TREE_SPREAD = 512;         // workgroups of chunks that are aimed at
+// Units of a workgroup's chunk at most, and workgroups of chunks that are aimed at: those
+// that are on the chip at once.  32 q / 8 kv heads of 128, bf16, chunks and shares, us: one
+// request, 16 nodes, of 700 tokens 13.8 and 17.2, of 6000 22 and 27; four of 1500 18.3 and
+// 22.3; 16 of 700 22.8 and 28.5.  Past 16 units a chunk gains where lengths are alike (16
+// requests of 1500, chunks of 24: 32 and 38) and loses more where they are not (16 of 50 ..
+// 1500, 1 .. 64 nodes: 49 and 36).  Twice the workgroups, in two turns: 16 requests of 500 ..
+// 1500, 1 .. 33 nodes, 64 us, in shares 39; one of 6000 36, not 22.
+constexpr int TREE_CHUNK = 16;
+constexpr int64_t TREE_SPREAD = TREE_WORKERS;
 constexpr int TREE_BATCH = 512;              // sequences of a launch: their lengths are in LDS
 // A lane's terms of a unit sum to this before the running maximum is raised: it need not
 // be the largest score, so most units look for none (64 trees of 64 nodes 440 us, with the
