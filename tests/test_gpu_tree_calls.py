@@ -10,7 +10,7 @@ import tree_cases as X
 from oracle import paged_ref as R
 from oracle import tree_ref as Q
 from oracle.bf16 import bf16_bits_to_f32, f32_to_bf16_bits
-from test_gpu_tree import _attend, _commit_inputs, _mask
+from test_gpu_tree import _attend, _check, _commit_inputs, _mask
 
 pytestmark = pytest.mark.gpu
 
@@ -201,3 +201,31 @@ def test_terms_are_not_too_large(cache, D, wide, heads):
                               torch.tensor([0, nodes], dtype=torch.int32, device="cuda"), max_new=nodes,
                               scale=1 / 1.4426950408889634)
     assert (o == 1).all()
+
+
+def test_rows_do_not_depend_on_the_workspace():
+    """Any contents of the workspace: NaN, ones, another call's; in shares and in chunks."""
+    from chenxing_amd import _lib
+    for name, wide in (("long_and_short", 0), ("long_and_short", 16384), ("edges_e4m3", 4096), ("full", 0)):
+        x = X.widen(X.attend_inputs(name, 12), wide)
+        want = _attend(x)
+        for byte in (0xFF, 0x7F, 0x01):
+            for buf in _lib._ws_tree.bufs.values():
+                buf.fill_(byte)
+            assert (_attend(x) == want).all(), (name, wide, byte)
+        _attend(X.attend_inputs("words"))
+        assert (_attend(x) == want).all()
+
+
+@pytest.mark.parametrize("cache,D", [("bf16", 64), ("e4m3", 128)])
+@pytest.mark.parametrize("B", [1, 31, 32, 33])
+@pytest.mark.parametrize("tokens", [511, 512, 513, 1500])
+def test_on_both_sides_of_the_chunks(cache, D, B, tokens):
+    """256 workgroups and more, 16 units and more, in tables as long as the longest."""
+    rng = np.random.default_rng(B * tokens + D)
+    lens = [tokens] + rng.integers(1, tokens, B - 1).tolist()
+    new = [int(rng.integers(1, min(n, 5) + 1)) for n in lens]
+    X.ATTEND["tmp"] = (cache, 8, 8, D, 16, lens, new, 1, 0, 0.0, "tree")
+    x = X.attend_inputs("tmp", B)
+    del X.ATTEND["tmp"]
+    _check(x, _attend(x))
