@@ -179,28 +179,35 @@ class PagedKVCache:
             raise ValueError("commit takes each sequence of the batch once, and path [sequences, width] "
                              "and count [sequences] on the pool's device")
         # in one copy to the host, what the moves go by
-        parts = [count, batch["kv_len"], table, path, *([] if start is None else [start])]
-        host = torch.cat([t.flatten() for t in parts]).cpu().numpy()
-        kept, lens, held, way, first = np.split(host, np.cumsum([B, B, B * M, B * width]))
-        kept, held, way = kept.tolist(), held.reshape(B, M), way.reshape(B, width)
-        new = [1] * B if start is None else np.diff(first).tolist()
-        if any(not 0 <= c <= min(n, width, self._seqs[s][1]) for s, c, n in zip(seqs, kept, new)):
-            raise ValueError("count must be in [0, new tokens of the sequence], and path that wide")
-        for s, n, row in zip(seqs, lens, held):
+        parts = [count, batch["kv_len"], path.flatten(), table.flatten()]
+        host = torch.cat(parts if start is None else [*parts, start]).cpu().numpy()
+        way = host[2 * B:(2 + width) * B].reshape(B, width)
+        held, ends = host[(2 + width) * B:], host[(2 + width + M) * B:]
+        kept, lens = host[:B].tolist(), host[B:2 * B].tolist()
+        new = [1] * B if start is None else (ends[1:] - ends[:-1]).tolist()
+        P, at, now, written = self.page_tokens, [], [], []
+        for i, (s, c, n, was) in enumerate(zip(seqs, kept, new, lens)):
             pages, length = self._seqs[s]
-            if n != length or row[:len(pages)].tolist() != pages:
-                raise ValueError("the sequences' lengths or pages are not those of the batch")
-        for s, c, n in zip(seqs, kept, new):
-            pages, length = self._seqs[s]
-            first, end = length - n, length - n + c
-            if c and any(self._refs[p] > 1 for p in pages[first // self.page_tokens:
-                                                          -(-end // self.page_tokens)]):
-                raise ValueError("commit moves tokens in pages that another sequence holds too: "
-                                 "commit first, then fork")
-        _lib.kv_commit_device(self.pool, self._head_dim, table, batch["kv_len"], path, count, start,
-                              self.page_tokens)
-        rises = (np.diff(way, axis=1, prepend=-1) > 0) & (way < np.reshape(new, (B, 1)))
-        if not (rises | (np.arange(width) >= np.reshape(kept, (B, 1)))).all():
+            if not 0 <= c <= min(n, width, length):
+                raise ValueError("count must be in [0, new tokens of the sequence], and path that wide")
+            p0, p1 = (length - n) // P, len(pages)
+            if was != length or p1 > M:
+                raise ValueError("the sequences' lengths are not those of the batch")
+            at += range(i * M + p0, i * M + p1)
+            now += pages[p0:]
+            if c:
+                written += pages[p0:-(-(length - n + c) // P)]
+        if held[at].tolist() != now:
+            raise ValueError("the sequences' pages are not those of the batch")
+        if any(self._refs[p] > 1 for p in written):
+            raise ValueError("commit moves tokens in pages that another sequence holds too: "
+                             "commit first, then fork")
+        _lib.kv_commit_device(self.pool, self._head_dim, table, batch["kv_len"], path, count, start, P)
+        moved = np.arange(width) < host[:B, None]
+        rises = way < np.reshape(new, (B, 1))
+        rises[:, :1] &= way[:, :1] >= 0
+        rises[:, 1:] &= way[:, 1:] > way[:, :-1]
+        if (moved & ~rises).any():             # the device has marked where those rows end
             kept = [min(c, [*row, -1].index(-1)) for row, c in zip(path.tolist(), kept)]
         for s, c, n in zip(seqs, kept, new):
             self.truncate(s, self._seqs[s][1] - n + c)
