@@ -772,7 +772,8 @@ def w4_linear_device(x, tiles, scales, N, dtype=None, out=None):
     [M, N] of ``dtype`` (float32, the default, or bfloat16) or in ``out``.
 
     ``tiles`` and ``scales`` as ``w4.pack`` lays them out (include/cx_sampler.h
-    has the format); the weights are read once for up to 64 rows of x."""
+    has the format).  The weights are read once for every 64 rows of x, or every 32
+    where N is small (up to 2048 for 64 rows)."""
     import torch
     lib = _lib or load()
     dev = x.get_device()

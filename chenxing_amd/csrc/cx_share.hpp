@@ -131,7 +131,9 @@ struct AttendLine {
   // what a row block costs beside its units, in units (64 ragged requests 99, 94
   // and 93 us with 0, 1 and 2; 32 verify rounds 48, 42, 39 and 35 us with 0 .. 3).  Trees,
   // whose workgroups take a unit or more a step: 32 ragged ones 84, 64, 55, 54 and 58 us
-  // with 2, 4, 6, 9 and 14, 64 full ones in row blocks of 256 484, 456, 439, 443 and 459
+  // with 2, 4, 6, 9 and 14, 64 full ones in row blocks of 256 484, 456, 439, 443 and 459.
+  // Ragged ones of 1 .. 64 nodes with 4, 9 and 16: 8 up to 4096 tokens 40 in each, 32 of them
+  // 84, 65 and 69, 16 up to 16000 126, 118 and 119, 100 up to 1500 114, 103 and 102
   static constexpr int PIECE = TREE ? (NT < 16 ? 9 : 6) : NT == 1 ? 2 : 4;
 
   // The sequence of new tokens tok0 .. end - 1 and len tokens in all.

@@ -19,7 +19,7 @@
 // K and V are read once for up to 256 rows, so trees of 64 nodes are bound by the matrix
 // cores (with the terms in two parts half as much again as the formula's products) and by
 // the softmax beside them: 2 sequences of 120001 .. 131072 tokens, 32 / 8 heads of 128,
-// bf16, 444 us, 587 TFLOP/s of the formula's; 64 of up to 8192, e4m3, 434 us.  Few rows are
+// bf16, 445 us, 586 TFLOP/s of the formula's; 64 of up to 8192, e4m3, 433 us.  Few rows are
 // bound by the start, a step's latency (1.2 us at D = 128) and a row block's own cost (about
 // 5 us: its rows, the groups' meeting, its part): 32 ragged trees of up to 33 nodes 52 us.
 #include <hip/hip_runtime.h>
@@ -655,7 +655,10 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         // two bf16 parts: the first cut off, the second never 0, so that an infinite
-        // value keeps its sign in both products (2^-23 of a term too much)
+        // value keeps its sign in both products (2^-23 of a term too much).  That is 2^-16
+        // of a term, and 0.3 to 0.5 % of the results are the other neighbour of what 64
+        // bits give, where a third part's products leave 0.03 to 0.1 % and take 518 us for
+        // 2 documents of 131072 tokens, not 445, 485 for 64 full trees, not 433
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
           const float p0 = p[nt][y][2 * d], p1 = p[nt][y][2 * d + 1];
@@ -966,8 +969,11 @@ __global__ __launch_bounds__(256) void tree_join_chunks(TreeArgs A) {
 }
 
 // Rows of a row block: the least of those that hold a sequence's on average (32 ragged
-// trees of 14 nodes, 4 heads a kv head: 64 us with 64 rows, 70 with 128; D = 256, e4m3, 2
-// heads a kv head, 13 nodes: 34.0 us with 32, 38.3 with 64).
+// trees of 14 nodes, 4 heads a kv head: 64 us with 64 rows, 70 with 128).  D = 256, e4m3, 2
+// heads a kv head, 4 kv heads, with 32 and with 64 rows: 64 requests up to 3000 tokens of 8
+// rows a sequence on average 48 and 59, of 26 58 and 57, of 32 69 and 65, of 60 97 and 81;
+// 19 up to 6000 of 13 34.5 and 38.4, of 60 50 and 53; four up to 20000, whose few row blocks
+// leave the chip to their units' shares, 56 and 69, 41 and 65 of 32, 45 and 63 of 60.
 static int tree_rows(int64_t rows, int D, bool f8) {
   if (D == 256) return rows <= 32 && f8 ? 32 : rows <= 64 ? 64 : 128;  // (32 of bf16: the ring passes LDS)
   return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;

@@ -38,13 +38,15 @@ struct W4Args {
   int bf16;                   // out is
 };
 
-// Tiles of codes that a wave has asked for: 4 are no faster in any case (72 against 65 us at
-// 16 rows, N = 128256, K = 4096; 36 against 22 at 61 rows, N = 14336).
+// Tiles of codes that a wave has asked for, 2 and 4 (K = 4096, us, weights from memory): 1 row
+// N = 4096 7.9 and 8.0, N = 14336 11.0 and 12.3; 16 rows N = 14336 12.8 and 14.5, N = 128256
+// 71.3 and 72.8; 61 rows N = 14336 21.7 and 23.0.
 constexpr int W4_AHEAD = 2;
 // The waves that a product should have, of the chip's 8192: two of a SIMD keep enough loads
-// in flight, and each further one has less work for its x and its sums.  16 rows, K = 4096,
-// with 2004 and twice as many waves: N = 128256 60 and 70 us; N = 14336 with 1792, half,
-// a quarter: 11.4, 16.4, 26.0 us.
+// in flight, and each further one has less work for its x and its sums.  K = 4096, us, with
+// 768, 1536 and 3072 (weights from memory): 16 rows, N = 6144 11.4, 9.1, 12.9; N = 14336 17.3,
+// 12.8, 15.2; N = 50257 56, 35, 40; N = 128256 71, 71, 77; 61 rows, N = 14336 30.6, 21.7, 21.6;
+// 30 rows, N = 50257 56, 40, 36.
 constexpr int W4_WAVES = 1536;
 constexpr int W4_CUS = 256;
 // Rows of x so far apart that 16 of them pass 32 bits take the other kernel.

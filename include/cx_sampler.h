@@ -479,7 +479,8 @@ int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int
  *  group      32, 64 or 128; K a multiple of it; N, K < 2^28, M < 2^21
  *  out        [M, ldo] fp32, or bf16 bits if out_bf16
  * Rows of the last tile past N are read and not used.  The weights are read once for
- * up to 64 rows of x.  Device pointers, stream-ordered, no synchronisation, no
+ * up to 32 rows of x; 33 to 64 rows read them once where N is above 2048, else twice,
+ * and more rows as often as that many times 64 or 32.  Device pointers, stream-ordered, no synchronisation, no
  * allocation.
  */
 int cx_w4_linear_bf16(const uint16_t* x, int64_t ldx, const uint32_t* tiles,
