@@ -34,6 +34,7 @@
 #include "cx_dma.hpp"
 #include "cx_internal.hpp"
 #include "cx_kv.hpp"
+#include "cx_lanes.hpp"
 #include "cx_sampler.h"
 #include "cx_share.hpp"
 #include "cx_timing.hpp"
@@ -81,10 +82,6 @@ struct TreeArgs {
   float* part;                // [slots, ROWS, D], in the order of join's lanes
 };
 
-__device__ __forceinline__ uint64_t tree_scalar(uint64_t x) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
-         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
-}
 // The kernel's arguments in memory (its first, at the segment's start), for the parts
 // that run once a piece: what they need is read there again, so the loop keeps its
 // scalar registers.
@@ -99,23 +96,6 @@ __device__ __forceinline__ int rare_lane() {
   asm volatile("" : "+v"(l));
   return l;
 }
-// The largest, or the sum, of the four lane groups' values, in every group.
-__device__ __forceinline__ float tree_groups_max(float x) {
-  uint32_t a = __float_as_uint(x);
-  auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  a = __float_as_uint(x);
-  r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float tree_groups_sum(float x) {
-  uint32_t a = __float_as_uint(x);
-  auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
-  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  a = __float_as_uint(x);
-  r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 // Sequence b of a launch, its lengths by scalar loads.
 template <class Line>
 __device__ __forceinline__ AttendSeq tree_seq(const TreeArgs& A, int b) {
@@ -127,22 +107,7 @@ __device__ __forceinline__ AttendSeq tree_seq(const TreeArgs& A, int b) {
   return Line::seq(ShareBatch{A.G, A.kv.heads, A.window, A.kv.n_pages ? A.kv.M << A.kv.logP : 0}, s0, s1,
                    const_load(A.kv.kv_len + b));
 }
-// Eight e4m3 codes as bf16.
-__device__ __forceinline__ bf16x8 tree_e4m3x8(uint32_t a, uint32_t b) {
-  const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false);
-  const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
-  const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false);
-  const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
-  return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-}
-// The sign bits say which of two bf16 are NaN or infinite; a mask of the others.
-__device__ __forceinline__ uint32_t tree_nonfinite(uint32_t x) { return (x & 0x7F807F80u) + 0x00800080u; }
-__device__ __forceinline__ uint32_t tree_finite(uint32_t x) {
-  const uint32_t m = tree_nonfinite(x) & 0x80008000u;
-  return ~(m | (m - (m >> 15)));
-}
-
-// The same from a scalar base, and 4 bytes a lane.
+// load_lds16 from a scalar base, and 4 bytes a lane.
 __device__ __forceinline__ void load_lds16_at(const char* base, uint32_t at, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(to), "v"(at), "s"(base) : "memory", "m0");
@@ -261,10 +226,10 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     if (b < C.B) s_pref[b + 1] = x;
     if (tid == 0) s_pref[0] = 0;
     __syncthreads();
-    const uint64_t line = tree_scalar(s_pref[C.B]);
+    const uint64_t line = scalar64(s_pref[C.B]);
     split = share_split(line, TREE_WORKERS, TREE_LEAST);
-    split.per = tree_scalar(split.per);
-    split.more = tree_scalar(split.more);
+    split.per = scalar64(split.per);
+    split.more = scalar64(split.more);
     if (worker == 0 && tid == 0) *A.entries = split.by_block ? (int)line_blocks(line) : TREE_WORKERS;
     for (int b = blockIdx.x; b < C.B; b += TREE_WORKERS)
       if (s_pref[b + 1] == s_pref[b]) nothing(first(b), seqs.starts ? seqs.end(b) : first(b) + 1);
@@ -320,7 +285,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
                         joined |= j.last >= 0;
                         if (tid == 0) A.join[entry] = j;
                       });
-      u = tree_scalar(u);
+      u = scalar64(u);
       if (p.cnt == 0) return false;
     } else {
       // its chunk; then, where a sequence has more new tokens than the caller said, the
@@ -435,7 +400,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       if (wr + WR * j >= 2 * KB / 1024) break;                  // (uniform)
       const int f = (wr + WR * j) * 64 + l;
       const u32x4 x = *(const CX_LDS u32x4*)(raw + 16 * f);
-      const bf16x8 lo = tree_e4m3x8(x[0], x[1]), hi = tree_e4m3x8(x[2], x[3]);
+      const bf16x8 lo = e4m3x8(x[0], x[1]), hi = e4m3x8(x[2], x[3]);
       // K: chunk rows of 32 slots; V: of D dims
       const int fv = f - KB / 16;
       const int at = fv < 0 ? (f / 32 * 2) * 32 + f % 32 : 2 * KB / 16 + fv / D * 2 * D + fv % D;
@@ -540,7 +505,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       for (int x = 0; x < N; ++x)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const bf16x8 k = NARROW ? tree_e4m3x8(ka[x][y][0], ka[x][y][1]) : __builtin_bit_cast(bf16x8, ka[x][y]);
+          const bf16x8 k = NARROW ? e4m3x8(ka[x][y][0], ka[x][y][1]) : __builtin_bit_cast(bf16x8, ka[x][y]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             v[nt][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, __builtin_bit_cast(bf16x8, qr[nt][x0 + x]),
@@ -625,7 +590,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
         for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int j = 0; j < 4; ++j) top = fmaxf(top, to2 * v[nt][y][j]);
-        const float m1 = fmaxf(m[nt], tree_groups_max(top));
+        const float m1 = fmaxf(m[nt], groups_max(top));
         const float alpha = m[nt] == m1 ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m1);
         m[nt] = m1;
         sum[nt] *= alpha;
@@ -692,7 +657,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
 #pragma unroll
       for (int n = 0; n < EARLY; ++n) {
         x[n] = va[n];
-        if (NARROW) x[n] = __builtin_bit_cast(u32x4, tree_e4m3x8(x[n][0], x[n][1]));
+        if (NARROW) x[n] = __builtin_bit_cast(u32x4, e4m3x8(x[n][0], x[n][1]));
       }
       if (masked) {
         const int g = rare_lane() >> 4;
@@ -702,8 +667,8 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
           for (int d = 0; d < 4; ++d) {
             const uint32_t two = valid >> (8 * g + 2 * d);
             x[n][d] &= (two & 1 ? 0xFFFFu : 0) | (two & 2 ? 0xFFFF0000u : 0);
-            bad |= tree_nonfinite(x[n][d]);
-            x[n][d] &= tree_finite(x[n][d]);
+            bad |= nonfinite_sign<false>(x[n][d]);
+            x[n][d] &= finite_mask<false>(x[n][d]);
           }
       }
       if (n0 + EARLY < DT) {
@@ -813,7 +778,7 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
     const int l = rare_lane(), g = l >> 4, c = l & 15;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float L = tree_groups_sum(sum[nt]);
+      const float L = groups_sum(sum[nt]);
       const int r = 16 * (NT * wr + nt) + c;
       if (cur.slot < 0) {
         if (r >= cur.R) continue;
