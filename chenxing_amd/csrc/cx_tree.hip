@@ -621,9 +621,9 @@ __global__ __launch_bounds__(TREE_WG) void tree_split(TreeArgs A) {
       for (int y = 0; y < 2; ++y) {
         // two bf16 parts: the first cut off, the second never 0, so that an infinite
         // value keeps its sign in both products (2^-23 of a term too much).  That is 2^-16
-        // of a term, and 0.3 to 0.5 % of the results are the other neighbour of what 64
-        // bits give, where a third part's products leave 0.03 to 0.1 % and take 518 us for
-        // 2 documents of 131072 tokens, not 445, 485 for 64 full trees, not 433
+        // of a term, and 0.2 to 0.5 % of the results are the other neighbour of what 64
+        // bits round to, where a third part leaves 0.03 to 0.13 % and its products take 518
+        // us for 2 documents of 131072 tokens, not 445, and 485 for 64 full trees, not 433
 #pragma unroll
         for (int d = 0; d < 2; ++d) {
           const float p0 = p[nt][y][2 * d], p1 = p[nt][y][2 * d + 1];
