@@ -51,9 +51,12 @@ constexpr int TREE_LEAST = 2;                // the least share, in units
 // 22.3; 16 of 700 22.8 and 28.5.  Past 16 units a chunk gains where lengths are alike (16
 // requests of 1500, chunks of 24: 32 and 38) and loses more where they are not (16 of 50 ..
 // 1500, 1 .. 64 nodes: 49 and 36).  Twice the workgroups, in two turns: 16 requests of 500 ..
-// 1500, 1 .. 33 nodes, 64 us, in shares 39; one of 6000 36, not 22.
+// 1500, 1 .. 33 nodes, 64 us, in shares 39; one of 6000 36, not 22.  Row blocks, a chunk each,
+// may be twice the workgroups, no more: requests of 20 .. 500 tokens, 64 of 1 .. 16 nodes
+// (512 row blocks) 34 and 36, of 1 .. 33 nodes 24 (576) 28 and 29, 64 63 and 47, 256 232 and
+// 131.
 constexpr int TREE_CHUNK = 16;
-constexpr int64_t TREE_SPREAD = TREE_WORKERS;
+constexpr int64_t TREE_SPREAD = TREE_WORKERS, TREE_BLOCKS = 2 * TREE_WORKERS;
 constexpr int TREE_BATCH = 512;              // sequences of a launch: their lengths are in LDS
 // A lane's terms of a unit sum to this before the running maximum is raised: it need not
 // be the largest score, so most units look for none (64 trees of 64 nodes 440 us, with the
@@ -969,11 +972,11 @@ static int launch_tree(TreeArgs A, int64_t max_new, hipStream_t s) {
   // (a table without columns: one empty chunk, whose rows are 0)
   const int64_t units = std::max<int64_t>((span + TREE_UNIT - 1) / TREE_UNIT, 1);
   const int64_t tiles = (A.G * max_new + ROWS - 1) / ROWS, blocks = A.kv.B * A.kv.heads * tiles;
-  // Chunks where the longest context is short for the workgroups there are ..
+  // Chunks where the longest context is short for the workgroups that there are ..
   const int64_t most = tree_slots(ROWS) / blocks;               // parts of a row block at most
   int64_t chunks = std::max<int64_t>(std::min({TREE_SPREAD / blocks, most, (units + Sh::WT - 1) / Sh::WT}), 1);
   const int64_t chunk = (units + chunks - 1) / chunks;
-  if (chunk <= TREE_CHUNK) {
+  if (chunk <= TREE_CHUNK && blocks <= TREE_BLOCKS) {
     chunks = (units + chunk - 1) / chunk;
     A.tiles = (int)tiles;
     A.chunks = (int)chunks;

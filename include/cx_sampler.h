@@ -437,8 +437,9 @@ int cx_tree_accept(const int32_t* parents, const int32_t* tokens, const int32_t*
  * tokens begin in slot s = kv_len[b] - n, slot s + j becomes a copy of slot
  * s + path[b][j] for j < count[b], as if every slot were read before any is written.
  * A row of path ends before an entry that is not above the one before it, or not
- * below n; where that is before j reaches count[b], the entry becomes -1.  A move from or to a slot without a page in the pool is left out.  No
- * page that is written to may be another sequence's too.
+ * below n; where that is before j reaches count[b], the entry becomes -1.  A move from
+ * or to a slot without a page in the pool is left out.  No page that is written to may
+ * be another sequence's too.
  *
  *  kv         pages: layer 0's; layer l's are layer_stride bytes further each, not 0
  *  path       [B, width] int32
@@ -480,8 +481,8 @@ int cx_kv_copy_pages(void* pages, int64_t layer_stride, int64_t page_stride, int
  *  out        [M, ldo] fp32, or bf16 bits if out_bf16
  * Rows of the last tile past N are read and not used.  The weights are read once for
  * up to 32 rows of x; 33 to 64 rows read them once where N is above 2048, else twice,
- * and more rows as often as that many times 64 or 32.  Device pointers, stream-ordered, no synchronisation, no
- * allocation.
+ * and more rows as often as they are 64 or, where N is small, 32.  Device pointers,
+ * stream-ordered, no synchronisation, no allocation.
  */
 int cx_w4_linear_bf16(const uint16_t* x, int64_t ldx, const uint32_t* tiles,
                       const uint16_t* scales, int32_t shifts, int32_t group, int32_t M, int32_t N,

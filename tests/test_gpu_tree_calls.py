@@ -218,10 +218,11 @@ def test_rows_do_not_depend_on_the_workspace():
 
 
 @pytest.mark.parametrize("cache,D", [("bf16", 64), ("e4m3", 128)])
-@pytest.mark.parametrize("B", [1, 31, 32, 33])
-@pytest.mark.parametrize("tokens", [511, 512, 513, 1500])
+@pytest.mark.parametrize("B,tokens", [(1, 511), (1, 512), (1, 513), (1, 1500), (31, 512), (31, 1500),
+                                      (32, 511), (32, 512), (32, 513), (32, 1500), (33, 512), (33, 513),
+                                      (64, 200), (65, 200)])
 def test_on_both_sides_of_the_chunks(cache, D, B, tokens):
-    """256 workgroups and more, 16 units and more, in tables as long as the longest."""
+    """256 and 512 workgroups and more, 16 units and more, in tables as long as the longest."""
     rng = np.random.default_rng(B * tokens + D)
     lens = [tokens] + rng.integers(1, tokens, B - 1).tolist()
     new = [int(rng.integers(1, min(n, 5) + 1)) for n in lens]
