@@ -44,9 +44,9 @@ struct W4Args {
 constexpr int W4_AHEAD = 2;
 // The waves that a product should have, of the chip's 8192: two of a SIMD keep enough loads
 // in flight, and each further one has less work for its x and its sums.  K = 4096, us, with
-// half as many, these and twice as many (weights from memory): 16 rows, N = 6144 11.4, 9.1, 12.9; N = 14336 17.3,
-// 12.8, 15.2; N = 50257 56, 35, 40; N = 128256 71, 71, 77; 61 rows, N = 14336 30.6, 21.7, 21.6;
-// 30 rows, N = 50257 56, 40, 36.
+// half as many, these and twice as many (weights from memory): 16 rows, N = 6144 11.4, 9.1,
+// 12.9; N = 14336 17.3, 12.8, 15.2; N = 50257 56, 35, 40; N = 128256 71, 71, 77; 61 rows, N =
+// 14336 30.6, 21.7, 21.6; 30 rows, N = 50257 56, 40, 36.
 constexpr int W4_WAVES = 1536;
 constexpr int W4_CUS = 256;
 // Rows of x so far apart that 16 of them pass 32 bits take the other kernel.
